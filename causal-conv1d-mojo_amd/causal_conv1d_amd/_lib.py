@@ -1,8 +1,8 @@
 """ctypes binding of ``libcc1d_amd.so`` (the C ABI in ``include/cc1d.h``).
 
 The structures below mirror ``cc1d_fwd_params`` / ``cc1d_bwd_params`` /
-``cc1d_bwd_grads`` / ``cc1d_update_params`` / ``cc1d_varlen_params`` field
-for field. The library
+``cc1d_bwd_grads`` / ``cc1d_update_params`` / ``cc1d_varlen_params`` and the
+scan's and norm's params field for field. The library
 is loaded on first use; a missing or stale build raises instead of falling
 back to anything else.
 """
@@ -80,6 +80,63 @@ class VarlenParams(ctypes.Structure):
     ]
 
 
+_i64x4 = _i64 * 4
+
+
+class ScanParams(ctypes.Structure):
+    _fields_ = [
+        ("u", _vp), ("delta", _vp), ("z", _vp), ("A", _vp), ("B", _vp), ("C", _vp), ("D", _vp),
+        ("delta_bias", _vp), ("seq_idx", _vp), ("cu_seqlens", _vp), ("initial_states", _vp),
+        ("out", _vp), ("final_states", _vp), ("tile_states", _vp),
+        ("batch", _i64), ("dim", _i64), ("seqlen", _i64), ("dstate", _i64), ("groups", _i64), ("num_seqs", _i64),
+        ("u_stride", _i64x3), ("delta_stride", _i64x3), ("z_stride", _i64x3), ("A_stride", _i64x2),
+        ("B_stride", _i64x4), ("C_stride", _i64x4), ("D_stride", _i64), ("delta_bias_stride", _i64),
+        ("seq_idx_stride", _i64x2), ("initial_states_stride", _i64x3), ("out_stride", _i64x3),
+        ("final_states_stride", _i64x3),
+        ("dtype", _i32), ("delta_softplus", _i32),
+    ]
+
+
+class ScanBwdParams(ctypes.Structure):
+    _fields_ = [
+        ("fwd", ScanParams), ("dout", _vp), ("dfinal_states", _vp), ("du", _vp), ("ddelta", _vp), ("dz", _vp),
+        ("dA", _vp), ("dB", _vp), ("dC", _vp), ("dD", _vp), ("ddelta_bias", _vp), ("dinitial_states", _vp),
+        ("workspace", _vp), ("workspace_floats", _i64),
+        ("dout_stride", _i64x3), ("dfinal_states_stride", _i64x3), ("du_stride", _i64x3),
+        ("ddelta_stride", _i64x3), ("dz_stride", _i64x3),
+    ]
+
+
+class ScanUpdateParams(ctypes.Structure):
+    _fields_ = [
+        ("u", _vp), ("delta", _vp), ("z", _vp), ("A", _vp), ("B", _vp), ("C", _vp), ("D", _vp),
+        ("delta_bias", _vp), ("ssm_state", _vp), ("ssm_state_indices", _vp), ("out", _vp),
+        ("batch", _i64), ("dim", _i64), ("seqlen", _i64), ("dstate", _i64), ("groups", _i64), ("state_rows", _i64),
+        ("u_stride", _i64x3), ("delta_stride", _i64x3), ("z_stride", _i64x3), ("A_stride", _i64x2),
+        ("B_stride", _i64x4), ("C_stride", _i64x4), ("D_stride", _i64), ("delta_bias_stride", _i64),
+        ("ssm_state_stride", _i64x3), ("out_stride", _i64x3),
+        ("dtype", _i32), ("delta_softplus", _i32),
+    ]
+
+
+class NormParams(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("weight", _vp), ("bias", _vp), ("y", _vp), ("sum", _vp), ("stats", _vp),
+        ("rows", _i64), ("dim", _i64),
+        ("x_stride", _i64), ("residual_stride", _i64), ("weight_stride", _i64), ("bias_stride", _i64),
+        ("y_stride", _i64), ("sum_stride", _i64),
+        ("eps", ctypes.c_double), ("dtype", _i32), ("residual_dtype", _i32), ("rms", _i32),
+    ]
+
+
+class NormBwdParams(ctypes.Structure):
+    _fields_ = [
+        ("fwd", NormParams), ("dy", _vp), ("dsum", _vp), ("dx", _vp), ("dresidual", _vp), ("dweight", _vp),
+        ("dbias", _vp), ("workspace", _vp), ("workspace_floats", _i64),
+        ("dy_stride", _i64), ("dsum_stride", _i64), ("dx_stride", _i64), ("dresidual_stride", _i64),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "cc1d_abi_version",
     "cc1d_strerror",
@@ -90,6 +147,14 @@ EXPORTED_SYMBOLS = (
     "cc1d_bwd_typed_noalloc",
     "cc1d_update",
     "cc1d_varlen_states",
+    "cc1d_scan_fwd",
+    "cc1d_scan_tile_floats",
+    "cc1d_scan_bwd",
+    "cc1d_scan_bwd_workspace_floats",
+    "cc1d_scan_update",
+    "cc1d_norm_fwd",
+    "cc1d_norm_bwd",
+    "cc1d_norm_bwd_workspace_floats",
 )
 
 _lib = None
@@ -121,12 +186,18 @@ def load():
     lib.cc1d_strerror.restype = ctypes.c_char_p
     lib.cc1d_strerror.argtypes = [ctypes.c_int]
     for name, st in (("cc1d_fwd", FwdParams), ("cc1d_bwd", BwdParams), ("cc1d_update", UpdateParams),
-                     ("cc1d_varlen_states", VarlenParams)):
+                     ("cc1d_varlen_states", VarlenParams), ("cc1d_scan_fwd", ScanParams),
+                     ("cc1d_scan_bwd", ScanBwdParams), ("cc1d_scan_update", ScanUpdateParams),
+                     ("cc1d_norm_fwd", NormParams), ("cc1d_norm_bwd", NormBwdParams)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(st), _vp]
-    lib.cc1d_bwd_workspace_floats.restype = ctypes.c_int64
-    lib.cc1d_bwd_workspace_floats.argtypes = [ctypes.POINTER(BwdParams)]
+    for name, st in (("cc1d_bwd_workspace_floats", BwdParams), ("cc1d_scan_tile_floats", ScanParams),
+                     ("cc1d_scan_bwd_workspace_floats", ScanBwdParams),
+                     ("cc1d_norm_bwd_workspace_floats", NormBwdParams)):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int64
+        fn.argtypes = [ctypes.POINTER(st)]
     for name in ("cc1d_bwd_typed", "cc1d_bwd_typed_noalloc"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int

@@ -53,6 +53,38 @@ int bwd_typed_entry(const cc1d_bwd_params* p, const cc1d_bwd_grads* g, void* str
     return launch_bwd_typed(*p, *g, s);
 }
 
+// Sizes and options of a scan, before its pointers.
+int check_scan(const cc1d_scan_params& p) {
+    if (!valid_dtype(p.dtype)) return CC1D_ERR_DTYPE;
+    if (p.dstate < 1 || p.dstate > CC1D_MAX_DSTATE) return CC1D_ERR_DSTATE;
+    if (p.batch < 0 || p.dim < 0 || p.seqlen < 0) return CC1D_ERR_SHAPE;
+    if (p.groups < 1 || p.dim % p.groups != 0) return CC1D_ERR_GROUPS;
+    if (p.seq_idx != nullptr &&
+        (p.initial_states != nullptr || p.final_states != nullptr || p.cu_seqlens != nullptr))
+        return CC1D_ERR_EXCLUSIVE;
+    if (p.cu_seqlens != nullptr && (p.batch != 1 || p.num_seqs < 0 || (p.num_seqs == 0 && p.seqlen > 0)))
+        return CC1D_ERR_SHAPE;
+    const int64_t seqs = p.cu_seqlens != nullptr ? p.num_seqs : p.batch;
+    // a block per sequence and channel at most, a thread per value of dB and dC, 32-bit positions
+    const double blocks = (double)seqs * (double)p.dim;
+    const double values = (double)p.batch * (double)p.groups * (double)p.dstate * (double)p.seqlen;
+    if (blocks >= (double)kMaxBlocks || values / 256 + 1 >= (double)kMaxBlocks || p.seqlen >= ((int64_t)1 << 31) - 4096)
+        return CC1D_ERR_SHAPE;
+    return CC1D_OK;
+}
+
+bool scan_empty(const cc1d_scan_params& p) {
+    return p.dim == 0 || (p.cu_seqlens != nullptr ? p.num_seqs == 0 : p.batch == 0);
+}
+
+int check_norm(const cc1d_norm_params& p) {
+    if (!valid_dtype(p.dtype) || (p.residual_dtype != p.dtype && p.residual_dtype != CC1D_DTYPE_FP32))
+        return CC1D_ERR_DTYPE;
+    if (p.rows < 0 || p.rows >= kMaxBlocks) return CC1D_ERR_SHAPE;
+    if (p.dim < 1 || p.dim > CC1D_MAX_NORM_DIM) return CC1D_ERR_NORM_DIM;
+    return CC1D_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -73,6 +105,9 @@ const char* cc1d_strerror(int status) {
     case CC1D_ERR_SCRATCH_LIMIT:
         return "problem needs more workspace than the static scratch of cc1d_bwd_typed_noalloc "
                "(CC1D_NOALLOC_WORKSPACE_FLOATS floats)";
+    case CC1D_ERR_DSTATE: return "dstate must be in 1..256";
+    case CC1D_ERR_GROUPS: return "dim must be a multiple of groups";
+    case CC1D_ERR_NORM_DIM: return "norm dim must be in 1..32768";
     default: return "unknown status";
     }
 }
@@ -162,6 +197,90 @@ int cc1d_varlen_states(const cc1d_varlen_params* p, void* stream) {
     if (p->cu_seqlens == nullptr || p->states == nullptr || (p->x == nullptr && p->total_tokens > 0))
         return CC1D_ERR_NULL_POINTER;
     return launch_varlen_states(*p, static_cast<hipStream_t>(stream));
+}
+
+int cc1d_scan_fwd(const cc1d_scan_params* p, void* stream) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const int st = check_scan(*p);
+    if (st != CC1D_OK) return st;
+    if (scan_empty(*p)) return CC1D_OK;
+    // without positions only the states are read and written
+    if (p->seqlen == 0 && p->final_states == nullptr) return CC1D_OK;
+    if (p->A == nullptr) return CC1D_ERR_NULL_POINTER;
+    if (p->seqlen > 0 && (p->u == nullptr || p->delta == nullptr || p->B == nullptr || p->C == nullptr || p->out == nullptr))
+        return CC1D_ERR_NULL_POINTER;
+    return launch_scan_fwd(*p, static_cast<hipStream_t>(stream));
+}
+
+int64_t cc1d_scan_tile_floats(const cc1d_scan_params* p) {
+    if (p == nullptr || check_scan(*p) != CC1D_OK) return -1;
+    return scan_empty(*p) ? 0 : scan_tile_floats(*p);
+}
+
+int cc1d_scan_bwd(const cc1d_scan_bwd_params* b, void* stream) {
+    if (b == nullptr) return CC1D_ERR_NULL_POINTER;
+    const cc1d_scan_params& p = b->fwd;
+    const int st = check_scan(p);
+    if (st != CC1D_OK) return st;
+    if (p.seq_idx != nullptr && (b->dfinal_states != nullptr || b->dinitial_states != nullptr)) return CC1D_ERR_EXCLUSIVE;
+    if (p.dim == 0) return CC1D_OK;
+    if (b->dA == nullptr || p.A == nullptr) return CC1D_ERR_NULL_POINTER;
+    if (p.batch * p.seqlen > 0 &&
+        (p.u == nullptr || p.delta == nullptr || p.B == nullptr || p.C == nullptr || p.tile_states == nullptr ||
+         b->dout == nullptr || b->du == nullptr || b->ddelta == nullptr || b->dB == nullptr || b->dC == nullptr ||
+         (p.z != nullptr && b->dz == nullptr)))
+        return CC1D_ERR_NULL_POINTER;
+    const int64_t need = scan_empty(p) ? 0 : scan_bwd_workspace_floats(*b);
+    if (b->workspace_floats < need) return CC1D_ERR_WORKSPACE;
+    if (need > 0 && b->workspace == nullptr) return CC1D_ERR_NULL_POINTER;
+    return launch_scan_bwd(*b, static_cast<hipStream_t>(stream));
+}
+
+int64_t cc1d_scan_bwd_workspace_floats(const cc1d_scan_bwd_params* b) {
+    if (b == nullptr || check_scan(b->fwd) != CC1D_OK) return -1;
+    return scan_empty(b->fwd) ? 0 : scan_bwd_workspace_floats(*b);
+}
+
+int cc1d_scan_update(const cc1d_scan_update_params* p, void* stream) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    if (!valid_dtype(p->dtype)) return CC1D_ERR_DTYPE;
+    if (p->dstate < 1 || p->dstate > CC1D_MAX_DSTATE) return CC1D_ERR_DSTATE;
+    if (p->batch < 0 || p->dim < 0 || p->seqlen < 0 || p->state_rows < 0) return CC1D_ERR_SHAPE;
+    if (p->groups < 1 || p->dim % p->groups != 0) return CC1D_ERR_GROUPS;
+    if (p->ssm_state_indices == nullptr && p->state_rows < p->batch) return CC1D_ERR_SHAPE;
+    if (p->batch == 0 || p->dim == 0 || p->seqlen == 0) return CC1D_OK;
+    if ((double)p->batch * (double)p->dim >= (double)kMaxBlocks) return CC1D_ERR_SHAPE;  // a block per channel at most
+    if (p->u == nullptr || p->delta == nullptr || p->A == nullptr || p->B == nullptr || p->C == nullptr ||
+        p->out == nullptr || (p->ssm_state == nullptr && p->state_rows > 0))
+        return CC1D_ERR_NULL_POINTER;
+    return launch_scan_update(*p, static_cast<hipStream_t>(stream));
+}
+
+int cc1d_norm_fwd(const cc1d_norm_params* p, void* stream) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const int st = check_norm(*p);
+    if (st != CC1D_OK) return st;
+    if (p->rows == 0) return CC1D_OK;
+    if (p->x == nullptr || p->weight == nullptr || p->y == nullptr) return CC1D_ERR_NULL_POINTER;
+    return launch_norm_fwd(*p, static_cast<hipStream_t>(stream));
+}
+
+int cc1d_norm_bwd(const cc1d_norm_bwd_params* b, void* stream) {
+    if (b == nullptr) return CC1D_ERR_NULL_POINTER;
+    const cc1d_norm_params& p = b->fwd;
+    const int st = check_norm(p);
+    if (st != CC1D_OK) return st;
+    if (b->dweight == nullptr || p.weight == nullptr) return CC1D_ERR_NULL_POINTER;
+    if (p.rows > 0 && ((p.x == nullptr && p.residual == nullptr) || p.stats == nullptr || b->dy == nullptr ||
+                       b->dx == nullptr || b->workspace == nullptr))
+        return CC1D_ERR_NULL_POINTER;
+    if (b->workspace_floats < norm_bwd_workspace_floats(*b)) return CC1D_ERR_WORKSPACE;
+    return launch_norm_bwd(*b, static_cast<hipStream_t>(stream));
+}
+
+int64_t cc1d_norm_bwd_workspace_floats(const cc1d_norm_bwd_params* b) {
+    if (b == nullptr || check_norm(b->fwd) != CC1D_OK) return -1;
+    return norm_bwd_workspace_floats(*b);
 }
 
 }  // extern "C"

@@ -32,6 +32,15 @@ int launch_varlen_states(const cc1d_varlen_params& p, hipStream_t stream);
 // element size of a varlen gather: elem_bytes, or the size of dtype when it is 0
 int varlen_elem_bytes(const cc1d_varlen_params& p);
 
+int launch_scan_fwd(const cc1d_scan_params& p, hipStream_t stream);
+int64_t scan_tile_floats(const cc1d_scan_params& p);
+int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream);
+int64_t scan_bwd_workspace_floats(const cc1d_scan_bwd_params& b);
+int launch_scan_update(const cc1d_scan_update_params& p, hipStream_t stream);
+int launch_norm_fwd(const cc1d_norm_params& p, hipStream_t stream);
+int launch_norm_bwd(const cc1d_norm_bwd_params& b, hipStream_t stream);
+int64_t norm_bwd_workspace_floats(const cc1d_norm_bwd_params& b);
+
 // Compile-time dispatch over the runtime dtype code / width / flags.
 template <typename F> int with_dtype(int dtype, F&& f) {
     switch (dtype) {

@@ -61,9 +61,15 @@ enum cc1d_status {
     CC1D_ERR_STATE_LEN = 6,         /* conv_state length < width - 1 */
     CC1D_ERR_LAUNCH = 7,            /* the HIP runtime refused a kernel launch */
     CC1D_ERR_WORKSPACE = 8,         /* workspace smaller than cc1d_bwd_workspace_floats() */
-    CC1D_ERR_SCRATCH_LIMIT = 9      /* cc1d_bwd_typed_noalloc: the problem needs more than
+    CC1D_ERR_SCRATCH_LIMIT = 9,     /* cc1d_bwd_typed_noalloc: the problem needs more than
                                        CC1D_NOALLOC_WORKSPACE_FLOATS floats of workspace */
+    CC1D_ERR_DSTATE = 10,           /* dstate outside 1..CC1D_MAX_DSTATE */
+    CC1D_ERR_GROUPS = 11,           /* groups < 1, or dim not a multiple of it */
+    CC1D_ERR_NORM_DIM = 12          /* norm dim outside 1..CC1D_MAX_NORM_DIM */
 };
+
+#define CC1D_MAX_DSTATE 256
+#define CC1D_MAX_NORM_DIM 32768
 
 /* Size (fp32 elements) of the static device scratch of cc1d_bwd_typed_noalloc: 8 MiB, reserved on
    every GPU where the library's kernels are loaded, whether or not cc1d_bwd_typed_noalloc is called
@@ -205,6 +211,159 @@ typedef struct cc1d_varlen_params {
     int32_t elem_bytes;            /* 0, or 1 / 2 / 4 / 8 / 16 */
 } cc1d_varlen_params;
 
+/*
+ * Selective state space scan over prompts. With dt = delta + delta_bias, its
+ * softplus when delta_softplus is set,
+ *     h[t] = exp(dt[t] A) h[t-1] + dt[t] u[t] B[t]       (per channel, dstate values)
+ *     y[t] = sum_n C[t,n] h[t,n] + D u[t],  out = z given ? y * silu(z) : y.
+ * Sequences are the batch rows (h before the first position is
+ * initial_states, or 0), or with cu_seqlens the runs [cu[i], cu[i+1]) of the
+ * one batch row (states then have num_seqs rows). With seq_idx, h starts at 0
+ * wherever the id differs from the one before, and positions with an id < 0
+ * take no part: out is 0 there and nothing they hold reaches another position.
+ * Positions that no sequence of cu_seqlens covers get 0 (its values are
+ * clamped to [0, seqlen] and have to be non-decreasing).
+ * Parameters and states are fp32; u, delta, z, B, C and out share dtype.
+ * Arithmetic and states are fp32; each output is rounded once.
+ */
+typedef struct cc1d_scan_params {
+    const void* u;                 /* (batch, dim, seqlen) */
+    const void* delta;             /* (batch, dim, seqlen) */
+    const void* z;                 /* (batch, dim, seqlen) or NULL */
+    const float* A;                /* (dim, dstate) */
+    const void* B;                 /* (batch, groups, dstate, seqlen) */
+    const void* C;                 /* (batch, groups, dstate, seqlen) */
+    const float* D;                /* (dim,) or NULL */
+    const float* delta_bias;       /* (dim,) or NULL */
+    const int32_t* seq_idx;        /* (batch, seqlen) or NULL; not with states or cu_seqlens */
+    const int32_t* cu_seqlens;     /* (num_seqs + 1,) contiguous or NULL; batch is 1 */
+    const float* initial_states;   /* (sequences, dim, dstate) or NULL */
+    void* out;                     /* (batch, dim, seqlen) */
+    float* final_states;           /* (sequences, dim, dstate) or NULL */
+    float* tile_states;            /* cc1d_scan_tile_floats() floats for the backward, or NULL */
+    int64_t batch, dim, seqlen, dstate, groups, num_seqs;
+    int64_t u_stride[3];
+    int64_t delta_stride[3];
+    int64_t z_stride[3];
+    int64_t A_stride[2];
+    int64_t B_stride[4];
+    int64_t C_stride[4];
+    int64_t D_stride, delta_bias_stride;
+    int64_t seq_idx_stride[2];
+    int64_t initial_states_stride[3];
+    int64_t out_stride[3];
+    int64_t final_states_stride[3];
+    int32_t dtype;
+    int32_t delta_softplus;
+} cc1d_scan_params;
+
+/*
+ * Backward of the scan: `fwd` as it was given to cc1d_scan_fwd (tile_states
+ * as that call filled it; out and final_states are not read), dout and
+ * dfinal_states the gradients of its results. Every sum runs in a fixed
+ * order, so the same inputs give the same bits. Gradient outputs that are
+ * not wanted are NULL, except du, ddelta, dA, dB and dC. dA, dB, dC, dD,
+ * ddelta_bias and dinitial_states are contiguous; dB and dC have dtype.
+ */
+typedef struct cc1d_scan_bwd_params {
+    cc1d_scan_params fwd;
+    const void* dout;              /* (batch, dim, seqlen) */
+    const float* dfinal_states;    /* (sequences, dim, dstate) or NULL */
+    void* du;                      /* (batch, dim, seqlen) */
+    void* ddelta;                  /* (batch, dim, seqlen) */
+    void* dz;                      /* (batch, dim, seqlen); required when z is given */
+    float* dA;                     /* (dim, dstate) */
+    void* dB;                      /* (batch, groups, dstate, seqlen) */
+    void* dC;                      /* (batch, groups, dstate, seqlen) */
+    float* dD;                     /* (dim,) or NULL */
+    float* ddelta_bias;            /* (dim,) or NULL */
+    float* dinitial_states;        /* (sequences, dim, dstate) or NULL */
+    float* workspace;              /* cc1d_scan_bwd_workspace_floats() floats */
+    int64_t workspace_floats;
+    int64_t dout_stride[3];
+    int64_t dfinal_states_stride[3];
+    int64_t du_stride[3];
+    int64_t ddelta_stride[3];
+    int64_t dz_stride[3];
+} cc1d_scan_bwd_params;
+
+/*
+ * The scan for `seqlen` new tokens (one or a few) per sequence of a decode
+ * batch, on a state pool updated in place. ssm_state_indices redirects batch
+ * entry b to that row of the pool; an index < 0 (padding) or >= state_rows
+ * zeroes out[b] and leaves the pool untouched. Live entries name distinct rows.
+ */
+typedef struct cc1d_scan_update_params {
+    const void* u;                 /* (batch, dim, seqlen) */
+    const void* delta;
+    const void* z;                 /* or NULL */
+    const float* A;                /* (dim, dstate) */
+    const void* B;                 /* (batch, groups, dstate, seqlen) */
+    const void* C;
+    const float* D;                /* (dim,) or NULL */
+    const float* delta_bias;       /* (dim,) or NULL */
+    float* ssm_state;              /* (state_rows, dim, dstate), updated */
+    const int32_t* ssm_state_indices; /* (batch,) contiguous or NULL */
+    void* out;                     /* (batch, dim, seqlen) */
+    int64_t batch, dim, seqlen, dstate, groups, state_rows;
+    int64_t u_stride[3];
+    int64_t delta_stride[3];
+    int64_t z_stride[3];
+    int64_t A_stride[2];
+    int64_t B_stride[4];
+    int64_t C_stride[4];
+    int64_t D_stride, delta_bias_stride;
+    int64_t ssm_state_stride[3];
+    int64_t out_stride[3];
+    int32_t dtype;
+    int32_t delta_softplus;
+} cc1d_scan_update_params;
+
+/*
+ * Residual add and norm over rows of `dim` values:
+ *     r = x + residual;  y = (r - mean) * rstd * weight + bias
+ * with mean = 0 when rms is set and rstd = 1 / sqrt(mean((r - mean)^2) + eps).
+ * The statistics and y are taken from the fp32 sum; sum (optional) receives
+ * it rounded to the residual's dtype. Rows are `*_stride` elements apart and
+ * contiguous inside. stats receives mean and rstd of each row (2 * rows
+ * floats) for the backward, or is NULL.
+ */
+typedef struct cc1d_norm_params {
+    const void* x;                 /* (rows, dim) */
+    const void* residual;          /* (rows, dim) or NULL */
+    const float* weight;           /* (dim,) */
+    const float* bias;             /* (dim,) or NULL */
+    void* y;                       /* (rows, dim), dtype */
+    void* sum;                     /* (rows, dim), residual_dtype, or NULL */
+    float* stats;                  /* 2 * rows floats or NULL */
+    int64_t rows, dim;
+    int64_t x_stride, residual_stride, weight_stride, bias_stride, y_stride, sum_stride;
+    double eps;
+    int32_t dtype;                 /* of x and y */
+    int32_t residual_dtype;        /* of residual and sum: dtype, or fp32 */
+    int32_t rms;
+} cc1d_norm_params;
+
+/*
+ * Backward: x, residual, weight, stats and the flags as in the forward (a
+ * caller that kept an fp32 sum may give it as residual with x NULL). dsum is
+ * the gradient of the forward's sum. dx = dresidual up to their dtypes;
+ * dresidual is NULL where it is not wanted or would repeat dx. The parameter
+ * gradients are summed in a fixed order over partial sums in the workspace.
+ */
+typedef struct cc1d_norm_bwd_params {
+    cc1d_norm_params fwd;
+    const void* dy;                /* (rows, dim), dtype */
+    const void* dsum;              /* (rows, dim), residual_dtype, or NULL */
+    void* dx;                      /* (rows, dim), dtype */
+    void* dresidual;               /* (rows, dim), residual_dtype, or NULL */
+    float* dweight;                /* (dim,) contiguous */
+    float* dbias;                  /* (dim,) contiguous or NULL */
+    float* workspace;              /* cc1d_norm_bwd_workspace_floats() floats */
+    int64_t workspace_floats;
+    int64_t dy_stride, dsum_stride, dx_stride, dresidual_stride;
+} cc1d_norm_bwd_params;
+
 int cc1d_abi_version(void);
 const char* cc1d_strerror(int status);
 
@@ -242,6 +401,20 @@ int cc1d_bwd_typed(const cc1d_bwd_params* params, const cc1d_bwd_grads* grads, v
 int cc1d_bwd_typed_noalloc(const cc1d_bwd_params* params, const cc1d_bwd_grads* grads, void* stream);
 int cc1d_update(const cc1d_update_params* params, void* stream);
 int cc1d_varlen_states(const cc1d_varlen_params* params, void* stream);
+
+/*
+ * Scan, decode step and norm. The workspace sizes depend on the sizes and
+ * flags of the params alone (< 0 for invalid ones); what a workspace holds
+ * before a call is not read.
+ */
+int cc1d_scan_fwd(const cc1d_scan_params* params, void* stream);
+int64_t cc1d_scan_tile_floats(const cc1d_scan_params* params);
+int cc1d_scan_bwd(const cc1d_scan_bwd_params* params, void* stream);
+int64_t cc1d_scan_bwd_workspace_floats(const cc1d_scan_bwd_params* params);
+int cc1d_scan_update(const cc1d_scan_update_params* params, void* stream);
+int cc1d_norm_fwd(const cc1d_norm_params* params, void* stream);
+int cc1d_norm_bwd(const cc1d_norm_bwd_params* params, void* stream);
+int64_t cc1d_norm_bwd_workspace_floats(const cc1d_norm_bwd_params* params);
 
 #ifdef __cplusplus
 }
