@@ -26,7 +26,7 @@ MAX_DSTATE = 256
 
 def scan_tile(seqlen: int) -> int:
     """Positions between the states that a training forward keeps for the backward (csrc/cc1d_scan_device.hpp)."""
-    return 256
+    return 256 if seqlen <= 256 else 512
 
 
 def scan_tile_floats(u: torch.Tensor, A: torch.Tensor, cu_seqlens: torch.Tensor | None) -> int:

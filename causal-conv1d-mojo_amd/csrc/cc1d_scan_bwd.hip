@@ -9,218 +9,391 @@
 namespace cc1d {
 namespace {
 
-constexpr int K = 4;
-constexpr int TILE = 64 * K;
-
 struct ScanBwdArgs {
     cc1d_scan_bwd_params p;
-    float *pB, *pC;  // (batch, dim, dstate, seqlen): each channel's terms of dB and dC
-    float *pA;       // (sequences, dim, dstate)
-    float *pD, *pbias;  // (sequences, dim)
+    float* carry;        // (sequences, dim, dstate): a g of the position after the tile being worked on
+    float* pA;           // (sequences, dim, dstate)
+    float *pD, *pbias;   // (sequences, dim)
+    float* pBC;          // (batch, groups, group_blocks, [B, C], dstate, seqlen): each block's share of dB and dC
+    int64_t group_blocks;
+    int rounds;          // times a block takes its wavefronts' channels, in every tile
 };
 
-template <typename T> __device__ void zero_uncovered(const ScanBwdArgs& a, int64_t d, int64_t from, int64_t to) {
-    const cc1d_scan_bwd_params& p = a.p;
-    for (int64_t t = from + threadIdx.x; t < to; t += 64) {
+template <typename T> __device__ void zero_uncovered(const cc1d_scan_bwd_params& p, int64_t d, int64_t from, int64_t to) {
+    for (int64_t t = from + (threadIdx.x & 63); t < to; t += 64) {
         static_cast<T*>(p.du)[d * p.du_stride[1] + t * p.du_stride[2]] = T{};
         static_cast<T*>(p.ddelta)[d * p.ddelta_stride[1] + t * p.ddelta_stride[2]] = T{};
-        if (p.dz) static_cast<T*>(p.dz)[d * p.dz_stride[1] + t * p.dz_stride[2]] = T{};
-        for (int64_t n = 0; n < p.fwd.dstate; ++n) {
-            a.pB[(d * p.fwd.dstate + n) * p.fwd.seqlen + t] = 0.0f;
-            a.pC[(d * p.fwd.dstate + n) * p.fwd.seqlen + t] = 0.0f;
-        }
+        if (p.fwd.z) static_cast<T*>(p.dz)[d * p.dz_stride[1] + t * p.dz_stride[2]] = T{};
     }
 }
 
-// One wavefront per (sequence, channel), every layout.
-template <typename T> __global__ void __launch_bounds__(64) scan_bwd_kernel(const ScanBwdArgs arg) {
-    __shared__ float carry[CC1D_MAX_DSTATE];  // a g of the position after the tile
-    __shared__ float dA[CC1D_MAX_DSTATE];
+// What one channel's tile holds in registers.
+template <int K> struct Channel {
+    float dt[K], du[K], dy[K];       // du: dt u
+    float y[K], along[K], wsum[K];   // sums over the states: C h, g B, A w
+    float step_sum;
+};
+
+// One state of CHW channels. before / after: h ahead of the tile and a g behind
+// it; on return after is a g of the tile's first position. dB, dC: the
+// channels' terms. dA: the lane's share of the state's dA.
+template <int K, int CHW, bool CUT>
+__device__ __forceinline__ void scan_state_bwd(Channel<K> (&ch)[CHW], const float (&A)[CHW], const float (&before)[CHW],
+                                               float (&after)[CHW], float (&dA)[CHW], const float (&B)[K], const float (&C)[K],
+                                               float (&dB)[K], float (&dC)[K], const Cuts<K>& cuts, int lane) {
+    float a[CHW][K], h[CHW][K], H[CHW], P[CHW], Pr[CHW], Q[CHW], first[CHW];
+#pragma unroll
+    for (int c = 0; c < CHW; ++c) {
+        const float A2 = A[c] * kLog2e;
+#pragma unroll
+        for (int j = 0; j < K; ++j) a[c][j] = __builtin_amdgcn_exp2f(ch[c].dt[j] * A2);
+        P[c] = __builtin_amdgcn_exp2f(ch[c].step_sum * A2);
+        // the lanes in reverse, for the prefix from the end
+        Pr[c] = lane_get(P[c], 63 - lane);
+        float v = ch[c].du[0] * B[0];
+#pragma unroll
+        for (int j = 1; j < K; ++j) {
+            const float b = ch[c].du[j] * B[j];
+            v = CUT && cuts.at[j] ? b : __builtin_fmaf(a[c][j], v, b);
+        }
+        first[c] = lane == 0 ? before[c] : 0.0f;
+        const float entered = __builtin_fmaf(P[c], first[c], v);
+        H[c] = CUT && (cuts.met || lane != 0) ? v : entered;
+        // Q = a g of the lane's first position
+        float x = 0.0f;
+#pragma unroll
+        for (int j = K - 1; j >= 0; --j) {
+            x = a[c][j] * __builtin_fmaf(C[j], ch[c].dy[j], x);
+            if (CUT && cuts.at[j]) x = 0.0f;
+        }
+        Q[c] = lane_get(x, 63 - lane);
+    }
+    const bool met_back = CUT && __shfl((int)cuts.met, 63 - lane) != 0;
+    float behind[CHW];
+#pragma unroll
+    for (int c = 0; c < CHW; ++c) {
+        behind[c] = lane == 0 ? after[c] : 0.0f;
+        const float entered = __builtin_fmaf(Pr[c], behind[c], Q[c]);
+        Q[c] = CUT && (met_back || lane != 0) ? Q[c] : entered;
+    }
+    if constexpr (CUT) {
+#pragma unroll
+        for (int c = 0; c < CHW; ++c) {
+            wave_prefix_cut(H[c], P[c], cuts.absorb);
+            wave_prefix_cut(Q[c], Pr[c], cuts.back);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < CHW; ++c) wave_prefix2(H[c], P[c], Q[c], Pr[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < CHW; ++c) {
+        const float ahead = dpp_keep<kDppWaveShr1, 0xf>(first[c], H[c]);  // h before the lane's first position
+        float x = dpp_keep<kDppWaveShr1, 0xf>(behind[c], Q[c]);           // a g after its last one, lanes in reverse
+        after[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q[c]), 63));
+        x = lane_get(x, 63 - lane);
+        float v = ahead;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const float b = ch[c].du[j] * B[j];
+            v = CUT && cuts.at[j] ? b : __builtin_fmaf(a[c][j], v, b);
+            h[c][j] = v;
+            ch[c].y[j] = __builtin_fmaf(C[j], v, ch[c].y[j]);
+            dC[j] = c == 0 ? ch[c].dy[j] * v : __builtin_fmaf(ch[c].dy[j], v, dC[j]);
+        }
+        float dAc = 0.0f;
+#pragma unroll
+        for (int j = K - 1; j >= 0; --j) {
+            const float g = __builtin_fmaf(C[j], ch[c].dy[j], x);
+            dB[j] = c == 0 ? g * ch[c].du[j] : __builtin_fmaf(g, ch[c].du[j], dB[j]);
+            ch[c].along[j] = __builtin_fmaf(g, B[j], ch[c].along[j]);
+            x = a[c][j] * g;
+            float w = x * (j > 0 ? h[c][j > 0 ? j - 1 : 0] : ahead);
+            if (CUT && cuts.at[j]) x = w = 0.0f;
+            ch[c].wsum[j] = __builtin_fmaf(A[c], w, ch[c].wsum[j]);
+            dAc = __builtin_fmaf(ch[c].dt[j], w, dAc);
+        }
+        dA[c] = dAc;
+    }
+}
+
+// A block: NW wavefronts of CHW channels each, `rounds` times, of one group and
+// sequence; tiles from the last to the first. In a tile, each round's channels
+// run through 16 states at a time, each wavefront at another one (state i + its
+// own offset in step i), so that the block's sums for dB and dC of a state, in
+// LDS, belong to one wavefront at a time and grow in a fixed order.
+template <typename T, int K, int CHW, int NW, bool SEQ, bool UNIT, bool TIME>
+__global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdArgs arg) {
+    constexpr int TILE = 64 * K;
+    __shared__ __attribute__((aligned(16))) float BC[2 * kStates * TILE];
+    __shared__ __attribute__((aligned(16))) float acc[2 * kStates * TILE];
     const cc1d_scan_bwd_params& b = arg.p;
     const cc1d_scan_params& p = b.fwd;
-    const int lane = threadIdx.x;
-    const int64_t s = blockIdx.x / p.dim, d = blockIdx.x % p.dim;
+    const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
+    const int64_t per = p.dim / p.groups;
+    const int64_t blk = blockIdx.x % arg.group_blocks, grp = blockIdx.x / arg.group_blocks % p.groups,
+                  s = blockIdx.x / arg.group_blocks / p.groups;
     const ScanSpan q = scan_span(p, s, TILE);
-    if (p.cu_seqlens != nullptr) {
-        if (s == 0) zero_uncovered<T>(arg, d, 0, q.start);
-        if (s == p.num_seqs - 1) zero_uncovered<T>(arg, d, q.start + q.len, p.seqlen);
-    }
-    const T* u = static_cast<const T*>(p.u) + q.row * p.u_stride[0] + d * p.u_stride[1];
-    const T* delta = static_cast<const T*>(p.delta) + q.row * p.delta_stride[0] + d * p.delta_stride[1];
-    const T* z = p.z ? static_cast<const T*>(p.z) + q.row * p.z_stride[0] + d * p.z_stride[1] : nullptr;
-    const T* dout = static_cast<const T*>(b.dout) + q.row * b.dout_stride[0] + d * b.dout_stride[1];
-    T* du_out = static_cast<T*>(b.du) + q.row * b.du_stride[0] + d * b.du_stride[1];
-    T* dd_out = static_cast<T*>(b.ddelta) + q.row * b.ddelta_stride[0] + d * b.ddelta_stride[1];
-    T* dz_out = z ? static_cast<T*>(b.dz) + q.row * b.dz_stride[0] + d * b.dz_stride[1] : nullptr;
-    const int64_t grp = d / (p.dim / p.groups);
+    const int N = (int)p.dstate;
+    const int begin = (int)q.start, end = (int)(q.start + q.len), size = (int)p.seqlen;
     const T* Bp = static_cast<const T*>(p.B) + q.row * p.B_stride[0] + grp * p.B_stride[1];
     const T* Cp = static_cast<const T*>(p.C) + q.row * p.C_stride[0] + grp * p.C_stride[1];
-    const int32_t* ids = p.seq_idx ? p.seq_idx + q.row * p.seq_idx_stride[0] : nullptr;
-    const float bias = p.delta_bias ? p.delta_bias[d * p.delta_bias_stride] : 0.0f;
-    const float skip = p.D ? p.D[d * p.D_stride] : 0.0f;
-    const int N = (int)p.dstate;
-    for (int n = lane; n < N; n += 64) {
-        carry[n] = b.dfinal_states ? b.dfinal_states[s * b.dfinal_states_stride[0] + d * b.dfinal_states_stride[1] +
-                                                     n * b.dfinal_states_stride[2]]
-                                   : 0.0f;
-        dA[n] = 0.0f;
-    }
-    float dD = 0.0f, dbias = 0.0f;
-    __syncthreads();
-    const int64_t tiles = (q.len + TILE - 1) / TILE;
-    for (int64_t i = tiles - 1; i >= 0; --i) {
-        const int64_t tl = i * TILE + lane * K;
-        float uu[K], raw[K], dt[K], dy[K], y[K], along[K], wsum[K], zz[K], dd[K];
-        bool live[K], cut[K];
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const int64_t t = q.start + tl + j;
-            live[j] = tl + j < q.len;
-            cut[j] = false;
-            if (live[j] && ids) {
-                const int32_t id = ids[t * p.seq_idx_stride[1]];
-                cut[j] = t == 0 || ids[(t - 1) * p.seq_idx_stride[1]] != id;
-                live[j] = id >= 0;
+    float* pBC = arg.pBC + ((q.row * p.groups + grp) * arg.group_blocks + blk) * 2 * N * p.seqlen;
+    const int32_t* ids = SEQ ? p.seq_idx + q.row * p.seq_idx_stride[0] : nullptr;
+    const int64_t is = SEQ ? p.seq_idx_stride[1] : 0;
+    const int tiles = (int)((q.len + TILE - 1) / TILE);
+    const int64_t block_first = blk * arg.rounds * (NW * CHW);  // the block's first channel in the group
+    const int rounds = (int)(per - block_first + NW * CHW - 1 < (int64_t)arg.rounds * NW * CHW
+                                 ? (per - block_first + NW * CHW - 1) / (NW * CHW) : arg.rounds);
+
+    if (tiles == 0 || p.cu_seqlens) {
+        for (int64_t i = wave; i < (int64_t)rounds * NW * CHW; i += NW) {
+            if (block_first + i >= per) break;
+            const int64_t d = grp * per + block_first + i;
+            if (p.cu_seqlens && s == 0) zero_uncovered<T>(b, d, 0, q.start);
+            if (p.cu_seqlens && s == p.num_seqs - 1) zero_uncovered<T>(b, d, q.start + q.len, p.seqlen);
+            if (tiles > 0) continue;
+            for (int n = lane; n < N; n += 64) {
+                arg.pA[(s * p.dim + d) * N + n] = 0.0f;
+                if (b.dinitial_states)
+                    b.dinitial_states[(s * p.dim + d) * N + n] =
+                        b.dfinal_states ? b.dfinal_states[s * b.dfinal_states_stride[0] + d * b.dfinal_states_stride[1] +
+                                                          n * b.dfinal_states_stride[2]]
+                                        : 0.0f;
             }
-            uu[j] = live[j] ? to_f32(u[t * p.u_stride[2]]) : 0.0f;
-            raw[j] = live[j] ? to_f32(delta[t * p.delta_stride[2]]) + bias : 0.0f;
-            dt[j] = live[j] ? (p.delta_softplus ? softplus(raw[j]) : raw[j]) : 0.0f;
-            zz[j] = live[j] && z ? to_f32(z[t * p.z_stride[2]]) : 0.0f;
-            dd[j] = live[j] ? to_f32(dout[t * b.dout_stride[2]]) : 0.0f;
-            dy[j] = z ? dd[j] * silu(zz[j]) : dd[j];
-            y[j] = skip * uu[j];
-            along[j] = wsum[j] = 0.0f;
-        }
-        for (int n = 0; n < N; ++n) {
-            const float A = p.A[d * p.A_stride[0] + n * p.A_stride[1]];
-            const float A2 = A * kLog2e;
-            float a[K], Bn[K], h[K], P = 1.0f, H = 0.0f;
-            bool met = false;
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                const int64_t t = q.start + tl + j;
-                a[j] = __builtin_amdgcn_exp2f(dt[j] * A2);
-                Bn[j] = live[j] ? to_f32(Bp[n * p.B_stride[2] + t * p.B_stride[3]]) : 0.0f;
-                const float bj = live[j] ? dt[j] * uu[j] * Bn[j] : 0.0f;
-                H = cut[j] ? bj : __builtin_fmaf(a[j], H, bj);
-                P *= a[j];
-                met |= cut[j];
-            }
-            const float own = P;
-            const float before = p.tile_states[((q.slot + i) * p.dim + d) * N + n];
-            if (lane == 0 && !met) H = __builtin_fmaf(P, before, H);
-            int reach = met;
-            for (int w = 1; w < 64; w *= 2) {
-                const float Hw = __shfl_up(H, w), Pw = __shfl_up(P, w);
-                const int rw = __shfl_up(reach, w);
-                if (lane >= w && !reach) {
-                    H = __builtin_fmaf(P, Hw, H);
-                    P *= Pw;
-                    reach |= rw;
-                }
-            }
-            float hp = __shfl_up(H, 1);
-            if (lane == 0) hp = before;
-            const float entered = hp;
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                const float bj = live[j] ? dt[j] * uu[j] * Bn[j] : 0.0f;
-                h[j] = hp = cut[j] ? bj : __builtin_fmaf(a[j], hp, bj);
-            }
-            // the same over the lanes from the end: Q = a g of the lane's first position
-            float c[K], Q = 0.0f;
-            P = own;
-#pragma unroll
-            for (int j = K - 1; j >= 0; --j) {
-                const int64_t t = q.start + tl + j;
-                const float Cn = live[j] ? to_f32(Cp[n * p.C_stride[2] + t * p.C_stride[3]]) : 0.0f;
-                if (live[j]) y[j] = __builtin_fmaf(Cn, h[j], y[j]);
-                c[j] = Cn * dy[j];
-                Q = cut[j] ? 0.0f : a[j] * (c[j] + Q);
-                if (tl + j < q.len) {
-                    const int64_t at = ((q.row * p.dim + d) * N + n) * p.seqlen + t;
-                    arg.pC[at] = live[j] ? dy[j] * h[j] : 0.0f;
-                }
-            }
-            const float after = carry[n];
-            if (lane == 63 && !met) Q = __builtin_fmaf(P, after, Q);
-            reach = met;
-            for (int w = 1; w < 64; w *= 2) {
-                const float Qw = __shfl_down(Q, w), Pw = __shfl_down(P, w);
-                const int rw = __shfl_down(reach, w);
-                if (lane + w < 64 && !reach) {
-                    Q = __builtin_fmaf(P, Qw, Q);
-                    P *= Pw;
-                    reach |= rw;
-                }
-            }
-            float x = __shfl_down(Q, 1);
-            if (lane == 63) x = after;
-            __syncthreads();
-            if (lane == 0) carry[n] = Q;
-            float dAn = 0.0f;
-#pragma unroll
-            for (int j = K - 1; j >= 0; --j) {
-                const float gj = c[j] + x;
-                x = cut[j] ? 0.0f : a[j] * gj;
-                const float prior = j > 0 ? h[j > 0 ? j - 1 : 0] : entered;
-                const float w = cut[j] ? 0.0f : x * prior;
-                if (live[j]) {
-                    along[j] = __builtin_fmaf(gj, Bn[j], along[j]);
-                    wsum[j] = __builtin_fmaf(A, w, wsum[j]);
-                    dAn = __builtin_fmaf(dt[j], w, dAn);
-                }
-                if (tl + j < q.len) {
-                    const int64_t at = ((q.row * p.dim + d) * N + n) * p.seqlen + q.start + tl + j;
-                    arg.pB[at] = live[j] ? gj * dt[j] * uu[j] : 0.0f;
-                }
-            }
-            dAn = wave_sum(dAn);
-            if (lane == 0) dA[n] += dAn;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            if (tl + j >= q.len) break;
-            const int64_t t = q.start + tl + j;
-            float ddt = __builtin_fmaf(uu[j], along[j], wsum[j]);
-            if (p.delta_softplus) ddt *= sigmoid(raw[j]);
-            du_out[t * b.du_stride[2]] = from_f32<T>(live[j] ? __builtin_fmaf(skip, dy[j], dt[j] * along[j]) : 0.0f);
-            dd_out[t * b.ddelta_stride[2]] = from_f32<T>(live[j] ? ddt : 0.0f);
-            if (z) dz_out[t * b.dz_stride[2]] = from_f32<T>(live[j] ? dd[j] * y[j] * silu_grad(zz[j]) : 0.0f);
-            if (live[j]) {
-                dD = __builtin_fmaf(dy[j], uu[j], dD);
-                dbias += ddt;
-            }
+            if (lane == 0) arg.pD[s * p.dim + d] = arg.pbias[s * p.dim + d] = 0.0f;
         }
     }
-    dD = wave_sum(dD);
-    dbias = wave_sum(dbias);
-    if (lane == 0) {
-        arg.pD[s * p.dim + d] = dD;
-        arg.pbias[s * p.dim + d] = dbias;
-    }
-    for (int n = lane; n < N; n += 64) {
-        arg.pA[(s * p.dim + d) * N + n] = dA[n];
-        if (b.dinitial_states) b.dinitial_states[(s * p.dim + d) * N + n] = carry[n];
+
+    for (int tile = tiles - 1; tile >= 0; --tile) {
+        const int t0 = begin + tile * TILE, t = t0 + lane * K;
+        const bool full = end - t0 >= TILE, last = tile == tiles - 1;
+        Cuts<K> cuts;
+        bool live[K];
+#pragma unroll
+        for (int j = 0; j < K; ++j) live[j] = t + j < end;
+        if constexpr (SEQ) cuts.read(ids, is, t, end - t, live);
+        else cuts.none();
+        auto input = [&](Raw<T, K>& r, const void* base, const int64_t* stride, int64_t d) {
+            const T* row = static_cast<const T*>(base) + q.row * stride[0] + d * stride[1];
+            if constexpr (UNIT) r.load(row, t, size);
+            else r.each(row, stride[2], t, end);
+        };
+        auto fix = [&](Raw<T, K>& r) {
+            if (UNIT && !full) r.fix(t, end, size);
+        };
+        // With more than 16 states a block has one round, and its channels keep
+        // their sums in registers from one lot of states to the next.
+        for (int round = 0; round < rounds; ++round) {
+            Channel<K> ch[CHW];
+            int64_t d[CHW];
+            bool mine[CHW];  // a missing channel is the group's last one with u, dout and states 0, and stores nothing
+            {
+                Raw<T, K> ru[CHW], rd[CHW], rz[CHW], ro[CHW];
+#pragma unroll
+                for (int c = 0; c < CHW; ++c) {
+                    const int64_t at = block_first + (int64_t)(round * NW + wave) * CHW + c;
+                    mine[c] = at < per;
+                    d[c] = grp * per + (mine[c] ? at : per - 1);
+                    input(ru[c], p.u, p.u_stride, d[c]);
+                    input(rd[c], p.delta, p.delta_stride, d[c]);
+                    input(ro[c], b.dout, b.dout_stride, d[c]);
+                    if (p.z) input(rz[c], p.z, p.z_stride, d[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < CHW; ++c) {
+                    const float bias = p.delta_bias ? ld_uniform(p.delta_bias + d[c] * p.delta_bias_stride) : 0.0f;
+                    fix(ru[c]);
+                    fix(rd[c]);
+                    fix(ro[c]);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < K; ++j) {
+                        const float raw = rd[c].get(j) + bias;
+                        ch[c].dt[j] = p.delta_softplus ? softplus(raw) : raw;
+                        if (SEQ || !full) ch[c].dt[j] = live[j] ? ch[c].dt[j] : 0.0f;
+                        ch[c].du[j] = mine[c] && (!SEQ || live[j]) ? ch[c].dt[j] * ru[c].get(j) : 0.0f;
+                        ch[c].dy[j] = mine[c] && (!SEQ || live[j]) ? ro[c].get(j) : 0.0f;
+                        sum += ch[c].dt[j];
+                        ch[c].y[j] = ch[c].along[j] = ch[c].wsum[j] = 0.0f;
+                    }
+                    if (p.z) {
+                        fix(rz[c]);
+#pragma unroll
+                        for (int j = 0; j < K; ++j)
+                            if (mine[c] && (!SEQ || live[j])) ch[c].dy[j] *= silu(rz[c].get(j));
+                    }
+                    ch[c].step_sum = sum;
+                }
+            }
+            for (int n0 = 0; n0 < N; n0 += kStates) {
+                const int nn = N - n0 < kStates ? N - n0 : kStates;
+                // lane i holds state n0 + i's
+                float before_l[CHW], after_l[CHW], dA_l[CHW];
+#pragma unroll
+                for (int c = 0; c < CHW; ++c) {
+                    before_l[c] = after_l[c] = dA_l[c] = 0.0f;
+                    if (lane < nn && mine[c]) {
+                        const int n = n0 + lane;
+                        before_l[c] = p.tile_states[((q.slot + tile) * p.dim + d[c]) * N + n];
+                        if (!last) after_l[c] = arg.carry[(s * p.dim + d[c]) * N + n];
+                        else if (b.dfinal_states)
+                            after_l[c] = b.dfinal_states[s * b.dfinal_states_stride[0] + d[c] * b.dfinal_states_stride[1] +
+                                                         n * b.dfinal_states_stride[2]];
+                        if (!last) dA_l[c] = arg.pA[(s * p.dim + d[c]) * N + n];
+                    }
+                }
+                if (round == 0) {
+                    StateRows<T, K, NW, TIME> rows;
+                    rows.load(p, Bp, Cp, n0, nn, t0, end, size);
+                    __syncthreads();  // the last lot is done with
+                    rows.store(BC, nn, t0, end, size, ids, is);
+                    for (int i = threadIdx.x; i < 2 * kStates * TILE / 4; i += 64 * NW)
+                        reinterpret_cast<f32x4*>(acc)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                __syncthreads();
+#pragma unroll 1
+                for (int i = 0; i < kStates; ++i) {
+                    const int n = (i + wave * (kStates / NW)) % kStates;
+                    if (n < nn) {
+                        float A[CHW], before[CHW], after[CHW], dA[CHW], B[K], C[K], dB[K], dC[K];
+#pragma unroll
+                        for (int c = 0; c < CHW; ++c) {
+                            A[c] = ld_uniform(p.A + d[c] * p.A_stride[0] + (n0 + n) * p.A_stride[1]);
+                            before[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(before_l[c]), n));
+                            after[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(after_l[c]), n));
+                        }
+                        read_state<K>(BC, n, lane, B);
+                        read_state<K>(BC + kStates * TILE, n, lane, C);
+                        if (SEQ && cuts.any) scan_state_bwd<K, CHW, true>(ch, A, before, after, dA, B, C, dB, dC, cuts, lane);
+                        else scan_state_bwd<K, CHW, false>(ch, A, before, after, dA, B, C, dB, dC, cuts, lane);
+#pragma unroll
+                        for (int c = 0; c < CHW; ++c) {
+                            const float sum = wave_sum(dA[c]);
+                            dA_l[c] = lane == n ? dA_l[c] + sum : dA_l[c];
+                            after_l[c] = lane == n ? after[c] : after_l[c];
+                        }
+                        float* aB = acc + n * TILE;
+                        float* aC = aB + kStates * TILE;
+#pragma unroll
+                        for (int k = 0; k < K / 4; ++k) {
+                            f32x4* vB = reinterpret_cast<f32x4*>(aB + (k * 64 + lane) * 4);
+                            f32x4* vC = reinterpret_cast<f32x4*>(aC + (k * 64 + lane) * 4);
+                            *vB += f32x4{dB[4 * k], dB[4 * k + 1], dB[4 * k + 2], dB[4 * k + 3]};
+                            *vC += f32x4{dC[4 * k], dC[4 * k + 1], dC[4 * k + 2], dC[4 * k + 3]};
+                        }
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int c = 0; c < CHW; ++c) {
+                    if (lane >= nn || !mine[c]) continue;
+                    const int64_t at = (s * p.dim + d[c]) * N + n0 + lane;
+                    arg.pA[at] = dA_l[c];
+                    if (tile > 0) arg.carry[at] = after_l[c];
+                    else if (b.dinitial_states) b.dinitial_states[at] = after_l[c];
+                }
+                if (round == rounds - 1) {
+                    constexpr int ROWS = 2 * kStates / NW;
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        const int row = wave * ROWS + r, n = row % kStates;
+                        if (n >= nn) continue;
+                        float v[K];
+                        read_state<K>(acc, row, lane, v);
+                        float* to = pBC + ((row / kStates) * N + n0 + n) * p.seqlen + t;
+                        if (t + K <= end) {
+#pragma unroll
+                            for (int k = 0; k < K / 4; ++k)
+                                *reinterpret_cast<AnyAddr<4>::v4*>(to + 4 * k) =
+                                    u32x4{__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
+                                          __float_as_uint(v[4 * k + 3])};
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < K; ++j)
+                                if (t + j < end) to[j] = v[j];
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < CHW; ++c) {
+                if (!mine[c]) continue;
+                Raw<T, K> ru, rd, rz, ro;
+                input(ru, p.u, p.u_stride, d[c]);
+                input(rd, p.delta, p.delta_stride, d[c]);
+                if (p.z) {
+                    input(rz, p.z, p.z_stride, d[c]);
+                    input(ro, b.dout, b.dout_stride, d[c]);
+                    fix(rz);
+                    fix(ro);
+                }
+                fix(ru);
+                fix(rd);
+                const float bias = p.delta_bias ? ld_uniform(p.delta_bias + d[c] * p.delta_bias_stride) : 0.0f;
+                const float skip = p.D ? ld_uniform(p.D + d[c] * p.D_stride) : 0.0f;
+                float du[K], dd[K], dD = 0.0f, dbias = 0.0f;
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    const float u = SEQ && !live[j] ? 0.0f : ru.get(j);
+                    du[j] = __builtin_fmaf(skip, ch[c].dy[j], ch[c].dt[j] * ch[c].along[j]);
+                    dd[j] = __builtin_fmaf(u, ch[c].along[j], ch[c].wsum[j]);
+                    if (p.delta_softplus) dd[j] *= SEQ && !live[j] ? 0.0f : sigmoid(rd.get(j) + bias);
+                    dD = __builtin_fmaf(ch[c].dy[j], u, dD);
+                    if (SEQ || !full) dd[j] = live[j] ? dd[j] : 0.0f;
+                    dbias += dd[j];
+                }
+                store_steps<T, K>(static_cast<T*>(b.du) + q.row * b.du_stride[0] + d[c] * b.du_stride[1], b.du_stride[2], t, end, du);
+                store_steps<T, K>(static_cast<T*>(b.ddelta) + q.row * b.ddelta_stride[0] + d[c] * b.ddelta_stride[1],
+                                  b.ddelta_stride[2], t, end, dd);
+                if (p.z) {
+                    float dz[K];
+#pragma unroll
+                    for (int j = 0; j < K; ++j) {
+                        const float u = SEQ && !live[j] ? 0.0f : ru.get(j);
+                        dz[j] = ro.get(j) * __builtin_fmaf(skip, u, ch[c].y[j]) * silu_grad(rz.get(j));
+                        if (SEQ && !live[j]) dz[j] = 0.0f;
+                    }
+                    store_steps<T, K>(static_cast<T*>(b.dz) + q.row * b.dz_stride[0] + d[c] * b.dz_stride[1], b.dz_stride[2], t, end, dz);
+                }
+                dD = wave_sum(dD);
+                dbias = wave_sum(dbias);
+                if (lane == 0) {
+                    const int64_t at = s * p.dim + d[c];
+                    arg.pD[at] = last ? dD : arg.pD[at] + dD;
+                    arg.pbias[at] = last ? dbias : arg.pbias[at] + dbias;
+                }
+            }
+        }
     }
 }
 
-// dB and dC: one thread per element, the channels of its group in order.
+// dB and dC: four positions per thread, the shares of the group's blocks in order.
 template <typename T> __global__ void __launch_bounds__(256) scan_bwd_reduce_bc(const ScanBwdArgs arg, int64_t items) {
     const cc1d_scan_params& p = arg.p.fwd;
+    const int64_t quads = (p.seqlen + 3) / 4;
     const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (idx >= items) return;
-    const int64_t t = idx % p.seqlen, n = idx / p.seqlen % p.dstate, g = idx / (p.seqlen * p.dstate) % p.groups,
-                  row = idx / (p.seqlen * p.dstate * p.groups), per = p.dim / p.groups;
-    float sB = 0.0f, sC = 0.0f;
-    for (int64_t d = g * per; d < (g + 1) * per; ++d) {
-        const int64_t at = ((row * p.dim + d) * p.dstate + n) * p.seqlen + t;
-        sB += arg.pB[at];
-        sC += arg.pC[at];
+    const int64_t t = idx % quads * 4, row = idx / quads, n2 = row % (2 * p.dstate), rg = row / (2 * p.dstate);
+    const int64_t lo = p.cu_seqlens ? clamp_pos(p.cu_seqlens[0], p.seqlen) : 0;
+    const int64_t hi = p.cu_seqlens ? clamp_pos(p.cu_seqlens[p.num_seqs], p.seqlen) : p.seqlen;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* from = arg.pBC + (rg * arg.group_blocks * 2 * p.dstate + n2) * p.seqlen + t;
+    const int64_t step = 2 * p.dstate * p.seqlen;
+    const int have = (int)(p.seqlen - t < 4 ? p.seqlen - t : 4);
+    if (have == 4) {
+#pragma unroll 4
+        for (int64_t k = 0; k < arg.group_blocks; ++k) {
+            const u32x4 v = *reinterpret_cast<const AnyAddr<4>::v4*>(from + k * step);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += __uint_as_float(v[j]);
+        }
+    } else {
+        for (int64_t k = 0; k < arg.group_blocks; ++k)
+            for (int j = 0; j < have; ++j) sum[j] += from[k * step + j];
     }
-    static_cast<T*>(arg.p.dB)[idx] = from_f32<T>(sB);
-    static_cast<T*>(arg.p.dC)[idx] = from_f32<T>(sC);
+    T* to = static_cast<T*>(n2 < p.dstate ? arg.p.dB : arg.p.dC) + (rg * p.dstate + n2 % p.dstate) * p.seqlen + t;
+    for (int j = 0; j < have; ++j) to[j] = from_f32<T>(t + j >= lo && t + j < hi ? sum[j] : 0.0f);
 }
 
 // dA, dD and ddelta_bias: one thread per channel and state, and two more per channel; the sequences in order.
@@ -249,29 +422,77 @@ __global__ void __launch_bounds__(256) scan_bwd_reduce_params(const ScanBwdArgs 
     to[i] = sum;
 }
 
+#ifndef BWD_CHW
+#define BWD_CHW 2
+#endif
+#ifndef BWD_NW
+#define BWD_NW (16 / BWD_CHW)
+#endif
+constexpr int kChw = BWD_CHW, kWaves = BWD_NW, kRound = kChw * kWaves;  // channels a round
+
+// Rounds of a block: a CU holds one (128 KB of LDS), so the choice that leaves
+// the card the least to do one after the other, and of equals the largest,
+// whose dB and dC have the fewest shares to add. More than 16 states: one.
+int bwd_rounds(const cc1d_scan_params& p) {
+    if (p.dstate > kStates) return 1;
+    const int64_t per = p.dim / p.groups, rows = scan_sequences(p) * p.groups;
+    int best = 1;
+    int64_t least = -1;
+    for (int r = 1; r <= 8; ++r) {
+        const int64_t cost = ceil_div(rows * ceil_div(per, kRound * r), 256) * r;
+        if (least < 0 || cost <= least) {
+            least = cost;
+            best = r;
+        }
+    }
+    return best;
+}
+
+template <typename T, int K> int launch_rows(const ScanBwdArgs& a, hipStream_t stream) {
+    const cc1d_scan_bwd_params& b = a.p;
+    const cc1d_scan_params& p = b.fwd;
+    const dim3 grid((unsigned)(a.group_blocks * p.groups * scan_sequences(p))), block(64 * kWaves);
+    const bool unit = p.seqlen >= K && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && b.dout_stride[2] == 1 &&
+                      (!p.z || p.z_stride[2] == 1);
+    const bool time = p.seqlen >= K && p.B_stride[3] == 1 && p.C_stride[3] == 1;
+    return with_flag(p.seq_idx != nullptr, [&](auto seq) {
+        return with_flag(unit, [&](auto u) {
+            return with_flag(time, [&](auto tm) {
+                return launch(scan_bwd_rows<T, K, kChw, kWaves, decltype(seq)::value, decltype(u)::value, decltype(tm)::value>,
+                              grid, block, stream, a);
+            });
+        });
+    });
+}
+
 }  // namespace
 
 int64_t scan_bwd_workspace_floats(const cc1d_scan_bwd_params& b) {
     const cc1d_scan_params& p = b.fwd;
-    return 2 * p.batch * p.dim * p.dstate * p.seqlen + scan_sequences(p) * p.dim * (p.dstate + 2);
+    const int64_t blocks = ceil_div(p.dim / p.groups, kRound * bwd_rounds(p));
+    return 2 * p.batch * p.groups * blocks * p.dstate * p.seqlen + scan_sequences(p) * p.dim * (2 * p.dstate + 2);
 }
 
 int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
     const cc1d_scan_params& p = b.fwd;
-    const int64_t seqs = scan_sequences(p);
-    ScanBwdArgs a{b, nullptr, nullptr, nullptr, nullptr, nullptr};
-    a.pB = b.workspace;
-    a.pC = a.pB + p.batch * p.dim * p.dstate * p.seqlen;
-    a.pA = a.pC + p.batch * p.dim * p.dstate * p.seqlen;
-    a.pD = a.pA + seqs * p.dim * p.dstate;
+    const int64_t seqs = scan_sequences(p), states = seqs * p.dim * p.dstate;
+    ScanBwdArgs a{};
+    a.p = b;
+    a.rounds = bwd_rounds(p);
+    a.group_blocks = ceil_div(p.dim / p.groups, kRound * a.rounds);
+    a.carry = b.workspace;
+    a.pA = a.carry + states;
+    a.pD = a.pA + states;
     a.pbias = a.pD + seqs * p.dim;
-    const int64_t nbc = p.batch * p.groups * p.dstate * p.seqlen;
+    a.pBC = a.pbias + seqs * p.dim;
+    const int64_t items = p.batch * p.groups * 2 * p.dstate * ceil_div(p.seqlen, 4);
     return with_dtype(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         int st = CC1D_OK;
-        if (seqs > 0) st = launch(scan_bwd_kernel<T>, dim3((unsigned)(seqs * p.dim)), dim3(64), stream, a);
-        if (st == CC1D_OK && nbc > 0)
-            st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)ceil_div(nbc, 256)), dim3(256), stream, a, nbc);
+        if (seqs > 0)
+            st = scan_tile(p.seqlen) == 512 ? launch_rows<T, 8>(a, stream) : launch_rows<T, 4>(a, stream);
+        if (st == CC1D_OK && items > 0)
+            st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)ceil_div(items, 256)), dim3(256), stream, a, items);
         if (st == CC1D_OK)
             st = launch(scan_bwd_reduce_params, dim3((unsigned)ceil_div(p.dim * (p.dstate + 2), 256)), dim3(256), stream,
                         a, seqs);

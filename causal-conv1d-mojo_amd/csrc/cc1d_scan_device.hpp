@@ -6,37 +6,42 @@
 // lane: each lane runs its K steps from 0, the lanes' pairs are combined over
 // the wavefront, and each lane runs its steps again from the state that
 // reaches it. The decay over a lane's steps is one exponential, exp(A sum dt).
+//
+// Time lies along the lanes, and not channels, because a (batch, channel) row
+// is then a wavefront's work of its own: 768 channels already fill the card
+// without cutting the sequence into chunks that are walked twice. Per position
+// and state the steps cost 7 issue slots (one exponential is two, measured 8
+// cycles a wavefront against 4 for a multiply-add) and the wavefront's prefix
+// 17 per K; channels along the lanes cost 6, but fill the card from 5120
+// channels x 4 rows on only, and 11 with the sequence cut into chunks.
 #pragma once
 
 #include "cc1d_internal.hpp"
 
 namespace cc1d {
 
+// Positions of a wavefront's tile, a rule on seqlen alone: 512 (8 a lane), or
+// 256 where the row has no more, which would leave half the lanes idle.
+__host__ __device__ constexpr int64_t scan_tile(int64_t seqlen) { return seqlen <= 256 ? 256 : 512; }
+
 // dt = softplus(raw) = max(raw, 0) + log1p(e), e = exp(-|raw|), with
-// log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the odd series up to s^15,
-// whose first omitted term is 9^-8 / 17 of the result. Steps are small
-// numbers (1e-3 and below), so the relative error counts, and log2(1 + e)
-// would lose it. The exponent's rounding (|raw| log2(e) may reach 20) is
-// taken back with the product's remainder.
-__device__ __forceinline__ float exp_neg(float x) {  // exp(-x), x >= 0
-    const float q = -kLog2e * x;
-    const float lo = __builtin_fmaf(-kLog2e, x, -q) - 1.9259629911e-8f * x;  // log2(e) - float(log2(e))
-    const float e = __builtin_amdgcn_exp2f(q);
-    return __builtin_fmaf(e * lo, kLn2, e);
-}
+// log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, and atanh(s) / s a polynomial
+// in s^2, fitted on [0, 1/9] at Chebyshev points (4e-9 off at most). Steps are
+// small numbers (1e-3 and below), so the relative error counts, and
+// log2(1 + e) would lose it. The exponent's rounding (|raw| log2(e) may reach
+// 20) is taken back with the product's remainder.
 __device__ __forceinline__ float softplus(float raw) {
-    const float e = exp_neg(fminf(__builtin_fabsf(raw), 80.0f));
+    const float x = fminf(__builtin_fabsf(raw), 100.0f);
+    const float q = -kLog2e * x;
+    const float near = __builtin_amdgcn_exp2f(q);
+    const float e = __builtin_fmaf(near * kLn2, __builtin_fmaf(-kLog2e, x, -q), near);
     const float s = e * __builtin_amdgcn_rcpf(2.0f + e);
-    const float q = s * s;
-    float p = __builtin_fmaf(q, 1.0f / 15.0f, 1.0f / 13.0f);
-    p = __builtin_fmaf(q, p, 1.0f / 11.0f);
-    p = __builtin_fmaf(q, p, 1.0f / 9.0f);
-    p = __builtin_fmaf(q, p, 1.0f / 7.0f);
-    p = __builtin_fmaf(q, p, 1.0f / 5.0f);
-    p = __builtin_fmaf(q, p, 1.0f / 3.0f);
-    p = __builtin_fmaf(q, p, 1.0f);
-    const float r = __builtin_fmaf(2.0f * s, p, fmaxf(raw, 0.0f));
-    return raw != raw ? raw : r;  // min and max drop a NaN
+    const float s2 = s * s;
+    float p = __builtin_fmaf(s2, 0.1408732831f, 0.1398070902f);
+    p = __builtin_fmaf(s2, p, 0.2001242638f);
+    p = __builtin_fmaf(s2, p, 0.3333315849f);
+    p = __builtin_fmaf(s2, p, 1.0f);
+    return __builtin_fmaf(s + s, p, raw < 0.0f ? 0.0f : raw);  // (a NaN is not below 0)
 }
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
@@ -58,8 +63,285 @@ __device__ __forceinline__ ScanSpan scan_span(const cc1d_scan_params& p, int64_t
 }
 
 inline int64_t scan_sequences(const cc1d_scan_params& p) { return p.cu_seqlens != nullptr ? p.num_seqs : p.batch; }
-inline int64_t scan_slots(const cc1d_scan_params& p, int64_t tile) {
+inline int64_t scan_slots(const cc1d_scan_params& p) {
+    const int64_t tile = scan_tile(p.seqlen);
     return p.cu_seqlens != nullptr ? p.seqlen / tile + p.num_seqs : p.batch * ceil_div(p.seqlen, tile);
+}
+
+// Where a lane's steps and the wavefront's prefix must not reach across a
+// sequence's start (seq_idx). All of it is the same for every state.
+template <int K> struct Cuts {
+    bool at[K];      // the state starts at 0 at the lane's step j
+    bool met;        // ... at one of them
+    bool absorb[6];  // level i of the prefix may take in the lanes it reads
+    bool back[6];    // ... of the prefix from the end, lanes in reverse
+    bool any;        // a lane of the wavefront has a cut
+
+    __device__ __forceinline__ void none() {
+        any = met = false;
+#pragma unroll
+        for (int j = 0; j < K; ++j) at[j] = false;
+    }
+    // ids of the row from its position 0; t the lane's first position, count of them in the row
+    __device__ __forceinline__ void read(const int32_t* ids, int64_t stride, int64_t t, int count, bool (&live)[K]) {
+        const int lane = threadIdx.x & 63;
+        int32_t prev = t > 0 && count > 0 ? ids[(t - 1) * stride] : 0;
+        met = false;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const int32_t id = j < count ? ids[(t + j) * stride] : prev;
+            at[j] = j < count && (id != prev || t + j == 0);
+            live[j] = j < count && id >= 0;
+            met |= at[j];
+            prev = id;
+        }
+        const uint64_t m = __ballot(met);
+        any = m != 0;
+        const uint64_t upto = m & (~0ull >> (63 - lane));
+        const int last = upto ? 63 - __builtin_clzll(upto) : -1;  // the nearest lane at or before this one with a cut
+#pragma unroll
+        for (int i = 0; i < 4; ++i) absorb[i] = last + (1 << i) <= lane;
+        absorb[4] = last < (lane & ~15);
+        absorb[5] = last < 32;
+        const uint64_t from = __builtin_bitreverse64(m) & (~0ull >> (63 - lane));
+        const int next = from ? 63 - __builtin_clzll(from) : -1;  // the same of the reversed lanes
+#pragma unroll
+        for (int i = 0; i < 4; ++i) back[i] = next + (1 << i) <= lane;
+        back[4] = next < (lane & ~15);
+        back[5] = next < 32;
+    }
+};
+
+constexpr int kDppWaveShr1 = 0x138;  // lane l takes lane l - 1's value
+constexpr int kDppRowShr = 0x110;    // + w: lane l takes lane l - w's, within 16 lanes
+
+// Inclusive prefix over the 64 lanes of the pairs (P, H): H becomes
+// H + P H' + P P' H'' ... over the lanes before. A DPP operand reads the
+// other lane's value in the multiply-add itself; lanes without a source (the
+// row's first, or rows outside row_mask) keep what they hold. VALU results
+// need two wait states before a DPP read, which asm has to provide itself.
+#define CC1D_SCAN_LEVEL(H, P, CTRL) "v_fmac_f32_dpp " H ", " H ", " P " " CTRL "\n\t"
+#define CC1D_SCAN_DECAY(P, CTRL) "v_mul_f32_dpp " P ", " P ", " P " " CTRL "\n\t"
+#define CC1D_ROW(w) "row_shr:" w " row_mask:0xf bank_mask:0xf"
+#define CC1D_B15 "row_bcast:15 row_mask:0xa bank_mask:0xf"
+#define CC1D_B31 "row_bcast:31 row_mask:0xc bank_mask:0xf"
+__device__ __forceinline__ void wave_prefix(float& H, float& P) {
+    asm("s_nop 1\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("1")) CC1D_SCAN_DECAY("%1", CC1D_ROW("1")) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("2")) CC1D_SCAN_DECAY("%1", CC1D_ROW("2")) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("4")) CC1D_SCAN_DECAY("%1", CC1D_ROW("4")) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("8")) CC1D_SCAN_DECAY("%1", CC1D_ROW("8")) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_B15) CC1D_SCAN_DECAY("%1", CC1D_B15) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_B31) "s_nop 1"
+        : "+v"(H), "+v"(P));
+}
+// Two prefixes at once: each fills the other's wait states.
+__device__ __forceinline__ void wave_prefix2(float& H0, float& P0, float& H1, float& P1) {
+#define CC1D_BOTH(CTRL) \
+    CC1D_SCAN_LEVEL("%0", "%1", CTRL) CC1D_SCAN_LEVEL("%2", "%3", CTRL) CC1D_SCAN_DECAY("%1", CTRL) CC1D_SCAN_DECAY("%3", CTRL)
+    asm("s_nop 1\n\t"
+        CC1D_BOTH(CC1D_ROW("1")) CC1D_BOTH(CC1D_ROW("2")) CC1D_BOTH(CC1D_ROW("4")) CC1D_BOTH(CC1D_ROW("8"))
+        CC1D_BOTH(CC1D_B15) CC1D_SCAN_LEVEL("%0", "%1", CC1D_B31) CC1D_SCAN_LEVEL("%2", "%3", CC1D_B31) "s_nop 1"
+        : "+v"(H0), "+v"(P0), "+v"(H1), "+v"(P1));
+#undef CC1D_BOTH
+}
+template <int CTRL, int ROW_MASK> __device__ __forceinline__ float dpp_keep(float keep, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(keep), __float_as_int(v), CTRL, ROW_MASK, 0xf, false));
+}
+// The prefix where lanes with cuts take in nothing from before them: selected,
+// not multiplied by 0, so that a non-finite state stays with its sequence.
+__device__ __forceinline__ void wave_prefix_cut(float& H, float& P, const bool (&absorb)[6]) {
+#define CC1D_CUT_LEVEL(I, CTRL, MASK)                                  \
+    {                                                                  \
+        const float h = dpp_keep<CTRL, MASK>(0.0f, H);                 \
+        const float d = dpp_keep<CTRL, MASK>(1.0f, P);                 \
+        H = absorb[I] ? __builtin_fmaf(P, h, H) : H;                 \
+        P *= d;                                                        \
+    }
+    CC1D_CUT_LEVEL(0, kDppRowShr + 1, 0xf)
+    CC1D_CUT_LEVEL(1, kDppRowShr + 2, 0xf)
+    CC1D_CUT_LEVEL(2, kDppRowShr + 4, 0xf)
+    CC1D_CUT_LEVEL(3, kDppRowShr + 8, 0xf)
+    CC1D_CUT_LEVEL(4, kDppRowBcast15, 0xa)
+    CC1D_CUT_LEVEL(5, kDppRowBcast31, 0xc)
+#undef CC1D_CUT_LEVEL
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// K consecutive positions of a row as they lie in memory.
+template <typename T, int K> struct Raw {
+    static constexpr int DW = K * (int)sizeof(T) / 4;  // dwords: 2 (four 16-bit positions), 4 or 8
+    uint32_t w[DW];
+
+    __device__ __forceinline__ void vector(const T* p) {
+        if constexpr (DW == 2) {
+            const u32x2 v = *reinterpret_cast<const typename AnyAddr<sizeof(T)>::v2*>(p);
+            w[0] = v[0];
+            w[1] = v[1];
+        } else {
+#pragma unroll
+            for (int q = 0; q < DW / 4; ++q) {
+                const u32x4 v = vload_any(p + q * elems16<T>::value);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[4 * q + i] = v[i];
+            }
+        }
+    }
+    // Positions t .. t + K - 1 of a row of `size` >= K positions with unit
+    // stride. Lanes that would read past the row read its last K positions
+    // instead, for fix() to put in place.
+    __device__ __forceinline__ void load(const T* row, int t, int size) { vector(row + (t + K <= size ? t : size - K)); }
+    // After load(): positions from `end` on are 0.
+    __device__ __forceinline__ void fix(int t, int end, int size) {
+        shift(t + K <= size ? 0 : (t < size ? t + K - size : K));
+        constexpr int PER = 4 / (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < DW; ++i) {
+            if constexpr (PER == 1) w[i] = t + i < end ? w[i] : 0u;
+            else w[i] &= t + 2 * i + 1 < end ? ~0u : (t + 2 * i < end ? 0xffffu : 0u);
+        }
+    }
+    // drops the first s positions (0 .. K), the others move up, zeros follow
+    __device__ __forceinline__ void shift(int s) {
+        constexpr int PER = 4 / (int)sizeof(T);
+        if constexpr (PER == 2) {
+            const bool odd = (s & 1) != 0;
+#pragma unroll
+            for (int i = 0; i < DW; ++i) {
+                const uint32_t up = i + 1 < DW ? w[i + 1] : 0u;
+                w[i] = odd ? (w[i] >> 16) | (up << 16) : w[i];
+            }
+        }
+        const int d = s / PER;
+#pragma unroll
+        for (int b = 1; b <= DW; b *= 2) {
+            const bool on = (d & b) != 0;
+#pragma unroll
+            for (int i = 0; i < DW; ++i) w[i] = on ? (i + b < DW ? w[i + b < DW ? i + b : 0] : 0u) : w[i];
+        }
+    }
+    // One by one, any stride; positions from `end` on are 0. Not unrolled: the
+    // vector forms are the ones to be fast, and share their registers with it.
+    __device__ __forceinline__ void each(const T* row, int64_t stride, int t, int end) {
+        constexpr int PER = 4 / (int)sizeof(T);
+#pragma unroll 1
+        for (int j = K - 1; j >= 0; --j) {
+            uint32_t v = 0u;
+            if (t + j < end) {
+                if constexpr (PER == 1) v = __builtin_bit_cast(uint32_t, row[(t + j) * stride]);
+                else v = row[(t + j) * stride].bits;
+            }
+#pragma unroll
+            for (int i = DW - 1; i >= 0; --i) {
+                const uint32_t low = i > 0 ? w[i > 0 ? i - 1 : 0] : 0u;
+                if constexpr (PER == 1) w[i] = i > 0 ? low : v;
+                else w[i] = (w[i] << 16) | (i > 0 ? low >> 16 : v);
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+        else if constexpr (__is_same(T, bf16)) return (j & 1) ? __uint_as_float(w[j / 2] & 0xffff0000u) : __uint_as_float(w[j / 2] << 16);
+        else return to_f32(f16{(uint16_t)((j & 1) ? w[j / 2] >> 16 : w[j / 2] & 0xffffu)});
+    }
+};
+template <typename T, int K>
+__device__ __forceinline__ void store_steps(T* row, int64_t stride, int t, int end, const float (&v)[K]) {
+    if (stride == 1 && t + K <= end) {
+        if constexpr (sizeof(T) == 2 && K == 4) {
+            *reinterpret_cast<typename AnyAddr<2>::v2*>(row + t) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+        } else {
+            constexpr int E = elems16<T>::value;
+#pragma unroll
+            for (int q = 0; q < K / E; ++q)
+                *reinterpret_cast<typename AnyAddr<sizeof(T)>::v4*>(row + t + q * E) = vpack<T>(v + q * E);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+        if (t + j < end) row[(t + j) * stride] = from_f32<T>(v[j]);
+}
+
+// A block's B and C of up to 16 states of a tile, fp32 in LDS as [B, C]
+// [state][K / 4][lane] of four positions: a lane reads 16 bytes, the
+// wavefront's contiguous. load() issues the reads, store() waits and writes,
+// so the next tile's values travel while the current ones are used. Positions
+// past the sequence and of an id < 0 are 0.
+//   TIME   unit time stride: a wavefront of W carries 32 / W of the 32 rows
+//   else   unit state stride (any other: one by one): a thread carries 16
+//          bytes of states of one position, positions along the lanes
+constexpr int kStates = 16;
+template <typename T, int K, int WAVES, bool TIME> struct StateRows {
+    static constexpr int E = elems16<T>::value, TILE = 64 * K, Q = K / 4, OCT = kStates / E;
+    static constexpr int ROWS = TIME ? 2 * kStates / WAVES : 2 * OCT * TILE / (64 * WAVES);
+    Raw<T, TIME ? K : E> raw[ROWS];
+
+    // B, C: the batch row's and group's position 0 (rows of `size` positions); a tile from t0 on of a sequence
+    // that ends at end
+    __device__ __forceinline__ void load(const cc1d_scan_params& p, const T* B, const T* C, int n0, int nn, int t0, int end, int size) {
+        const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
+        if constexpr (TIME) {
+            const bool isC = wave * ROWS >= kStates;
+            const int64_t ns = isC ? p.C_stride[2] : p.B_stride[2];
+            const T* row = (isC ? C : B) + (n0 + wave * ROWS % kStates) * ns;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                if (wave * ROWS % kStates + r < nn) raw[r].load(row + r * ns, t0 + lane * K, size);
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int item = r * 64 * WAVES + (int)threadIdx.x, rest = item / TILE;
+                const bool isC = rest >= OCT;
+                const int t = t0 + item % TILE, n = rest % OCT * E, have = t < end ? (nn - n < E ? nn - n : E) : 0;
+                const int64_t ns = isC ? p.C_stride[2] : p.B_stride[2], ts = isC ? p.C_stride[3] : p.B_stride[3];
+                const T* at = (isC ? C : B) + (t < end ? t : 0) * ts + n0 * ns;
+                if (ns == 1 && have == E) raw[r].vector(at + n);
+                else raw[r].each(at, ns, n, n + have);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* lds, int nn, int t0, int end, int size, const int32_t* ids, int64_t id_stride) {
+        const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
+        if constexpr (TIME) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                if (wave * ROWS % kStates + r >= nn) continue;
+                if (end - t0 < TILE) raw[r].fix(t0 + lane * K, end, size);
+                float v[K];
+#pragma unroll
+                for (int j = 0; j < K; ++j) v[j] = raw[r].get(j);
+                if (ids) {
+#pragma unroll
+                    for (int j = 0; j < K; ++j)
+                        if (t0 + lane * K + j < end && ids[(t0 + lane * K + j) * id_stride] < 0) v[j] = 0.0f;
+                }
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    *reinterpret_cast<f32x4*>(lds + (((wave * ROWS + r) * Q + q) * 64 + lane) * 4) =
+                        f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int item = r * 64 * WAVES + (int)threadIdx.x, rest = item / TILE, t = item % TILE;
+                const bool dead = ids && t0 + t < end && ids[(t0 + t) * id_stride] < 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    lds[((((rest / OCT) * kStates + rest % OCT * E + e) * Q + (t / 4) % Q) * 64 + t / K) * 4 + t % 4] =
+                        dead ? 0.0f : raw[r].get(e);
+            }
+        }
+    }
+};
+template <int K> __device__ __forceinline__ void read_state(const float* lds, int n, int lane, float (&v)[K]) {
+#pragma unroll
+    for (int q = 0; q < K / 4; ++q) {
+        const f32x4 w = *reinterpret_cast<const f32x4*>(lds + ((n * (K / 4) + q) * 64 + lane) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * q + j] = w[j];
+    }
 }
 
 }  // namespace cc1d

@@ -4,123 +4,295 @@
 namespace cc1d {
 namespace {
 
-constexpr int K = 4;          // positions per lane
-constexpr int TILE = 64 * K;  // positions per wavefront and step
+// A block: 8 wavefronts and `chans` channels (1, 2, 4, 8, or 16 with two per
+// wavefront) of one group and sequence. With fewer than 8 channels the
+// wavefronts of a channel take its states in turns and add their outputs.
+struct ScanFwdArgs {
+    cc1d_scan_params p;
+    int64_t group_blocks;  // blocks per group
+    int split;             // wavefronts per channel
+};
 
-// The positions of batch row 0 that no sequence covers: before the first and after the last.
-template <typename T> __device__ void zero_uncovered(const cc1d_scan_params& p, int64_t s, int64_t d, const ScanSpan& q) {
+// Positions of batch row 0 that no sequence covers: before the first and after the last.
+template <typename T>
+__device__ void zero_uncovered(const cc1d_scan_params& p, int64_t s, int64_t d, const ScanSpan& q) {
+    const int lane = threadIdx.x & 63;
     T* out = static_cast<T*>(p.out) + d * p.out_stride[1];
     if (s == 0)
-        for (int64_t t = threadIdx.x; t < q.start; t += 64) out[t * p.out_stride[2]] = T{};
+        for (int64_t t = lane; t < q.start; t += 64) out[t * p.out_stride[2]] = T{};
     if (s == p.num_seqs - 1)
-        for (int64_t t = q.start + q.len + threadIdx.x; t < p.seqlen; t += 64) out[t * p.out_stride[2]] = T{};
+        for (int64_t t = q.start + q.len + lane; t < p.seqlen; t += 64) out[t * p.out_stride[2]] = T{};
 }
 
-// One wavefront per (sequence, channel), every layout.
-template <typename T> __global__ void __launch_bounds__(64) scan_fwd_kernel(const cc1d_scan_params p) {
-    __shared__ float carry[CC1D_MAX_DSTATE];
-    const int lane = threadIdx.x;
-    const int64_t s = blockIdx.x / p.dim, d = blockIdx.x % p.dim;
-    const ScanSpan q = scan_span(p, s, TILE);
-    if (p.cu_seqlens != nullptr) zero_uncovered<T>(p, s, d, q);
-    const T* u = static_cast<const T*>(p.u) + q.row * p.u_stride[0] + d * p.u_stride[1];
-    const T* delta = static_cast<const T*>(p.delta) + q.row * p.delta_stride[0] + d * p.delta_stride[1];
-    const T* z = p.z ? static_cast<const T*>(p.z) + q.row * p.z_stride[0] + d * p.z_stride[1] : nullptr;
-    T* out = static_cast<T*>(p.out) + q.row * p.out_stride[0] + d * p.out_stride[1];
-    const int64_t g = d / (p.dim / p.groups);
-    const T* Bp = static_cast<const T*>(p.B) + q.row * p.B_stride[0] + g * p.B_stride[1];
-    const T* Cp = static_cast<const T*>(p.C) + q.row * p.C_stride[0] + g * p.C_stride[1];
-    const int32_t* ids = p.seq_idx ? p.seq_idx + q.row * p.seq_idx_stride[0] : nullptr;
-    const float bias = p.delta_bias ? p.delta_bias[d * p.delta_bias_stride] : 0.0f;
-    const float skip = p.D ? p.D[d * p.D_stride] : 0.0f;
-    const int N = (int)p.dstate;
-    for (int n = lane; n < N; n += 64)
-        carry[n] = p.initial_states ? p.initial_states[s * p.initial_states_stride[0] + d * p.initial_states_stride[1] +
-                                                       n * p.initial_states_stride[2]]
-                                    : 0.0f;
-    __syncthreads();
-    for (int64_t t0 = 0, slot = q.slot; t0 < q.len; t0 += TILE, ++slot) {
-        if (p.tile_states)
-            for (int n = lane; n < N; n += 64) p.tile_states[(slot * p.dim + d) * N + n] = carry[n];
-        const int64_t tl = t0 + lane * K;
-        float uu[K], dt[K], du[K], y[K];
-        bool live[K], cut[K];  // the position takes part; h starts at 0 there
+// What one channel's tile holds in registers.
+template <int K> struct Channel {
+    float dt[K], du[K], y[K], step_sum;
+};
+
+// One state of CHW channels: see cc1d_scan_device.hpp.
+template <int K, int CHW, bool CUT>
+__device__ __forceinline__ void scan_state(Channel<K> (&ch)[CHW], const float* A2, float* const* carry, int n,
+                                           const float (&B)[K], const float (&C)[K], const Cuts<K>& cuts, int lane) {
+    float a[CHW][K], H[CHW], P[CHW], first[CHW];
+#pragma unroll
+    for (int c = 0; c < CHW; ++c) {
+        const float before = carry[c][n];
+#pragma unroll
+        for (int j = 0; j < K; ++j) a[c][j] = __builtin_amdgcn_exp2f(ch[c].dt[j] * A2[c]);
+        P[c] = __builtin_amdgcn_exp2f(ch[c].step_sum * A2[c]);
+        float h = ch[c].du[0] * B[0];
+#pragma unroll
+        for (int j = 1; j < K; ++j) {
+            const float b = ch[c].du[j] * B[j];
+            h = CUT && cuts.at[j] ? b : __builtin_fmaf(a[c][j], h, b);
+        }
+        first[c] = lane == 0 ? before : 0.0f;
+        const float entered = __builtin_fmaf(P[c], first[c], h);
+        H[c] = CUT && (cuts.met || lane != 0) ? h : entered;
+    }
+    if constexpr (CUT) {
+#pragma unroll
+        for (int c = 0; c < CHW; ++c) wave_prefix_cut(H[c], P[c], cuts.absorb);
+    } else if constexpr (CHW == 2) {
+        wave_prefix2(H[0], P[0], H[1], P[1]);
+    } else {
+        wave_prefix(H[0], P[0]);
+    }
+#pragma unroll
+    for (int c = 0; c < CHW; ++c) {
+        float h = dpp_keep<kDppWaveShr1, 0xf>(first[c], H[c]);
+        if (lane == 63) carry[c][n] = H[c];
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            const int64_t t = q.start + tl + j;
-            live[j] = tl + j < q.len;
-            cut[j] = false;
-            if (live[j] && ids) {
-                const int32_t id = ids[t * p.seq_idx_stride[1]];
-                cut[j] = t == 0 || ids[(t - 1) * p.seq_idx_stride[1]] != id;
-                live[j] = id >= 0;
-            }
-            uu[j] = live[j] ? to_f32(u[t * p.u_stride[2]]) : 0.0f;
-            const float raw = live[j] ? to_f32(delta[t * p.delta_stride[2]]) + bias : 0.0f;
-            dt[j] = live[j] ? (p.delta_softplus ? softplus(raw) : raw) : 0.0f;
-            du[j] = dt[j] * uu[j];
-            y[j] = skip * uu[j];
-        }
-        for (int n = 0; n < N; ++n) {
-            const float A2 = p.A[d * p.A_stride[0] + n * p.A_stride[1]] * kLog2e;
-            float a[K], b[K], c[K], P = 1.0f, H = 0.0f;
-            bool met = false;  // the lane's span has a start
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                const int64_t t = q.start + tl + j;
-                a[j] = __builtin_amdgcn_exp2f(dt[j] * A2);
-                b[j] = live[j] ? du[j] * to_f32(Bp[n * p.B_stride[2] + t * p.B_stride[3]]) : 0.0f;
-                c[j] = live[j] ? to_f32(Cp[n * p.C_stride[2] + t * p.C_stride[3]]) : 0.0f;
-                H = cut[j] ? b[j] : __builtin_fmaf(a[j], H, b[j]);
-                P *= a[j];
-                met |= cut[j];
-            }
-            const float before = carry[n];
-            if (lane == 0 && !met) H = __builtin_fmaf(P, before, H);
-            int reach = met;
-            for (int w = 1; w < 64; w *= 2) {
-                const float Hw = __shfl_up(H, w), Pw = __shfl_up(P, w);
-                const int rw = __shfl_up(reach, w);
-                if (lane >= w && !reach) {
-                    H = __builtin_fmaf(P, Hw, H);
-                    P *= Pw;
-                    reach |= rw;
-                }
-            }
-            float h = __shfl_up(H, 1);
-            if (lane == 0) h = before;
-            __syncthreads();
-            if (lane == 63) carry[n] = H;
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                h = cut[j] ? b[j] : __builtin_fmaf(a[j], h, b[j]);
-                if (live[j]) y[j] = __builtin_fmaf(c[j], h, y[j]);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            if (tl + j >= q.len) break;
-            const int64_t t = q.start + tl + j;
-            float v = y[j];
-            if (z && live[j]) v *= silu(to_f32(z[t * p.z_stride[2]]));
-            out[t * p.out_stride[2]] = from_f32<T>(live[j] ? v : 0.0f);
+            const float b = ch[c].du[j] * B[j];
+            h = CUT && cuts.at[j] ? b : __builtin_fmaf(a[c][j], h, b);
+            ch[c].y[j] = __builtin_fmaf(C[j], h, ch[c].y[j]);
         }
     }
-    if (p.final_states)
-        for (int n = lane; n < N; n += 64)
-            p.final_states[s * p.final_states_stride[0] + d * p.final_states_stride[1] + n * p.final_states_stride[2]] =
-                carry[n];
+}
+
+// UNIT: the time strides of u, delta, z and out are 1; TIME: those of B and C (and the rows hold K positions).
+template <typename T, int K, int CHW, int NCAP, bool SEQ, bool UNIT, bool TIME>
+__global__ void __launch_bounds__(512, UNIT && TIME ? 4 : 2) scan_fwd_rows(const ScanFwdArgs arg) {
+    constexpr int TILE = 64 * K;
+    __shared__ __attribute__((aligned(16))) float BC[2 * kStates * TILE];
+    __shared__ float carries[8 * CHW * NCAP];
+    const cc1d_scan_params& p = arg.p;
+    const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
+    const int split = arg.split, part = wave % split;
+    const int64_t per = p.dim / p.groups;
+    const int64_t blk = blockIdx.x % arg.group_blocks, g = blockIdx.x / arg.group_blocks % p.groups,
+                  s = blockIdx.x / arg.group_blocks / p.groups;
+    const ScanSpan q = scan_span(p, s, TILE);
+    const int64_t in_group = (blk * (8 / split) + wave / split) * CHW;  // the wavefront's first channel
+    const int channels = (int)(per - in_group < CHW ? (per - in_group < 0 ? 0 : per - in_group) : CHW);
+    const int N = (int)p.dstate;
+    const int begin = (int)q.start, end = (int)(q.start + q.len), size = (int)p.seqlen;
+
+    // A missing channel repeats the group's last one, and stores nothing.
+    float* carry[CHW];
+    float bias[CHW], skip[CHW];
+    const T *pu[CHW], *pd[CHW], *pz[CHW];
+    T* po[CHW];
+    const float* pA[CHW];
+    float* tiles[CHW];
+    const int64_t us = UNIT ? 1 : p.u_stride[2], ds = UNIT ? 1 : p.delta_stride[2], zs = UNIT ? 1 : p.z_stride[2],
+                  os = UNIT ? 1 : p.out_stride[2];
+#pragma unroll
+    for (int c = 0; c < CHW; ++c) {
+        const int64_t d = g * per + (in_group + c < per ? in_group + c : per - 1);
+        carry[c] = carries + (wave / split * CHW + c) * NCAP;
+        bias[c] = p.delta_bias ? ld_uniform(p.delta_bias + d * p.delta_bias_stride) : 0.0f;
+        skip[c] = p.D && part == 0 ? ld_uniform(p.D + d * p.D_stride) : 0.0f;
+        pu[c] = static_cast<const T*>(p.u) + q.row * p.u_stride[0] + d * p.u_stride[1];
+        pd[c] = static_cast<const T*>(p.delta) + q.row * p.delta_stride[0] + d * p.delta_stride[1];
+        pz[c] = p.z ? static_cast<const T*>(p.z) + q.row * p.z_stride[0] + d * p.z_stride[1] : nullptr;
+        po[c] = static_cast<T*>(p.out) + q.row * p.out_stride[0] + d * p.out_stride[1];
+        pA[c] = p.A + d * p.A_stride[0];
+        tiles[c] = p.tile_states && c < channels ? p.tile_states + (q.slot * p.dim + d) * N : nullptr;
+        if (p.cu_seqlens != nullptr && c < channels && part == 0) zero_uncovered<T>(p, s, d, q);
+        const float* from = p.initial_states ? p.initial_states + s * p.initial_states_stride[0] + d * p.initial_states_stride[1] : nullptr;
+        for (int n = part * 64 + lane; n < N; n += 64 * split) carry[c][n] = from ? from[n * p.initial_states_stride[2]] : 0.0f;
+    }
+    const T* Bp = static_cast<const T*>(p.B) + q.row * p.B_stride[0] + g * p.B_stride[1];
+    const T* Cp = static_cast<const T*>(p.C) + q.row * p.C_stride[0] + g * p.C_stride[1];
+    const int32_t* ids = SEQ ? p.seq_idx + q.row * p.seq_idx_stride[0] : nullptr;
+    const int64_t is = SEQ ? p.seq_idx_stride[1] : 0;
+
+    Raw<T, K> ru[CHW], rd[CHW];
+    StateRows<T, K, 8, TIME> rows;
+    auto fetch = [&](Raw<T, K>& r, const T* row, int64_t stride, int t0) {
+        if constexpr (UNIT) r.load(row, t0 + lane * K, size);
+        else r.each(row, stride, t0 + lane * K, end);
+    };
+    auto fetch_inputs = [&](int t0) {
+#pragma unroll
+        for (int c = 0; c < CHW; ++c) {
+            fetch(ru[c], pu[c], us, t0);
+            fetch(rd[c], pd[c], ds, t0);
+        }
+    };
+    auto fetch_states = [&](int t0, int n0) { rows.load(p, Bp, Cp, n0, N - n0 < kStates ? N - n0 : kStates, t0, end, size); };
+    if (begin < end) {
+        fetch_inputs(begin);
+        fetch_states(begin, 0);
+    }
+    __syncthreads();
+
+    for (int t0 = begin; t0 < end; t0 += TILE) {
+        const int t = t0 + lane * K;
+        const bool full = end - t0 >= TILE;
+        Channel<K> ch[CHW];
+        Raw<T, K> rz[CHW];
+        Cuts<K> cuts;
+        bool live[K];
+#pragma unroll
+        for (int j = 0; j < K; ++j) live[j] = t + j < end;
+        if constexpr (SEQ) cuts.read(ids, is, t, end - t, live);
+        else cuts.none();
+#pragma unroll
+        for (int c = 0; c < CHW; ++c) {
+            if (tiles[c]) {
+                for (int n = part * 64 + lane; n < N; n += 64 * split) tiles[c][n] = carry[c][n];
+                tiles[c] += p.dim * N;
+            }
+            if (UNIT && !full) {
+                ru[c].fix(t, end, size);
+                rd[c].fix(t, end, size);
+            }
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                const float raw = rd[c].get(j) + bias[c];
+                ch[c].dt[j] = p.delta_softplus ? softplus(raw) : raw;
+            }
+            if (SEQ || !full) {
+#pragma unroll
+                for (int j = 0; j < K; ++j) ch[c].dt[j] = live[j] ? ch[c].dt[j] : 0.0f;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                const float u = SEQ && !live[j] ? 0.0f : ru[c].get(j);
+                ch[c].du[j] = ch[c].dt[j] * u;
+                ch[c].y[j] = skip[c] * u;
+                sum += ch[c].dt[j];
+            }
+            ch[c].step_sum = sum;
+        }
+        for (int n0 = 0; n0 < N; n0 += kStates) {
+            const int nn = N - n0 < kStates ? N - n0 : kStates;
+            rows.store(BC, nn, t0, end, size, ids, is);
+            __syncthreads();
+            // the next values travel while these are used
+            if (n0 + kStates < N) fetch_states(t0, n0 + kStates);
+            else if (t0 + TILE < end) fetch_states(t0 + TILE, 0);
+            if (n0 == 0) {
+                if (t0 + TILE < end) fetch_inputs(t0 + TILE);
+                if (p.z) {
+#pragma unroll
+                    for (int c = 0; c < CHW; ++c) fetch(rz[c], pz[c], zs, t0);
+                }
+            }
+#pragma unroll 1
+            for (int n = part; n < nn; n += split) {
+                float A2[CHW], B[K], C[K];
+#pragma unroll
+                for (int c = 0; c < CHW; ++c) A2[c] = ld_uniform(pA[c] + (n0 + n) * p.A_stride[1]) * kLog2e;
+                read_state<K>(BC, n, lane, B);
+                read_state<K>(BC + kStates * TILE, n, lane, C);
+                if (SEQ && cuts.any) scan_state<K, CHW, true>(ch, A2, carry, n0 + n, B, C, cuts, lane);
+                else scan_state<K, CHW, false>(ch, A2, carry, n0 + n, B, C, cuts, lane);
+            }
+            __syncthreads();
+        }
+        if (CHW == 1 && split > 1) {  // the channel's first wavefront adds the parts in order
+            float* own = BC + wave * TILE;
+#pragma unroll
+            for (int qd = 0; qd < K / 4; ++qd)
+                *reinterpret_cast<f32x4*>(own + (qd * 64 + lane) * 4) =
+                    f32x4{ch[0].y[4 * qd], ch[0].y[4 * qd + 1], ch[0].y[4 * qd + 2], ch[0].y[4 * qd + 3]};
+            __syncthreads();
+            if (part == 0) {
+                for (int w = 1; w < split; ++w) {
+#pragma unroll
+                    for (int qd = 0; qd < K / 4; ++qd) {
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(own + w * TILE + (qd * 64 + lane) * 4);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) ch[0].y[4 * qd + j] += v[j];
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (part == 0) {
+#pragma unroll
+            for (int c = 0; c < CHW; ++c) {
+                if (c >= channels) break;
+                if (p.z) {
+                    if (UNIT && !full) rz[c].fix(t, end, size);
+#pragma unroll
+                    for (int j = 0; j < K; ++j) ch[c].y[j] *= silu(rz[c].get(j));
+                }
+                if constexpr (SEQ) {
+#pragma unroll
+                    for (int j = 0; j < K; ++j)
+                        if (!live[j]) ch[c].y[j] = 0.0f;
+                }
+                store_steps<T, K>(po[c], os, t, end, ch[c].y);
+            }
+        }
+    }
+    if (p.final_states) {
+#pragma unroll
+        for (int c = 0; c < CHW; ++c) {
+            if (c >= channels) break;
+            float* to = p.final_states + s * p.final_states_stride[0] + (g * per + in_group + c) * p.final_states_stride[1];
+            for (int n = part * 64 + lane; n < N; n += 64 * split) to[n * p.final_states_stride[2]] = carry[c][n];
+        }
+    }
+}
+
+template <typename T, int K, int CHW, int NCAP> int launch_rows(const ScanFwdArgs& a, hipStream_t stream) {
+    const cc1d_scan_params& p = a.p;
+    const dim3 grid((unsigned)(a.group_blocks * p.groups * scan_sequences(p))), block(512);
+    const bool unit = p.seqlen >= K && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && p.out_stride[2] == 1 && (!p.z || p.z_stride[2] == 1);
+    const bool time = p.seqlen >= K && p.B_stride[3] == 1 && p.C_stride[3] == 1;
+    return with_flag(p.seq_idx != nullptr, [&](auto seq) {
+        return with_flag(unit, [&](auto u) {
+            return with_flag(time, [&](auto tm) {
+                return launch(scan_fwd_rows<T, K, CHW, NCAP, decltype(seq)::value, decltype(u)::value, decltype(tm)::value>,
+                              grid, block, stream, a);
+            });
+        });
+    });
 }
 
 }  // namespace
 
-int64_t scan_tile_floats(const cc1d_scan_params& p) { return scan_slots(p, TILE) * p.dim * p.dstate; }
+int64_t scan_tile_floats(const cc1d_scan_params& p) { return scan_slots(p) * p.dim * p.dstate; }
 
 int launch_scan_fwd(const cc1d_scan_params& p, hipStream_t stream) {
+    ScanFwdArgs a{p, 0, 8};
+    const int64_t channels = scan_sequences(p) * p.dim, per = p.dim / p.groups;
+    while (a.split > 1 && channels > 512 * (8 / a.split) && per > 8 / a.split && a.split > 1) a.split /= 2;
+#ifdef PROBE_TWO
+    const bool two = a.split == 1 && channels >= 8192 && per >= 16;
+#else
+    const bool two = false;
+#endif
+    a.group_blocks = ceil_div(per, (8 / a.split) * (two ? 2 : 1));
     return with_dtype(p.dtype, [&](auto t) {
-        const dim3 grid((unsigned)(scan_sequences(p) * p.dim));
-        return launch(scan_fwd_kernel<decltype(t)>, grid, dim3(64), stream, p);
+        typedef decltype(t) T;
+        return with_flag(scan_tile(p.seqlen) == 512, [&](auto wide) {
+            constexpr int K = decltype(wide)::value ? 8 : 4;
+            return with_flag(p.dstate <= 16, [&](auto few) {
+                constexpr int NCAP = decltype(few)::value ? 16 : CC1D_MAX_DSTATE;
+#ifdef PROBE_TWO
+                if (two) return launch_rows<T, K, 2, NCAP>(a, stream);
+#endif
+                return launch_rows<T, K, 1, NCAP>(a, stream);
+            });
+        });
     });
 }
 
