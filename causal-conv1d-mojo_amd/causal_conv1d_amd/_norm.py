@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 
+from causal_conv1d_amd import _host
 from causal_conv1d_amd._dtype import _DTYPE_CODE
 from causal_conv1d_amd._native import native_norm_bwd, native_norm_fwd
 
@@ -161,6 +162,11 @@ def add_norm_fn(
 
     Returns y (x's dtype), or (y, residual stream). Gradients reach x, weight, bias and residual.
     """
+    if getattr(x, "is_cuda", False) and not torch.compiler.is_compiling():
+        # an ordinary call, checked, recorded and launched in native code
+        r = _host.native().add_norm(x, weight, bias, residual, eps, rms, return_residual)
+        if r is not NotImplemented:
+            return r
     if x.dtype not in _DTYPE_CODE:
         raise NotImplementedError(f"unsupported dtype {x.dtype}; only fp16/bf16/fp32 are supported")
     if x.dim() < 1:

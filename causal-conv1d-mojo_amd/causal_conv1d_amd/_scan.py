@@ -18,7 +18,9 @@ from __future__ import annotations
 
 import torch
 
+from causal_conv1d_amd import _host
 from causal_conv1d_amd._dtype import _DTYPE_CODE
+from causal_conv1d_amd._fn import _match_layout
 from causal_conv1d_amd._native import native_scan_bwd, native_scan_fwd
 
 MAX_DSTATE = 256
@@ -176,7 +178,7 @@ class _SsmScanFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grad_outputs):
         u, delta, A, B, C, D, z, delta_bias, seq_idx, cu_seqlens, initial_states, tiles = ctx.saved_tensors
-        dout = grad_outputs[0]
+        dout = _match_layout(grad_outputs[0], u)
         dfinal = grad_outputs[1] if ctx.has_final else None
         new = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
         flat = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
@@ -256,6 +258,12 @@ def ssm_scan_fn(
     Returns out (batch, dim, seqlen) in u's dtype and layout, or (out, final_states). Gradients reach every
     float argument and flow through final_states.
     """
+    if getattr(u, "is_cuda", False) and not torch.compiler.is_compiling():
+        # an ordinary call, checked, recorded and launched in native code
+        r = _host.native().ssm_scan(u, delta, A, B, C, D, z, delta_bias, delta_softplus, seq_idx, cu_seqlens,
+                                    initial_states, return_final_states)
+        if r is not NotImplemented:
+            return r
     if u.dim() != 3:
         raise ValueError(f"expected u of shape (batch, dim, seqlen); got {tuple(u.shape)}")
     batch, dim, seqlen = u.shape

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import torch
 
+from causal_conv1d_amd import _host
 from causal_conv1d_amd._native import native_scan_update
 from causal_conv1d_amd._scan import _check_int32, _check_like, _check_parameters
 
@@ -33,6 +34,12 @@ def ssm_scan_update(
 
     Returns: out, same shape as u (0 for padding, whose state rows stay as they are).
     """
+    if getattr(u, "is_cuda", False) and not torch.compiler.is_compiling():
+        # an ordinary call, checked and launched in native code
+        out = _host.native().ssm_scan_update(u, ssm_state, delta, A, B, C, D, z, delta_bias, delta_softplus,
+                                             ssm_state_indices)
+        if out is not NotImplemented:
+            return out
     if u.dim() not in (2, 3) or ssm_state.dim() != 3:
         raise ValueError(
             f"expected u (batch, dim[, seqlen]) and ssm_state (rows, dim, dstate); "

@@ -7,7 +7,7 @@ with hipcc (in parallel), then linked into
 (bandwidth floors that ``bench.py`` times beside the kernels; measurement
 code, not part of the package) is linked on its own into
 ``libcc1d_floor.so`` beside ``bench.py`` at the repository root. The native
-host path, ``host/cc1d_host.cpp``, is compiled for the host against the
+host path, ``host/*.cpp``, is compiled for the host against the
 running interpreter's torch into ``causal_conv1d_amd/_lib/cc1d_host.so``.
 
 Usage: ``python causal-conv1d-mojo_amd/csrc/build.py [--jobs N] [--verbose]``.
@@ -35,7 +35,7 @@ LIB_PATH = LIB_DIR / "libcc1d_amd.so"
 FLOOR_SRC = CSRC / "bench" / "cc1d_floor.hip"
 FLOOR_PATH = REPO / "libcc1d_floor.so"
 # host path: a CPython extension over libtorch, no device code
-HOST_SRC = CSRC / "host" / "cc1d_host.cpp"
+HOST_SRCS = (CSRC / "host" / "cc1d_host.cpp", CSRC / "host" / "cc1d_host_ssm.cpp")
 HOST_PATH = LIB_DIR / "cc1d_host.so"
 ARCH = "gfx950"
 
@@ -102,7 +102,7 @@ def _build_host(verbose: bool) -> None:
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
         f"-I{INCLUDE}", "-isystem", str(root / "include"), "-isystem",
         str(root / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(rocm / "include"),
-        "-isystem", sysconfig.get_paths()["include"], str(HOST_SRC), "-o", str(tmp),
+        "-isystem", sysconfig.get_paths()["include"], *map(str, HOST_SRCS), "-o", str(tmp),
         f"-L{root / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python",
     ]
     if verbose:

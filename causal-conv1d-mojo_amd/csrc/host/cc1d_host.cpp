@@ -17,29 +17,11 @@
 // The interpreter lock is given up while a call allocates and launches: a
 // launch waits when the stream's queue is full, and other threads run on.
 // Nothing is kept from one call for the next.
-#include <Python.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/utils/pybind.h>
-#include <ATen/ATen.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/record_function.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPStream.h>
+#include "cc1d_host.hpp"
 
-#include <optional>
-
-#include "cc1d.h"
+using namespace cc1d_host;
 
 namespace {
-
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using torch::autograd::variable_list;
 
 // entry points of the loaded library (set once by bind())
 struct Api {
@@ -51,62 +33,14 @@ struct Api {
     decltype(&cc1d_varlen_states) varlen = nullptr;
 } api;
 
-void check(int status) {
+}  // namespace
+
+void cc1d_host::check(int status) {
     TORCH_CHECK_WITH(Error, status == CC1D_OK, "causal_conv1d_amd native call failed: ", api.strerror(status),
                      " (status ", status, ")");
 }
 
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-// No dispatch or torch-function mode, transform or tracer in force on this
-// thread: what the dispatcher would send straight to the backend.
-bool plain_thread() {
-    if (c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled()) return false;
-    const auto tls = c10::impl::tls_local_dispatch_key_set();
-    return (tls.included_ - c10::default_included_set - c10::autocast_dispatch_keyset).empty();
-}
-
-// A strided GPU tensor without a subclass, lazy bit, wrapper or tangent.
-bool plain(const Tensor& t) {
-    static const auto allowed = c10::DispatchKeySet(c10::DispatchKey::CUDA) |
-                                c10::DispatchKeySet(c10::DispatchKey::AutogradCUDA) |
-                                c10::DispatchKeySet(c10::DispatchKey::ADInplaceOrView) |
-                                c10::DispatchKeySet(c10::DispatchKey::AutocastCUDA);
-    return t.defined() && t.is_cuda() && t.layout() == at::kStrided &&
-           (t.key_set().raw_repr() & ~allowed.raw_repr()) == 0 && !t._fw_grad(0).defined();
-}
-
-bool plain(PyObject* o) { return THPVariable_CheckExact(o) && plain(THPVariable_Unpack(o)); }
-bool plain_or_none(PyObject* o) { return o == Py_None || plain(o); }
-Tensor tensor_or_none(PyObject* o) { return o == Py_None ? Tensor() : THPVariable_Unpack(o); }
-
-int dtype_code(const Tensor& t) {
-    switch (t.scalar_type()) {
-    case at::kHalf: return CC1D_DTYPE_FP16;
-    case at::kBFloat16: return CC1D_DTYPE_BF16;
-    case at::kFloat: return CC1D_DTYPE_FP32;
-    default: return -1;
-    }
-}
-
-// 0: no activation, 1: SiLU, -1: not one of the accepted values
-int activation_code(PyObject* o) {
-    if (o == Py_None) return 0;
-    if (!PyUnicode_CheckExact(o)) return -1;
-    return PyUnicode_CompareWithASCIIString(o, "silu") == 0 || PyUnicode_CompareWithASCIIString(o, "swish") == 0 ? 1 : -1;
-}
-
-bool same(const Tensor& t, const Tensor& like) {
-    return t.scalar_type() == like.scalar_type() && t.device() == like.device();
-}
-bool shaped(const Tensor& t, at::IntArrayRef s) { return t.sizes() == s; }
-
-const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
-
-template <int N> void strides(int64_t (&dst)[N], const Tensor& t) {
-    for (int i = 0; i < N; ++i) dst[i] = t.defined() ? t.stride(i) : 0;
-}
+namespace {
 
 // ---- forward / backward ------------------------------------------------
 
@@ -179,13 +113,6 @@ void launch_bwd(const Tensor& x, const Tensor& weight, const Tensor& bias, const
     check(api.bwd(&p, &g, stream_of(x)));
 }
 
-// dout in x's layout: a copy only where the time strides differ (or any, in a layout without unit time stride)
-Tensor match_layout(const Tensor& t, const Tensor& like) {
-    if (t.strides() == like.strides()) return t;
-    if (like.stride(-1) == 1) return t.stride(-1) == 1 ? t : t.contiguous();
-    return at::empty_like(like).copy_(t);
-}
-
 struct Conv1dFn : public torch::autograd::Function<Conv1dFn> {
     // backward() depends on its arguments and on what ctx saved alone
     static constexpr bool is_traceable = true;
@@ -231,8 +158,6 @@ struct Conv1dFn : public torch::autograd::Function<Conv1dFn> {
         return {dx, dweight, dbias, Tensor(), dinit, Tensor(), Tensor()};
     }
 };
-
-PyObject* not_implemented() { Py_RETURN_NOTIMPLEMENTED; }
 
 // fn(x, weight, bias, seq_idx, initial_states, return_final_states, final_states_out, activation)
 PyObject* py_fn(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -391,7 +316,6 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-#define CC1D_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
 PyMethodDef methods[] = {
     {"bind", CC1D_FAST(py_bind), "the library's entry points"},
     {"fn", CC1D_FAST(py_fn), "causal_conv1d_fn's ordinary case, or NotImplemented"},
@@ -404,4 +328,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "cc1d_host", "native host path of c
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_cc1d_host(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_cc1d_host(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m != nullptr && PyModule_AddFunctions(m, ssm_methods) != 0) Py_CLEAR(m);
+    return m;
+}

@@ -308,3 +308,18 @@ def test_tile_states_size_is_the_librarys(L, N):
         cu = torch.empty(seqs + 1, dtype=torch.int32) if seqs else None
         p = _scan(batch=batch, seqlen=L, dstate=N, num_seqs=seqs, cu_seqlens=16 if seqs else None)
         assert scan_tile_floats(u, A, cu) == lib.cc1d_scan_tile_floats(ctypes.byref(p))
+
+
+def test_native_host_path_leaves_cpu_tensors_and_odd_arguments_to_python():
+    from causal_conv1d_amd import _host
+
+    ext = _host.load()
+    p = _bf16()
+    args = [p[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias")]
+    assert ext.ssm_scan(*args, True, None, None, None, False) is NotImplemented
+    assert ext.ssm_scan(None, *args[1:], 1, None, None, None, "x") is NotImplemented
+    assert ext.ssm_scan_update(args[0], torch.zeros(2, 4, 3), *args[1:], True, None) is NotImplemented
+    assert ext.add_norm(torch.zeros(2, 8), torch.ones(8), None, None, 1e-5, False, False) is NotImplemented
+    for f, n in ((ext.ssm_scan, 13), (ext.ssm_scan_update, 11), (ext.add_norm, 7), (ext.bind_ssm, 8)):
+        with pytest.raises(RuntimeError, match=f"takes {n}"):
+            f(None)
