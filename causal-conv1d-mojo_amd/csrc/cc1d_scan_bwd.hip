@@ -34,94 +34,77 @@ template <int K> struct Channel {
     float step_sum;
 };
 
-// One state of CHW channels. before / after: h ahead of the tile and a g behind
+// One state of a channel. before / after: h ahead of the tile and a g behind
 // it; on return after is a g of the tile's first position. dB, dC: the
-// channels' terms. dA: the lane's share of the state's dA.
-template <int K, int CHW, bool CUT>
-__device__ __forceinline__ void scan_state_bwd(Channel<K> (&ch)[CHW], const float (&A)[CHW], const float (&before)[CHW],
-                                               float (&after)[CHW], float (&dA)[CHW], const float (&B)[K], const float (&C)[K],
-                                               float (&dB)[K], float (&dC)[K], const Cuts<K>& cuts, int lane) {
-    float a[CHW][K], h[CHW][K], H[CHW], P[CHW], Pr[CHW], Q[CHW], first[CHW];
+// channel's terms are added. Returns the lane's share of the state's dA.
+template <int K, bool CUT>
+__device__ __forceinline__ float scan_state_bwd(Channel<K>& ch, float A, float before, float& after, const float (&B)[K],
+                                                const float (&C)[K], float (&dB)[K], float (&dC)[K], const Cuts<K>& cuts,
+                                                bool met_back, int lane) {
+    float a[K], h[K];
+    const float A2 = A * kLog2e;
 #pragma unroll
-    for (int c = 0; c < CHW; ++c) {
-        const float A2 = A[c] * kLog2e;
+    for (int j = 0; j < K; ++j) a[j] = __builtin_amdgcn_exp2f(ch.dt[j] * A2);
+    float P = __builtin_amdgcn_exp2f(ch.step_sum * A2);
+    float Pr = lane_get(P, 63 - lane);  // the lanes in reverse, for the prefix from the end
+    float H = ch.du[0] * B[0];
 #pragma unroll
-        for (int j = 0; j < K; ++j) a[c][j] = __builtin_amdgcn_exp2f(ch[c].dt[j] * A2);
-        P[c] = __builtin_amdgcn_exp2f(ch[c].step_sum * A2);
-        // the lanes in reverse, for the prefix from the end
-        Pr[c] = lane_get(P[c], 63 - lane);
-        float v = ch[c].du[0] * B[0];
-#pragma unroll
-        for (int j = 1; j < K; ++j) {
-            const float b = ch[c].du[j] * B[j];
-            v = CUT && cuts.at[j] ? b : __builtin_fmaf(a[c][j], v, b);
-        }
-        first[c] = lane == 0 ? before[c] : 0.0f;
-        const float entered = __builtin_fmaf(P[c], first[c], v);
-        H[c] = CUT && (cuts.met || lane != 0) ? v : entered;
-        // Q = a g of the lane's first position
-        float x = 0.0f;
-#pragma unroll
-        for (int j = K - 1; j >= 0; --j) {
-            x = a[c][j] * __builtin_fmaf(C[j], ch[c].dy[j], x);
-            if (CUT && cuts.at[j]) x = 0.0f;
-        }
-        Q[c] = lane_get(x, 63 - lane);
+    for (int j = 1; j < K; ++j) {
+        const float b = ch.du[j] * B[j];
+        H = CUT && cuts.at[j] ? b : __builtin_fmaf(a[j], H, b);
     }
-    const bool met_back = CUT && __shfl((int)cuts.met, 63 - lane) != 0;
-    float behind[CHW];
+    // Q = a g of the lane's first position
+    float x = 0.0f;
 #pragma unroll
-    for (int c = 0; c < CHW; ++c) {
-        behind[c] = lane == 0 ? after[c] : 0.0f;
-        const float entered = __builtin_fmaf(Pr[c], behind[c], Q[c]);
-        Q[c] = CUT && (met_back || lane != 0) ? Q[c] : entered;
+    for (int j = K - 1; j >= 0; --j) {
+        x = a[j] * __builtin_fmaf(C[j], ch.dy[j], x);
+        if (CUT && cuts.at[j]) x = 0.0f;
     }
+    float Q = lane_get(x, 63 - lane);
+    const float first = lane == 0 ? before : 0.0f, behind = lane == 0 ? after : 0.0f;
+    const float Hin = __builtin_fmaf(P, first, H), Qin = __builtin_fmaf(Pr, behind, Q);
+    H = CUT && (cuts.met || lane != 0) ? H : Hin;
+    Q = CUT && (met_back || lane != 0) ? Q : Qin;
     if constexpr (CUT) {
-#pragma unroll
-        for (int c = 0; c < CHW; ++c) {
-            wave_prefix_cut(H[c], P[c], cuts.absorb);
-            wave_prefix_cut(Q[c], Pr[c], cuts.back);
-        }
+        wave_prefix_cut(H, P, cuts.absorb);
+        wave_prefix_cut(Q, Pr, cuts.back);
     } else {
-#pragma unroll
-        for (int c = 0; c < CHW; ++c) wave_prefix2(H[c], P[c], Q[c], Pr[c]);
+        wave_prefix2(H, P, Q, Pr);
     }
+    const float ahead = dpp_keep<kDppWaveShr1, 0xf>(first, H);  // h before the lane's first position
+    x = dpp_keep<kDppWaveShr1, 0xf>(behind, Q);                 // a g after its last one, lanes in reverse
+    after = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q), 63));
+    x = lane_get(x, 63 - lane);
+    float v = ahead;
 #pragma unroll
-    for (int c = 0; c < CHW; ++c) {
-        const float ahead = dpp_keep<kDppWaveShr1, 0xf>(first[c], H[c]);  // h before the lane's first position
-        float x = dpp_keep<kDppWaveShr1, 0xf>(behind[c], Q[c]);           // a g after its last one, lanes in reverse
-        after[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q[c]), 63));
-        x = lane_get(x, 63 - lane);
-        float v = ahead;
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const float b = ch[c].du[j] * B[j];
-            v = CUT && cuts.at[j] ? b : __builtin_fmaf(a[c][j], v, b);
-            h[c][j] = v;
-            ch[c].y[j] = __builtin_fmaf(C[j], v, ch[c].y[j]);
-            dC[j] = c == 0 ? ch[c].dy[j] * v : __builtin_fmaf(ch[c].dy[j], v, dC[j]);
-        }
-        float dAc = 0.0f;
-#pragma unroll
-        for (int j = K - 1; j >= 0; --j) {
-            const float g = __builtin_fmaf(C[j], ch[c].dy[j], x);
-            dB[j] = c == 0 ? g * ch[c].du[j] : __builtin_fmaf(g, ch[c].du[j], dB[j]);
-            ch[c].along[j] = __builtin_fmaf(g, B[j], ch[c].along[j]);
-            x = a[c][j] * g;
-            float w = x * (j > 0 ? h[c][j > 0 ? j - 1 : 0] : ahead);
-            if (CUT && cuts.at[j]) x = w = 0.0f;
-            ch[c].wsum[j] = __builtin_fmaf(A[c], w, ch[c].wsum[j]);
-            dAc = __builtin_fmaf(ch[c].dt[j], w, dAc);
-        }
-        dA[c] = dAc;
+    for (int j = 0; j < K; ++j) {
+        const float b = ch.du[j] * B[j];
+        v = CUT && cuts.at[j] ? b : __builtin_fmaf(a[j], v, b);
+        h[j] = v;
+        ch.y[j] = __builtin_fmaf(C[j], v, ch.y[j]);
+        dC[j] = __builtin_fmaf(ch.dy[j], v, dC[j]);
     }
+    float dA = 0.0f;
+#pragma unroll
+    for (int j = K - 1; j >= 0; --j) {
+        const float g = __builtin_fmaf(C[j], ch.dy[j], x);
+        dB[j] = __builtin_fmaf(g, ch.du[j], dB[j]);
+        ch.along[j] = __builtin_fmaf(g, B[j], ch.along[j]);
+        x = a[j] * g;
+        float w = x * (j > 0 ? h[j > 0 ? j - 1 : 0] : ahead);
+        if (CUT && cuts.at[j]) x = w = 0.0f;
+        ch.wsum[j] = __builtin_fmaf(A, w, ch.wsum[j]);
+        dA = __builtin_fmaf(ch.dt[j], w, dA);
+    }
+    return dA;
 }
 
 // A block: NW wavefronts of CHW channels each, `rounds` times, of one group and
 // sequence; tiles from the last to the first. In a tile, each round's channels
-// run through 16 states at a time, each wavefront at another one (state i + its
-// own offset in step i), so that the block's sums for dB and dC of a state, in
-// LDS, belong to one wavefront at a time and grow in a fixed order.
+// run through 16 states at a time, each wavefront at others (in step i the
+// 16 / NW from (i + its number) mod NW on), so that the block's sums for dB and
+// dC of a state, in LDS, belong to one wavefront at a time and grow in a fixed
+// order.
 template <typename T, int K, int CHW, int NW, bool SEQ, bool UNIT, bool TIME>
 __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdArgs arg) {
     constexpr int TILE = 64 * K;
@@ -174,6 +157,7 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
         for (int j = 0; j < K; ++j) live[j] = t + j < end;
         if constexpr (SEQ) cuts.read(ids, is, t, end - t, live);
         else cuts.none();
+        const bool met_back = SEQ && __shfl((int)cuts.met, 63 - lane) != 0;
         auto input = [&](Raw<T, K>& r, const void* base, const int64_t* stride, int64_t d) {
             const T* row = static_cast<const T*>(base) + q.row * stride[0] + d * stride[1];
             if constexpr (UNIT) r.load(row, t, size);
@@ -207,10 +191,9 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                     fix(rd[c]);
                     fix(ro[c]);
                     float sum = 0.0f;
+                    steps<K>(rd[c], bias, p.delta_softplus != 0, ch[c].dt);
 #pragma unroll
                     for (int j = 0; j < K; ++j) {
-                        const float raw = rd[c].get(j) + bias;
-                        ch[c].dt[j] = p.delta_softplus ? softplus(raw) : raw;
                         if (SEQ || !full) ch[c].dt[j] = live[j] ? ch[c].dt[j] : 0.0f;
                         ch[c].du[j] = mine[c] && (!SEQ || live[j]) ? ch[c].dt[j] * ru[c].get(j) : 0.0f;
                         ch[c].dy[j] = mine[c] && (!SEQ || live[j]) ? ro[c].get(j) : 0.0f;
@@ -253,34 +236,36 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                 }
                 __syncthreads();
 #pragma unroll 1
-                for (int i = 0; i < kStates; ++i) {
-                    const int n = (i + wave * (kStates / NW)) % kStates;
-                    if (n < nn) {
-                        float A[CHW], before[CHW], after[CHW], dA[CHW], B[K], C[K], dB[K], dC[K];
-#pragma unroll
-                        for (int c = 0; c < CHW; ++c) {
-                            A[c] = ld_uniform(p.A + d[c] * p.A_stride[0] + (n0 + n) * p.A_stride[1]);
-                            before[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(before_l[c]), n));
-                            after[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(after_l[c]), n));
-                        }
+                for (int i = 0; i < NW; ++i) {
+#pragma unroll 1
+                    for (int k = 0; k < kStates / NW; ++k) {
+                        const int n = (i + wave) % NW * (kStates / NW) + k;
+                        if (n >= nn) break;
+                        float B[K], C[K], dB[K], dC[K];
                         read_state<K>(BC, n, lane, B);
                         read_state<K>(BC + kStates * TILE, n, lane, C);
-                        if (SEQ && cuts.any) scan_state_bwd<K, CHW, true>(ch, A, before, after, dA, B, C, dB, dC, cuts, lane);
-                        else scan_state_bwd<K, CHW, false>(ch, A, before, after, dA, B, C, dB, dC, cuts, lane);
+                        read_state<K>(acc, n, lane, dB);
+                        read_state<K>(acc + kStates * TILE, n, lane, dC);
 #pragma unroll
                         for (int c = 0; c < CHW; ++c) {
-                            const float sum = wave_sum(dA[c]);
+                            const float A = ld_uniform(p.A + d[c] * p.A_stride[0] + (n0 + n) * p.A_stride[1]);
+                            const float before = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(before_l[c]), n));
+                            float after = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(after_l[c]), n));
+                            const float dA = SEQ && cuts.any
+                                ? scan_state_bwd<K, true>(ch[c], A, before, after, B, C, dB, dC, cuts, met_back, lane)
+                                : scan_state_bwd<K, false>(ch[c], A, before, after, B, C, dB, dC, cuts, met_back, lane);
+                            const float sum = wave_sum(dA);
                             dA_l[c] = lane == n ? dA_l[c] + sum : dA_l[c];
-                            after_l[c] = lane == n ? after[c] : after_l[c];
+                            after_l[c] = lane == n ? after : after_l[c];
+                            // one channel after the other: both at once would need more registers than there are
+                            __builtin_amdgcn_sched_barrier(0);
                         }
-                        float* aB = acc + n * TILE;
-                        float* aC = aB + kStates * TILE;
 #pragma unroll
-                        for (int k = 0; k < K / 4; ++k) {
-                            f32x4* vB = reinterpret_cast<f32x4*>(aB + (k * 64 + lane) * 4);
-                            f32x4* vC = reinterpret_cast<f32x4*>(aC + (k * 64 + lane) * 4);
-                            *vB += f32x4{dB[4 * k], dB[4 * k + 1], dB[4 * k + 2], dB[4 * k + 3]};
-                            *vC += f32x4{dC[4 * k], dC[4 * k + 1], dC[4 * k + 2], dC[4 * k + 3]};
+                        for (int q = 0; q < K / 4; ++q) {
+                            *reinterpret_cast<f32x4*>(acc + ((n * (K / 4) + q) * 64 + lane) * 4) =
+                                f32x4{dB[4 * q], dB[4 * q + 1], dB[4 * q + 2], dB[4 * q + 3]};
+                            *reinterpret_cast<f32x4*>(acc + kStates * TILE + ((n * (K / 4) + q) * 64 + lane) * 4) =
+                                f32x4{dC[4 * q], dC[4 * q + 1], dC[4 * q + 2], dC[4 * q + 3]};
                         }
                     }
                     __syncthreads();
@@ -343,9 +328,9 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                     if (SEQ || !full) dd[j] = live[j] ? dd[j] : 0.0f;
                     dbias += dd[j];
                 }
-                store_steps<T, K>(static_cast<T*>(b.du) + q.row * b.du_stride[0] + d[c] * b.du_stride[1], b.du_stride[2], t, end, du);
+                store_steps<T, K>(static_cast<T*>(b.du) + q.row * b.du_stride[0] + d[c] * b.du_stride[1], UNIT ? 1 : b.du_stride[2], t, end, du);
                 store_steps<T, K>(static_cast<T*>(b.ddelta) + q.row * b.ddelta_stride[0] + d[c] * b.ddelta_stride[1],
-                                  b.ddelta_stride[2], t, end, dd);
+                                  UNIT ? 1 : b.ddelta_stride[2], t, end, dd);
                 if (p.z) {
                     float dz[K];
 #pragma unroll
@@ -354,7 +339,7 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                         dz[j] = ro.get(j) * __builtin_fmaf(skip, u, ch[c].y[j]) * silu_grad(rz.get(j));
                         if (SEQ && !live[j]) dz[j] = 0.0f;
                     }
-                    store_steps<T, K>(static_cast<T*>(b.dz) + q.row * b.dz_stride[0] + d[c] * b.dz_stride[1], b.dz_stride[2], t, end, dz);
+                    store_steps<T, K>(static_cast<T*>(b.dz) + q.row * b.dz_stride[0] + d[c] * b.dz_stride[1], UNIT ? 1 : b.dz_stride[2], t, end, dz);
                 }
                 dD = wave_sum(dD);
                 dbias = wave_sum(dbias);
@@ -453,7 +438,7 @@ template <typename T, int K> int launch_rows(const ScanBwdArgs& a, hipStream_t s
     const cc1d_scan_params& p = b.fwd;
     const dim3 grid((unsigned)(a.group_blocks * p.groups * scan_sequences(p))), block(64 * kWaves);
     const bool unit = p.seqlen >= K && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && b.dout_stride[2] == 1 &&
-                      (!p.z || p.z_stride[2] == 1);
+                      b.du_stride[2] == 1 && b.ddelta_stride[2] == 1 && (!p.z || (p.z_stride[2] == 1 && b.dz_stride[2] == 1));
     const bool time = p.seqlen >= K && p.B_stride[3] == 1 && p.C_stride[3] == 1;
     return with_flag(p.seq_idx != nullptr, [&](auto seq) {
         return with_flag(unit, [&](auto u) {

@@ -69,6 +69,16 @@ inline int64_t scan_slots(const cc1d_scan_params& p) {
     return p.cu_seqlens != nullptr ? p.seqlen / tile + p.num_seqs : p.batch * ceil_div(p.seqlen, tile);
 }
 
+// dt of a lane's positions
+template <int K, typename R> __device__ __forceinline__ void steps(const R& raw, float bias, bool soft, float (&dt)[K]) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) dt[j] = raw.get(j) + bias;
+    if (soft) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) dt[j] = softplus(dt[j]);
+    }
+}
+
 // Where a lane's steps and the wavefront's prefix must not reach across a
 // sequence's start (seq_idx). All of it is the same for every state.
 template <int K> struct Cuts {

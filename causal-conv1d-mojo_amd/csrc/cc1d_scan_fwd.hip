@@ -160,11 +160,7 @@ __global__ void __launch_bounds__(512, UNIT && TIME ? 4 : 2) scan_fwd_rows(const
                 ru[c].fix(t, end, size);
                 rd[c].fix(t, end, size);
             }
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                const float raw = rd[c].get(j) + bias[c];
-                ch[c].dt[j] = p.delta_softplus ? softplus(raw) : raw;
-            }
+            steps<K>(rd[c], bias[c], p.delta_softplus != 0, ch[c].dt);
             if (SEQ || !full) {
 #pragma unroll
                 for (int j = 0; j < K; ++j) ch[c].dt[j] = live[j] ? ch[c].dt[j] : 0.0f;
