@@ -105,7 +105,7 @@ __device__ __forceinline__ float scan_state_bwd(Channel<K>& ch, float A, float b
 // 16 / NW from (i + its number) mod NW on), so that the block's sums for dB and
 // dC of a state, in LDS, belong to one wavefront at a time and grow in a fixed
 // order.
-template <typename T, int K, int CHW, int NW, bool SEQ, bool UNIT, bool TIME>
+template <typename T, int K, int CHW, int NW, bool SEQ, bool UNIT, StateMode MODE>
 __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdArgs arg) {
     constexpr int TILE = 64 * K;
     __shared__ __attribute__((aligned(16))) float BC[2 * kStates * TILE];
@@ -114,8 +114,9 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
     const cc1d_scan_params& p = b.fwd;
     const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
     const int64_t per = p.dim / p.groups;
-    const int64_t blk = blockIdx.x % arg.group_blocks, grp = blockIdx.x / arg.group_blocks % p.groups,
-                  s = blockIdx.x / arg.group_blocks / p.groups;
+    const uint32_t order = xcd_block(blockIdx.x, gridDim.x);
+    const int64_t blk = order % arg.group_blocks, grp = order / arg.group_blocks % p.groups,
+                  s = order / arg.group_blocks / p.groups;
     const ScanSpan q = scan_span(p, s, TILE);
     const int N = (int)p.dstate;
     const int begin = (int)q.start, end = (int)(q.start + q.len), size = (int)p.seqlen;
@@ -227,10 +228,10 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                     }
                 }
                 if (round == 0) {
-                    StateRows<T, K, NW, TIME> rows;
+                    StateRows<T, K, NW, MODE> rows;
                     rows.load(p, Bp, Cp, n0, nn, t0, end, size);
                     __syncthreads();  // the last lot is done with
-                    rows.store(BC, nn, t0, end, size, ids, is);
+                    rows.store(BC, n0, nn, N, t0, end, size, ids, is);
                     for (int i = threadIdx.x; i < 2 * kStates * TILE / 4; i += 64 * NW)
                         reinterpret_cast<f32x4*>(acc)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
@@ -439,14 +440,13 @@ template <typename T, int K> int launch_rows(const ScanBwdArgs& a, hipStream_t s
     const dim3 grid((unsigned)(a.group_blocks * p.groups * scan_sequences(p))), block(64 * kWaves);
     const bool unit = p.seqlen >= K && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && b.dout_stride[2] == 1 &&
                       b.du_stride[2] == 1 && b.ddelta_stride[2] == 1 && (!p.z || (p.z_stride[2] == 1 && b.dz_stride[2] == 1));
-    const bool time = p.seqlen >= K && p.B_stride[3] == 1 && p.C_stride[3] == 1;
+    const StateMode mode = state_mode<T, K>(p);
     return with_flag(p.seq_idx != nullptr, [&](auto seq) {
-        return with_flag(unit, [&](auto u) {
-            return with_flag(time, [&](auto tm) {
-                return launch(scan_bwd_rows<T, K, kChw, kWaves, decltype(seq)::value, decltype(u)::value, decltype(tm)::value>,
-                              grid, block, stream, a);
-            });
-        });
+        constexpr bool SEQ = decltype(seq)::value;
+        if (!unit || mode == kStateAny)
+            return launch(scan_bwd_rows<T, K, kChw, kWaves, SEQ, false, kStateAny>, grid, block, stream, a);
+        if (mode == kStateTime) return launch(scan_bwd_rows<T, K, kChw, kWaves, SEQ, true, kStateTime>, grid, block, stream, a);
+        return launch(scan_bwd_rows<T, K, kChw, kWaves, SEQ, true, kStateLast>, grid, block, stream, a);
     });
 }
 

@@ -183,20 +183,27 @@ __device__ __forceinline__ void wave_prefix_cut(float& H, float& P, const bool (
 // wavefront's contiguous. load() issues the reads, store() waits and writes,
 // so the next tile's values travel while the current ones are used. Positions
 // past the sequence and of an id < 0 are 0.
-//   TIME   unit time stride: a wavefront of W carries 32 / W of the 32 rows
-//   else   unit state stride (any other: one by one): a thread carries 16
-//          bytes of states of one position, positions along the lanes
+//   kStateTime   unit time stride: a wavefront of W carries 32 / W of the 32 rows
+//   kStateLast   unit state stride (and at least 16 bytes of states): a thread
+//                carries 16 bytes of states of one position, positions along
+//                the lanes
+//   kStateAny    the same, one by one, any strides
+enum StateMode { kStateTime = 0, kStateLast = 1, kStateAny = 2 };
 constexpr int kStates = 16;
-template <typename T, int K, int WAVES, bool TIME> struct StateRows {
+template <typename T, int K, int WAVES, StateMode MODE> struct StateRows {
     static constexpr int E = elems16<T>::value, TILE = 64 * K, Q = K / 4, OCT = kStates / E;
-    static constexpr int ROWS = TIME ? 2 * kStates / WAVES : 2 * OCT * TILE / (64 * WAVES);
-    Raw<T, TIME ? K : E> raw[ROWS];
+    static constexpr int ROWS = MODE == kStateTime ? 2 * kStates / WAVES : 2 * OCT * K / WAVES;
+    Raw<T, MODE == kStateTime ? K : E> raw[ROWS];
+
+    // kStateLast, kStateAny: which 16 bytes turn r is about (uniform), and the position in the tile
+    static __device__ __forceinline__ int unit(int r, int wave) { return (r * WAVES + wave) / K; }
+    static __device__ __forceinline__ int pos(int r, int wave, int lane) { return (r * WAVES + wave) % K * 64 + lane; }
 
     // B, C: the batch row's and group's position 0 (rows of `size` positions); a tile from t0 on of a sequence
     // that ends at end
     __device__ __forceinline__ void load(const cc1d_scan_params& p, const T* B, const T* C, int n0, int nn, int t0, int end, int size) {
         const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
-        if constexpr (TIME) {
+        if constexpr (MODE == kStateTime) {
             const bool isC = wave * ROWS >= kStates;
             const int64_t ns = isC ? p.C_stride[2] : p.B_stride[2];
             const T* row = (isC ? C : B) + (n0 + wave * ROWS % kStates) * ns;
@@ -206,19 +213,20 @@ template <typename T, int K, int WAVES, bool TIME> struct StateRows {
         } else {
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
-                const int item = r * 64 * WAVES + (int)threadIdx.x, rest = item / TILE;
-                const bool isC = rest >= OCT;
-                const int t = t0 + item % TILE, n = rest % OCT * E, have = t < end ? (nn - n < E ? nn - n : E) : 0;
+                const bool isC = unit(r, wave) >= OCT;
+                const int n = unit(r, wave) % OCT * E, t = t0 + pos(r, wave, lane);
+                if (n >= nn) continue;
                 const int64_t ns = isC ? p.C_stride[2] : p.B_stride[2], ts = isC ? p.C_stride[3] : p.B_stride[3];
-                const T* at = (isC ? C : B) + (t < end ? t : 0) * ts + n0 * ns;
-                if (ns == 1 && have == E) raw[r].vector(at + n);
-                else raw[r].each(at, ns, n, n + have);
+                const T* at = (isC ? C : B) + (t < end ? t : end - 1) * ts;
+                if constexpr (MODE == kStateLast) raw[r].load(at, n0 + n, (int)p.dstate);
+                else raw[r].each(at, ns, n0 + n, (int)p.dstate);
             }
         }
     }
-    __device__ __forceinline__ void store(float* lds, int nn, int t0, int end, int size, const int32_t* ids, int64_t id_stride) {
+    __device__ __forceinline__ void store(float* lds, int n0, int nn, int dstate, int t0, int end, int size, const int32_t* ids,
+                                          int64_t id_stride) {
         const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
-        if constexpr (TIME) {
+        if constexpr (MODE == kStateTime) {
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 if (wave * ROWS % kStates + r >= nn) continue;
@@ -239,12 +247,14 @@ template <typename T, int K, int WAVES, bool TIME> struct StateRows {
         } else {
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
-                const int item = r * 64 * WAVES + (int)threadIdx.x, rest = item / TILE, t = item % TILE;
-                const bool dead = ids && t0 + t < end && ids[(t0 + t) * id_stride] < 0;
+                const int n = unit(r, wave) % OCT * E, t = pos(r, wave, lane);
+                if (n >= nn) continue;
+                if (MODE == kStateLast && n0 + n + E > dstate) raw[r].fix(n0 + n, dstate, dstate);
+                const bool out = t0 + t >= end || (ids && ids[(t0 + t) * id_stride] < 0);
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    lds[((((rest / OCT) * kStates + rest % OCT * E + e) * Q + (t / 4) % Q) * 64 + t / K) * 4 + t % 4] =
-                        dead ? 0.0f : raw[r].get(e);
+                    lds[((((unit(r, wave) / OCT) * kStates + n + e) * Q + (t / 4) % Q) * 64 + t / K) * 4 + t % 4] =
+                        out ? 0.0f : raw[r].get(e);
             }
         }
     }
@@ -256,6 +266,135 @@ template <int K> __device__ __forceinline__ void read_state(const float* lds, in
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[4 * q + j] = w[j];
     }
+}
+
+// Tiles of channel-last tensors: a block's CB channels of TILE positions pass
+// through LDS, [channel][position] with 16 bytes between channels, so that both
+// sides are whole accesses: in memory CB contiguous channels per position, in
+// registers a lane's K consecutive positions of one channel. A thread carries
+// 16 bytes of channels at two neighbouring positions, which are one write of
+// two positions per channel in LDS.
+template <typename T, int K, int CB, int THREADS> struct ChannelTile {
+    static constexpr int TILE = 64 * K, E = elems16<T>::value, SEGS = CB / E, PAIRS = TILE / 2 * SEGS,
+                         TURNS = (PAIRS + THREADS - 1) / THREADS, ROW = TILE + E;
+    static constexpr int BYTES = CB * ROW * (int)sizeof(T);
+    Raw<T, E> r[TURNS][2];
+
+    static __device__ __forceinline__ bool has(int i) { return i * THREADS + (int)threadIdx.x < PAIRS; }
+    static __device__ __forceinline__ int seg(int i) { return (i * THREADS + (int)threadIdx.x) % SEGS * E; }   // first channel
+    static __device__ __forceinline__ int pos(int i) { return (i * THREADS + (int)threadIdx.x) / SEGS * 2; }   // first position
+
+    // base: the batch row's position 0 and channel 0; c0 the block's first channel of `dim`; positions t0 .. end - 1
+    __device__ __forceinline__ void load(const T* base, int64_t t_stride, int c0, int dim, int t0, int end) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            if (!has(i)) continue;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int t = t0 + pos(i) + k;
+                r[i][k].load(base + (t < end ? t : end - 1) * t_stride, c0 + seg(i), dim);  // (past the end: never used)
+            }
+        }
+    }
+    __device__ __forceinline__ void to_lds(T* buf, int c0, int dim) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            if (!has(i)) continue;
+            if (c0 + CB > dim) {
+                r[i][0].fix(c0 + seg(i), dim, dim);
+                r[i][1].fix(c0 + seg(i), dim, dim);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                T* at = buf + (seg(i) + e) * ROW + pos(i);
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<u32x2*>(at) = u32x2{r[i][0].w[e], r[i][1].w[e]};
+                } else {
+                    const uint32_t a = r[i][0].w[e / 2], b = r[i][1].w[e / 2];
+                    *reinterpret_cast<uint32_t*>(at) = (e & 1) ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
+                }
+            }
+        }
+    }
+    // A lane's K positions of channel c.
+    static __device__ __forceinline__ void row(const T* buf, int c, int lane, Raw<T, K>& v) {
+        const T* at = buf + c * ROW + lane * K;
+        if constexpr (Raw<T, K>::DW == 2) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+            v.w[0] = w[0];
+            v.w[1] = w[1];
+        } else {
+#pragma unroll
+            for (int q = 0; q < Raw<T, K>::DW / 4; ++q) {
+                const u32x4 w = reinterpret_cast<const u32x4*>(at)[q];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v.w[4 * q + j] = w[j];
+            }
+        }
+    }
+    static __device__ __forceinline__ void put_row(T* buf, int c, int lane, const float (&v)[K]) {
+        T* at = buf + c * ROW + lane * K;
+        if constexpr (Raw<T, K>::DW == 2) {
+            *reinterpret_cast<u32x2*>(at) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+        } else {
+#pragma unroll
+            for (int q = 0; q < Raw<T, K>::DW / 4; ++q) reinterpret_cast<u32x4*>(at)[q] = vpack<T>(v + q * E);
+        }
+    }
+    // LDS to memory: `channels` of them from c0 on.
+    static __device__ __forceinline__ void store(const T* buf, T* base, int64_t t_stride, int c0, int channels, int t0, int end) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            if (!has(i)) continue;
+            uint32_t a[4], b[4];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const T* at = buf + (seg(i) + e) * ROW + pos(i);
+                if constexpr (sizeof(T) == 4) {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+                    a[e] = w[0];
+                    b[e] = w[1];
+                } else {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
+                    a[e / 2] = (e & 1) ? a[e / 2] | (w << 16) : w & 0xffffu;
+                    b[e / 2] = (e & 1) ? b[e / 2] | (w & 0xffff0000u) : w >> 16;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int t = t0 + pos(i) + k;
+                if (t >= end) continue;
+                T* to = base + t * t_stride + c0 + seg(i);
+                const u32x4 v = k == 0 ? u32x4{a[0], a[1], a[2], a[3]} : u32x4{b[0], b[1], b[2], b[3]};
+                if (seg(i) + E <= channels) {
+                    *reinterpret_cast<typename AnyAddr<sizeof(T)>::v4*>(to) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (seg(i) + e < channels) st_elem<T>(to + e, v, e);
+                }
+            }
+        }
+    }
+};
+
+// Blocks in XCD order: the hardware deals blocks out to the 8 XCDs in turns;
+// here 8 neighbours run on one XCD and share its L2: the 128-byte lines that
+// hold their channels in channel-last tensors, B and C of their sequence. No
+// more than 8 in a row: sequences differ in length, and each has to be spread
+// over all XCDs (whole sequences on one XCD: 605 us, 380 with none of this
+// order, at eight prompts of 8192 positions x 4096 channels).
+__device__ __forceinline__ uint32_t xcd_block(uint32_t b, uint32_t total) {
+    const uint32_t base = b & ~63u;
+    if (base + 64 > total) return b;
+    return base + (b & 7) * 8 + ((b >> 3) & 7);
+}
+
+// How a call's B and C lie.
+template <typename T, int K> StateMode state_mode(const cc1d_scan_params& p) {
+    if (p.seqlen >= K && p.B_stride[3] == 1 && p.C_stride[3] == 1) return kStateTime;
+    if (p.dstate >= elems16<T>::value && p.B_stride[2] == 1 && p.C_stride[2] == 1) return kStateLast;
+    return kStateAny;
 }
 
 }  // namespace cc1d
