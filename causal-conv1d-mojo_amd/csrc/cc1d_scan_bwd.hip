@@ -99,17 +99,26 @@ __device__ __forceinline__ float scan_state_bwd(Channel<K>& ch, float A, float b
     return dA;
 }
 
-// A block: NW wavefronts of CHW channels each, `rounds` times, of one group and
+// How u, delta, z, dout and their gradients lie: unit time stride, unit channel
+// stride (through LDS), or any strides.
+enum Layout { kRows, kLast, kAny };
+
+// A block: 8 wavefronts of CHW channels each, `rounds` times, of one group and
 // sequence; tiles from the last to the first. In a tile, each round's channels
-// run through 16 states at a time, each wavefront at others (in step i the
-// 16 / NW from (i + its number) mod NW on), so that the block's sums for dB and
-// dC of a state, in LDS, belong to one wavefront at a time and grow in a fixed
-// order.
-template <typename T, int K, int CHW, int NW, bool SEQ, bool UNIT, StateMode MODE>
-__global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdArgs arg) {
-    constexpr int TILE = 64 * K;
+// run through 16 states at a time, each wavefront at others (of 16, in step i
+// the two from 2 ((i + its number) mod 8) on), so that the block's sums for dB
+// and dC of a state, in LDS, belong to one wavefront at a time and grow in a
+// fixed order.
+constexpr int kWaves = 8;
+template <typename T, int K, int CHW, bool SEQ, Layout LAY, StateMode MODE>
+__global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const ScanBwdArgs arg) {
+    constexpr int TILE = 64 * K, CB = kWaves * CHW;
+    constexpr bool UNIT = LAY == kRows, LAST = LAY == kLast;
+    // (16 channels of 512 positions in 32 bits fill the 160 KB of a CU with no gap between rows)
+    typedef ChannelTile<T, K, CB, 64 * kWaves, CB * TILE * sizeof(T) < 32768 ? elems16<T>::value : 0> Tile;
     __shared__ __attribute__((aligned(16))) float BC[2 * kStates * TILE];
     __shared__ __attribute__((aligned(16))) float acc[2 * kStates * TILE];
+    __shared__ __attribute__((aligned(16))) T buf[LAST ? Tile::BYTES / sizeof(T) : 16 / sizeof(T)];
     const cc1d_scan_bwd_params& b = arg.p;
     const cc1d_scan_params& p = b.fwd;
     const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
@@ -126,12 +135,12 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
     const int32_t* ids = SEQ ? p.seq_idx + q.row * p.seq_idx_stride[0] : nullptr;
     const int64_t is = SEQ ? p.seq_idx_stride[1] : 0;
     const int tiles = (int)((q.len + TILE - 1) / TILE);
-    const int64_t block_first = blk * arg.rounds * (NW * CHW);  // the block's first channel in the group
-    const int rounds = (int)(per - block_first + NW * CHW - 1 < (int64_t)arg.rounds * NW * CHW
-                                 ? (per - block_first + NW * CHW - 1) / (NW * CHW) : arg.rounds);
+    const int64_t block_first = blk * arg.rounds * CB;  // the block's first channel in the group
+    const int rounds = (int)(per - block_first + CB - 1 < (int64_t)arg.rounds * CB
+                                 ? (per - block_first + CB - 1) / CB : arg.rounds);
 
     if (tiles == 0 || p.cu_seqlens) {
-        for (int64_t i = wave; i < (int64_t)rounds * NW * CHW; i += NW) {
+        for (int64_t i = wave; i < (int64_t)rounds * CB; i += kWaves) {
             if (block_first + i >= per) break;
             const int64_t d = grp * per + block_first + i;
             if (p.cu_seqlens && s == 0) zero_uncovered<T>(b, d, 0, q.start);
@@ -158,56 +167,106 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
         for (int j = 0; j < K; ++j) live[j] = t + j < end;
         if constexpr (SEQ) cuts.read(ids, is, t, end - t, live);
         else cuts.none();
+        const uint32_t bits = live_bits<K>(live);
+        auto counts = [&](int j) { return SEQ ? live[j] : !LAST || full || live[j]; };  // (of rows, fix() clears the others)
         const bool met_back = SEQ && __shfl((int)cuts.met, 63 - lane) != 0;
-        auto input = [&](Raw<T, K>& r, const void* base, const int64_t* stride, int64_t d) {
-            const T* row = static_cast<const T*>(base) + q.row * stride[0] + d * stride[1];
-            if constexpr (UNIT) r.load(row, t, size);
-            else r.each(row, stride[2], t, end);
-        };
-        auto fix = [&](Raw<T, K>& r) {
-            if (UNIT && !full) r.fix(t, end, size);
-        };
         // With more than 16 states a block has one round, and its channels keep
         // their sums in registers from one lot of states to the next.
         for (int round = 0; round < rounds; ++round) {
             Channel<K> ch[CHW];
             int64_t d[CHW];
             bool mine[CHW];  // a missing channel is the group's last one with u, dout and states 0, and stores nothing
-            {
-                Raw<T, K> ru[CHW], rd[CHW], rz[CHW], ro[CHW];
+            const int64_t round_first = block_first + (int64_t)round * CB;
+            const int channels = (int)(per - round_first < CB ? per - round_first : CB), c0 = (int)(grp * per + round_first);
 #pragma unroll
-                for (int c = 0; c < CHW; ++c) {
-                    const int64_t at = block_first + (int64_t)(round * NW + wave) * CHW + c;
-                    mine[c] = at < per;
-                    d[c] = grp * per + (mine[c] ? at : per - 1);
-                    input(ru[c], p.u, p.u_stride, d[c]);
-                    input(rd[c], p.delta, p.delta_stride, d[c]);
-                    input(ro[c], b.dout, b.dout_stride, d[c]);
-                    if (p.z) input(rz[c], p.z, p.z_stride, d[c]);
+            for (int c = 0; c < CHW; ++c) {
+                mine[c] = wave * CHW + c < channels;
+                d[c] = c0 + (mine[c] ? wave * CHW + c : channels - 1);
+            }
+            // A round's share of a tensor: fetch() issues the loads, take() waits
+            // for them (kLast: through LDS), give() stores.
+            struct Rows {
+                Raw<T, K> r[CHW];
+            };
+            typedef typename std::conditional<LAST, Tile, Rows>::type In;
+            auto fetch = [&](In& in, const void* base, const int64_t* stride) {
+                const T* row = static_cast<const T*>(base) + q.row * stride[0];
+                if constexpr (LAST) {
+                    in.load(row, stride[2], c0, (int)p.dim, t0, end);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < CHW; ++c) {
+                        if constexpr (UNIT) in.r[c].load(row + d[c] * stride[1], t, size);
+                        else in.r[c].each(row + d[c] * stride[1], stride[2], t, end);
+                    }
+                }
+            };
+            auto take = [&](In& in, Raw<T, K> (&r)[CHW]) {
+                if constexpr (LAST) {
+                    __syncthreads();
+                    in.to_lds(buf, c0, (int)p.dim);
+                    __syncthreads();
                 }
 #pragma unroll
                 for (int c = 0; c < CHW; ++c) {
-                    const float bias = p.delta_bias ? ld_uniform(p.delta_bias + d[c] * p.delta_bias_stride) : 0.0f;
-                    fix(ru[c]);
-                    fix(rd[c]);
-                    fix(ro[c]);
-                    float sum = 0.0f;
-                    steps<K>(rd[c], bias, p.delta_softplus != 0, ch[c].dt);
+                    if constexpr (LAST) Tile::row(buf, (int)(d[c] - c0), lane, r[c]);
+                    else r[c] = in.r[c];
+                    if (UNIT && !full) r[c].fix(t, end, size);
+                }
+            };
+            auto give = [&](void* base, const int64_t* stride, auto value) {
+                T* row = static_cast<T*>(base) + q.row * stride[0];
+                if constexpr (LAST) {
+                    __syncthreads();
+#pragma unroll
+                    for (int c = 0; c < CHW; ++c) Tile::put_row(buf, wave * CHW + c, lane, value(c));
+                    __syncthreads();
+                    Tile::store(buf, row, stride[2], c0, channels, t0, end);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < CHW; ++c)
+                        if (mine[c]) store_steps<T, K>(row + d[c] * stride[1], UNIT ? 1 : stride[2], t, end, value(c));
+                }
+            };
+            float bias[CHW];
+#pragma unroll
+            for (int c = 0; c < CHW; ++c) bias[c] = p.delta_bias ? ld_uniform(p.delta_bias + d[c] * p.delta_bias_stride) : 0.0f;
+            {
+                In iu, id, iz, io;
+                Raw<T, K> r[CHW];
+                fetch(id, p.delta, p.delta_stride);
+                fetch(iu, p.u, p.u_stride);
+                fetch(io, b.dout, b.dout_stride);
+                if (p.z) fetch(iz, p.z, p.z_stride);
+                take(id, r);
+#pragma unroll
+                for (int c = 0; c < CHW; ++c) {
+                    steps<K>(r[c], bias[c], p.delta_softplus != 0, ch[c].dt);
+                    ch[c].step_sum = 0.0f;
 #pragma unroll
                     for (int j = 0; j < K; ++j) {
                         if (SEQ || !full) ch[c].dt[j] = live[j] ? ch[c].dt[j] : 0.0f;
-                        ch[c].du[j] = mine[c] && (!SEQ || live[j]) ? ch[c].dt[j] * ru[c].get(j) : 0.0f;
-                        ch[c].dy[j] = mine[c] && (!SEQ || live[j]) ? ro[c].get(j) : 0.0f;
-                        sum += ch[c].dt[j];
+                        ch[c].step_sum += ch[c].dt[j];
                         ch[c].y[j] = ch[c].along[j] = ch[c].wsum[j] = 0.0f;
                     }
-                    if (p.z) {
-                        fix(rz[c]);
+                }
+                take(iu, r);
+#pragma unroll
+                for (int c = 0; c < CHW; ++c)
+#pragma unroll
+                    for (int j = 0; j < K; ++j) ch[c].du[j] = mine[c] && counts(j) ? ch[c].dt[j] * r[c].get(j) : 0.0f;
+                take(io, r);
+#pragma unroll
+                for (int c = 0; c < CHW; ++c)
+#pragma unroll
+                    for (int j = 0; j < K; ++j) ch[c].dy[j] = mine[c] && counts(j) ? r[c].get(j) : 0.0f;
+                if (p.z) {
+                    take(iz, r);
+#pragma unroll
+                    for (int c = 0; c < CHW; ++c)
 #pragma unroll
                         for (int j = 0; j < K; ++j)
-                            if (mine[c] && (!SEQ || live[j])) ch[c].dy[j] *= silu(rz[c].get(j));
-                    }
-                    ch[c].step_sum = sum;
+                            if (mine[c] && counts(j)) ch[c].dy[j] *= silu(r[c].get(j));
                 }
             }
             for (int n0 = 0; n0 < N; n0 += kStates) {
@@ -228,19 +287,20 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                     }
                 }
                 if (round == 0) {
-                    StateRows<T, K, NW, MODE> rows;
+                    StateRows<T, K, kWaves, MODE> rows;
                     rows.load(p, Bp, Cp, n0, nn, t0, end, size);
                     __syncthreads();  // the last lot is done with
-                    rows.store(BC, n0, nn, N, t0, end, size, ids, is);
-                    for (int i = threadIdx.x; i < 2 * kStates * TILE / 4; i += 64 * NW)
+                    rows.store(BC, n0, nn, N, t0, end, size, bits);
+                    for (int i = threadIdx.x; i < 2 * kStates * TILE / 4; i += 64 * kWaves)
                         reinterpret_cast<f32x4*>(acc)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
                 __syncthreads();
+                const int turn = (nn + kWaves - 1) / kWaves;  // states per wavefront between two barriers
 #pragma unroll 1
-                for (int i = 0; i < NW; ++i) {
+                for (int i = 0; i < kWaves; ++i) {
 #pragma unroll 1
-                    for (int k = 0; k < kStates / NW; ++k) {
-                        const int n = (i + wave) % NW * (kStates / NW) + k;
+                    for (int k = 0; k < turn; ++k) {
+                        const int n = (i + wave) % kWaves * turn + k;
                         if (n >= nn) break;
                         float B[K], C[K], dB[K], dC[K];
                         read_state<K>(BC, n, lane, B);
@@ -280,7 +340,7 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                     else if (b.dinitial_states) b.dinitial_states[at] = after_l[c];
                 }
                 if (round == rounds - 1) {
-                    constexpr int ROWS = 2 * kStates / NW;
+                    constexpr int ROWS = 2 * kStates / kWaves;
 #pragma unroll
                     for (int r = 0; r < ROWS; ++r) {
                         const int row = wave * ROWS + r, n = row % kStates;
@@ -302,52 +362,65 @@ __global__ void __launch_bounds__(64 * NW, NW / 4) scan_bwd_rows(const ScanBwdAr
                     }
                 }
             }
+            // The inputs again, from L2: to have kept them would have cost the
+            // states' loop its registers. From here on along is du, wsum ddelta
+            // and y dz.
+            In iu, id, iz, io;
+            Raw<T, K> r[CHW];
+            fetch(iu, p.u, p.u_stride);
+            fetch(id, p.delta, p.delta_stride);
+            if (p.z) {
+                fetch(io, b.dout, b.dout_stride);
+                fetch(iz, p.z, p.z_stride);
+            }
+            float dD[CHW], dbias[CHW];
+            take(iu, r);
 #pragma unroll
             for (int c = 0; c < CHW; ++c) {
-                if (!mine[c]) continue;
-                Raw<T, K> ru, rd, rz, ro;
-                input(ru, p.u, p.u_stride, d[c]);
-                input(rd, p.delta, p.delta_stride, d[c]);
-                if (p.z) {
-                    input(rz, p.z, p.z_stride, d[c]);
-                    input(ro, b.dout, b.dout_stride, d[c]);
-                    fix(rz);
-                    fix(ro);
-                }
-                fix(ru);
-                fix(rd);
-                const float bias = p.delta_bias ? ld_uniform(p.delta_bias + d[c] * p.delta_bias_stride) : 0.0f;
                 const float skip = p.D ? ld_uniform(p.D + d[c] * p.D_stride) : 0.0f;
-                float du[K], dd[K], dD = 0.0f, dbias = 0.0f;
+                dD[c] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < K; ++j) {
-                    const float u = SEQ && !live[j] ? 0.0f : ru.get(j);
-                    du[j] = __builtin_fmaf(skip, ch[c].dy[j], ch[c].dt[j] * ch[c].along[j]);
-                    dd[j] = __builtin_fmaf(u, ch[c].along[j], ch[c].wsum[j]);
-                    if (p.delta_softplus) dd[j] *= SEQ && !live[j] ? 0.0f : sigmoid(rd.get(j) + bias);
-                    dD = __builtin_fmaf(ch[c].dy[j], u, dD);
-                    if (SEQ || !full) dd[j] = live[j] ? dd[j] : 0.0f;
-                    dbias += dd[j];
+                    const float u = counts(j) ? r[c].get(j) : 0.0f;
+                    ch[c].wsum[j] = __builtin_fmaf(u, ch[c].along[j], ch[c].wsum[j]);
+                    ch[c].along[j] = __builtin_fmaf(skip, ch[c].dy[j], ch[c].dt[j] * ch[c].along[j]);
+                    ch[c].y[j] = __builtin_fmaf(skip, u, ch[c].y[j]);
+                    dD[c] = __builtin_fmaf(ch[c].dy[j], u, dD[c]);
                 }
-                store_steps<T, K>(static_cast<T*>(b.du) + q.row * b.du_stride[0] + d[c] * b.du_stride[1], UNIT ? 1 : b.du_stride[2], t, end, du);
-                store_steps<T, K>(static_cast<T*>(b.ddelta) + q.row * b.ddelta_stride[0] + d[c] * b.ddelta_stride[1],
-                                  UNIT ? 1 : b.ddelta_stride[2], t, end, dd);
-                if (p.z) {
-                    float dz[K];
+            }
+            give(b.du, b.du_stride, [&](int c) -> const float(&)[K] { return ch[c].along; });
+            take(id, r);
 #pragma unroll
-                    for (int j = 0; j < K; ++j) {
-                        const float u = SEQ && !live[j] ? 0.0f : ru.get(j);
-                        dz[j] = ro.get(j) * __builtin_fmaf(skip, u, ch[c].y[j]) * silu_grad(rz.get(j));
-                        if (SEQ && !live[j]) dz[j] = 0.0f;
-                    }
-                    store_steps<T, K>(static_cast<T*>(b.dz) + q.row * b.dz_stride[0] + d[c] * b.dz_stride[1], UNIT ? 1 : b.dz_stride[2], t, end, dz);
+            for (int c = 0; c < CHW; ++c) {
+                dbias[c] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    if (p.delta_softplus) ch[c].wsum[j] *= counts(j) ? sigmoid(r[c].get(j) + bias[c]) : 0.0f;
+                    if (SEQ || !full) ch[c].wsum[j] = live[j] ? ch[c].wsum[j] : 0.0f;
+                    dbias[c] += ch[c].wsum[j];
                 }
-                dD = wave_sum(dD);
-                dbias = wave_sum(dbias);
-                if (lane == 0) {
+            }
+            give(b.ddelta, b.ddelta_stride, [&](int c) -> const float(&)[K] { return ch[c].wsum; });
+            if (p.z) {
+                take(io, r);
+#pragma unroll
+                for (int c = 0; c < CHW; ++c)
+#pragma unroll
+                    for (int j = 0; j < K; ++j) ch[c].y[j] *= r[c].get(j);
+                take(iz, r);
+#pragma unroll
+                for (int c = 0; c < CHW; ++c)
+#pragma unroll
+                    for (int j = 0; j < K; ++j) ch[c].y[j] = counts(j) ? ch[c].y[j] * silu_grad(r[c].get(j)) : 0.0f;
+                give(b.dz, b.dz_stride, [&](int c) -> const float(&)[K] { return ch[c].y; });
+            }
+#pragma unroll
+            for (int c = 0; c < CHW; ++c) {
+                const float sD = wave_sum(dD[c]), sb = wave_sum(dbias[c]);
+                if (lane == 0 && mine[c]) {
                     const int64_t at = s * p.dim + d[c];
-                    arg.pD[at] = last ? dD : arg.pD[at] + dD;
-                    arg.pbias[at] = last ? dbias : arg.pbias[at] + dbias;
+                    arg.pD[at] = last ? sD : arg.pD[at] + sD;
+                    arg.pbias[at] = last ? sb : arg.pbias[at] + sb;
                 }
             }
         }
@@ -408,45 +481,55 @@ __global__ void __launch_bounds__(256) scan_bwd_reduce_params(const ScanBwdArgs 
     to[i] = sum;
 }
 
-#ifndef BWD_CHW
-#define BWD_CHW 2
-#endif
-#ifndef BWD_NW
-#define BWD_NW (16 / BWD_CHW)
-#endif
-constexpr int kChw = BWD_CHW, kWaves = BWD_NW, kRound = kChw * kWaves;  // channels a round
+// What a block takes: its wavefronts' channels at a time (1 or 2), and how many
+// rounds of them.
+struct BwdPlan {
+    int chw, rounds;
+    int64_t group_blocks;
+};
 
-// Rounds of a block: a CU holds one (128 KB of LDS), so the choice that leaves
-// the card the least to do one after the other, and of equals the largest,
-// whose dB and dC have the fewest shares to add. More than 16 states: one.
-int bwd_rounds(const cc1d_scan_params& p) {
-    if (p.dstate > kStates) return 1;
+// A CU holds one block (128 KB of LDS), so the choice that leaves the card the
+// least to do one after the other; a round of one channel each takes about 2/3
+// of the time of one of two (854 us against 652 at 4 x 2048 x 2048 with 16
+// states, where either fills the card). Of equals the largest: its dB and dC
+// have the fewest shares to add. More than 16 states: one round.
+BwdPlan bwd_plan(const cc1d_scan_params& p) {
     const int64_t per = p.dim / p.groups, rows = scan_sequences(p) * p.groups;
-    int best = 1;
-    int64_t least = -1;
-    for (int r = 1; r <= 8; ++r) {
-        const int64_t cost = ceil_div(rows * ceil_div(per, kRound * r), 256) * r;
-        if (least < 0 || cost <= least) {
-            least = cost;
-            best = r;
+    BwdPlan best{0, 0, 0};
+    int64_t least = 0;
+    for (int r = 1; r <= (p.dstate > kStates ? 1 : 8); ++r)
+        for (int chw = 1; chw <= 2; ++chw) {
+            const int64_t blocks = ceil_div(per, kWaves * chw * r);
+            const int64_t cost = ceil_div(rows * blocks, 256) * r * (chw + 1);
+            if (best.chw == 0 || cost <= least) {
+                least = cost;
+                best = {chw, r, blocks};
+            }
         }
-    }
     return best;
 }
 
-template <typename T, int K> int launch_rows(const ScanBwdArgs& a, hipStream_t stream) {
+template <typename T, int K> int launch_rows(const ScanBwdArgs& a, int chw, hipStream_t stream) {
     const cc1d_scan_bwd_params& b = a.p;
     const cc1d_scan_params& p = b.fwd;
     const dim3 grid((unsigned)(a.group_blocks * p.groups * scan_sequences(p))), block(64 * kWaves);
-    const bool unit = p.seqlen >= K && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && b.dout_stride[2] == 1 &&
-                      b.du_stride[2] == 1 && b.ddelta_stride[2] == 1 && (!p.z || (p.z_stride[2] == 1 && b.dz_stride[2] == 1));
+    auto unit = [&](int i) {
+        return p.u_stride[i] == 1 && p.delta_stride[i] == 1 && b.dout_stride[i] == 1 && b.du_stride[i] == 1 &&
+               b.ddelta_stride[i] == 1 && (!p.z || (p.z_stride[i] == 1 && b.dz_stride[i] == 1));
+    };
     const StateMode mode = state_mode<T, K>(p);
+    const Layout lay = mode == kStateAny ? kAny : p.seqlen >= K && unit(2) ? kRows : p.dim >= elems16<T>::value && unit(1) ? kLast : kAny;
     return with_flag(p.seq_idx != nullptr, [&](auto seq) {
-        constexpr bool SEQ = decltype(seq)::value;
-        if (!unit || mode == kStateAny)
-            return launch(scan_bwd_rows<T, K, kChw, kWaves, SEQ, false, kStateAny>, grid, block, stream, a);
-        if (mode == kStateTime) return launch(scan_bwd_rows<T, K, kChw, kWaves, SEQ, true, kStateTime>, grid, block, stream, a);
-        return launch(scan_bwd_rows<T, K, kChw, kWaves, SEQ, true, kStateLast>, grid, block, stream, a);
+        return with_flag(chw == 2, [&](auto two) {
+            constexpr bool SEQ = decltype(seq)::value;
+            constexpr int CHW = decltype(two)::value ? 2 : 1;
+            if (lay == kAny) return launch(scan_bwd_rows<T, K, CHW, SEQ, kAny, kStateAny>, grid, block, stream, a);
+            return with_flag(mode == kStateTime, [&](auto tm) {
+                constexpr StateMode MODE = decltype(tm)::value ? kStateTime : kStateLast;
+                if (lay == kRows) return launch(scan_bwd_rows<T, K, CHW, SEQ, kRows, MODE>, grid, block, stream, a);
+                return launch(scan_bwd_rows<T, K, CHW, SEQ, kLast, MODE>, grid, block, stream, a);
+            });
+        });
     });
 }
 
@@ -454,7 +537,7 @@ template <typename T, int K> int launch_rows(const ScanBwdArgs& a, hipStream_t s
 
 int64_t scan_bwd_workspace_floats(const cc1d_scan_bwd_params& b) {
     const cc1d_scan_params& p = b.fwd;
-    const int64_t blocks = ceil_div(p.dim / p.groups, kRound * bwd_rounds(p));
+    const int64_t blocks = bwd_plan(p).group_blocks;
     return 2 * p.batch * p.groups * blocks * p.dstate * p.seqlen + scan_sequences(p) * p.dim * (2 * p.dstate + 2);
 }
 
@@ -463,8 +546,9 @@ int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
     const int64_t seqs = scan_sequences(p), states = seqs * p.dim * p.dstate;
     ScanBwdArgs a{};
     a.p = b;
-    a.rounds = bwd_rounds(p);
-    a.group_blocks = ceil_div(p.dim / p.groups, kRound * a.rounds);
+    const BwdPlan plan = bwd_plan(p);
+    a.rounds = plan.rounds;
+    a.group_blocks = plan.group_blocks;
     a.carry = b.workspace;
     a.pA = a.carry + states;
     a.pD = a.pA + states;
@@ -475,7 +559,7 @@ int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
         typedef decltype(t) T;
         int st = CC1D_OK;
         if (seqs > 0)
-            st = scan_tile(p.seqlen) == 512 ? launch_rows<T, 8>(a, stream) : launch_rows<T, 4>(a, stream);
+            st = scan_tile(p.seqlen) == 512 ? launch_rows<T, 8>(a, plan.chw, stream) : launch_rows<T, 4>(a, plan.chw, stream);
         if (st == CC1D_OK && items > 0)
             st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)ceil_div(items, 256)), dim3(256), stream, a, items);
         if (st == CC1D_OK)

@@ -79,6 +79,9 @@ template <int K, typename R> __device__ __forceinline__ void steps(const R& raw,
     }
 }
 
+constexpr int kDppWaveShr1 = 0x138;  // lane l takes lane l - 1's value
+constexpr int kDppRowShr = 0x110;    // + w: lane l takes lane l - w's, within 16 lanes
+
 // Where a lane's steps and the wavefront's prefix must not reach across a
 // sequence's start (seq_idx). All of it is the same for every state.
 template <int K> struct Cuts {
@@ -96,15 +99,27 @@ template <int K> struct Cuts {
     // ids of the row from its position 0; t the lane's first position, count of them in the row
     __device__ __forceinline__ void read(const int32_t* ids, int64_t stride, int64_t t, int count, bool (&live)[K]) {
         const int lane = threadIdx.x & 63;
-        int32_t prev = t > 0 && count > 0 ? ids[(t - 1) * stride] : 0;
+        int32_t id[K];
+        if (stride == 1 && count >= K) {
+#pragma unroll
+            for (int q = 0; q < K / 4; ++q) {
+                const u32x4 w = *reinterpret_cast<const AnyAddr<4>::v4*>(ids + t + 4 * q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) id[4 * q + j] = (int32_t)w[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < K; ++j) id[j] = j < count ? ids[(t + j) * stride] : 0;
+        }
+        const int32_t ahead = lane == 0 && t > 0 && count > 0 ? ids[(t - 1) * stride] : 0;
+        int32_t prev = __builtin_amdgcn_update_dpp(ahead, id[K - 1], kDppWaveShr1, 0xf, 0xf, false);
         met = false;
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            const int32_t id = j < count ? ids[(t + j) * stride] : prev;
-            at[j] = j < count && (id != prev || t + j == 0);
-            live[j] = j < count && id >= 0;
+            at[j] = j < count && (id[j] != prev || t + j == 0);
+            live[j] = j < count && id[j] >= 0;
             met |= at[j];
-            prev = id;
+            prev = id[j];
         }
         const uint64_t m = __ballot(met);
         any = m != 0;
@@ -122,9 +137,6 @@ template <int K> struct Cuts {
         back[5] = next < 32;
     }
 };
-
-constexpr int kDppWaveShr1 = 0x138;  // lane l takes lane l - 1's value
-constexpr int kDppRowShr = 0x110;    // + w: lane l takes lane l - w's, within 16 lanes
 
 // Inclusive prefix over the 64 lanes of the pairs (P, H): H becomes
 // H + P H' + P P' H'' ... over the lanes before. A DPP operand reads the
@@ -223,8 +235,8 @@ template <typename T, int K, int WAVES, StateMode MODE> struct StateRows {
             }
         }
     }
-    __device__ __forceinline__ void store(float* lds, int n0, int nn, int dstate, int t0, int end, int size, const int32_t* ids,
-                                          int64_t id_stride) {
+    // live: bit j for the lane's position j, if it counts
+    __device__ __forceinline__ void store(float* lds, int n0, int nn, int dstate, int t0, int end, int size, uint32_t live) {
         const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6);
         if constexpr (MODE == kStateTime) {
 #pragma unroll
@@ -233,12 +245,7 @@ template <typename T, int K, int WAVES, StateMode MODE> struct StateRows {
                 if (end - t0 < TILE) raw[r].fix(t0 + lane * K, end, size);
                 float v[K];
 #pragma unroll
-                for (int j = 0; j < K; ++j) v[j] = raw[r].get(j);
-                if (ids) {
-#pragma unroll
-                    for (int j = 0; j < K; ++j)
-                        if (t0 + lane * K + j < end && ids[(t0 + lane * K + j) * id_stride] < 0) v[j] = 0.0f;
-                }
+                for (int j = 0; j < K; ++j) v[j] = live >> j & 1 ? raw[r].get(j) : 0.0f;
 #pragma unroll
                 for (int q = 0; q < Q; ++q)
                     *reinterpret_cast<f32x4*>(lds + (((wave * ROWS + r) * Q + q) * 64 + lane) * 4) =
@@ -250,15 +257,21 @@ template <typename T, int K, int WAVES, StateMode MODE> struct StateRows {
                 const int n = unit(r, wave) % OCT * E, t = pos(r, wave, lane);
                 if (n >= nn) continue;
                 if (MODE == kStateLast && n0 + n + E > dstate) raw[r].fix(n0 + n, dstate, dstate);
-                const bool out = t0 + t >= end || (ids && ids[(t0 + t) * id_stride] < 0);
+                const bool in = (uint32_t)__shfl((int)live, t / K) >> (t % K) & 1;
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     lds[((((unit(r, wave) / OCT) * kStates + n + e) * Q + (t / 4) % Q) * 64 + t / K) * 4 + t % 4] =
-                        out ? 0.0f : raw[r].get(e);
+                        in ? raw[r].get(e) : 0.0f;
             }
         }
     }
 };
+template <int K> __device__ __forceinline__ uint32_t live_bits(const bool (&live)[K]) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) bits |= (uint32_t)live[j] << j;
+    return bits;
+}
 template <int K> __device__ __forceinline__ void read_state(const float* lds, int n, int lane, float (&v)[K]) {
 #pragma unroll
     for (int q = 0; q < K / 4; ++q) {
@@ -269,14 +282,14 @@ template <int K> __device__ __forceinline__ void read_state(const float* lds, in
 }
 
 // Tiles of channel-last tensors: a block's CB channels of TILE positions pass
-// through LDS, [channel][position] with 16 bytes between channels, so that both
+// through LDS, [channel][position] with PAD elements between channels, so that both
 // sides are whole accesses: in memory CB contiguous channels per position, in
 // registers a lane's K consecutive positions of one channel. A thread carries
 // 16 bytes of channels at two neighbouring positions, which are one write of
 // two positions per channel in LDS.
-template <typename T, int K, int CB, int THREADS> struct ChannelTile {
+template <typename T, int K, int CB, int THREADS, int PAD = elems16<T>::value> struct ChannelTile {
     static constexpr int TILE = 64 * K, E = elems16<T>::value, SEGS = CB / E, PAIRS = TILE / 2 * SEGS,
-                         TURNS = (PAIRS + THREADS - 1) / THREADS, ROW = TILE + E;
+                         TURNS = (PAIRS + THREADS - 1) / THREADS, ROW = TILE + PAD;
     static constexpr int BYTES = CB * ROW * (int)sizeof(T);
     Raw<T, E> r[TURNS][2];
 

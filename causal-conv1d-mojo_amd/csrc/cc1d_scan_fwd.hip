@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(512, UNIT && MODE == kStateTime ? 4 : 2) scan_
         for (int j = 0; j < K; ++j) live[j] = t + j < end;
         if constexpr (SEQ) cuts.read(ids, is, t, end - t, live);
         else cuts.none();
+        const uint32_t bits = live_bits<K>(live);
         if (tiles) {
             for (int n = part * 64 + lane; n < N; n += 64 * split) tiles[n] = carry[n];
             tiles += p.dim * N;
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(512, UNIT && MODE == kStateTime ? 4 : 2) scan_
         }
         for (int n0 = 0; n0 < N; n0 += kStates) {
             const int nn = N - n0 < kStates ? N - n0 : kStates;
-            rows.store(BC, n0, nn, N, t0, end, size, ids, is);
+            rows.store(BC, n0, nn, N, t0, end, size, bits);
             __syncthreads();
             // the next values travel while these are used
             if (n0 + kStates < N) fetch_states(t0, n0 + kStates);
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(512, sizeof(T) == 2 && NCAP <= 128 ? 4 : 2) sc
         for (int j = 0; j < K; ++j) live[j] = t + j < end;
         if constexpr (SEQ) cuts.read(ids, is, t, end - t, live);
         else cuts.none();
+        const uint32_t bits = live_bits<K>(live);
         Raw<T, K> ru, rd;
         __syncthreads();  // the last tile's outputs have left the buffer
         tu.to_lds(buf, c0, dim);
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(512, sizeof(T) == 2 && NCAP <= 128 ? 4 : 2) sc
         if (p.z) tz.load(pz, p.z_stride[2], c0, dim, t0, end);
         for (int n0 = 0; n0 < N; n0 += kStates) {
             const int nn = N - n0 < kStates ? N - n0 : kStates;
-            rows.store(BC, n0, nn, N, t0, end, size, ids, is);
+            rows.store(BC, n0, nn, N, t0, end, size, bits);
             __syncthreads();
             if (n0 + kStates < N) fetch_states(t0, n0 + kStates);
             else if (t0 + TILE < end) fetch_states(t0 + TILE, 0);
