@@ -135,14 +135,15 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
     const int32_t* ids = SEQ ? p.seq_idx + q.row * p.seq_idx_stride[0] : nullptr;
     const int64_t is = SEQ ? p.seq_idx_stride[1] : 0;
     const int tiles = (int)((q.len + TILE - 1) / TILE);
-    const int64_t block_first = blk * arg.rounds * CB;  // the block's first channel in the group
-    const int rounds = (int)(per - block_first + CB - 1 < (int64_t)arg.rounds * CB
-                                 ? (per - block_first + CB - 1) / CB : arg.rounds);
+    // In a round, neighbouring blocks take neighbouring channels: they share the lines of channel-last tensors.
+    auto first_of = [&](int round) { return (round * arg.group_blocks + blk) * CB; };
+    const int rounds = (int)(((per + CB - 1) / CB - blk + arg.group_blocks - 1) / arg.group_blocks);
 
     if (tiles == 0 || p.cu_seqlens) {
         for (int64_t i = wave; i < (int64_t)rounds * CB; i += kWaves) {
-            if (block_first + i >= per) break;
-            const int64_t d = grp * per + block_first + i;
+            const int64_t in_group = first_of((int)(i / CB)) + i % CB;
+            if (in_group >= per) break;
+            const int64_t d = grp * per + in_group;
             if (p.cu_seqlens && s == 0) zero_uncovered<T>(b, d, 0, q.start);
             if (p.cu_seqlens && s == p.num_seqs - 1) zero_uncovered<T>(b, d, q.start + q.len, p.seqlen);
             if (tiles > 0) continue;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
             Channel<K> ch[CHW];
             int64_t d[CHW];
             bool mine[CHW];  // a missing channel is the group's last one with u, dout and states 0, and stores nothing
-            const int64_t round_first = block_first + (int64_t)round * CB;
+            const int64_t round_first = first_of(round);
             const int channels = (int)(per - round_first < CB ? per - round_first : CB), c0 = (int)(grp * per + round_first);
 #pragma unroll
             for (int c = 0; c < CHW; ++c) {
@@ -236,9 +237,8 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
                 Raw<T, K> r[CHW];
                 fetch(id, p.delta, p.delta_stride);
                 fetch(iu, p.u, p.u_stride);
-                fetch(io, b.dout, b.dout_stride);
-                if (p.z) fetch(iz, p.z, p.z_stride);
                 take(id, r);
+                fetch(io, b.dout, b.dout_stride);
 #pragma unroll
                 for (int c = 0; c < CHW; ++c) {
                     steps<K>(r[c], bias[c], p.delta_softplus != 0, ch[c].dt);
@@ -250,7 +250,9 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
                         ch[c].y[j] = ch[c].along[j] = ch[c].wsum[j] = 0.0f;
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
                 take(iu, r);
+                if (p.z) fetch(iz, p.z, p.z_stride);
 #pragma unroll
                 for (int c = 0; c < CHW; ++c)
 #pragma unroll
@@ -369,10 +371,6 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
             Raw<T, K> r[CHW];
             fetch(iu, p.u, p.u_stride);
             fetch(id, p.delta, p.delta_stride);
-            if (p.z) {
-                fetch(io, b.dout, b.dout_stride);
-                fetch(iz, p.z, p.z_stride);
-            }
             float dD[CHW], dbias[CHW];
             take(iu, r);
 #pragma unroll
@@ -388,6 +386,8 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
                     dD[c] = __builtin_fmaf(ch[c].dy[j], u, dD[c]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            if (p.z) fetch(io, b.dout, b.dout_stride);
             give(b.du, b.du_stride, [&](int c) -> const float(&)[K] { return ch[c].along; });
             take(id, r);
 #pragma unroll
@@ -400,6 +400,8 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
                     dbias[c] += ch[c].wsum[j];
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            if (p.z) fetch(iz, p.z, p.z_stride);
             give(b.ddelta, b.ddelta_stride, [&](int c) -> const float(&)[K] { return ch[c].wsum; });
             if (p.z) {
                 take(io, r);
