@@ -57,6 +57,12 @@ template <int LPR, bool EVEN> struct Place {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[4 * q + j] = __uint_as_float(x[j]);
             }
+        } else if (stride == 1 && dim >= E) {
+            Raw<float, E> r;
+            r.load(w, at(i), dim);
+            if (!full(i)) r.fix(at(i), dim, dim);
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = r.get(j);
         } else {
 #pragma unroll
             for (int j = 0; j < E; ++j) v[j] = at(i) + j < dim ? w[(at(i) + j) * stride] : 0.0f;
