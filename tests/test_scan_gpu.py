@@ -126,6 +126,17 @@ def test_packed_rows(size, layout, dtype):
     check(make(B, D, L, N, G, dtype, layout, seed=3), ids=runs(B, L, seed=L))
 
 
+# More channels than the card takes at once: two a wavefront, and several rounds, in the backward's blocks.
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("layout", ["rows", "last", "odd"])
+@pytest.mark.parametrize("size", [(1, 4100, 21, 16, 1), (1, 4107, 520, 5, 1), (2, 1030, 300, 9, 1), (2, 4104, 21, 17, 2)],
+                         ids=str)
+@pytest.mark.parametrize("packed", [False, True], ids=["plain", "packed"])
+def test_many_channels(packed, size, layout, dtype):
+    B, D, L, N, G = size
+    check(make(B, D, L, N, G, dtype, layout, seed=5), ids=runs(B, L, seed=L) if packed else None, states=not packed)
+
+
 def test_every_position_its_own_sequence_and_only_padding():
     p = make(2, 6, 300, 16, 1, FP32)
     check(p, ids=torch.arange(300, dtype=torch.int32).repeat(2, 1))
