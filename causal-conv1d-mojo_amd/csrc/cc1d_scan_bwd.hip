@@ -486,30 +486,228 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
     }
 }
 
-// dB and dC: four positions per thread, the shares of the group's blocks in order.
-template <typename T> __global__ void __launch_bounds__(256) scan_bwd_reduce_bc(const ScanBwdArgs arg, int64_t items) {
+// Rows of at most 64 positions: a round of a block takes 32 channels. The LDS
+// sums have a copy for each of a wavefront's four channels, added at the end.
+template <typename T, bool SEQ, bool UNIT> __global__ void __launch_bounds__(512, 4) scan_bwd_short(const ScanBwdArgs arg) {
+    constexpr int K = kShortK, TILE = 64 * K;
+    __shared__ __attribute__((aligned(16))) float BC[2 * kStates * kShort];
+    __shared__ __attribute__((aligned(16))) float acc[2 * kStates * TILE];
+    const cc1d_scan_bwd_params& b = arg.p;
+    const cc1d_scan_params& p = b.fwd;
+    const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6), l = lane & 15, t = l * K;
+    const int end = (int)p.seqlen, N = (int)p.dstate;
+    const int64_t per = p.dim / p.groups;
+    const int64_t blk = blockIdx.x % arg.group_blocks, g = blockIdx.x / arg.group_blocks % p.groups, s = blockIdx.x / arg.group_blocks / p.groups;
+    const T* const Bp = static_cast<const T*>(p.B) + s * p.B_stride[0] + g * p.B_stride[1];
+    const T* const Cp = static_cast<const T*>(p.C) + s * p.C_stride[0] + g * p.C_stride[1];
+    float* const pBC = arg.pBC + ((s * p.groups + g) * arg.group_blocks + blk) * 2 * N * p.seqlen;
+    const int32_t* ids = SEQ ? p.seq_idx + s * p.seq_idx_stride[0] : nullptr;
+    const int64_t is = SEQ ? p.seq_idx_stride[1] : 0;
+    const int rounds = (int)(((per + 31) / 32 - blk + arg.group_blocks - 1) / arg.group_blocks);
+    ShortCuts cuts;
+    bool live[K];
+#pragma unroll
+    for (int j = 0; j < K; ++j) live[j] = t + j < end;
+    if constexpr (SEQ) cuts.read(ids, is, t, end, live);
+    else cuts.none();
+
+    // (more than 16 states: one round)
+    for (int round = 0; round < rounds; ++round) {
+        const int64_t in_group = (round * arg.group_blocks + blk) * 32 + threadIdx.x / 16;
+        const bool mine = in_group < per;  // a missing channel: the group's last one with u, dout and states 0
+        const int64_t d = g * per + (mine ? in_group : per - 1), sd = s * p.dim + d;
+        auto input = [&](Raw<T, K>& r, const void* base, const int64_t* stride) {
+            const T* row = static_cast<const T*>(base) + s * stride[0] + d * stride[1];
+            if constexpr (UNIT) r.load(row, t, end);
+            else r.each(row, stride[2], t, end);
+        };
+        Raw<T, K> ru, rd, rz, ro;
+        input(ru, p.u, p.u_stride);
+        input(rd, p.delta, p.delta_stride);
+        input(ro, b.dout, b.dout_stride);
+        if (p.z) input(rz, p.z, p.z_stride);
+        if constexpr (UNIT) {
+            ru.fix(t, end, end);
+            rd.fix(t, end, end);
+            ro.fix(t, end, end);
+            if (p.z) rz.fix(t, end, end);
+        }
+        const float bias = p.delta_bias ? p.delta_bias[d * p.delta_bias_stride] : 0.0f;
+        const float skip = p.D ? p.D[d * p.D_stride] : 0.0f;
+        float dt[K], du[K], dy[K], y[K], along[K], wsum[K], step_sum = 0.0f;
+        steps<K>(rd, bias, p.delta_softplus != 0, dt);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const bool in = mine && live[j];
+            dt[j] = live[j] ? dt[j] : 0.0f;
+            step_sum += dt[j];
+            du[j] = in ? dt[j] * ru.get(j) : 0.0f;
+            dy[j] = in ? ro.get(j) : 0.0f;
+            if (p.z && in) dy[j] *= silu(rz.get(j));
+            y[j] = along[j] = wsum[j] = 0.0f;
+        }
+        for (int n0 = 0; n0 < N; n0 += kStates) {
+            const int nn = N - n0 < kStates ? N - n0 : kStates;
+            float A_l = 0.0f, before_l = 0.0f, behind_l = 0.0f, dA_l = 0.0f, dinit_l = 0.0f;
+            if (l < nn) {
+                A_l = p.A[d * p.A_stride[0] + (n0 + l) * p.A_stride[1]];
+                if (mine) before_l = p.tile_states[sd * N + n0 + l];
+                if (mine && b.dfinal_states)
+                    behind_l = b.dfinal_states[s * b.dfinal_states_stride[0] + d * b.dfinal_states_stride[1] +
+                                               (n0 + l) * b.dfinal_states_stride[2]];
+            }
+            if (round == 0) {
+                __syncthreads();  // the last lot is done with
+                short_states<T>(BC, p, Bp, Cp, n0, nn, ids, is);
+                for (int i = threadIdx.x; i < 2 * kStates * TILE / 4; i += 512)
+                    reinterpret_cast<f32x4*>(acc)[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            __syncthreads();
+            const int turn = (nn + kWaves - 1) / kWaves;
+#pragma unroll 1
+            for (int i = 0; i < kWaves; ++i) {
+#pragma unroll 1
+                for (int k = 0; k < turn; ++k) {
+                    const int n = (i + wave) % kWaves * turn + k;
+                    if (n >= nn) break;
+                    float B[K], C[K], dB[K], dC[K], a[K], h[K];
+                    short_state(BC, n, l, B);
+                    short_state(BC, kStates + n, l, C);
+                    read_state<K>(acc, n, lane, dB);
+                    read_state<K>(acc + kStates * TILE, n, lane, dC);
+                    const float A = row_lane(A_l, n), A2 = A * kLog2e;
+                    const float before = row_lane(before_l, n), after = row_lane(behind_l, n);
+#pragma unroll
+                    for (int j = 0; j < K; ++j) a[j] = __builtin_amdgcn_exp2f(dt[j] * A2);
+                    float P = __builtin_amdgcn_exp2f(step_sum * A2), Pr = row_reverse(P);
+                    float H = du[0] * B[0];
+#pragma unroll
+                    for (int j = 1; j < K; ++j) {
+                        const float v = du[j] * B[j];
+                        H = SEQ && cuts.at[j] ? v : __builtin_fmaf(a[j], H, v);
+                    }
+                    float x = 0.0f;
+#pragma unroll
+                    for (int j = K - 1; j >= 0; --j) {
+                        x = a[j] * __builtin_fmaf(C[j], dy[j], x);
+                        if (SEQ && cuts.at[j]) x = 0.0f;
+                    }
+                    float Q = row_reverse(x);
+                    const float first = l == 0 ? before : 0.0f, behind = l == 0 ? after : 0.0f;
+                    const float Hin = __builtin_fmaf(P, first, H), Qin = __builtin_fmaf(Pr, behind, Q);
+                    H = SEQ && (cuts.met || l != 0) ? H : Hin;
+                    Q = SEQ && (cuts.met_back || l != 0) ? Q : Qin;
+                    if constexpr (SEQ) {
+                        row_prefix_cut(H, P, cuts.absorb);
+                        row_prefix_cut(Q, Pr, cuts.back);
+                    } else {
+                        row_prefix2(H, P, Q, Pr);
+                    }
+                    const float ahead = dpp_keep<kDppRowShr + 1, 0xf>(first, H);
+                    x = row_reverse(dpp_keep<kDppRowShr + 1, 0xf>(behind, Q));
+                    const float dinit = row_lane(Q, 15);
+                    float v = ahead;
+#pragma unroll
+                    for (int j = 0; j < K; ++j) {
+                        const float w = du[j] * B[j];
+                        v = SEQ && cuts.at[j] ? w : __builtin_fmaf(a[j], v, w);
+                        h[j] = v;
+                        y[j] = __builtin_fmaf(C[j], v, y[j]);
+                        dC[j] = __builtin_fmaf(dy[j], v, dC[j]);
+                    }
+                    float dA = 0.0f;
+#pragma unroll
+                    for (int j = K - 1; j >= 0; --j) {
+                        const float gr = __builtin_fmaf(C[j], dy[j], x);
+                        dB[j] = __builtin_fmaf(gr, du[j], dB[j]);
+                        along[j] = __builtin_fmaf(gr, B[j], along[j]);
+                        x = a[j] * gr;
+                        float w = x * (j > 0 ? h[j > 0 ? j - 1 : 0] : ahead);
+                        if (SEQ && cuts.at[j]) x = w = 0.0f;
+                        wsum[j] = __builtin_fmaf(A, w, wsum[j]);
+                        dA = __builtin_fmaf(dt[j], w, dA);
+                    }
+                    dA = lanes_sum<16>(dA);
+                    dA_l = l == n ? dA : dA_l;
+                    dinit_l = l == n ? dinit : dinit_l;
+                    *reinterpret_cast<f32x4*>(acc + (n * 64 + lane) * 4) = f32x4{dB[0], dB[1], dB[2], dB[3]};
+                    *reinterpret_cast<f32x4*>(acc + kStates * TILE + (n * 64 + lane) * 4) = f32x4{dC[0], dC[1], dC[2], dC[3]};
+                }
+                __syncthreads();
+            }
+            if (l < nn && mine) {
+                arg.pA[sd * N + n0 + l] = dA_l;
+                if (b.dinitial_states) b.dinitial_states[sd * N + n0 + l] = dinit_l;
+            }
+            if (round == rounds - 1) {
+                for (int i = threadIdx.x; i < 2 * nn * end; i += 512) {
+                    const int at = i % end, row = i / end, n = row < nn ? row : row - nn;
+                    const float* sums = acc + (row < nn ? 0 : kStates * TILE) + (n * 64 + at / K) * 4 + at % K;
+                    pBC[((row < nn ? 0 : N) + n0 + n) * p.seqlen + at] = (sums[0] + sums[64]) + (sums[128] + sums[192]);
+                }
+            }
+        }
+        float dD = 0.0f, dbias = 0.0f;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const float u = live[j] ? ru.get(j) : 0.0f;
+            wsum[j] = __builtin_fmaf(u, along[j], wsum[j]);
+            along[j] = __builtin_fmaf(skip, dy[j], dt[j] * along[j]);
+            dD = __builtin_fmaf(dy[j], u, dD);
+            if (p.delta_softplus) wsum[j] *= live[j] ? sigmoid(rd.get(j) + bias) : 0.0f;
+            wsum[j] = live[j] ? wsum[j] : 0.0f;
+            dbias += wsum[j];
+            if (p.z) y[j] = live[j] ? ro.get(j) * __builtin_fmaf(skip, u, y[j]) * silu_grad(rz.get(j)) : 0.0f;
+        }
+        dD = lanes_sum<16>(dD);
+        dbias = lanes_sum<16>(dbias);
+        if (!mine) continue;
+        auto give = [&](void* base, const int64_t* stride, const float (&v)[K]) {
+            store_steps<T, K>(static_cast<T*>(base) + s * stride[0] + d * stride[1], UNIT ? 1 : stride[2], t, end, v);
+        };
+        give(b.du, b.du_stride, along);
+        give(b.ddelta, b.ddelta_stride, wsum);
+        if (p.z) give(b.dz, b.dz_stride, y);
+        if (l == 0) {
+            arg.pD[sd] = dD;
+            arg.pbias[sd] = dbias;
+        }
+    }
+}
+
+// dB and dC: four positions per thread, the shares of the group's blocks in
+// order; where that leaves the card idle, `split` threads take every split-th
+// share each (1 x 6137 x 7, 8 states: 192 shares for 28 threads took 108 us).
+template <typename T> __global__ void __launch_bounds__(256) scan_bwd_reduce_bc(const ScanBwdArgs arg, int64_t items, int split) {
+    __shared__ f32x4 parts[256];
     const cc1d_scan_params& p = arg.p.fwd;
     const int64_t quads = (p.seqlen + 3) / 4;
-    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= items) return;
+    const int wide = 256 / split, part = (int)threadIdx.x / wide;
+    const int64_t idx = (int64_t)blockIdx.x * wide + threadIdx.x % wide;
     const int64_t t = idx % quads * 4, row = idx / quads, n2 = row % (2 * p.dstate), rg = row / (2 * p.dstate);
-    const int64_t lo = p.cu_seqlens ? clamp_pos(p.cu_seqlens[0], p.seqlen) : 0;
-    const int64_t hi = p.cu_seqlens ? clamp_pos(p.cu_seqlens[p.num_seqs], p.seqlen) : p.seqlen;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int have = idx < items ? (int)(p.seqlen - t < 4 ? p.seqlen - t : 4) : 0;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     const float* from = arg.pBC + (rg * arg.group_blocks * 2 * p.dstate + n2) * p.seqlen + t;
     const int64_t step = 2 * p.dstate * p.seqlen;
-    const int have = (int)(p.seqlen - t < 4 ? p.seqlen - t : 4);
     if (have == 4) {
 #pragma unroll 4
-        for (int64_t k = 0; k < arg.group_blocks; ++k) {
+        for (int64_t k = part; k < arg.group_blocks; k += split) {
             const u32x4 v = *reinterpret_cast<const AnyAddr<4>::v4*>(from + k * step);
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum[j] += __uint_as_float(v[j]);
         }
     } else {
-        for (int64_t k = 0; k < arg.group_blocks; ++k)
+        for (int64_t k = part; k < arg.group_blocks; k += split)
             for (int j = 0; j < have; ++j) sum[j] += from[k * step + j];
     }
+    if (split > 1) {
+        parts[threadIdx.x] = sum;
+        __syncthreads();
+        if (part > 0) return;
+        for (int k = 1; k < split; ++k) sum += parts[threadIdx.x + k * wide];
+    }
+    const int64_t lo = p.cu_seqlens ? clamp_pos(p.cu_seqlens[0], p.seqlen) : 0;
+    const int64_t hi = p.cu_seqlens ? clamp_pos(p.cu_seqlens[p.num_seqs], p.seqlen) : p.seqlen;
     T* to = static_cast<T*>(n2 < p.dstate ? arg.p.dB : arg.p.dC) + (rg * p.dstate + n2 % p.dstate) * p.seqlen + t;
     for (int j = 0; j < have; ++j) to[j] = from_f32<T>(t + j >= lo && t + j < hi ? sum[j] : 0.0f);
 }
@@ -554,6 +752,10 @@ struct BwdPlan {
 // have the fewest shares to add. More than 16 states: one round.
 BwdPlan bwd_plan(const cc1d_scan_params& p) {
     const int64_t per = p.dim / p.groups, rows = scan_sequences(p) * p.groups;
+    if (scan_is_short(p)) {  // rounds once 1024 blocks (four wavefronts a SIMD, twice over) have some
+        const int64_t blocks = ceil_div(per, 32), r = p.dstate > kStates ? 1 : ceil_div(rows * blocks, 1024);
+        return {0, (int)(r < blocks ? r : blocks), ceil_div(blocks, r)};
+    }
     BwdPlan best{0, 0, 0};
     int64_t least = 0;
     for (int r = 1; r <= (p.dstate > kStates ? 1 : 8); ++r)
@@ -592,6 +794,19 @@ template <typename T, int K> int launch_rows(const ScanBwdArgs& a, int chw, hipS
     });
 }
 
+template <typename T> int launch_short(const ScanBwdArgs& a, hipStream_t stream) {
+    const cc1d_scan_bwd_params& b = a.p;
+    const cc1d_scan_params& p = b.fwd;
+    const dim3 grid((unsigned)(a.group_blocks * p.groups * p.batch)), block(512);
+    const bool unit = p.seqlen >= kShortK && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && b.dout_stride[2] == 1 &&
+                      b.du_stride[2] == 1 && b.ddelta_stride[2] == 1 && (!p.z || (p.z_stride[2] == 1 && b.dz_stride[2] == 1));
+    return with_flag(p.seq_idx != nullptr, [&](auto seq) {
+        return with_flag(unit, [&](auto un) {
+            return launch(scan_bwd_short<T, decltype(seq)::value, decltype(un)::value>, grid, block, stream, a);
+        });
+    });
+}
+
 }  // namespace
 
 int64_t scan_bwd_workspace_floats(const cc1d_scan_bwd_params& b) {
@@ -614,13 +829,16 @@ int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
     a.pbias = a.pD + seqs * p.dim;
     a.pBC = a.pbias + seqs * p.dim;
     const int64_t items = p.batch * p.groups * 2 * p.dstate * ceil_div(p.seqlen, 4);
+    int split = 1;
+    while (split < 32 && items * split < 262144 && a.group_blocks >= 4 * split) split *= 2;
     return with_dtype(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         int st = CC1D_OK;
-        if (seqs > 0)
+        if (scan_is_short(p)) st = launch_short<T>(a, stream);
+        else if (seqs > 0)
             st = scan_tile(p.seqlen) == 512 ? launch_rows<T, 8>(a, plan.chw, stream) : launch_rows<T, 4>(a, plan.chw, stream);
         if (st == CC1D_OK && items > 0)
-            st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)ceil_div(items, 256)), dim3(256), stream, a, items);
+            st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)ceil_div(items * split, 256)), dim3(256), stream, a, items, split);
         if (st == CC1D_OK)
             st = launch(scan_bwd_reduce_params, dim3((unsigned)ceil_div(p.dim * (p.dstate + 2), 256)), dim3(256), stream,
                         a, seqs);

@@ -69,6 +69,13 @@ inline int64_t scan_slots(const cc1d_scan_params& p) {
     return p.cu_seqlens != nullptr ? p.seqlen / tile + p.num_seqs : p.batch * ceil_div(p.seqlen, tile);
 }
 
+constexpr int kShort = 64, kShortK = 4;
+
+// Rows for the kernels of four channels a wavefront.
+inline bool scan_is_short(const cc1d_scan_params& p) {
+    return p.cu_seqlens == nullptr && p.batch * p.dim > 0 && p.seqlen >= 1 && p.seqlen <= kShort;
+}
+
 // dt of a lane's positions
 template <int K, typename R> __device__ __forceinline__ void steps(const R& raw, float bias, bool soft, float (&dt)[K]) {
 #pragma unroll
@@ -187,7 +194,85 @@ __device__ __forceinline__ void wave_prefix_cut(float& H, float& P, const bool (
     CC1D_CUT_LEVEL(3, kDppRowShr + 8, 0xf)
     CC1D_CUT_LEVEL(4, kDppRowBcast15, 0xa)
     CC1D_CUT_LEVEL(5, kDppRowBcast31, 0xc)
-#undef CC1D_CUT_LEVEL
+}
+
+// Rows of at most 64 positions: a wavefront takes four channels, 16 lanes of 4
+// positions each, instead of one whose positions leave most lanes idle (bf16, 16
+// states, 8 x 4096 x 64: 32 us forward and 74 backward instead of 79 and 210; at
+// 14 x 6016 x 11 with 64 states 128 and 335 instead of 483 and 1718). What
+// is one channel's in the kernels above is 16 lanes' there: prefixes end after
+// four levels, and lane l holds what belongs to state l of 16.
+__device__ __forceinline__ float row_lane(float v, int n) { return __shfl(v, (threadIdx.x & 48) | n); }  // of the 16 lanes
+__device__ __forceinline__ float row_reverse(float v) { return dpp_f32<0x140, 0xf>(v); }
+__device__ __forceinline__ void row_prefix(float& H, float& P) {
+    asm("s_nop 1\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("1")) CC1D_SCAN_DECAY("%1", CC1D_ROW("1")) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("2")) CC1D_SCAN_DECAY("%1", CC1D_ROW("2")) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("4")) CC1D_SCAN_DECAY("%1", CC1D_ROW("4")) "s_nop 0\n\t"
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("8")) "s_nop 1"
+        : "+v"(H), "+v"(P));
+}
+__device__ __forceinline__ void row_prefix2(float& H0, float& P0, float& H1, float& P1) {
+#define CC1D_BOTH(CTRL) \
+    CC1D_SCAN_LEVEL("%0", "%1", CTRL) CC1D_SCAN_LEVEL("%2", "%3", CTRL) CC1D_SCAN_DECAY("%1", CTRL) CC1D_SCAN_DECAY("%3", CTRL)
+    asm("s_nop 1\n\t"
+        CC1D_BOTH(CC1D_ROW("1")) CC1D_BOTH(CC1D_ROW("2")) CC1D_BOTH(CC1D_ROW("4"))
+        CC1D_SCAN_LEVEL("%0", "%1", CC1D_ROW("8")) CC1D_SCAN_LEVEL("%2", "%3", CC1D_ROW("8")) "s_nop 1"
+        : "+v"(H0), "+v"(P0), "+v"(H1), "+v"(P1));
+#undef CC1D_BOTH
+}
+struct ShortCuts {
+    bool at[kShortK], met, met_back, absorb[4], back[4];
+
+    __device__ __forceinline__ void none() {
+        met = met_back = false;
+#pragma unroll
+        for (int j = 0; j < kShortK; ++j) at[j] = false;
+    }
+    // ids of the row; t the lane's first position
+    __device__ __forceinline__ void read(const int32_t* ids, int64_t stride, int t, int end, bool (&live)[kShortK]) {
+        const int l = threadIdx.x & 15;
+        int32_t prev = t > 0 && t < end ? ids[(t - 1) * stride] : 0;
+        met = false;
+#pragma unroll
+        for (int j = 0; j < kShortK; ++j) {
+            const int32_t id = t + j < end ? ids[(t + j) * stride] : prev;
+            at[j] = t + j < end && (id != prev || t + j == 0);
+            live[j] = t + j < end && id >= 0;
+            met |= at[j];
+            prev = id;
+        }
+        const uint32_t m = (uint32_t)__ballot(met) & 0xffffu, r = __builtin_bitreverse32(m) >> 16, mask = (2u << l) - 1;
+        const int last = (m & mask) ? 31 - __builtin_clz(m & mask) : -1, next = (r & mask) ? 31 - __builtin_clz(r & mask) : -1;
+        met_back = r >> l & 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            absorb[i] = last + (1 << i) <= l;
+            back[i] = next + (1 << i) <= l;
+        }
+    }
+};
+__device__ __forceinline__ void row_prefix_cut(float& H, float& P, const bool (&absorb)[4]) {
+    CC1D_CUT_LEVEL(0, kDppRowShr + 1, 0xf)
+    CC1D_CUT_LEVEL(1, kDppRowShr + 2, 0xf)
+    CC1D_CUT_LEVEL(2, kDppRowShr + 4, 0xf)
+    CC1D_CUT_LEVEL(3, kDppRowShr + 8, 0xf)
+}
+// B and C of states n0 .. n0 + nn - 1 (nn <= 16) of a short row to LDS, [B, C][state][position], by 512 threads.
+template <typename T>
+__device__ __forceinline__ void short_states(float* lds, const cc1d_scan_params& p, const T* B, const T* C, int n0, int nn,
+                                             const int32_t* ids, int64_t id_stride) {
+    for (int i = threadIdx.x; i < 2 * nn * kShort; i += 512) {
+        const int t = i % kShort, row = i / kShort, n = row < nn ? row : row - nn;
+        const bool in = t < (int)p.seqlen && (ids == nullptr || ids[t * id_stride] >= 0);
+        const T* at = row < nn ? B + (n0 + n) * p.B_stride[2] + t * p.B_stride[3] : C + (n0 + n) * p.C_stride[2] + t * p.C_stride[3];
+        lds[((row < nn ? 0 : 16) + n) * kShort + t] = in ? to_f32(*at) : 0.0f;
+    }
+}
+__device__ __forceinline__ void short_state(const float* lds, int n, int l, float (&v)[kShortK]) {
+    const f32x4 w = *reinterpret_cast<const f32x4*>(lds + n * kShort + 4 * l);
+#pragma unroll
+    for (int j = 0; j < kShortK; ++j) v[j] = w[j];
 }
 
 // A block's B and C of up to 16 states of a tile, fp32 in LDS as [B, C]

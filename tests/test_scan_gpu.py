@@ -129,7 +129,8 @@ def test_packed_rows(size, layout, dtype):
 # More channels than the card takes at once: two a wavefront, and several rounds, in the backward's blocks.
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("layout", ["rows", "last", "odd"])
-@pytest.mark.parametrize("size", [(1, 4100, 21, 16, 1), (1, 4107, 520, 5, 1), (2, 1030, 300, 9, 1), (2, 4104, 21, 17, 2)],
+@pytest.mark.parametrize("size", [(1, 4100, 21, 16, 1), (1, 4107, 520, 5, 1), (2, 1030, 300, 9, 1), (2, 4104, 21, 17, 2),
+                                  (9, 4100, 6, 3, 1)],
                          ids=str)
 @pytest.mark.parametrize("packed", [False, True], ids=["plain", "packed"])
 def test_many_channels(packed, size, layout, dtype):
