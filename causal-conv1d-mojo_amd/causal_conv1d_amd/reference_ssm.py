@@ -1,6 +1,6 @@
 """Plain PyTorch formulations of the scan, its decode step and the norm
 (``ssm_scan_ref``, ``ssm_scan_update_ref``, ``add_norm_ref``), for callers that
-want a checker: the recurrence position by position, on any device, in fp32 or
+want to compare results: the recurrence position by position, on any device, in fp32 or
 in the inputs' dtype where that is wider. Autograd runs through them. The
 package's kernels never call them.
 """
