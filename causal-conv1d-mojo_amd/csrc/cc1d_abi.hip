@@ -223,7 +223,13 @@ int cc1d_scan_bwd(const cc1d_scan_bwd_params* b, void* stream) {
     const int st = check_scan(p);
     if (st != CC1D_OK) return st;
     if (p.seq_idx != nullptr && (b->dfinal_states != nullptr || b->dinitial_states != nullptr)) return CC1D_ERR_EXCLUSIVE;
-    if (p.dim == 0) return CC1D_OK;
+    if (p.dim == 0) {  // no channel adds to dB and dC
+        const int64_t rows = p.batch * p.groups, strides[3] = {p.dstate * p.seqlen, p.seqlen, 1};
+        if (rows * p.seqlen > 0 && (b->dB == nullptr || b->dC == nullptr)) return CC1D_ERR_NULL_POINTER;
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        const int zeroed = launch_zero3(b->dB, esize(p.dtype), rows, p.dstate, p.seqlen, strides, s);
+        return zeroed != CC1D_OK ? zeroed : launch_zero3(b->dC, esize(p.dtype), rows, p.dstate, p.seqlen, strides, s);
+    }
     if (b->dA == nullptr || p.A == nullptr) return CC1D_ERR_NULL_POINTER;
     if (p.batch * p.seqlen > 0 &&
         (p.u == nullptr || p.delta == nullptr || p.B == nullptr || p.C == nullptr || p.tile_states == nullptr ||

@@ -227,6 +227,19 @@ def test_no_positions():
         assert all((got[k] == 0).all() for k in ("dA", "dD", "dbias"))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("prompts", [False, True])
+def test_no_channels(prompts, dtype):
+    """B and C of a layer without channels have gradients, of zeros."""
+    p = make(1 if prompts else 2, 0, 700, 16, 2, dtype)
+    for _ in range(4):  # (what their memory held before is not zeros)
+        torch.full_like(p["B"], float("nan"))
+    kw = {"cu_seqlens": torch.tensor([0, 300, 700], dtype=torch.int32, device=DEV)} if prompts else {}
+    got = own(p, True, **kw)
+    for k in ("dB", "dC"):
+        assert got[k].shape == p["B"].shape and (got[k] == 0).all(), k
+
+
 def test_extreme_steps():
     """Decays that underflow to 0, steps of 0 (a state that stays), large raw steps, growing states."""
     p = make(1, 16, 600, 16, 1, FP32, seed=9)

@@ -271,6 +271,20 @@ def test_scan_bwd_needs_its_workspace():
     assert lib.cc1d_scan_bwd(ctypes.byref(b), None) == 1
 
 
+def test_scan_bwd_without_channels_still_has_dB_and_dC():
+    """No channel adds to dB and dC: they are zeros to be written, not buffers to be left as they are."""
+    b = _lib.ScanBwdParams()
+    b.fwd = _scan(dim=0)
+    lib = _lib.load()
+    assert lib.cc1d_scan_bwd_workspace_floats(ctypes.byref(b)) == 0
+    assert lib.cc1d_scan_bwd(ctypes.byref(b), None) == 1  # nowhere to write them
+    b.dB = 16
+    assert lib.cc1d_scan_bwd(ctypes.byref(b), None) == 1
+    for kw in ({"seqlen": 0}, {"batch": 0}):  # no values of B either
+        b.fwd = _scan(dim=0, **kw)
+        assert lib.cc1d_scan_bwd(ctypes.byref(b), None) == 0
+
+
 @pytest.mark.parametrize("code,kw", [(2, {"dtype": 3}), (10, {"dstate": 257}), (11, {"groups": 3}),
                                      (4, {"state_rows": 0}), (1, {}), (0, {"batch": 0}), (0, {"seqlen": 0})])
 def test_scan_update_codes(code, kw):
