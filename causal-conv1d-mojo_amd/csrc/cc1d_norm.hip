@@ -341,7 +341,9 @@ int64_t norm_bwd_workspace_floats(const cc1d_norm_bwd_params& b) {
 
 int launch_norm_fwd(const cc1d_norm_params& p, hipStream_t stream) {
     const NormPlan n = norm_plan(p.dim);
-    const dim3 grid((unsigned)ceil_div(p.rows, n.slots())), block(64 * n.waves);
+    // a turn for all rows, or as many of them as a launch has threads for
+    const int64_t blocks = ceil_div(p.rows, n.slots()), most = UINT32_MAX / (64 * n.waves);
+    const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(64 * n.waves);
     return with_norm_types(p, [&](auto t, auto r) {
         return with_plan(p, n, [&](auto steps, auto lpr, auto even) {
             return launch(norm_fwd_kernel<decltype(t), decltype(r), decltype(steps)::value, decltype(lpr)::value,

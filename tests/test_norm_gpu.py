@@ -141,6 +141,22 @@ def test_past_32_bits():
     assert torch.equal(out[-2:], cc.add_norm_fn(p["x"], p["weight"], p["bias"]))
 
 
+def test_more_rows_than_one_turn_of_the_grid():
+    """Eight lanes a row: 2**29 rows are more threads than a launch counts, and blocks take several turns."""
+    rows = (1 << 29) + 3
+    x = torch.randn(4099, 1, device=DEV).bfloat16().repeat(rows // 4099 + 1, 1)[:rows].requires_grad_()
+    w, b = torch.tensor([1.5], device=DEV), torch.tensor([0.25], device=DEV)
+    y = cc.add_norm_fn(x, w, b, rms=True)
+    few = x.detach()[:4099].requires_grad_()
+    want = cc.add_norm_fn(few, w, b, rms=True)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    dwant, = torch.autograd.grad(want, few, few.detach())
+    for got, exact in ((y, want), (dx, dwant)):
+        for part in got.split(1 << 26):
+            at = part.storage_offset() % 4099
+            assert torch.equal(part, exact.roll(-at, 0).repeat(part.shape[0] // 4099 + 1, 1)[:part.shape[0]])
+
+
 def test_graph_compile_and_side_stream():
     p = make(33, 2560, BF16, "fp32")
     want = own(p)
