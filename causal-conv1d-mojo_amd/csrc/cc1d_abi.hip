@@ -65,7 +65,8 @@ int check_scan(const cc1d_scan_params& p) {
     if (p.cu_seqlens != nullptr && (p.batch != 1 || p.num_seqs < 0 || (p.num_seqs == 0 && p.seqlen > 0)))
         return CC1D_ERR_SHAPE;
     const int64_t seqs = p.cu_seqlens != nullptr ? p.num_seqs : p.batch;
-    // a block per sequence and channel at most, a thread per value of dB and dC, 32-bit positions
+    // a block per sequence and channel at most, a thread per value of dB and dC, 32-bit positions (launches check
+    // their threads, which depend on the kernel)
     const double blocks = (double)seqs * (double)p.dim;
     const double values = (double)p.batch * (double)p.groups * (double)p.dstate * (double)p.seqlen;
     if (blocks >= (double)kMaxBlocks || values / 256 + 1 >= (double)kMaxBlocks || p.seqlen >= ((int64_t)1 << 31) - 4096)

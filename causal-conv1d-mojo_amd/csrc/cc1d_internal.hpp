@@ -69,6 +69,9 @@ template <typename F> int with_flag(bool flag, F&& f) {
     return flag ? f(std::true_type{}) : f(std::false_type{});
 }
 
+// The runtime counts a launch's threads along an axis in 32 bits.
+inline bool threads_fit(int64_t blocks, int64_t threads) { return blocks * threads <= (int64_t)UINT32_MAX; }
+
 // Launches kernel k with the given arguments (converted to its parameter
 // types) and returns the status of this launch alone: hipLaunchKernel reports
 // it directly, so an error that an earlier, unrelated call left on the thread
@@ -77,6 +80,7 @@ template <typename F> int with_flag(bool flag, F&& f) {
 template <typename... P, typename... A>
 int launch(void (*k)(P...), dim3 grid, dim3 block, hipStream_t stream, const A&... args) {
     static_assert(sizeof...(P) == sizeof...(A), "one argument per kernel parameter");
+    if (!threads_fit(grid.x, block.x) || !threads_fit(grid.y, block.y)) return CC1D_ERR_SHAPE;
     std::tuple<std::decay_t<P>...> vals(args...);
     void* ptrs[sizeof...(P)];
     std::apply([&](auto&... v) {

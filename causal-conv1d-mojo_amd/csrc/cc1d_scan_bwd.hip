@@ -831,6 +831,10 @@ int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
     const int64_t items = p.batch * p.groups * 2 * p.dstate * ceil_div(p.seqlen, 4);
     int split = 1;
     while (split < 32 && items * split < 262144 && a.group_blocks >= 4 * split) split *= 2;
+    const int64_t blocks = a.group_blocks * p.groups * seqs, bc_blocks = ceil_div(items * split, 256),
+                  param_blocks = ceil_div(p.dim * (p.dstate + 2), 256);
+    if (!threads_fit(blocks, 64 * kWaves) || !threads_fit(bc_blocks, 256) || !threads_fit(param_blocks, 256))
+        return CC1D_ERR_SHAPE;  // before any of them runs
     return with_dtype(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         int st = CC1D_OK;
@@ -838,10 +842,9 @@ int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
         else if (seqs > 0)
             st = scan_tile(p.seqlen) == 512 ? launch_rows<T, 8>(a, plan.chw, stream) : launch_rows<T, 4>(a, plan.chw, stream);
         if (st == CC1D_OK && items > 0)
-            st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)ceil_div(items * split, 256)), dim3(256), stream, a, items, split);
+            st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)bc_blocks), dim3(256), stream, a, items, split);
         if (st == CC1D_OK)
-            st = launch(scan_bwd_reduce_params, dim3((unsigned)ceil_div(p.dim * (p.dstate + 2), 256)), dim3(256), stream,
-                        a, seqs);
+            st = launch(scan_bwd_reduce_params, dim3((unsigned)param_blocks), dim3(256), stream, a, seqs);
         return st;
     });
 }

@@ -259,6 +259,34 @@ def test_scan_codes(code, kw):
         assert lib.cc1d_scan_bwd(ctypes.byref(b), None) == code
 
 
+@pytest.mark.parametrize("kw", [{"batch": 1 << 16, "dim": 4096},  # rows of 16 positions: 32 channels a block of 512 threads
+                                {"num_seqs": 1 << 14, "cu_seqlens": 16, "dim": 4096, "seqlen": 512},
+                                {"batch": 1 << 14, "dim": 4096, "seqlen": 100}], ids=["short", "packed", "rows"])
+def test_scans_of_more_threads_than_a_launch_has_are_refused(kw):
+    """A launch counts its threads in 32 bits: what has more is refused as a shape, before anything runs."""
+    lib = _lib.load()
+    p = _scan(u=16, delta=16, A=16, B=16, C=16, out=16, tile_states=16, **kw)
+    assert lib.cc1d_scan_fwd(ctypes.byref(p), None) == 4
+
+
+def test_scan_bwd_of_more_threads_than_a_launch_has_is_refused():
+    lib = _lib.load()
+    b = _lib.ScanBwdParams()
+    for k in ("dout", "du", "ddelta", "dA", "dB", "dC", "workspace"):
+        setattr(b, k, 16)
+    b.workspace_floats = 1 << 62
+    b.fwd = _scan(u=16, delta=16, A=16, B=16, C=16, tile_states=16, dim=1 << 25, dstate=256, seqlen=4)
+    assert lib.cc1d_scan_bwd(ctypes.byref(b), None) == 4  # a thread per channel and state of dA
+
+
+def test_scan_update_of_more_threads_than_a_launch_has_is_refused():
+    p = _lib.ScanUpdateParams()
+    p.batch, p.dim, p.seqlen, p.dstate, p.groups, p.state_rows, p.dtype = 1 << 18, 4096, 1, 16, 1, 1 << 18, 1
+    for k in ("u", "delta", "A", "B", "C", "ssm_state", "out"):
+        setattr(p, k, 16)
+    assert _lib.load().cc1d_scan_update(ctypes.byref(p), None) == 4
+
+
 def test_scan_bwd_needs_its_workspace():
     b = _lib.ScanBwdParams()
     b.fwd = _scan(u=16, delta=16, A=16, B=16, C=16, tile_states=16)
