@@ -126,6 +126,42 @@ def test_packed_rows(size, layout, dtype):
     check(make(B, D, L, N, G, dtype, layout, seed=3), ids=runs(B, L, seed=L))
 
 
+def relay(p, layout, *names):
+    """p with some of its tensors laid out another way."""
+    return {**p, **{k: lay(p[k], layout) for k in names}}
+
+
+@pytest.mark.parametrize("packed", [False, True], ids=["plain", "packed"])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("pair", [("rows", "last"), ("last", "rows"), ("slice", "last"), ("last", "slice"), ("rows", "odd"),
+                                  ("last", "odd")], ids="+".join)
+@pytest.mark.parametrize("size", [(2, 20, 200, 16, 2), (1, 9, 1100, 24, 1), (1, 34, 60, 9, 2), (2, 40, 650, 16, 1)], ids=str)
+def test_layout_pairs(size, pair, dtype, packed):
+    """u, delta, z and dout one way, B and C another (as slices of a projection are beside rows from the convolution)."""
+    B, D, L, N, G = size
+    p = relay(make(B, D, L, N, G, dtype, pair[0], seed=L), pair[1], "B", "C")
+    check(p, ids=runs(B, L, seed=D) if packed else None, states=not packed)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("bc", ["last", "rows"])
+@pytest.mark.parametrize("size", [(1, 17, 300, 200, 1), (2, 9, 530, 131, 1), (1, 24, 90, 256, 2)], ids=str)
+def test_channel_last_with_many_states(size, bc, dtype):
+    B, D, L, N, G = size
+    check(relay(make(B, D, L, N, G, dtype, "last", seed=N), bc, "B", "C"), states=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("base", ["rows", "last"])
+@pytest.mark.parametrize("other", ["u", "delta", "z", "dout", "C"])
+@pytest.mark.parametrize("size", [(2, 20, 200, 16, 2), (1, 18, 600, 20, 1)], ids=str)
+def test_one_tensor_lies_otherwise(size, other, base, dtype):
+    B, D, L, N, G = size
+    p = make(B, D, L, N, G, dtype, base, seed=L)
+    for layout in ("last" if base == "rows" else "rows", "odd"):
+        check(relay(p, layout, other), states=True)
+
+
 # More channels than the card takes at once: two a wavefront, and several rounds, in the backward's blocks.
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("layout", ["rows", "last", "odd"])
@@ -136,6 +172,15 @@ def test_packed_rows(size, layout, dtype):
 def test_many_channels(packed, size, layout, dtype):
     B, D, L, N, G = size
     check(make(B, D, L, N, G, dtype, layout, seed=5), ids=runs(B, L, seed=L) if packed else None, states=not packed)
+
+
+@pytest.mark.parametrize("packed", [False, True], ids=["plain", "packed"])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("pair", [("rows", "last"), ("last", "rows")], ids="+".join)
+@pytest.mark.parametrize("L", [200, 520])
+def test_layout_pairs_of_many_channels(L, pair, dtype, packed):
+    p = relay(make(1, 4107, L, 9, 1, dtype, pair[0], seed=L), pair[1], "B", "C")
+    check(p, ids=runs(1, L, seed=L) if packed else None, states=not packed)
 
 
 def test_every_position_its_own_sequence_and_only_padding():
