@@ -14,9 +14,12 @@ struct ScanBwdArgs {
     float* carry;        // (sequences, dim, dstate): a g of the position after the tile being worked on
     float* pA;           // (sequences, dim, dstate)
     float *pD, *pbias;   // (sequences, dim)
-    float* pBC;          // (batch, groups, group_blocks, [B, C], dstate, seqlen): each block's share of dB and dC
+    float* pBC;          // (rows, groups, group_blocks, [B, C], dstate, span): each block's share of dB and dC
     int64_t group_blocks;
-    int rounds;          // times a block takes its wavefronts' channels, in every tile
+    // What this launch works on: rows (sequences) from `first` on, and of each its tiles tile0 .. tile1 - 1, which
+    // are positions from t0 on, `span` at most.
+    int64_t first, t0, span;
+    int tile0, tile1;
 };
 
 template <typename T> __device__ void zero_uncovered(const cc1d_scan_bwd_params& p, int64_t d, int64_t from, int64_t to) {
@@ -161,13 +164,13 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
     const int64_t per = p.dim / p.groups;
     const uint32_t order = xcd_block(blockIdx.x, gridDim.x);
     const int64_t blk = order % arg.group_blocks, grp = order / arg.group_blocks % p.groups,
-                  s = order / arg.group_blocks / p.groups;
+                  s = arg.first + order / arg.group_blocks / p.groups;
     const ScanSpan q = scan_span(p, s, TILE);
     const int N = (int)p.dstate;
     const int begin = (int)q.start, end = (int)(q.start + q.len), size = (int)p.seqlen;
     const T* Bp = static_cast<const T*>(p.B) + q.row * p.B_stride[0] + grp * p.B_stride[1];
     const T* Cp = static_cast<const T*>(p.C) + q.row * p.C_stride[0] + grp * p.C_stride[1];
-    float* pBC = arg.pBC + ((q.row * p.groups + grp) * arg.group_blocks + blk) * 2 * N * p.seqlen;
+    float* pBC = arg.pBC + (((q.row - arg.first) * p.groups + grp) * arg.group_blocks + blk) * 2 * N * arg.span;
     const int32_t* ids = SEQ ? p.seq_idx + q.row * p.seq_idx_stride[0] : nullptr;
     const int64_t is = SEQ ? p.seq_idx_stride[1] : 0;
     const int tiles = (int)((q.len + TILE - 1) / TILE);
@@ -195,7 +198,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
         }
     }
 
-    for (int tile = tiles - 1; tile >= 0; --tile) {
+    for (int tile = (tiles < arg.tile1 ? tiles : arg.tile1) - 1; tile >= arg.tile0; --tile) {
         const int t0 = begin + tile * TILE, t = t0 + lane * K;
         const bool full = end - t0 >= TILE, last = tile == tiles - 1;
         Cuts<K> cuts;
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const S
                         if (n >= nn) continue;
                         float v[K];
                         read_state<K>(acc, row, lane, v);
-                        float* to = pBC + ((row / kStates) * N + n0 + n) * p.seqlen + t;
+                        float* to = pBC + ((row / kStates) * N + n0 + n) * arg.span + (t - arg.tile0 * TILE);
                         if (t + K <= end) {
 #pragma unroll
                             for (int k = 0; k < K / 4; ++k)
@@ -497,10 +500,11 @@ template <typename T, bool SEQ, bool UNIT> __global__ void __launch_bounds__(512
     const int lane = threadIdx.x & 63, wave = (int)uniform32(threadIdx.x >> 6), l = lane & 15, t = l * K;
     const int end = (int)p.seqlen, N = (int)p.dstate;
     const int64_t per = p.dim / p.groups;
-    const int64_t blk = blockIdx.x % arg.group_blocks, g = blockIdx.x / arg.group_blocks % p.groups, s = blockIdx.x / arg.group_blocks / p.groups;
+    const int64_t blk = blockIdx.x % arg.group_blocks, g = blockIdx.x / arg.group_blocks % p.groups,
+                  row = blockIdx.x / arg.group_blocks / p.groups, s = arg.first + row;
     const T* const Bp = static_cast<const T*>(p.B) + s * p.B_stride[0] + g * p.B_stride[1];
     const T* const Cp = static_cast<const T*>(p.C) + s * p.C_stride[0] + g * p.C_stride[1];
-    float* const pBC = arg.pBC + ((s * p.groups + g) * arg.group_blocks + blk) * 2 * N * p.seqlen;
+    float* const pBC = arg.pBC + ((row * p.groups + g) * arg.group_blocks + blk) * 2 * N * p.seqlen;
     const int32_t* ids = SEQ ? p.seq_idx + s * p.seq_idx_stride[0] : nullptr;
     const int64_t is = SEQ ? p.seq_idx_stride[1] : 0;
     const int rounds = (int)(((per + 31) / 32 - blk + arg.group_blocks - 1) / arg.group_blocks);
@@ -675,20 +679,20 @@ template <typename T, bool SEQ, bool UNIT> __global__ void __launch_bounds__(512
     }
 }
 
-// dB and dC: four positions per thread, the shares of the group's blocks in
-// order; where that leaves the card idle, `split` threads take every split-th
+// dB and dC of the launch's rows and positions (`count` of them): four positions
+// per thread, the shares of the group's blocks in order; where that leaves the card idle, `split` threads take every split-th
 // share each (1 x 6137 x 7, 8 states: 192 shares for 28 threads took 108 us).
-template <typename T> __global__ void __launch_bounds__(256) scan_bwd_reduce_bc(const ScanBwdArgs arg, int64_t items, int split) {
+template <typename T> __global__ void __launch_bounds__(256) scan_bwd_reduce_bc(const ScanBwdArgs arg, int64_t items, int64_t count, int split) {
     __shared__ f32x4 parts[256];
     const cc1d_scan_params& p = arg.p.fwd;
-    const int64_t quads = (p.seqlen + 3) / 4;
+    const int64_t quads = (count + 3) / 4;
     const int wide = 256 / split, part = (int)threadIdx.x / wide;
     const int64_t idx = (int64_t)blockIdx.x * wide + threadIdx.x % wide;
     const int64_t t = idx % quads * 4, row = idx / quads, n2 = row % (2 * p.dstate), rg = row / (2 * p.dstate);
-    const int have = idx < items ? (int)(p.seqlen - t < 4 ? p.seqlen - t : 4) : 0;
+    const int have = idx < items ? (int)(count - t < 4 ? count - t : 4) : 0;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    const float* from = arg.pBC + (rg * arg.group_blocks * 2 * p.dstate + n2) * p.seqlen + t;
-    const int64_t step = 2 * p.dstate * p.seqlen;
+    const float* from = arg.pBC + (rg * arg.group_blocks * 2 * p.dstate + n2) * arg.span + t;
+    const int64_t step = 2 * p.dstate * arg.span;
     if (have == 4) {
 #pragma unroll 4
         for (int64_t k = part; k < arg.group_blocks; k += split) {
@@ -708,8 +712,10 @@ template <typename T> __global__ void __launch_bounds__(256) scan_bwd_reduce_bc(
     }
     const int64_t lo = p.cu_seqlens ? clamp_pos(p.cu_seqlens[0], p.seqlen) : 0;
     const int64_t hi = p.cu_seqlens ? clamp_pos(p.cu_seqlens[p.num_seqs], p.seqlen) : p.seqlen;
-    T* to = static_cast<T*>(n2 < p.dstate ? arg.p.dB : arg.p.dC) + (rg * p.dstate + n2 % p.dstate) * p.seqlen + t;
-    for (int j = 0; j < have; ++j) to[j] = from_f32<T>(t + j >= lo && t + j < hi ? sum[j] : 0.0f);
+    const int64_t at = arg.t0 + t;
+    T* to = static_cast<T*>(n2 < p.dstate ? arg.p.dB : arg.p.dC) +
+            ((arg.first * p.groups + rg) * p.dstate + n2 % p.dstate) * p.seqlen + at;
+    for (int j = 0; j < have; ++j) to[j] = from_f32<T>(at + j >= lo && at + j < hi ? sum[j] : 0.0f);
 }
 
 // dA, dD and ddelta_bias: one thread per channel and state, and two more per channel; the sequences in order.
@@ -738,12 +744,26 @@ __global__ void __launch_bounds__(256) scan_bwd_reduce_params(const ScanBwdArgs 
     to[i] = sum;
 }
 
-// What a block takes: its wavefronts' channels at a time (1 or 2), and how many
-// rounds of them.
+// What a block takes: its wavefronts' channels at a time (1 or 2), and with
+// group_blocks how many rounds of them. What a launch takes: `rows` rows and
+// `tiles` tiles of each, `span` positions.
 struct BwdPlan {
-    int chw, rounds;
-    int64_t group_blocks;
+    int chw;
+    int64_t group_blocks, rows, tiles, span;
 };
+
+// `all` in parts of at most `most` (one at least), of about one size
+int64_t evenly(int64_t all, int64_t most) { return ceil_div(all, ceil_div(all, most > 1 ? most : 1)); }
+
+// The shares of dB and dC would otherwise grow with everything at once (17 GB
+// at 8 x 8192 x 4096 with 128 states, where u has 0.5), so a call of more than
+// this, 4 GiB, takes several launches, each followed by its sum: tiles from
+// the last to the first, which leaves every launch all rows, and where one
+// tile of all rows is too much, rows. That costs nothing (43.0 ms either way
+// at that size); parts of 1 GiB cost up to 5% (45.0 there), as fewer blocks
+// run beside each other at the end of each. Packed prompts (cu_seqlens) have
+// one row and lengths that only the device knows: one launch.
+constexpr double kShareFloats = 1 << 30;
 
 // A CU holds one block (128 KB of LDS), so the choice that leaves the card the
 // least to do one after the other; a round of one channel each takes about 2/3
@@ -754,9 +774,12 @@ BwdPlan bwd_plan(const cc1d_scan_params& p) {
     const int64_t per = p.dim / p.groups, rows = scan_sequences(p) * p.groups;
     if (scan_is_short(p)) {  // rounds once 1024 blocks (four wavefronts a SIMD, twice over) have some
         const int64_t blocks = ceil_div(per, 32), r = p.dstate > kStates ? 1 : ceil_div(rows * blocks, 1024);
-        return {0, (int)(r < blocks ? r : blocks), ceil_div(blocks, r)};
+        BwdPlan plan{0, ceil_div(blocks, r), p.batch, 1, p.seqlen};
+        const double row = 2.0 * p.groups * plan.group_blocks * p.dstate * p.seqlen;
+        if (p.batch * row > kShareFloats) plan.rows = evenly(p.batch, (int64_t)(kShareFloats / row));
+        return plan;
     }
-    BwdPlan best{0, 0, 0};
+    BwdPlan best{0, 0, p.batch, INT32_MAX, p.seqlen};
     int64_t least = 0;
     for (int r = 1; r <= (p.dstate > kStates ? 1 : 8); ++r)
         for (int chw = 1; chw <= 2; ++chw) {
@@ -764,16 +787,25 @@ BwdPlan bwd_plan(const cc1d_scan_params& p) {
             const int64_t cost = ceil_div(rows * blocks, 256) * r * (chw + 1);
             if (best.chw == 0 || cost <= least) {
                 least = cost;
-                best = {chw, r, blocks};
+                best.chw = chw;
+                best.group_blocks = blocks;
             }
         }
+    const int64_t tile = scan_tile(p.seqlen);
+    const double one = 2.0 * p.groups * best.group_blocks * p.dstate * tile;  // a tile's of a row
+    if (p.cu_seqlens == nullptr && p.batch * (one / tile) * p.seqlen > kShareFloats) {
+        best.tiles = evenly(ceil_div(p.seqlen, tile), (int64_t)(kShareFloats / (p.batch * one)));
+        if (best.tiles == 1 && p.batch * one > kShareFloats) best.rows = evenly(p.batch, (int64_t)(kShareFloats / one));
+        if (best.tiles * tile < p.seqlen) best.span = best.tiles * tile;
+    }
     return best;
 }
 
-template <typename T, int K> int launch_rows(const ScanBwdArgs& a, int chw, hipStream_t stream) {
+// rows: of the launch
+template <typename T, int K> int launch_rows(const ScanBwdArgs& a, int chw, int64_t rows, hipStream_t stream) {
     const cc1d_scan_bwd_params& b = a.p;
     const cc1d_scan_params& p = b.fwd;
-    const dim3 grid((unsigned)(a.group_blocks * p.groups * scan_sequences(p))), block(64 * kWaves);
+    const dim3 grid((unsigned)(a.group_blocks * p.groups * rows)), block(64 * kWaves);
     auto unit = [&](int i) {
         return p.u_stride[i] == 1 && p.delta_stride[i] == 1 && b.dout_stride[i] == 1 && b.du_stride[i] == 1 &&
                b.ddelta_stride[i] == 1 && (!p.z || (p.z_stride[i] == 1 && b.dz_stride[i] == 1));
@@ -794,10 +826,10 @@ template <typename T, int K> int launch_rows(const ScanBwdArgs& a, int chw, hipS
     });
 }
 
-template <typename T> int launch_short(const ScanBwdArgs& a, hipStream_t stream) {
+template <typename T> int launch_short(const ScanBwdArgs& a, int64_t rows, hipStream_t stream) {
     const cc1d_scan_bwd_params& b = a.p;
     const cc1d_scan_params& p = b.fwd;
-    const dim3 grid((unsigned)(a.group_blocks * p.groups * p.batch)), block(512);
+    const dim3 grid((unsigned)(a.group_blocks * p.groups * rows)), block(512);
     const bool unit = p.seqlen >= kShortK && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && b.dout_stride[2] == 1 &&
                       b.du_stride[2] == 1 && b.ddelta_stride[2] == 1 && (!p.z || (p.z_stride[2] == 1 && b.dz_stride[2] == 1));
     return with_flag(p.seq_idx != nullptr, [&](auto seq) {
@@ -811,40 +843,53 @@ template <typename T> int launch_short(const ScanBwdArgs& a, hipStream_t stream)
 
 int64_t scan_bwd_workspace_floats(const cc1d_scan_bwd_params& b) {
     const cc1d_scan_params& p = b.fwd;
-    const int64_t blocks = bwd_plan(p).group_blocks;
-    return 2 * p.batch * p.groups * blocks * p.dstate * p.seqlen + scan_sequences(p) * p.dim * (2 * p.dstate + 2);
+    const BwdPlan plan = bwd_plan(p);
+    return 2 * plan.rows * p.groups * plan.group_blocks * p.dstate * plan.span + scan_sequences(p) * p.dim * (2 * p.dstate + 2);
 }
 
 int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
     const cc1d_scan_params& p = b.fwd;
-    const int64_t seqs = scan_sequences(p), states = seqs * p.dim * p.dstate;
+    const int64_t seqs = scan_sequences(p), states = seqs * p.dim * p.dstate, tile = scan_tile(p.seqlen);
+    const BwdPlan plan = bwd_plan(p);
     ScanBwdArgs a{};
     a.p = b;
-    const BwdPlan plan = bwd_plan(p);
-    a.rounds = plan.rounds;
     a.group_blocks = plan.group_blocks;
+    a.span = plan.span;
     a.carry = b.workspace;
     a.pA = a.carry + states;
     a.pD = a.pA + states;
     a.pbias = a.pD + seqs * p.dim;
     a.pBC = a.pbias + seqs * p.dim;
-    const int64_t items = p.batch * p.groups * 2 * p.dstate * ceil_div(p.seqlen, 4);
+    // of a launch: rows (with cu_seqlens the sequences of the one row), and threads of its sum
+    const int64_t rows = p.cu_seqlens != nullptr ? seqs : plan.rows;
+    const int64_t most = plan.rows * p.groups * 2 * p.dstate * ceil_div(plan.span, 4);
     int split = 1;
-    while (split < 32 && items * split < 262144 && a.group_blocks >= 4 * split) split *= 2;
-    const int64_t blocks = a.group_blocks * p.groups * seqs, bc_blocks = ceil_div(items * split, 256),
-                  param_blocks = ceil_div(p.dim * (p.dstate + 2), 256);
-    if (!threads_fit(blocks, 64 * kWaves) || !threads_fit(bc_blocks, 256) || !threads_fit(param_blocks, 256))
+    while (split < 32 && most * split < 262144 && a.group_blocks >= 4 * split) split *= 2;
+    const int64_t param_blocks = ceil_div(p.dim * (p.dstate + 2), 256);
+    if (!threads_fit(a.group_blocks * p.groups * rows, 64 * kWaves) || !threads_fit(ceil_div(most * split, 256), 256) ||
+        !threads_fit(param_blocks, 256))
         return CC1D_ERR_SHAPE;  // before any of them runs
     return with_dtype(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         int st = CC1D_OK;
-        if (scan_is_short(p)) st = launch_short<T>(a, stream);
-        else if (seqs > 0)
-            st = scan_tile(p.seqlen) == 512 ? launch_rows<T, 8>(a, plan.chw, stream) : launch_rows<T, 4>(a, plan.chw, stream);
-        if (st == CC1D_OK && items > 0)
-            st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)bc_blocks), dim3(256), stream, a, items, split);
-        if (st == CC1D_OK)
-            st = launch(scan_bwd_reduce_params, dim3((unsigned)param_blocks), dim3(256), stream, a, seqs);
+        for (a.first = 0; st == CC1D_OK && a.first < seqs; a.first += rows) {
+            const int64_t count = seqs - a.first < rows ? seqs - a.first : rows;  // of sequences
+            const int64_t in_rows = p.cu_seqlens != nullptr ? 1 : count, all = ceil_div(p.seqlen, tile);
+            for (int64_t w = all > plan.tiles ? ceil_div(all, plan.tiles) - 1 : 0; st == CC1D_OK && w >= 0; --w) {
+                a.tile0 = (int)(w * plan.tiles);
+                a.tile1 = (int)(plan.tiles < all ? (w + 1) * plan.tiles : INT32_MAX);
+                a.t0 = a.tile0 * tile;
+                const int64_t positions = p.seqlen - a.t0 < plan.span ? p.seqlen - a.t0 : plan.span;
+                const int64_t items = in_rows * p.groups * 2 * p.dstate * ceil_div(positions, 4);
+                if (scan_is_short(p)) st = launch_short<T>(a, count, stream);
+                else
+                    st = tile == 512 ? launch_rows<T, 8>(a, plan.chw, count, stream) : launch_rows<T, 4>(a, plan.chw, count, stream);
+                if (st == CC1D_OK && items > 0)
+                    st = launch(scan_bwd_reduce_bc<T>, dim3((unsigned)ceil_div(items * split, 256)), dim3(256), stream, a, items,
+                                positions, split);
+            }
+        }
+        if (st == CC1D_OK) st = launch(scan_bwd_reduce_params, dim3((unsigned)param_blocks), dim3(256), stream, a, seqs);
         return st;
     });
 }

@@ -406,6 +406,9 @@ int cc1d_varlen_states(const cc1d_varlen_params* params, void* stream);
  * Scan, decode step and norm. The workspace sizes depend on the sizes and
  * flags of the params alone (< 0 for invalid ones); what a workspace holds
  * before a call is not read.
+ * The scan backward's shares of dB and dC are 4 GiB at most (a larger call
+ * runs in parts), except with cu_seqlens, where they grow with dim, dstate and
+ * seqlen, and where one tile's shares of one row are more.
  */
 int cc1d_scan_fwd(const cc1d_scan_params* params, void* stream);
 int64_t cc1d_scan_tile_floats(const cc1d_scan_params* params);

@@ -295,6 +295,52 @@ def test_extreme_steps():
     check(p, states=True)
 
 
+def live_channels(p, live):
+    """p with u and dout 0 in all channels but those, and the part of it that they are: the others add nothing."""
+    rest = torch.ones(p["u"].shape[1], dtype=torch.bool, device=DEV)
+    rest[live] = False
+    for k in ("u", "dout", "init", "dfinal"):
+        p[k][:, rest] = 0
+    return {k: v if v is None or k in ("B", "C") else (v[live] if k in ("A", "D", "bias") else v[:, live])
+            for k, v in p.items()}
+
+
+@pytest.mark.parametrize("layout", ["rows", "last"])
+@pytest.mark.parametrize("size", [(1, 8192, 4300, 256), (3, 4096, 2800, 256)], ids=str)
+def test_backward_in_parts_of_the_sequence(size, layout):
+    """More shares of dB and dC than a launch takes: tiles in several launches."""
+    B, D, L, N = size
+    p = make(B, D, L, N, 1, BF16, layout, seed=8)
+    live = torch.tensor([0, 7, 8, 300, 1023, 1024, 1500, D - 9, D - 1], device=DEV)
+    part = live_channels(p, live)
+    got = own(p, True, init=True)
+    e, s = exact(part, True, states=True), exact(part, True, states=True, mag=True)
+    for k, v in got.items():
+        pick = v if k in ("dB", "dC") else (v[live] if k in ("dA", "dD", "dbias") else v[:, live])
+        close(pick, e[k], s[k], L * (B + D), k)
+
+
+@pytest.mark.parametrize("size", [(8300, 128, 64, 256), (1800, 64, 300, 256), (1040, 64, 700, 256)], ids=str)
+def test_backward_in_parts_of_the_batch(size):
+    """More shares of one tile than a launch takes: rows in several launches. A row is what it is alone."""
+    B, D, L, N = size
+    p = make(B, D, L, N, 1, BF16, seed=9)
+    got = own(p, True, init=True)
+    rows = torch.tensor([0, B // 3, B // 2 - 1, B // 2, B // 2 + 1, B - 1], device=DEV)
+    few = {k: v if k in ("A", "D", "bias") else v[rows] for k, v in p.items()}
+    e, s = exact(few, True, states=True), exact(few, True, states=True, mag=True)
+    for k, v in got.items():
+        if k not in ("dA", "dD", "dbias"):
+            close(v[rows], e[k], s[k], L * (B + D), k)
+    dA = torch.zeros_like(p["A"], dtype=torch.float64)  # the parameters' gradients: of parts that one launch takes
+    mag = torch.zeros_like(dA)
+    for at in torch.arange(B, device=DEV).split(500):
+        one = own({k: v if k in ("A", "D", "bias") else v[at] for k, v in p.items()}, True, init=True)
+        dA += one["dA"].double()
+        mag += one["dA"].double().abs()
+    assert ((got["dA"].double() - dA).abs() <= 4 * B * 2.0**-24 * mag + 1e-6).all()
+
+
 def test_states_carry_over_chunks():
     """A prompt in pieces, the state handed on, is the prompt at once (up to fp32 rounding)."""
     p = make(2, 24, 1500, 16, 1, FP32, "rows")

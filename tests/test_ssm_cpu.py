@@ -287,6 +287,19 @@ def test_scan_update_of_more_threads_than_a_launch_has_is_refused():
     assert _lib.load().cc1d_scan_update(ctypes.byref(p), None) == 4
 
 
+@pytest.mark.parametrize("batch,dim,seqlen,dstate,groups", [
+    (4, 5120, 2048, 16, 1), (4, 5120, 2048, 17, 1), (4, 5120, 2048, 64, 1), (4, 5120, 2048, 128, 1), (8, 8192, 4096, 128, 1),
+    (1, 5120, 16384, 128, 1), (512, 1024, 300, 256, 1), (4096, 4096, 64, 64, 1), (65536, 64, 64, 256, 1),
+    (64, 4096, 8192, 16, 8), (1, 8192, 1 << 20, 256, 1), (1, 2048, 2048, 64, 8)])
+def test_scan_bwd_workspace_does_not_grow_with_everything(batch, dim, seqlen, dstate, groups):
+    """The shares of dB and dC are those of a part of the call: 2**30 floats at most (of these sizes)."""
+    b = _lib.ScanBwdParams()
+    b.fwd = _scan(batch=batch, dim=dim, seqlen=seqlen, dstate=dstate, groups=groups)
+    params = batch * dim * (2 * dstate + 2)
+    shares = _lib.load().cc1d_scan_bwd_workspace_floats(ctypes.byref(b)) - params
+    assert 2 * groups * dstate <= shares <= 1 << 30
+
+
 def test_scan_bwd_needs_its_workspace():
     b = _lib.ScanBwdParams()
     b.fwd = _scan(u=16, delta=16, A=16, B=16, C=16, tile_states=16)
