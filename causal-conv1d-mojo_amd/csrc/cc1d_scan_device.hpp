@@ -27,7 +27,7 @@ __host__ __device__ constexpr int64_t scan_tile(int64_t seqlen) { return seqlen 
 
 // dt = softplus(raw) = max(raw, 0) + log1p(e), e = exp(-|raw|), with
 // log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, and atanh(s) / s a polynomial
-// in s^2, fitted on [0, 1/9] at Chebyshev points (4e-9 off at most). Steps are
+// in s^2, fitted on [0, 1/9] at Chebyshev points (8e-9 off at most). Steps are
 // small numbers (1e-3 and below), so the relative error counts, and
 // log2(1 + e) would lose it. The exponent's rounding (|raw| log2(e) may reach
 // 20) is taken back with the product's remainder.

@@ -5,6 +5,7 @@ torch formulations, argument checks, the C ABI's refusals and struct layouts."""
 from __future__ import annotations
 
 import ctypes
+import re
 import subprocess
 from pathlib import Path
 
@@ -121,6 +122,22 @@ def test_references_agree_with_each_other():
         torch.testing.assert_close(got, out[..., t])
     torch.testing.assert_close(state[3], fin[0])
     assert torch.equal(state[:3], init) and torch.equal(state[4:], init[1:])
+
+
+def test_softplus_polynomial_is_as_close_as_it_says():
+    """The kernels' atanh(s) / s, with the coefficients and the bound read from the source."""
+    src = (ROOT / "causal-conv1d-mojo_amd" / "csrc" / "cc1d_scan_device.hpp").read_text()
+    said = float(re.search(r"Chebyshev points \(([\d.e-]+) off at most\)", src).group(1))
+    body = src[src.index("float softplus(float raw)"):src.index("float sigmoid(float x)")]
+    first = re.search(r"p = __builtin_fmaf\(s2, ([\d.]+)f, ([\d.]+)f\)", body).groups()
+    coefficients = [float(torch.tensor(float(c))) for c in (*first, *re.findall(r"fmaf\(s2, p, ([\d.]+)f\)", body))]
+    assert len(coefficients) == 5
+    s = torch.linspace(1e-6, 1 / 3, 200001, dtype=torch.float64)
+    p = torch.zeros_like(s)
+    for c in coefficients:
+        p = p * s * s + c
+    off = (p - torch.atanh(s) / s).abs().max().item()
+    assert said / 2 < off <= said
 
 
 # ---------------------------------------------------------------- refusals
