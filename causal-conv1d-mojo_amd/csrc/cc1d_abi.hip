@@ -99,10 +99,10 @@ const char* cc1d_strerror(int status) {
     case CC1D_ERR_DTYPE: return "unsupported dtype code (expected 0=fp16, 1=bf16, 2=fp32) or element size";
     case CC1D_ERR_WIDTH: return "width must be in 2..9";
     case CC1D_ERR_SHAPE: return "invalid or too large shape";
-    case CC1D_ERR_EXCLUSIVE: return "seq_idx is mutually exclusive with initial_states and final_states";
+    case CC1D_ERR_EXCLUSIVE: return "seq_idx is mutually exclusive with initial_states and final_states (in a scan also with cu_seqlens)";
     case CC1D_ERR_STATE_LEN: return "conv_state length must be >= width - 1";
     case CC1D_ERR_LAUNCH: return "kernel launch failed";
-    case CC1D_ERR_WORKSPACE: return "workspace smaller than cc1d_bwd_workspace_floats()";
+    case CC1D_ERR_WORKSPACE: return "workspace smaller than the entry point's *_workspace_floats()";
     case CC1D_ERR_SCRATCH_LIMIT:
         return "problem needs more workspace than the static scratch of cc1d_bwd_typed_noalloc "
                "(CC1D_NOALLOC_WORKSPACE_FLOATS floats)";

@@ -57,10 +57,11 @@ enum cc1d_status {
     CC1D_ERR_WIDTH = 3,             /* width outside 2..9 */
     CC1D_ERR_SHAPE = 4,             /* negative size, or a size/stride too large for the kernels */
     CC1D_ERR_EXCLUSIVE = 5,         /* seq_idx given together with initial_states or final_states
-                                       (backward: or with dfinal_states / dinitial_states) */
+                                       (backward: or with dfinal_states / dinitial_states; scan: or
+                                       with cu_seqlens) */
     CC1D_ERR_STATE_LEN = 6,         /* conv_state length < width - 1 */
     CC1D_ERR_LAUNCH = 7,            /* the HIP runtime refused a kernel launch */
-    CC1D_ERR_WORKSPACE = 8,         /* workspace smaller than cc1d_bwd_workspace_floats() */
+    CC1D_ERR_WORKSPACE = 8,         /* workspace smaller than the entry point's *_workspace_floats() */
     CC1D_ERR_SCRATCH_LIMIT = 9,     /* cc1d_bwd_typed_noalloc: the problem needs more than
                                        CC1D_NOALLOC_WORKSPACE_FLOATS floats of workspace */
     CC1D_ERR_DSTATE = 10,           /* dstate outside 1..CC1D_MAX_DSTATE */

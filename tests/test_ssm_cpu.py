@@ -304,6 +304,14 @@ def test_scan_update_of_more_threads_than_a_launch_has_is_refused():
     assert _lib.load().cc1d_scan_update(ctypes.byref(p), None) == 4
 
 
+def test_messages_fit_the_scan_and_the_norm():
+    """The codes that the convolution's entry points also give name what these lack."""
+    lib = _lib.load()
+    assert "cu_seqlens" in lib.cc1d_strerror(5).decode()
+    workspace = lib.cc1d_strerror(8).decode()
+    assert "cc1d_bwd" not in workspace and "_workspace_floats()" in workspace
+
+
 @pytest.mark.parametrize("batch,dim,seqlen,dstate,groups", [
     (4, 5120, 2048, 16, 1), (4, 5120, 2048, 17, 1), (4, 5120, 2048, 64, 1), (4, 5120, 2048, 128, 1), (8, 8192, 4096, 128, 1),
     (1, 5120, 16384, 128, 1), (512, 1024, 300, 256, 1), (4096, 4096, 64, 64, 1), (65536, 64, 64, 256, 1),
