@@ -243,7 +243,9 @@ def ssm_scan_fn(
     return_final_states: bool = False,
 ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """
-    u, delta, z: (batch, dim, seqlen), fp16 / bf16 / fp32; channel-first and channel-last layouts are fast
+    u, delta, z: (batch, dim, seqlen), fp16 / bf16 / fp32; channel-first and channel-last layouts are fast where
+        the three lie alike; B and C may lie either way beside them. Other strides, or one tensor unlike the rest,
+        are read element by element (two to three times as long)
     A: (dim, dstate) fp32 (real), dstate in 1..256; D, delta_bias: (dim,) fp32
     B, C: (batch, dstate, seqlen) or (batch, groups, dstate, seqlen), dtype of u; dim a multiple of groups
     delta_softplus: dt = softplus(delta + delta_bias) instead of delta + delta_bias

@@ -1,10 +1,18 @@
 // cc1d_norm.hip -- residual add and layer / rms norm, forward and backward.
 //
-// Bandwidth kernels: every value is read once and stays in registers, 8 per
+// Bandwidth kernels: every value is read once and stays on the chip, 8 per
 // lane and step, while its row's sums are formed (the mean first, then the
 // spread around it), so rows go through the card once each way. At 8192 x 2560
 // bf16 with an fp32 residual: forward 56 us (4.5 TB/s), backward 77 (4.4) and its
 // reduction 9; a copy reaches 6.3 with non-temporal accesses, 5.0 without.
+//
+// Rows of up to 8192 columns (one step a lane) fit in registers. Wider ones
+// have 2 to 4 steps a lane in blocks of up to 16 wavefronts, whose 128 registers
+// a lane do not hold them: the backward spills 216, 652 and 980 bytes a lane at
+// 2, 3 and 4 steps (forward 0, 68, 256, or 188 to 844 where the width is no
+// multiple of 8). Same bytes, bf16 with an fp32 residual: 2048 x 8192 takes 54
+// and 67 us, 2048 x 12288 (half as much again) 78 and 198, 1024 x 32768 (twice)
+// 213 and 636.
 #include "cc1d_internal.hpp"
 #include "cc1d_steps.hpp"
 
@@ -304,7 +312,10 @@ NormPlan norm_plan(int64_t dim) {
     return {lpr, wpr, steps, wpr <= 2 ? 4 : wpr};
 }
 // Shares of the parameter gradients: three blocks a CU (15 wavefronts at 2560
-// columns; a fourth would not fit beside them and run alone at the end)
+// columns; a fourth would not fit beside them and run alone at the end). With
+// two, three and four a CU, kernel and reduction in a row of launches, us:
+// 8192 x 2560 bf16 + fp32 74, 86, 92; 2048 x 8192 70, 79, 89; 4099 x 1533 fp32
+// 35, 36, 39; 16384 x 1024 bf16 43, 38, 38; 32768 x 256 bf16 22, 22, 24.
 constexpr int64_t kBwdBlocks = 768;
 
 int64_t bwd_blocks(const cc1d_norm_params& p, const NormPlan& n) {

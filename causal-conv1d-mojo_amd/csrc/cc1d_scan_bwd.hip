@@ -139,10 +139,18 @@ template <typename R> __device__ __forceinline__ void kept(const uint32_t* lds, 
 // fixed order. (Added to by LDS atomics instead, 3870 us against 700 at
 // 4 x 5120 x 2048 with 16 states.)
 //
-// Vector issue bounds it: 28.5 instructions per position, channel and state,
-// of which the state's loop is 22.7; at that size they fill 75% of the time.
-// What remains is the barrier per two states (one per state: 724 us against
-// 652) and the start and end of each tile, which one block a CU does not cover.
+// Vector issue bounds it: 28.6 instructions per position, channel and state,
+// which fill 74% of the time at that size. What remains is the barrier per two
+// states and the start and end of each tile, which one block a CU does not
+// cover. A barrier per state instead of two, in a row of launches at 4 x 5120 x
+// 2048: 682 us against 719, channel-last 1100 against 1060, with ids 1092
+// against 1081, fp32 854 against 858.
+//
+// Two channels a wavefront and their loads in flight are more than 256 registers
+// hold in most forms: bytes of scratch a lane at 512 positions, 16-bit types and
+// fp32: rows 0 and 136 (with ids 152 and 292), channel-last 276 and 560 (444 and
+// 740), any strides 360 and 640 (540 and 812). Channel-last takes 1010 to 1060
+// us at that size (fp32 1670), with ids in rows 1065.
 constexpr int kWaves = 8;
 template <typename T, int K, int CHW, bool SEQ, Layout LAY, StateMode MODE>
 __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) scan_bwd_rows(const ScanBwdArgs arg) {
@@ -765,14 +773,19 @@ int64_t evenly(int64_t all, int64_t most) { return ceil_div(all, ceil_div(all, m
 // one row and lengths that only the device knows: one launch.
 constexpr double kShareFloats = 1 << 30;
 
-// A CU holds one block (128 KB of LDS), so the choice that leaves the card the
-// least to do one after the other; a round of one channel each takes about 2/3
-// of the time of one of two (854 us against 652 at 4 x 2048 x 2048 with 16
-// states, where either fills the card). Of equals the largest: its dB and dC
-// have the fewest shares to add. More than 16 states: one round.
+// A CU holds one block (128 KB of LDS and more; tiles of 256 positions have half
+// of that, which is not counted), so the choice that leaves the card the least
+// to do one after the other; a round of one channel each is taken for 2/3 of one
+// of two. Measured where either fills the card, with 16 states, one and two
+// channels, us: 4 x 5120 x 2048 bf16 850 and 719 (0.59 a round), channel-last
+// 1150 and 1051, with ids 1137 and 1080, fp32 870 and 856; 4 x 2048 x 2048 fp32
+// channel-last 693 and 713; 4 x 5120 x 200 122 and 129. Of equals the largest:
+// its dB and dC have the fewest shares to add. More than 16 states: one round.
 BwdPlan bwd_plan(const cc1d_scan_params& p) {
     const int64_t per = p.dim / p.groups, rows = scan_sequences(p) * p.groups;
-    if (scan_is_short(p)) {  // rounds once 1024 blocks (four wavefronts a SIMD, twice over) have some
+    // Short rows: rounds once 1024 blocks (four wavefronts a SIMD, twice over) have some. From 512, 1024 and 4096 on, us,
+    // 16 states bf16: 8 x 4096 x 64 53, 56, 56; 64 x 4096 x 64 297, 291, 305; 32 x 8192 x 64 288, 280, 297.
+    if (scan_is_short(p)) {
         const int64_t blocks = ceil_div(per, 32), r = p.dstate > kStates ? 1 : ceil_div(rows * blocks, 1024);
         BwdPlan plan{0, ceil_div(blocks, r), p.batch, 1, p.seqlen};
         const double row = 2.0 * p.groups * plan.group_blocks * p.dstate * p.seqlen;
@@ -863,6 +876,9 @@ int launch_scan_bwd(const cc1d_scan_bwd_params& b, hipStream_t stream) {
     // of a launch: rows (with cu_seqlens the sequences of the one row), and threads of its sum
     const int64_t rows = p.cu_seqlens != nullptr ? seqs : plan.rows;
     const int64_t most = plan.rows * p.groups * 2 * p.dstate * ceil_div(plan.span, 4);
+    // Shares of dB and dC per thread of their sum: 1024 blocks of threads fill the card. Against one thread for all of
+    // them and 32 everywhere, backward in all, us: 1 x 4096 x 512 with 16 states 57 (73 and 56), 4 x 2048 x 2041 326 (345
+    // and 332), 4 x 5120 x 2048 721 (725 and 725), 1 x 8192 x 16384 2415 (2404 and 2426).
     int split = 1;
     while (split < 32 && most * split < 262144 && a.group_blocks >= 4 * split) split *= 2;
     const int64_t param_blocks = ceil_div(p.dim * (p.dstate + 2), 256);

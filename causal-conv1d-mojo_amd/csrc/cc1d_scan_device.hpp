@@ -12,8 +12,10 @@
 // without cutting the sequence into chunks that are walked twice. Per position
 // and state the steps cost 7 issue slots (one exponential is two, measured 8
 // cycles a wavefront against 4 for a multiply-add) and the wavefront's prefix
-// 17 per K; channels along the lanes cost 6, but fill the card from 5120
-// channels x 4 rows on only, and 11 with the sequence cut into chunks.
+// 17 per K; channels along the lanes would cost 6, but fill the card from 5120
+// channels x 4 rows on only, and 11 with the sequence cut into chunks. (Counts:
+// that form was not built, nor one that also spreads a channel's states over
+// wavefronts, which fills the card with fewer channels.)
 #pragma once
 
 #include "cc1d_internal.hpp"

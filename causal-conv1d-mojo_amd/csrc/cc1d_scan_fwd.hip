@@ -1,8 +1,8 @@
 // cc1d_scan_fwd.hip -- forward of the selective state space scan.
 //
-// Vector issue bounds it: 12.1 instructions per position, channel and state
-// with 16 states (the state's loop 9.4 of them), which fill 88% of the time:
-// 255 us at 4 x 5120 x 2048 bf16. Its 341 MB would take 54.
+// Vector issue bounds it: 12.7 instructions per position, channel and state
+// with 16 states, which fill 97% of the time (13.4 and 88% channel-last): 250
+// to 260 us at 4 x 5120 x 2048 bf16. Its 341 MB would take 54.
 #include "cc1d_scan_device.hpp"
 
 namespace cc1d {
@@ -498,7 +498,10 @@ int launch_scan_fwd(const cc1d_scan_params& p, hipStream_t stream) {
     const ScanFwdArgs a{p, 0, 1};
     return with_dtype(p.dtype, [&](auto t) {
         typedef decltype(t) T;
-        // (few channels of many states: several wavefronts a channel, 27 us against 37 at 1 x 1024 x 40 with 128 states)
+        // Four channels a wavefront against one, or fewer channels with their states over several, us, 1 x dim x 40
+        // bf16: the former's time hardly depends on dim (N = 16: 7.5, 32: 11.5, 64: 19.7, 128: 35.7, 256: 68), the
+        // latter's does (N = 16: 6.1 at 64 channels, 9.4 at 1024; 64: 9.9, 14.1 at 512, 16.7 at 1024, 21.6 at 1536, 32
+        // at 4096; 128: 26 at 1024, 36 at 1536 and 2048, 57 at 4096; 256: 66 at 1536 and 2048, 108 at 4096).
         if (scan_is_short(p) && (p.dstate <= 64 || p.batch * p.dim >= 2048))
             return launch_short<T>(a, p.seqlen >= kShortK && p.u_stride[2] == 1 && p.delta_stride[2] == 1 && p.out_stride[2] == 1 &&
                                           (!p.z || p.z_stride[2] == 1), stream);
