@@ -770,7 +770,10 @@ int64_t evenly(int64_t all, int64_t most) { return ceil_div(all, ceil_div(all, m
 // tile of all rows is too much, rows. That costs nothing (43.0 ms either way
 // at that size); parts of 1 GiB cost up to 5% (45.0 there), as fewer blocks
 // run beside each other at the end of each. Packed prompts (cu_seqlens) have
-// one row and lengths that only the device knows: one launch.
+// one row and lengths that only the device knows: one launch. (Parts of the row,
+// with the tiles that start in them: four prompts of 16384 x 1024 channels with
+// 256 states run one after the other, 44.2 ms against 21.9, and the tiles' bounds
+// kept in scalars cost other forms up to 5%.)
 constexpr double kShareFloats = 1 << 30;
 
 // A CU holds one block (128 KB of LDS and more; tiles of 256 positions have half
