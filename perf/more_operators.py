@@ -15,6 +15,7 @@ returning the new ones; ``packed`` the same packing without states; ``states`` o
 
 from __future__ import annotations
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -32,7 +33,9 @@ STEP_LARGEST = 128 * 40 * 128 * 128               # state elements of the larges
 ROTARY_LARGEST = 4 * 2048 * (40 + 40) * 128       # values of the largest listed rotation
 
 
+@functools.lru_cache(maxsize=None)
 def _cc():
+    """The package, imported once as a program imports it."""
     pkg = str(Path(__file__).resolve().parent.parent / "causal-conv1d-mojo_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
