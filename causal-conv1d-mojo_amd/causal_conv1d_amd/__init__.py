@@ -15,13 +15,22 @@ same manner: ``ssm_scan_fn`` (the selective scan over prompts, forward +
 autograd backward), ``ssm_scan_update`` (its decode step) and ``add_norm_fn``
 (residual add and layer / rms norm, forward + autograd backward), with
 plain-torch formulations ``ssm_scan_ref``, ``ssm_scan_update_ref`` and
-``add_norm_ref``.
+``add_norm_ref``. So does the mixer whose state is a matrix for each head:
+``linear_attn_fn`` (linear attention with a decay for each head over prompts,
+forward + autograd backward), ``linear_attn_update`` (its decode step) and
+``head_norm_rotary_fn`` (norm of each query and key head and rotation by
+position, forward + autograd backward; ``rotary_frequencies`` gives the
+frequencies), with ``linear_attn_ref``, ``linear_attn_update_ref`` and
+``head_norm_rotary_ref``.
 """
 
 from __future__ import annotations
 
+from causal_conv1d_amd._attn import linear_attn_fn
+from causal_conv1d_amd._attn_update import linear_attn_update
 from causal_conv1d_amd._fn import causal_conv1d_fn
 from causal_conv1d_amd._norm import add_norm_fn
+from causal_conv1d_amd._rotary import head_norm_rotary_fn, rotary_frequencies
 from causal_conv1d_amd._scan import ssm_scan_fn
 from causal_conv1d_amd._scan_update import ssm_scan_update
 from causal_conv1d_amd._update import causal_conv1d_update
@@ -30,6 +39,7 @@ from causal_conv1d_amd.causal_conv1d_varlen import (
     causal_conv1d_varlen_states_ref,
 )
 from causal_conv1d_amd.reference import causal_conv1d_ref, causal_conv1d_update_ref
+from causal_conv1d_amd.reference_attn import head_norm_rotary_ref, linear_attn_ref, linear_attn_update_ref
 from causal_conv1d_amd.reference_ssm import add_norm_ref, ssm_scan_ref, ssm_scan_update_ref
 
 __version__ = "1.6.1"
@@ -43,6 +53,13 @@ __all__ = [
     "causal_conv1d_update_ref",
     "causal_conv1d_varlen_states",
     "causal_conv1d_varlen_states_ref",
+    "head_norm_rotary_fn",
+    "head_norm_rotary_ref",
+    "linear_attn_fn",
+    "linear_attn_ref",
+    "linear_attn_update",
+    "linear_attn_update_ref",
+    "rotary_frequencies",
     "ssm_scan_fn",
     "ssm_scan_ref",
     "ssm_scan_update",

@@ -17,6 +17,8 @@ _ENTRIES = ("cc1d_strerror", "cc1d_fwd", "cc1d_bwd_workspace_floats", "cc1d_bwd_
             "cc1d_varlen_states")
 _SSM_ENTRIES = ("cc1d_scan_fwd", "cc1d_scan_tile_floats", "cc1d_scan_bwd", "cc1d_scan_bwd_workspace_floats",
                 "cc1d_scan_update", "cc1d_norm_fwd", "cc1d_norm_bwd", "cc1d_norm_bwd_workspace_floats")
+_ATTN_ENTRIES = ("cc1d_attn_fwd", "cc1d_attn_workspace_floats", "cc1d_attn_bwd", "cc1d_attn_bwd_workspace_floats",
+                 "cc1d_attn_update", "cc1d_rotary_fwd", "cc1d_rotary_bwd", "cc1d_rotary_bwd_workspace_floats")
 
 _ext = None
 
@@ -36,6 +38,7 @@ def load():
         address = lambda name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value  # noqa: E731
         ext.bind(*map(address, _ENTRIES))
         ext.bind_ssm(*map(address, _SSM_ENTRIES))
+        ext.bind_attn(*map(address, _ATTN_ENTRIES))
         _ext = ext
     return _ext
 

@@ -2,7 +2,7 @@
 
 The structures below mirror ``cc1d_fwd_params`` / ``cc1d_bwd_params`` /
 ``cc1d_bwd_grads`` / ``cc1d_update_params`` / ``cc1d_varlen_params`` and the
-scan's and norm's params field for field. The library
+params of the scan, the norm, linear attention and the rotation field for field. The library
 is loaded on first use; a missing or stale build raises instead of falling
 back to anything else.
 """
@@ -137,6 +137,56 @@ class NormBwdParams(ctypes.Structure):
     ]
 
 
+class AttnParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("g", _vp), ("cu_seqlens", _vp), ("initial_states", _vp),
+        ("out", _vp), ("final_states", _vp), ("workspace", _vp), ("workspace_floats", _i64),
+        ("batch", _i64), ("seqlen", _i64), ("heads", _i64), ("key_heads", _i64), ("dk", _i64), ("dv", _i64),
+        ("num_seqs", _i64),
+        ("q_stride", _i64x4), ("k_stride", _i64x4), ("v_stride", _i64x4), ("g_stride", _i64x3),
+        ("initial_states_stride", _i64x4),
+        ("scale", ctypes.c_double), ("dtype", _i32),
+    ]
+
+
+class AttnBwdParams(ctypes.Structure):
+    _fields_ = [
+        ("fwd", AttnParams), ("dout", _vp), ("dfinal_states", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("dg", _vp), ("dinitial_states", _vp), ("workspace", _vp), ("workspace_floats", _i64),
+        ("dout_stride", _i64x4), ("dfinal_states_stride", _i64x4),
+    ]
+
+
+class AttnUpdateParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("g", _vp), ("attn_state", _vp), ("attn_state_indices", _vp), ("out", _vp),
+        ("batch", _i64), ("tokens", _i64), ("heads", _i64), ("key_heads", _i64), ("dk", _i64), ("dv", _i64),
+        ("state_rows", _i64),
+        ("q_stride", _i64x4), ("k_stride", _i64x4), ("v_stride", _i64x4), ("g_stride", _i64x3),
+        ("attn_state_stride", _i64x4),
+        ("scale", ctypes.c_double), ("dtype", _i32),
+    ]
+
+
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("q_weight", _vp), ("k_weight", _vp), ("inv_freq", _vp), ("positions", _vp),
+        ("q_out", _vp), ("k_out", _vp),
+        ("batch", _i64), ("seqlen", _i64), ("q_heads", _i64), ("k_heads", _i64), ("dim", _i64), ("rotated", _i64),
+        ("q_stride", _i64x4), ("k_stride", _i64x4), ("positions_stride", _i64x2),
+        ("eps", ctypes.c_double), ("amplitude", ctypes.c_double),
+        ("dtype", _i32), ("positions_bytes", _i32), ("interleaved", _i32),
+    ]
+
+
+class RotaryBwdParams(ctypes.Structure):
+    _fields_ = [
+        ("fwd", RotaryParams), ("dq_out", _vp), ("dk_out", _vp), ("dq", _vp), ("dk", _vp), ("dq_weight", _vp),
+        ("dk_weight", _vp), ("workspace", _vp), ("workspace_floats", _i64),
+        ("dq_out_stride", _i64x4), ("dk_out_stride", _i64x4),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "cc1d_abi_version",
     "cc1d_strerror",
@@ -155,6 +205,14 @@ EXPORTED_SYMBOLS = (
     "cc1d_norm_fwd",
     "cc1d_norm_bwd",
     "cc1d_norm_bwd_workspace_floats",
+    "cc1d_attn_fwd",
+    "cc1d_attn_workspace_floats",
+    "cc1d_attn_bwd",
+    "cc1d_attn_bwd_workspace_floats",
+    "cc1d_attn_update",
+    "cc1d_rotary_fwd",
+    "cc1d_rotary_bwd",
+    "cc1d_rotary_bwd_workspace_floats",
 )
 
 _lib = None
@@ -188,13 +246,19 @@ def load():
     for name, st in (("cc1d_fwd", FwdParams), ("cc1d_bwd", BwdParams), ("cc1d_update", UpdateParams),
                      ("cc1d_varlen_states", VarlenParams), ("cc1d_scan_fwd", ScanParams),
                      ("cc1d_scan_bwd", ScanBwdParams), ("cc1d_scan_update", ScanUpdateParams),
-                     ("cc1d_norm_fwd", NormParams), ("cc1d_norm_bwd", NormBwdParams)):
+                     ("cc1d_norm_fwd", NormParams), ("cc1d_norm_bwd", NormBwdParams),
+                     ("cc1d_attn_fwd", AttnParams), ("cc1d_attn_bwd", AttnBwdParams),
+                     ("cc1d_attn_update", AttnUpdateParams), ("cc1d_rotary_fwd", RotaryParams),
+                     ("cc1d_rotary_bwd", RotaryBwdParams)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(st), _vp]
     for name, st in (("cc1d_bwd_workspace_floats", BwdParams), ("cc1d_scan_tile_floats", ScanParams),
                      ("cc1d_scan_bwd_workspace_floats", ScanBwdParams),
-                     ("cc1d_norm_bwd_workspace_floats", NormBwdParams)):
+                     ("cc1d_norm_bwd_workspace_floats", NormBwdParams),
+                     ("cc1d_attn_workspace_floats", AttnParams),
+                     ("cc1d_attn_bwd_workspace_floats", AttnBwdParams),
+                     ("cc1d_rotary_bwd_workspace_floats", RotaryBwdParams)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int64
         fn.argtypes = [ctypes.POINTER(st)]

@@ -169,8 +169,9 @@ def native_varlen_states(x, cu_seqlens, states) -> None:
     _lib.check(lib.cc1d_varlen_states(ctypes.byref(p), _stream(x)))
 
 
-def _set4(arr, t: torch.Tensor) -> None:
-    arr[0], arr[1], arr[2], arr[3] = t.stride()
+def _set4(arr, t: torch.Tensor | None) -> None:
+    if t is not None:
+        arr[0], arr[1], arr[2], arr[3] = t.stride()
 
 
 def _stride0(t: torch.Tensor | None) -> int:
@@ -294,3 +295,116 @@ def native_norm_bwd(x, weight, residual, stats, rms, dy, dsum, dx, dresidual, dw
     ws = torch.empty(max(n, 1), dtype=torch.float32, device=dy.device)
     b.workspace, b.workspace_floats = ws.data_ptr(), ws.numel()
     _lib.check(lib.cc1d_norm_bwd(ctypes.byref(b), _stream(dy)))
+
+
+def _attn_params(q, k, v, g, cu_seqlens, initial_states, scale):
+    p = _lib.AttnParams()
+    p.q, p.k, p.v, p.g = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr()
+    p.cu_seqlens, p.initial_states = _ptr(cu_seqlens), _ptr(initial_states)
+    p.batch, p.seqlen, p.key_heads, p.dk = q.shape
+    p.heads, p.dv = v.shape[2:]
+    p.num_seqs = 0 if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    _set4(p.q_stride, q)
+    _set4(p.k_stride, k)
+    _set4(p.v_stride, v)
+    _set3(p.g_stride, g)
+    _set4(p.initial_states_stride, initial_states)
+    p.scale, p.dtype = scale, _DTYPE_CODE[q.dtype]
+    return p
+
+
+def _workspace(n, like):
+    """(tensor or None, floats) of a workspace of n floats (n <= 0: none)."""
+    if n <= 0:
+        return None, 0
+    return torch.empty(n, dtype=torch.float32, device=like.device), n
+
+
+def native_attn_fwd(q, k, v, g, cu_seqlens, initial_states, scale, out, final_states) -> None:
+    _require_device(q)
+    lib = _lib.load()
+    p = _attn_params(q, k, v, g, cu_seqlens, initial_states, scale)
+    p.out, p.final_states = out.data_ptr(), _ptr(final_states)
+    ws, p.workspace_floats = _workspace(lib.cc1d_attn_workspace_floats(ctypes.byref(p)), q)
+    p.workspace = _ptr(ws)
+    with torch.cuda.device(q.device):
+        _lib.check(lib.cc1d_attn_fwd(ctypes.byref(p), _stream(q)))
+
+
+def native_attn_bwd(q, k, v, g, cu_seqlens, initial_states, scale, dout, dfinal_states, dq, dk, dv, dg,
+                    dinitial_states) -> None:
+    _require_device(q)
+    lib = _lib.load()
+    b = _lib.AttnBwdParams()
+    b.fwd = _attn_params(q, k, v, g, cu_seqlens, initial_states, scale)
+    b.dout, b.dfinal_states = dout.data_ptr(), _ptr(dfinal_states)
+    b.dq, b.dk, b.dv, b.dg = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr()
+    b.dinitial_states = _ptr(dinitial_states)
+    _set4(b.dout_stride, dout)
+    _set4(b.dfinal_states_stride, dfinal_states)
+    ws, b.workspace_floats = _workspace(lib.cc1d_attn_bwd_workspace_floats(ctypes.byref(b)), q)
+    b.workspace = _ptr(ws)
+    with torch.cuda.device(q.device):
+        _lib.check(lib.cc1d_attn_bwd(ctypes.byref(b), _stream(q)))
+
+
+def native_attn_update(q, attn_state, k, v, g, scale, attn_state_indices, out) -> None:
+    """Tensors with a token axis."""
+    _require_device(q)
+    lib = _lib.load()
+    p = _lib.AttnUpdateParams()
+    p.q, p.k, p.v, p.g = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr()
+    p.attn_state, p.attn_state_indices, p.out = attn_state.data_ptr(), _ptr(attn_state_indices), out.data_ptr()
+    p.batch, p.tokens, p.key_heads, p.dk = q.shape
+    p.heads, p.dv = v.shape[2:]
+    p.state_rows = attn_state.shape[0]
+    _set4(p.q_stride, q)
+    _set4(p.k_stride, k)
+    _set4(p.v_stride, v)
+    _set3(p.g_stride, g)
+    _set4(p.attn_state_stride, attn_state)
+    p.scale, p.dtype = scale, _DTYPE_CODE[q.dtype]
+    with torch.cuda.device(q.device):
+        _lib.check(lib.cc1d_attn_update(ctypes.byref(p), _stream(q)))
+
+
+def _rotary_params(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved, amplitude):
+    p = _lib.RotaryParams()
+    p.q, p.k, p.q_weight, p.k_weight = q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight)
+    p.inv_freq, p.positions = _ptr(inv_freq), _ptr(positions)
+    p.batch, p.seqlen, p.q_heads, p.dim = q.shape
+    p.k_heads = k.shape[2]
+    p.rotated = 0 if inv_freq is None else 2 * inv_freq.shape[0]
+    _set4(p.q_stride, q)
+    _set4(p.k_stride, k)
+    _set2(p.positions_stride, positions)
+    p.positions_bytes = 4 if positions is None else positions.element_size()
+    p.eps, p.amplitude, p.interleaved = eps, amplitude, int(interleaved)
+    p.dtype = _DTYPE_CODE[q.dtype]
+    return p
+
+
+def native_rotary_fwd(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved, amplitude, q_out, k_out) -> None:
+    _require_device(q)
+    lib = _lib.load()
+    p = _rotary_params(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved, amplitude)
+    p.q_out, p.k_out = q_out.data_ptr(), k_out.data_ptr()
+    with torch.cuda.device(q.device):
+        _lib.check(lib.cc1d_rotary_fwd(ctypes.byref(p), _stream(q)))
+
+
+def native_rotary_bwd(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved, amplitude, dq_out, dk_out, dq,
+                      dk, dq_weight, dk_weight) -> None:
+    _require_device(dq_out)
+    lib = _lib.load()
+    b = _lib.RotaryBwdParams()
+    b.fwd = _rotary_params(dq_out if q is None else q, dk_out if k is None else k, q_weight, k_weight, inv_freq,
+                           positions, eps, interleaved, amplitude)
+    b.dq_out, b.dk_out, b.dq, b.dk = dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr()
+    b.dq_weight, b.dk_weight = _ptr(dq_weight), _ptr(dk_weight)
+    _set4(b.dq_out_stride, dq_out)
+    _set4(b.dk_out_stride, dk_out)
+    ws, b.workspace_floats = _workspace(lib.cc1d_rotary_bwd_workspace_floats(ctypes.byref(b)), dq_out)
+    b.workspace = _ptr(ws)
+    with torch.cuda.device(dq_out.device):
+        _lib.check(lib.cc1d_rotary_bwd(ctypes.byref(b), _stream(dq_out)))

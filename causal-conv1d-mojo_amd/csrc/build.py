@@ -35,7 +35,7 @@ LIB_PATH = LIB_DIR / "libcc1d_amd.so"
 FLOOR_SRC = CSRC / "bench" / "cc1d_floor.hip"
 FLOOR_PATH = REPO / "libcc1d_floor.so"
 # host path: a CPython extension over libtorch, no device code
-HOST_SRCS = (CSRC / "host" / "cc1d_host.cpp", CSRC / "host" / "cc1d_host_ssm.cpp")
+HOST_SRCS = tuple(CSRC / "host" / f"cc1d_host{unit}.cpp" for unit in ("", "_ssm", "_attn"))
 HOST_PATH = LIB_DIR / "cc1d_host.so"
 ARCH = "gfx950"
 

@@ -86,6 +86,35 @@ int check_norm(const cc1d_norm_params& p) {
     return CC1D_OK;
 }
 
+bool attn_dim(int64_t d) { return d >= 1 && d <= CC1D_MAX_ATTN_DIM; }
+
+// Sizes of linear attention, before its pointers.
+int check_attn(const cc1d_attn_params& p) {
+    if (!valid_dtype(p.dtype)) return CC1D_ERR_DTYPE;
+    if (!attn_dim(p.dk) || !attn_dim(p.dv)) return CC1D_ERR_HEAD_DIM;
+    if (p.batch < 0 || p.seqlen < 0 || p.heads < 0) return CC1D_ERR_SHAPE;
+    if (p.key_heads < 1 || p.heads % p.key_heads != 0) return CC1D_ERR_HEADS;
+    if (p.cu_seqlens != nullptr && (p.batch != 1 || p.num_seqs < 0 || (p.num_seqs == 0 && p.seqlen > 0))) return CC1D_ERR_SHAPE;
+    return attn_fits(p) ? CC1D_OK : CC1D_ERR_SHAPE;
+}
+
+bool attn_empty(const cc1d_attn_params& p) {
+    return p.heads == 0 || (p.cu_seqlens != nullptr ? p.num_seqs == 0 : p.batch == 0);
+}
+
+// Sizes of the head norm with rotation.
+int check_rotary(const cc1d_rotary_params& p) {
+    if (!valid_dtype(p.dtype)) return CC1D_ERR_DTYPE;
+    if (p.dim < 1 || p.dim > CC1D_MAX_ROTARY_DIM) return CC1D_ERR_HEAD_DIM;
+    if (p.rotated < 0 || p.rotated > p.dim || p.rotated % 2 != 0) return CC1D_ERR_ROTATED;
+    if (p.batch < 0 || p.seqlen < 0 || p.q_heads < 0 || p.k_heads < 0) return CC1D_ERR_SHAPE;
+    if (p.positions != nullptr && p.positions_bytes != 4 && p.positions_bytes != 8) return CC1D_ERR_DTYPE;
+    // a block a token at most
+    if ((double)p.batch * (double)p.seqlen >= (double)(1 << 24) || p.q_heads >= kMaxBlocks || p.k_heads >= kMaxBlocks) return CC1D_ERR_SHAPE;
+    if (p.rotated > 0 && p.inv_freq == nullptr && p.batch * p.seqlen > 0) return CC1D_ERR_NULL_POINTER;
+    return CC1D_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -109,6 +138,9 @@ const char* cc1d_strerror(int status) {
     case CC1D_ERR_DSTATE: return "dstate must be in 1..256";
     case CC1D_ERR_GROUPS: return "dim must be a multiple of groups";
     case CC1D_ERR_NORM_DIM: return "norm dim must be in 1..32768";
+    case CC1D_ERR_HEADS: return "heads must be a multiple of key_heads";
+    case CC1D_ERR_HEAD_DIM: return "a head's size must be in 1..128 (rotation: 1..256)";
+    case CC1D_ERR_ROTATED: return "rotated must be even and at most the head's size";
     default: return "unknown status";
     }
 }
@@ -288,6 +320,104 @@ int cc1d_norm_bwd(const cc1d_norm_bwd_params* b, void* stream) {
 int64_t cc1d_norm_bwd_workspace_floats(const cc1d_norm_bwd_params* b) {
     if (b == nullptr || check_norm(b->fwd) != CC1D_OK) return -1;
     return norm_bwd_workspace_floats(*b);
+}
+
+int cc1d_attn_fwd(const cc1d_attn_params* p, void* stream) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const int st = check_attn(*p);
+    if (st != CC1D_OK) return st;
+    if (attn_empty(*p)) return CC1D_OK;
+    // without positions only the states are read and written
+    if (p->seqlen == 0 && p->final_states == nullptr) return CC1D_OK;
+    if (p->seqlen > 0 && (p->q == nullptr || p->k == nullptr || p->v == nullptr || p->g == nullptr || p->out == nullptr))
+        return CC1D_ERR_NULL_POINTER;
+    const int64_t need = attn_workspace_floats(*p);
+    if (p->workspace_floats < need) return CC1D_ERR_WORKSPACE;
+    if (need > 0 && p->workspace == nullptr) return CC1D_ERR_NULL_POINTER;
+    return launch_attn_fwd(*p, static_cast<hipStream_t>(stream));
+}
+
+int64_t cc1d_attn_workspace_floats(const cc1d_attn_params* p) {
+    if (p == nullptr || check_attn(*p) != CC1D_OK) return -1;
+    return attn_empty(*p) ? 0 : attn_workspace_floats(*p);
+}
+
+int cc1d_attn_bwd(const cc1d_attn_bwd_params* b, void* stream) {
+    if (b == nullptr) return CC1D_ERR_NULL_POINTER;
+    const cc1d_attn_params& p = b->fwd;
+    const int st = check_attn(p);
+    if (st != CC1D_OK) return st;
+    if (attn_empty(p)) {
+        // no head adds to the gradients of q and k
+        const int64_t n = p.batch * p.seqlen * p.key_heads, strides[3] = {p.dk, 0, 1};
+        if (n == 0) return CC1D_OK;
+        if (b->dq == nullptr || b->dk == nullptr) return CC1D_ERR_NULL_POINTER;
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        const int zeroed = launch_zero3(b->dq, esize(p.dtype), n, 1, p.dk, strides, s);
+        return zeroed != CC1D_OK ? zeroed : launch_zero3(b->dk, esize(p.dtype), n, 1, p.dk, strides, s);
+    }
+    if (p.batch * p.seqlen > 0 &&
+        (p.q == nullptr || p.k == nullptr || p.v == nullptr || p.g == nullptr || b->dout == nullptr || b->dq == nullptr ||
+         b->dk == nullptr || b->dv == nullptr || b->dg == nullptr))
+        return CC1D_ERR_NULL_POINTER;
+    if (p.seqlen == 0 && b->dinitial_states == nullptr) return CC1D_OK;
+    const int64_t need = attn_bwd_workspace_floats(*b);
+    if (b->workspace_floats < need) return CC1D_ERR_WORKSPACE;
+    if (need > 0 && b->workspace == nullptr) return CC1D_ERR_NULL_POINTER;
+    return launch_attn_bwd(*b, static_cast<hipStream_t>(stream));
+}
+
+int64_t cc1d_attn_bwd_workspace_floats(const cc1d_attn_bwd_params* b) {
+    if (b == nullptr || check_attn(b->fwd) != CC1D_OK) return -1;
+    return attn_empty(b->fwd) ? 0 : attn_bwd_workspace_floats(*b);
+}
+
+int cc1d_attn_update(const cc1d_attn_update_params* p, void* stream) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    if (!valid_dtype(p->dtype)) return CC1D_ERR_DTYPE;
+    if (!attn_dim(p->dk) || !attn_dim(p->dv)) return CC1D_ERR_HEAD_DIM;
+    if (p->batch < 0 || p->tokens < 0 || p->heads < 0 || p->state_rows < 0) return CC1D_ERR_SHAPE;
+    if (p->key_heads < 1 || p->heads % p->key_heads != 0) return CC1D_ERR_HEADS;
+    if (p->attn_state_indices == nullptr && p->state_rows < p->batch) return CC1D_ERR_SHAPE;
+    if (p->batch == 0 || p->heads == 0 || p->tokens == 0) return CC1D_OK;
+    // a block per entry and head; a block's outputs are counted in 32 bits
+    if ((double)p->batch * (double)p->heads >= (double)(1 << 24) || p->tokens >= (1 << 23)) return CC1D_ERR_SHAPE;
+    if (p->q == nullptr || p->k == nullptr || p->v == nullptr || p->g == nullptr || p->out == nullptr ||
+        (p->attn_state == nullptr && p->state_rows > 0))
+        return CC1D_ERR_NULL_POINTER;
+    return launch_attn_update(*p, static_cast<hipStream_t>(stream));
+}
+
+int cc1d_rotary_fwd(const cc1d_rotary_params* p, void* stream) {
+    if (p == nullptr) return CC1D_ERR_NULL_POINTER;
+    const int st = check_rotary(*p);
+    if (st != CC1D_OK) return st;
+    if (p->batch * p->seqlen == 0 || p->q_heads + p->k_heads == 0) return CC1D_OK;
+    if ((p->q_heads > 0 && (p->q == nullptr || p->q_out == nullptr)) || (p->k_heads > 0 && (p->k == nullptr || p->k_out == nullptr)))
+        return CC1D_ERR_NULL_POINTER;
+    return launch_rotary_fwd(*p, static_cast<hipStream_t>(stream));
+}
+
+int cc1d_rotary_bwd(const cc1d_rotary_bwd_params* b, void* stream) {
+    if (b == nullptr) return CC1D_ERR_NULL_POINTER;
+    const cc1d_rotary_params& p = b->fwd;
+    const int st = check_rotary(p);
+    if (st != CC1D_OK) return st;
+    if ((p.q_weight != nullptr && b->dq_weight == nullptr) || (p.k_weight != nullptr && b->dk_weight == nullptr)) return CC1D_ERR_NULL_POINTER;
+    // (without tokens or heads the weights' gradients are sums over no terms: the kernels run)
+    if (p.batch * p.seqlen > 0 &&
+        ((p.q_heads > 0 && (b->dq_out == nullptr || b->dq == nullptr || (p.q_weight != nullptr && p.q == nullptr))) ||
+         (p.k_heads > 0 && (b->dk_out == nullptr || b->dk == nullptr || (p.k_weight != nullptr && p.k == nullptr)))))
+        return CC1D_ERR_NULL_POINTER;
+    const int64_t need = rotary_bwd_workspace_floats(*b);
+    if (b->workspace_floats < need) return CC1D_ERR_WORKSPACE;
+    if (need > 0 && b->workspace == nullptr) return CC1D_ERR_NULL_POINTER;
+    return launch_rotary_bwd(*b, static_cast<hipStream_t>(stream));
+}
+
+int64_t cc1d_rotary_bwd_workspace_floats(const cc1d_rotary_bwd_params* b) {
+    if (b == nullptr || check_rotary(b->fwd) != CC1D_OK) return -1;
+    return rotary_bwd_workspace_floats(*b);
 }
 
 }  // extern "C"

@@ -1,0 +1,404 @@
+// cc1d_attn.hip -- linear attention with a decay for each head: the plan of a
+// call (segments, workspace, jobs), and what runs beside its main kernel
+// (cc1d_attn_kernels.hpp): the states handed from segment to segment, the
+// gradient of the decays, and the sums over heads that share their queries.
+#include "cc1d_attn_kernels.hpp"
+
+namespace cc1d {
+namespace {
+
+constexpr int64_t kAlign = 4;  // floats
+
+int chunk_of(int dtype) { return dtype == CC1D_DTYPE_BF16 ? AttnType<bf16>::chunk : AttnType<float>::chunk; }
+
+struct Plan {
+    int64_t seqs, seg, slots, per_row;
+    bool cut() const { return slots > seqs; }
+};
+
+// Sequences run as one block per head where those fill the chip; longer ones
+// are cut into segments that run side by side, from states that a first pass
+// over keys and values alone provides.
+Plan plan_of(const cc1d_attn_params& p, int jobs) {
+    Plan pl;
+    pl.seqs = p.cu_seqlens ? p.num_seqs : p.batch;
+    const double work = (double)p.batch * (double)p.seqlen * (double)p.heads * jobs;
+    const int64_t c = chunk_of(p.dtype);
+    int64_t seg = (int64_t)(work / 768.0);
+    seg = ceil_div(seg < 256 ? 256 : seg, c) * c;
+    if (seg >= p.seqlen) {
+        pl.seg = ceil_div(p.seqlen > 0 ? p.seqlen : 1, c) * c;
+        pl.per_row = 1;
+        // (with cu_seqlens a slot starts at cu[i] / seg + i: seg has to be more than the last start)
+        if (p.cu_seqlens) pl.seg += c;
+        pl.slots = pl.seqs;
+    } else {
+        pl.seg = seg;
+        pl.per_row = ceil_div(p.seqlen, seg);
+        pl.slots = p.cu_seqlens ? p.seqlen / seg + p.num_seqs : p.batch * pl.per_row;
+    }
+    return pl;
+}
+
+int64_t aligned(int64_t n) { return ceil_div(n, kAlign) * kAlign; }
+
+AttnArgs args_of(const cc1d_attn_params& p, const Plan& pl, int jobs) {
+    AttnArgs a{};
+    a.g = p.g;
+    for (int i = 0; i < 3; ++i) a.g_stride[i] = p.g_stride[i];
+    a.cu = p.cu_seqlens;
+    a.batch = p.batch;
+    a.seqlen = p.seqlen;
+    a.num_seqs = pl.seqs;
+    a.seg = pl.seg;
+    a.heads = (uint32_t)p.heads;
+    a.jobs = (uint32_t)jobs;
+    a.slots = (uint32_t)pl.slots;
+    a.per_row = (uint32_t)pl.per_row;
+    a.heads_div = FastDiv(a.heads);
+    a.jobs_div = FastDiv(a.jobs);
+    a.row_div = FastDiv(a.per_row);
+    a.blocks = (uint32_t)(pl.slots * p.heads * jobs);
+    return a;
+}
+
+AttnOperand operand(const void* ptr, const int64_t (&s)[4], int64_t div) {
+    AttnOperand o{ptr, {}, (uint32_t)div};
+    for (int i = 0; i < 4; ++i) o.s[i] = s[i];
+    return o;
+}
+
+// (n, heads, rows, cols) contiguous
+AttnState state(float* ptr, int64_t heads, int64_t rows, int64_t cols) { return {ptr, {heads * rows * cols, rows * cols, cols, 1}}; }
+AttnState strided(const float* ptr, const int64_t (&s)[4]) { return {const_cast<float*>(ptr), {s[0], s[1], s[2], s[3]}}; }
+AttnState turned(AttnState s) {
+    const int64_t t = s.s[2];
+    s.s[2] = s.s[3];
+    s.s[3] = t;
+    return s;
+}
+
+int launch_jobs(int dtype, const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
+    return with_dtype(dtype, [&](auto t) { return launch_attn_jobs<decltype(t)>(a, da, dc, states, stream); });
+}
+
+// ---- states from segment to segment
+
+struct CombineArgs {
+    AttnArgs a;  // the segments (jobs of the first pass)
+    uint32_t pieces;  // of 256 values
+};
+
+// The first pass left in every slot what its segment adds to a state of 0;
+// afterwards a slot holds the state at its segment's start (a sequence's first
+// one is left out). A thread per value; the walk over the segments is serial.
+__global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg) {
+    const AttnArgs& a = arg.a;
+    const uint32_t rest = blockIdx.x / arg.pieces, jn = rest / a.heads, h = rest - jn * a.heads;
+    const AttnJob& job = a.job[jn];
+    const int64_t per = (int64_t)job.da * job.dc, e = (int64_t)(blockIdx.x - rest * arg.pieces) * 256 + threadIdx.x;
+    if (e >= per) return;
+    const int64_t row = e / job.dc, col = e % job.dc;
+    for (int64_t seq = blockIdx.y; seq < a.num_seqs; seq += gridDim.y) {
+        int64_t slot, len;
+        if (a.cu == nullptr) {
+            slot = seq * a.per_row;
+            len = a.seqlen;
+        } else {
+            const int64_t first = clamp_pos(a.cu[seq], a.seqlen);
+            len = clamp_pos(a.cu[seq + 1], a.seqlen) - first;
+            slot = first / a.seg + seq;
+        }
+        int64_t segs = len <= a.seg ? 1 : (len + a.seg - 1) / a.seg;
+        if (slot + segs > a.slots) segs = a.slots - slot;
+        if (segs < 2) continue;
+        float* at = job.seg.p + slot * job.seg.s[0] + h * job.seg.s[1] + row * job.seg.s[2] + col * job.seg.s[3];
+        float cur = job.first.p ? job.first.p[seq * job.first.s[0] + h * job.first.s[1] + row * job.first.s[2] + col * job.first.s[3]] : 0.0f;
+        float adds = *at;
+        for (int64_t i = 0; i + 1 < segs; ++i) {
+            cur = __builtin_fmaf(job.decay[(slot + i) * a.heads + h], cur, adds);
+            at += job.seg.s[0];
+            if (i + 2 < segs) adds = *at;
+            *at = cur;
+        }
+    }
+}
+
+int run_segments(const cc1d_attn_params& p, const Plan& pl, const AttnArgs& a, int da, int dc, hipStream_t stream) {
+    const int st = launch_jobs(p.dtype, a, da, dc, true, stream);
+    if (st != CC1D_OK) return st;
+    const uint32_t pieces = (uint32_t)ceil_div((int64_t)da * dc, 256);
+    const dim3 grid((unsigned)(pieces * p.heads * a.jobs), (unsigned)(pl.seqs < 1024 ? pl.seqs : 1024));
+    return launch(attn_combine_kernel, grid, dim3(256), stream, CombineArgs{a, pieces});
+}
+
+// ---- the gradient of the decays
+
+struct DecayGradArgs {
+    const float* row_dots;  // q . dq, (heads, tokens)
+    const float* col_dots;  // k . dk
+    const void* g;
+    void* dg;               // (tokens, heads)
+    AttnState dfinal, fin;  // p null: the final states are not used
+    int64_t g_stride[3];
+    const int32_t* cu;
+    int64_t seqlen, num_seqs, tokens, heads;
+    int32_t dk, dv;
+};
+
+// dg[t] = <G, S> after the sequence's last position + sum over s >= t of
+// (q . dq - k . dk)[s]: a position's decay carries all that is written before
+// it and read from it on, and what is written and read on one side cancels.
+// The sums run in 64 bits. A block per sequence and head; 4 bytes twice a
+// position, read once.
+template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_kernel(const DecayGradArgs a) {
+    __shared__ double part[4];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int64_t seq = blockIdx.x / (uint32_t)a.heads, h = blockIdx.x - (uint32_t)seq * (uint32_t)a.heads;
+    int64_t first = 0, len = a.seqlen, row = seq;
+    if (a.cu) {
+        row = 0;
+        first = clamp_pos(ld_uniform(a.cu + seq), a.seqlen);
+        len = clamp_pos(ld_uniform(a.cu + seq + 1), a.seqlen) - first;
+        if (len < 0) len = 0;
+    }
+    auto block_sum = [&](double v) {  // of everybody's
+        const double s = lane63(wave_prefix_f64(v));
+        __syncthreads();
+        if (lane == 0) part[wave] = s;
+        __syncthreads();
+        return (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    double carry = 0.0;
+    if (a.dfinal.p) {
+        const float* x = a.dfinal.p + seq * a.dfinal.s[0] + h * a.dfinal.s[1];
+        const float* y = a.fin.p + seq * a.fin.s[0] + h * a.fin.s[1];
+        double s = 0.0;
+        for (int i = tid; i < a.dk * a.dv; i += 256) {
+            const int64_t r = i / a.dv, c = i % a.dv;
+            s += (double)x[r * a.dfinal.s[2] + c * a.dfinal.s[3]] * (double)y[r * a.fin.s[2] + c * a.fin.s[3]];
+        }
+        carry = block_sum(s);
+    }
+    const int64_t base = row * a.seqlen;
+    T* const dg = static_cast<T*>(a.dg);
+    const T* const g = static_cast<const T*>(a.g) + row * a.g_stride[0] + h * a.g_stride[2];
+    constexpr int K = 4;  // positions a thread
+    for (int64_t end = first + len; end > first; end -= 256 * K) {
+        // thread t has positions end - 1 - K t - i
+        double v[K], sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int64_t t = end - 1 - K * tid - i;
+            if (t >= first) {
+                const int64_t at = h * a.tokens + base + t;
+                sum += (double)a.row_dots[at] - (double)a.col_dots[at];
+            }
+            v[i] = sum;
+        }
+        const double incl = wave_prefix_f64(sum);
+        __syncthreads();
+        if (lane == 63) part[wave] = incl;
+        __syncthreads();
+        double before = carry + incl - sum;
+        for (int w = 0; w < wave; ++w) before += part[w];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int64_t t = end - 1 - K * tid - i;
+            // nothing is carried over a decay of 0
+            if (t >= first) dg[(base + t) * a.heads + h] = from_f32<T>(to_f32(g[t * a.g_stride[1]]) < -1e5f ? 0.0f : (float)(before + v[i]));
+        }
+        carry += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    if (a.cu) {
+        if (seq == 0)
+            for (int64_t t = tid; t < first; t += 256) dg[t * a.heads + h] = from_f32<T>(0.0f);
+        if (seq == a.num_seqs - 1)
+            for (int64_t t = first + len + tid; t < a.seqlen; t += 256) dg[t * a.heads + h] = from_f32<T>(0.0f);
+    }
+}
+
+// ---- sums over the heads that share a key head
+
+struct GroupSumArgs {
+    const float* part[2];  // (tokens, heads, dk)
+    void* out[2];          // (tokens, key_heads, dk)
+    int64_t n;             // values of out
+    int32_t each, dk;      // heads to a key head
+};
+
+template <typename T> __global__ void __launch_bounds__(256) attn_group_sum_kernel(const GroupSumArgs a) {
+    const float* const part = a.part[blockIdx.y];
+    T* const out = static_cast<T*>(a.out[blockIdx.y]);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n; i += (int64_t)gridDim.x * 256) {
+        const int64_t head = i / a.dk, c = i - head * a.dk;
+        const float* at = part + head * a.each * a.dk + c;
+        float s = 0.0f;
+        for (int r = 0; r < a.each; ++r) s += at[(int64_t)r * a.dk];
+        out[i] = from_f32<T>(s);
+    }
+}
+
+// The backward's workspace, in floats.
+struct Room {
+    int64_t dots, part, seg, decay, fin, total;
+};
+Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
+    const cc1d_attn_params& p = b.fwd;
+    const int64_t tokens = p.batch * p.seqlen, per = p.heads * p.dk * p.dv;
+    Room r;
+    r.dots = aligned(tokens * p.heads);
+    r.part = p.heads == p.key_heads ? 0 : aligned(tokens * p.heads * p.dk);
+    r.seg = pl.cut() ? aligned(pl.slots * per) : 0;
+    r.decay = pl.cut() ? aligned(pl.slots * p.heads) : 0;
+    r.fin = b.dfinal_states ? aligned(pl.seqs * per) : 0;
+    r.total = 2 * r.dots + 2 * r.part + 2 * r.seg + 2 * r.decay + r.fin;
+    return r;
+}
+
+}  // namespace
+
+bool attn_fits(const cc1d_attn_params& p) {
+    // blocks of 256 threads, 32-bit thread counts: one a slot, head and job, or one a piece of 256 values of a state
+    const double seqs = p.cu_seqlens ? (double)p.num_seqs : (double)p.batch;
+    if ((double)p.heads >= (double)(1 << 20) || seqs * (double)p.heads * kAttnJobs >= (double)(1 << 23)) return false;
+    if ((double)p.batch * (double)p.seqlen >= (double)((int64_t)1 << 40) || p.seqlen >= ((int64_t)1 << 31) - 4096) return false;
+    return (double)plan_of(p, kAttnJobs).slots * (double)p.heads * kAttnJobs < (double)(1 << 24) &&
+           (double)plan_of(p, 1).slots * (double)p.heads < (double)(1 << 24) && (double)p.heads * 2 * 64 < (double)(1 << 24);
+}
+
+int64_t attn_workspace_floats(const cc1d_attn_params& p) {
+    const Plan pl = plan_of(p, 1);
+    return pl.cut() ? aligned(pl.slots * p.heads * p.dk * p.dv) + aligned(pl.slots * p.heads) : 0;
+}
+
+int launch_attn_fwd(const cc1d_attn_params& p, hipStream_t stream) {
+    const Plan pl = plan_of(p, 1);
+    const int64_t per = p.heads / p.key_heads;
+    AttnArgs a = args_of(p, pl, 1);
+    AttnJob& j = a.job[0];
+    j.a = operand(p.q, p.q_stride, per);
+    j.b = operand(p.k, p.k_stride, per);
+    j.c = operand(p.v, p.v_stride, 1);
+    j.first = strided(p.initial_states, p.initial_states_stride);
+    j.last = state(p.final_states, p.heads, p.dk, p.dv);
+    j.out = p.out;
+    j.da = (int32_t)p.dk;
+    j.dc = (int32_t)p.dv;
+    j.p_scale = j.in_scale = (float)p.scale;
+    j.w_scale = 1.0f;
+    if (pl.cut()) {
+        j.seg = state(p.workspace, p.heads, p.dk, p.dv);
+        j.decay = p.workspace + aligned(pl.slots * p.heads * p.dk * p.dv);
+        const int st = run_segments(p, pl, a, (int)p.dk, (int)p.dv, stream);
+        if (st != CC1D_OK) return st;
+    }
+    return launch_jobs(p.dtype, a, (int)p.dk, (int)p.dv, false, stream);
+}
+
+int64_t attn_bwd_workspace_floats(const cc1d_attn_bwd_params& b) { return room_of(b, plan_of(b.fwd, kAttnJobs)).total; }
+
+int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
+    const cc1d_attn_params& p = b.fwd;
+    const Plan pl = plan_of(p, kAttnJobs);
+    const Room room = room_of(b, pl);
+    const int64_t per = p.heads / p.key_heads, tokens = p.batch * p.seqlen;
+    const int dk = (int)p.dk, dv = (int)p.dv;
+    const bool shared = per > 1;
+    float* ws = b.workspace;
+    auto take = [&ws](int64_t n) {
+        float* at = n ? ws : nullptr;
+        ws += n;
+        return at;
+    };
+    float *const row_dots = take(room.dots), *const col_dots = take(room.dots);
+    float *const dq_part = take(room.part), *const dk_part = take(room.part);
+    float *const seg_s = take(room.seg), *const seg_g = take(room.seg);
+    float *const decay_s = take(room.decay), *const decay_g = take(room.decay);
+    float* const fin = take(room.fin);
+
+    const AttnOperand q = operand(p.q, p.q_stride, per), k = operand(p.k, p.k_stride, per), v = operand(p.v, p.v_stride, 1);
+    const AttnOperand d = operand(b.dout, b.dout_stride, 1);
+    const AttnState first = strided(p.initial_states, p.initial_states_stride);
+    const AttnState last_grad = strided(b.dfinal_states, b.dfinal_states_stride);
+    const float scale = (float)p.scale;
+
+    AttnJob jq{}, jk{}, jv{};
+    jq.a = d; jq.b = v; jq.c = k; jq.x = q;
+    jq.first = turned(first);
+    jq.last = turned(state(fin, p.heads, dk, dv));
+    jq.seg = turned(state(seg_s, p.heads, dk, dv));
+    jq.decay = decay_s;
+    jq.out = shared ? dq_part : b.dq;
+    jq.dots = row_dots;
+    jq.da = dv; jq.dc = dk;
+    jq.p_scale = jq.in_scale = scale; jq.w_scale = 1.0f;
+    jq.out_f32 = shared;
+
+    jk.a = v; jk.b = d; jk.c = q; jk.x = k;
+    jk.first = turned(last_grad);
+    jk.seg = turned(state(seg_g, p.heads, dk, dv));
+    jk.decay = decay_g;
+    jk.out = shared ? dk_part : b.dk;
+    jk.dots = col_dots;
+    jk.da = dv; jk.dc = dk;
+    jk.p_scale = jk.w_scale = scale; jk.in_scale = 1.0f;
+    jk.reverse = 1;
+    jk.out_f32 = shared;
+
+    jv.a = k; jv.b = q; jv.c = d;
+    jv.first = last_grad;
+    jv.last = state(b.dinitial_states, p.heads, dk, dv);
+    jv.seg = state(seg_g, p.heads, dk, dv);
+    jv.decay = decay_g;
+    jv.out = b.dv;
+    jv.da = dk; jv.dc = dv;
+    jv.p_scale = jv.w_scale = scale; jv.in_scale = 1.0f;
+    jv.reverse = 1;
+
+    if (pl.cut()) {
+        // both states as (dk, dv): K^T V forwards, Q^T dO backwards
+        AttnArgs s = args_of(p, pl, 2);
+        s.job[0] = jv;
+        s.job[0].b = k; s.job[0].c = v;
+        s.job[0].first = first;
+        s.job[0].seg = state(seg_s, p.heads, dk, dv);
+        s.job[0].decay = decay_s;
+        s.job[0].w_scale = 1.0f;
+        s.job[0].reverse = 0;
+        s.job[1] = jv;
+        const int st = run_segments(p, pl, s, dk, dv, stream);
+        if (st != CC1D_OK) return st;
+    }
+    int st;
+    const bool alike = (dk <= 64) == (dv <= 64);  // one kernel for all
+    if (alike) {
+        AttnArgs a = args_of(p, pl, 3);
+        a.job[0] = jq; a.job[1] = jk; a.job[2] = jv;
+        st = launch_jobs(p.dtype, a, dk, dv, false, stream);
+    } else {
+        AttnArgs a = args_of(p, pl, 2);
+        a.job[0] = jq; a.job[1] = jk;
+        st = launch_jobs(p.dtype, a, dv, dk, false, stream);
+        if (st != CC1D_OK) return st;
+        AttnArgs c = args_of(p, pl, 1);
+        c.job[0] = jv;
+        st = launch_jobs(p.dtype, c, dk, dv, false, stream);
+    }
+    if (st != CC1D_OK) return st;
+    if (tokens == 0) return CC1D_OK;
+    DecayGradArgs dg{row_dots, col_dots, p.g, b.dg, last_grad, state(fin, p.heads, dk, dv), {}, p.cu_seqlens,
+                     p.seqlen, pl.seqs, tokens, p.heads, dk, dv};
+    for (int i = 0; i < 3; ++i) dg.g_stride[i] = p.g_stride[i];
+    st = with_dtype(p.dtype, [&](auto t) {
+        return launch(attn_decay_grad_kernel<decltype(t)>, dim3((unsigned)(p.heads * pl.seqs)), dim3(256), stream, dg);
+    });
+    if (st != CC1D_OK || !shared) return st;
+    const GroupSumArgs gs{{dq_part, dk_part}, {b.dq, b.dk}, tokens * p.key_heads * p.dk, (int32_t)per, dk};
+    const int64_t blocks = ceil_div(gs.n, 256);
+    return with_dtype(p.dtype, [&](auto t) {
+        return launch(attn_group_sum_kernel<decltype(t)>, dim3((unsigned)(blocks < 65536 ? blocks : 65536), 2), dim3(256), stream, gs);
+    });
+}
+
+}  // namespace cc1d

@@ -1,0 +1,10 @@
+// cc1d_attn_fp32.hip -- linear attention's kernels for fp32.
+#include "cc1d_attn_kernels.hpp"
+
+namespace cc1d {
+
+template <> int launch_attn_jobs<float>(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
+    return states ? launch_attn_sizes<float, true>(a, da, dc, stream) : launch_attn_sizes<float, false>(a, da, dc, stream);
+}
+
+}  // namespace cc1d

@@ -1,0 +1,670 @@
+// cc1d_attn_kernels.hpp -- linear attention with a decay for each head, on
+// the matrix cores.
+//
+// Per sequence and head S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T and out[t] =
+// scale q[t]^T S[t]. Over a chunk of C positions with c the inclusive sums of
+// its g and M[i][j] = exp(c_i - c_j) for i >= j, else 0,
+//     O     = scale (Q K^T o M) V + diag(exp c) scale Q S_in
+//     S_out = exp(c_last) S_in + (diag(exp(c_last - c)) K)^T V,
+// four matrix products a chunk. No exponent is ever positive for g <= 0, so
+// nothing overflows however long the chunk's decay is.
+//
+// The gradients are the same operator on other operands (G the gradient of S
+// after a position):
+//     dQ: rows dO, columns V,  values K, state S^T, forwards in time
+//     dK: rows V,  columns dO, values Q, state G^T, backwards
+//     dV: rows K,  columns Q,  values dO, state G,  backwards
+// (run backwards the decay between two positions is the same product, so g
+// comes shifted by one position). One kernel computes all of them; a job says
+// which operands it reads, which way, and where the scale goes.
+//
+// Precision: operands are held in LDS as bf16 planes whose sum is the value:
+// one for bf16, two for fp16, three for fp32 (8 bits each), and products of
+// planes are summed in fp32 by the MFMAs until what is left out is below the
+// result's own rounding: planes a + b <= 1 (2^-17) where only 16-bit outputs
+// follow, a + b <= 2 (2^-25) in fp32 and for the states, which are fp32
+// whatever the type. bf16 planes have fp32's range, so nothing overflows on
+// the way that fp32 holds.
+#pragma once
+
+#include "cc1d_internal.hpp"
+#include "cc1d_scan_device.hpp"
+
+namespace cc1d {
+
+// Pointers and strides (batch, position, head, element) of one operand; head h
+// reads the operand's head h / div.
+struct AttnOperand {
+    const void* p;
+    int64_t s[4];
+    uint32_t div;
+};
+
+struct AttnState {
+    float* p;
+    int64_t s[4];  // (sequence or segment slot, head, row, column)
+};
+
+struct AttnJob {
+    AttnOperand a, b, c;  // rows, columns, values
+    AttnOperand x;        // dotted with the outputs; p null: no dots
+    AttnState first;      // state before the first position; p null: 0
+    AttnState last;       // state after the last; p null: not wanted
+    AttnState seg;        // state at the start of each segment but a sequence's first; p null: whole sequences
+    float* decay;         // (slots, heads): a segment's decay
+    void* out;            // (batch * seqlen, heads, dc) contiguous
+    float* dots;          // (heads, batch * seqlen)
+    int32_t da, dc;       // sizes of rows and columns, of values
+    float p_scale, in_scale, w_scale;  // on the pairs, on what the state gives, on what it takes
+    int32_t reverse, out_f32;
+};
+
+constexpr int kAttnJobs = 3;
+
+struct AttnArgs {
+    AttnJob job[kAttnJobs];
+    const void* g;
+    int64_t g_stride[3];
+    const int32_t* cu;
+    int64_t batch, seqlen, num_seqs;
+    int64_t seg;  // positions of a segment, a multiple of the chunk
+    uint32_t heads, jobs, slots, per_row;  // slots of all sequences; of one (without cu)
+    FastDiv heads_div, jobs_div, row_div;
+    uint32_t blocks;
+};
+
+template <typename T> struct AttnType;
+template <> struct AttnType<bf16> { static constexpr int planes = 1, chunk = 64, order = 1; };
+template <> struct AttnType<f16> { static constexpr int planes = 2, chunk = 32, order = 1; };
+template <> struct AttnType<float> { static constexpr int planes = 3, chunk = 32, order = 2; };
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// 2 N values as P planes of bf16, two to a dword
+template <int P, int N> __device__ __forceinline__ void to_planes(const float (&v)[2 * N], uint32_t (&out)[P][N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const uint32_t w = pack2<bf16>(a, b);
+            out[p][i] = w;
+            if (p + 1 < P) {
+                a -= __uint_as_float(w << 16);
+                b -= __uint_as_float(w & 0xffff0000u);
+            }
+        }
+    }
+}
+__device__ __forceinline__ bf16x8 as_frag(const uint32_t (&w)[4]) { return __builtin_bit_cast(bf16x8, w); }
+
+// 16-byte block `blk` of an LDS row, permuted so that neither the rows that a
+// fragment takes nor the columns that a transposing store takes share banks
+template <int BLKS> __device__ __forceinline__ int swizzle(int row, int blk) {
+    if constexpr (BLKS >= 8) return blk ^ ((row ^ (row >> 3)) & 7);
+    else return blk ^ (((row >> 1) ^ (row >> 3)) & (BLKS - 1));
+}
+
+// exp2 of a sum held in two floats: the second is at most an ulp of the first
+__device__ __forceinline__ float exp2_sum(float hi, float lo) {
+    return __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
+}
+
+// Inclusive prefix sums over 64 lanes, in 64 bits.
+template <int CTRL, int ROW_MASK> __device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROW_MASK, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROW_MASK, 0xf, true);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_prefix_f64(double v) {
+    v += dpp_f64<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_f64<0x112, 0xf>(v);
+    v += dpp_f64<0x114, 0xf>(v);
+    v += dpp_f64<0x118, 0xf>(v);
+    v += dpp_f64<kDppRowBcast15, 0xa>(v);
+    v += dpp_f64<kDppRowBcast31, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ double lane63(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, 63), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
+// A log decay as the sums take it: -1e5 stands for everything below (its
+// exponential is 0), so that sums of -inf have differences.
+__device__ __forceinline__ double log_decay(float g) { return g < -1e5f ? -1e5 : (double)g; }
+
+// Where a block works: a sequence's segment.
+struct AttnSpan {
+    int64_t seq, first, len;  // the sequence; its first position and length
+    int64_t slot;             // of its first segment
+    int64_t segs, index;      // its segments, and which of them this is
+    bool live;
+};
+
+__device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, uint32_t slot) {
+    AttnSpan s;
+    if (a.cu == nullptr) {
+        s.seq = a.row_div.div(slot);
+        s.first = 0;
+        s.len = a.seqlen;
+        s.slot = s.seq * a.per_row;
+    } else {
+        // sequence i has the slots from cu[i] / seg + i on: the last that starts at or before this one
+        int64_t lo = 0, hi = a.num_seqs - 1;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) >> 1;
+            if (clamp_pos(ld_uniform(a.cu + mid), a.seqlen) / a.seg + mid <= slot) lo = mid;
+            else hi = mid - 1;
+        }
+        s.seq = lo;
+        s.first = clamp_pos(ld_uniform(a.cu + lo), a.seqlen);
+        s.len = clamp_pos(ld_uniform(a.cu + lo + 1), a.seqlen) - s.first;
+        if (s.len < 0) s.len = 0;
+        s.slot = s.first / a.seg + lo;
+    }
+    s.segs = s.len <= a.seg ? 1 : (s.len + a.seg - 1) / a.seg;
+    s.index = (int64_t)slot - s.slot;
+    s.live = s.index >= 0 && s.index < s.segs;
+    return s;
+}
+
+// What one thread carries of a chunk of one operand from HBM to LDS: units of
+// 4 positions x one 16-byte vector, so that four positions of a column leave
+// for the transposed image in one store.
+template <typename T, int C, int D> struct AttnTile {
+    static constexpr int EPV = elems16<T>::value, CGS = D / EPV, UNITS = C / 4 * CGS, N = (UNITS + 255) / 256;
+    static constexpr int P = AttnType<T>::planes;
+    u32x4 v[N][4];
+
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = n * 256 + threadIdx.x, row = u / CGS * 4, col = u % CGS * EPV;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[n][i] = vzero();
+                if ((UNITS % 256 == 0 || u < UNITS) && row + i < rows && col < d) {
+                    const T* at = base + (row + i) * row_stride + col * elem_stride;
+                    if (elem_stride == 1 && col + EPV <= d) {
+                        v[n][i] = vload_any(at);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < EPV; ++e)
+                            if (col + e < d) put(v[n][i], e, at[e * elem_stride]);
+                    }
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void put(u32x4& w, int e, T x) {
+        if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(to_f32(x));
+        else w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, x) << (16 * (e & 1));
+    }
+    // whether anything is infinite or NaN
+    __device__ __forceinline__ bool wild() const {
+        constexpr uint32_t M = sizeof(T) == 4 ? 0x7f800000u : (std::is_same_v<T, bf16> ? 0x7f807f80u : 0x7c007c00u);
+        bool w = false;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t x = v[n][i][d] & M;
+                    w = w || (x >> 16) == (M >> 16) || (sizeof(T) == 2 && (x & 0xffffu) == (M & 0xffffu));
+                }
+        return w;
+    }
+    // rows[plane][position][column] and / or cols[plane][column][position]
+    template <bool ROWS, bool COLS> __device__ __forceinline__ void store(uint16_t* rows, uint16_t* cols) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = n * 256 + threadIdx.x, row = u / CGS * 4, col = u % CGS * EPV;
+            if (UNITS % 256 != 0 && u >= UNITS) continue;
+            uint32_t w[4][P][EPV / 2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (std::is_same_v<T, bf16>) {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) w[i][0][d] = v[n][i][d];
+                } else {
+                    float f[EPV];
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) f[e] = vget<T>(v[n][i], e);
+                    to_planes<P, EPV / 2>(f, w[i]);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                if constexpr (ROWS) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint16_t* at = rows + (p * C + row + i) * D + swizzle<D / 8>(row + i, col >> 3) * 8 + (col & 7);
+                        if constexpr (EPV == 8) *reinterpret_cast<u32x4*>(at) = u32x4{w[i][p][0], w[i][p][1], w[i][p][2], w[i][p][3]};
+                        else *reinterpret_cast<u32x2*>(at) = u32x2{w[i][p][0], w[i][p][1]};
+                    }
+                }
+                if constexpr (COLS) {
+#pragma unroll
+                    for (int e = 0; e < EPV; ++e) {
+                        const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;  // the high or the low halves of two dwords
+                        const u32x2 q = {__builtin_amdgcn_perm(w[1][p][e >> 1], w[0][p][e >> 1], sel),
+                                         __builtin_amdgcn_perm(w[3][p][e >> 1], w[2][p][e >> 1], sel)};
+                        *reinterpret_cast<u32x2*>(cols + (p * D + col + e) * C + swizzle<C / 8>(col + e, row >> 3) * 8 + (row & 7)) = q;
+                    }
+                }
+            }
+        }
+    }
+};
+
+// One job of one segment of one head. Four wavefronts; each holds 16 * NT of
+// the state's columns with all its rows in registers (the accumulators of
+// S += K^T V), where they are at once the left operand of Q S: an accumulator
+// has four neighbouring rows of a column, and the order in which a product
+// runs over its inner index is free, so Q's fragments are read in that order.
+// The pairs' products are shared: each wavefront forms a quarter of their
+// tiles and passes them through LDS.
+// STATES: the state alone, of the segments that another one follows.
+template <typename T, int DA, int DC, bool STATES> __global__ void __launch_bounds__(256, 2) attn_kernel(const AttnArgs args) {
+    typedef AttnType<T> Ty;
+    constexpr int C = Ty::chunk, P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
+    constexpr int NT = DC / 64, TA = DA / 16, SC = C / 32, SA = DA / 32, IT = C / 16;
+    constexpr int TILES = C == 64 ? 12 : 4;  // of the pairs, with the empty ones that a product reads
+    constexpr int kA = STATES ? 0 : P * C * DA, kPairs = PP * C * C;
+    constexpr int kB = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
+    __shared__ __attribute__((aligned(16))) uint16_t lds[kA + kB + P * DA * C + P * DC * C];
+    __shared__ __attribute__((aligned(16))) float sums_hi[2][C], sums_lo[2][C], into[2][C], left[2][C], whole[2];
+    __shared__ float dot_lds[4][C];
+    __shared__ int wild_flag;
+    uint16_t *const ldsA = lds, *const ldsB = lds + kA, *const ldsBT = lds + kA + kB, *const ldsCT = ldsBT + P * DA * C;
+    uint16_t* const ldsP = ldsB;  // the columns are dead once the pairs' products are formed
+
+    const int tid = threadIdx.x, wave = uniform32(tid >> 6), lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+    const uint32_t id = xcd_block(blockIdx.x, args.blocks);
+    const uint32_t rest = args.jobs_div.div(id), jn = id - rest * args.jobs;
+    const uint32_t slot = args.heads_div.div(rest), h = rest - slot * args.heads;
+    const AttnJob& job = args.job[jn];
+    const AttnSpan sp = attn_span(args, slot);
+    if (!sp.live || (STATES && sp.index + 1 == sp.segs)) return;
+    const int64_t r0_seg = sp.index * args.seg, r1_seg = r0_seg + args.seg < sp.len ? r0_seg + args.seg : sp.len;
+    const int64_t row0 = args.cu ? 0 : sp.seq;  // batch row
+    const int da = job.da, dc = job.dc;
+    const bool reverse = job.reverse;
+    const int64_t dir = reverse ? -1 : 1, p0 = reverse ? sp.first + sp.len - 1 : sp.first;
+
+    auto base = [&](const AttnOperand& o) {
+        return static_cast<const T*>(o.p) + row0 * o.s[0] + p0 * o.s[1] + (int64_t)(h / o.div) * o.s[2];
+    };
+    const T *const pa = base(job.a), *const pb = base(job.b), *const pc = base(job.c);
+    const int64_t sa = dir * job.a.s[1], sb = dir * job.b.s[1], sc = dir * job.c.s[1];
+    const T* const pg = static_cast<const T*>(args.g) + row0 * args.g_stride[0] + h * args.g_stride[2];
+
+    // ---- the state at the segment's start
+    const int col0 = wave * 16 * NT + l16;  // this lane's column (of its first tile)
+    f32x4 S[TA][NT];
+    {
+        const bool from_seg = sp.index > 0;
+        const AttnState& st = from_seg ? job.seg : job.first;
+        const float* at = st.p == nullptr || STATES ? nullptr : st.p + (from_seg ? (int64_t)slot : sp.seq) * st.s[0] + h * st.s[1];
+#pragma unroll
+        for (int t = 0; t < TA; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * t + 4 * g4 + r, col = col0 + 16 * n;
+                    S[t][n][r] = at != nullptr && row < da && col < dc ? at[row * st.s[2] + col * st.s[3]] : 0.0f;
+                }
+    }
+
+    // ---- decays of the rows from r on (by one wavefront)
+    double total = 0.0;
+    auto g_load = [&](int64_t r, int n) {
+        if (lane >= n) return 0.0f;
+        // backwards, a position's decay is the one of the position after it, and the sequence's last has none
+        const int64_t at = reverse ? p0 - (r + lane) + 1 : p0 + r + lane;
+        return reverse && r + lane == 0 ? 0.0f : to_f32(pg[at * args.g_stride[1]]);
+    };
+    auto decays = [&](float g, int buf) {
+        const double c = wave_prefix_f64(log_decay(g) * 1.4426950408889634), end = lane63(c);
+        total += end;
+        const float hi = (float)c, lo = (float)(c - (double)hi);
+        const float ehi = (float)end, elo = (float)(end - (double)ehi);
+        if (lane < C) {
+            sums_hi[buf][lane] = hi;
+            sums_lo[buf][lane] = lo;
+            into[buf][lane] = exp2_sum(hi, lo) * job.in_scale;
+            left[buf][lane] = __builtin_amdgcn_exp2f((ehi - hi) + (elo - lo)) * job.w_scale;
+        }
+        if (lane == 0) whole[buf] = exp2_sum(ehi, elo);
+    };
+
+    AttnTile<T, C, DA> ta, tb;
+    AttnTile<T, C, DC> tc;
+    auto load = [&](int64_t r, int n) {
+        if constexpr (!STATES) ta.load(pa + r * sa, sa, job.a.s[3], n, da);
+        tb.load(pb + r * sb, sb, job.b.s[3], n, da);
+        tc.load(pc + r * sc, sc, job.c.s[3], n, dc);
+    };
+    auto rows_at = [&](int64_t r) { return (int)(r1_seg - r < C ? r1_seg - r : C); };
+
+    int64_t r = r0_seg, single = 0;  // rows before `single` go one by one
+    int n = rows_at(r), buf = 0;
+    float g_next = 0.0f;
+    if (tid == 0) wild_flag = 0;
+    if (n > 0) {
+        load(r, n);
+        if (wave == 3) decays(g_load(r, n), 0);
+    }
+    __syncthreads();
+    while (r < r1_seg) {
+        // ---- the chunk into LDS
+        ta.template store<true, false>(ldsA, nullptr);
+        if constexpr (STATES) tb.template store<false, true>(nullptr, ldsBT);
+        else tb.template store<true, true>(ldsB, ldsBT);
+        tc.template store<false, true>(nullptr, ldsCT);
+        if constexpr (!STATES)
+            if (tc.wild()) wild_flag = 1;
+        __syncthreads();
+        // An infinite or NaN value is multiplied with the zeros of the pairs that come before it: such a chunk goes
+        // position by position, so that it reaches the later ones alone.
+        if (!STATES && wild_flag && n > 1) {
+            single = r + n;
+            n = 1;
+            load(r, 1);
+            const float g = wave == 3 ? g_load(r, 1) : 0.0f;
+            __syncthreads();
+            if (wave == 3) decays(g, buf);
+            if (tid == 0) wild_flag = 0;
+            __syncthreads();
+            continue;
+        }
+        const int64_t r_next = r + n;
+        const int n_next = r_next >= r1_seg ? 0 : (r_next < single ? 1 : rows_at(r_next));
+        if (n_next > 0) {
+            load(r_next, n_next);
+            if (wave == 3) g_next = g_load(r_next, n_next);
+        }
+
+        f32x4 O[IT][NT];
+        float x[IT][NT][4];
+        if constexpr (!STATES) {
+            if (job.dots != nullptr) {
+                const T* px = base(job.x);
+#pragma unroll
+                for (int it = 0; it < IT; ++it)
+#pragma unroll
+                    for (int m = 0; m < NT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 16 * it + l16, col = wave * 16 * NT + 16 * m + 4 * g4 + e;
+                            x[it][m][e] = i < n && col < dc ? to_f32(px[dir * (r + i) * job.x.s[1] + col * job.x.s[3]]) : 0.0f;
+                        }
+            }
+            // ---- pairs: tile (rows it, columns jt) transposed, so that a lane gets four columns of a row
+            uint32_t pw[TILES / 4][PP][2];
+#pragma unroll
+            for (int k = 0; k < TILES / 4; ++k) {
+                const int tile = k * 4 + wave;
+                int it, jt;
+                if constexpr (C == 64) {
+                    it = tile < 2 ? 0 : tile < 4 ? 1 : tile < 8 ? 2 : 3;
+                    jt = tile < 4 ? tile & 1 : tile & 3;
+                } else {
+                    it = tile >> 1;
+                    jt = tile & 1;
+                }
+                float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (jt <= it) {
+                    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < SA; ++s) {
+                        bf16x8 fa[P], fb[P];
+                        const int ia = 16 * it + l16, ib = 16 * jt + l16;
+#pragma unroll
+                        for (int p = 0; p < P; ++p) {
+                            fa[p] = *reinterpret_cast<const bf16x8*>(ldsA + (p * C + ia) * DA + swizzle<DA / 8>(ia, 4 * s + g4) * 8);
+                            fb[p] = *reinterpret_cast<const bf16x8*>(ldsB + (p * C + ib) * DA + swizzle<DA / 8>(ib, 4 * s + g4) * 8);
+                        }
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+#pragma unroll
+                            for (int q = 0; q < P; ++q)
+                                if (p + q <= ORD) acc = mfma(fb[p], fa[q], acc);
+                    }
+                    const int i = 16 * it + l16;
+                    const float hi = sums_hi[buf][i], lo = sums_lo[buf][i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = 16 * jt + 4 * g4 + e;
+                        const float m = __builtin_amdgcn_exp2f((hi - sums_hi[buf][j]) + (lo - sums_lo[buf][j])) * job.p_scale;
+                        f[e] = j <= i ? acc[e] * m : 0.0f;
+                    }
+                }
+                to_planes<PP, 2>(f, pw[k]);
+            }
+            // ---- what the state gives
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+#pragma unroll
+                for (int m = 0; m < NT; ++m) O[it][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < SA; ++s) {
+                uint32_t sw[NT][PP][4];
+#pragma unroll
+                for (int m = 0; m < NT; ++m) {
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f[e] = S[2 * s][m][e];
+                        f[4 + e] = S[2 * s + 1][m][e];
+                    }
+                    to_planes<PP, 4>(f, sw[m]);
+                }
+#pragma unroll
+                for (int it = 0; it < IT; ++it) {
+                    const int i = 16 * it + l16;
+#pragma unroll
+                    for (int q = 0; q < P; ++q) {
+                        const uint16_t* at = ldsA + (q * C + i) * DA + (g4 & 1) * 4;
+                        const u32x2 w0 = *reinterpret_cast<const u32x2*>(at + swizzle<DA / 8>(i, 4 * s + (g4 >> 1)) * 8);
+                        const u32x2 w1 = *reinterpret_cast<const u32x2*>(at + swizzle<DA / 8>(i, 4 * s + 2 + (g4 >> 1)) * 8);
+                        const uint32_t w[4] = {w0[0], w0[1], w1[0], w1[1]};
+#pragma unroll
+                        for (int p = 0; p < PP; ++p)
+#pragma unroll
+                            for (int m = 0; m < NT; ++m)
+                                if (p + q <= ORD) O[it][m] = mfma(as_frag(sw[m][p]), as_frag(w), O[it][m]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
+                const float e = into[buf][16 * it + l16];
+#pragma unroll
+                for (int m = 0; m < NT; ++m) O[it][m] *= e;
+            }
+            __syncthreads();
+            if (tid == 0) wild_flag = 0;
+            // ---- the pairs to everybody
+#pragma unroll
+            for (int k = 0; k < TILES / 4; ++k) {
+                const int tile = k * 4 + wave;
+                int it, jt;
+                if constexpr (C == 64) {
+                    it = tile < 2 ? 0 : tile < 4 ? 1 : tile < 8 ? 2 : 3;
+                    jt = tile < 4 ? tile & 1 : tile & 3;
+                } else {
+                    it = tile >> 1;
+                    jt = tile & 1;
+                }
+                const int i = 16 * it + l16;
+#pragma unroll
+                for (int p = 0; p < PP; ++p)
+                    *reinterpret_cast<u32x2*>(ldsP + (p * C + i) * C + swizzle<C / 8>(i, 2 * jt + (g4 >> 1)) * 8 + (g4 & 1) * 4) =
+                        u32x2{pw[k][p][0], pw[k][p][1]};
+            }
+            __syncthreads();
+        }
+        const float decay = whole[buf];
+#pragma unroll
+        for (int t = 0; t < TA; ++t)
+#pragma unroll
+            for (int m = 0; m < NT; ++m) S[t][m] *= decay;
+#pragma unroll
+        for (int s = 0; s < SC; ++s) {
+            bf16x8 fc[NT][P];
+            uint32_t ww[NT][3][4];
+            float w8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w8[e] = left[buf][32 * s + 8 * g4 + e];
+#pragma unroll
+            for (int m = 0; m < NT; ++m) {
+                const int col = col0 + 16 * m;
+                float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int p = P - 1; p >= 0; --p) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(ldsCT + (p * DC + col) * C + swizzle<C / 8>(col, 4 * s + g4) * 8);
+                    fc[m][p] = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] += vget<bf16>(w, e);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= w8[e];
+                to_planes<3, 4>(f, ww[m]);
+            }
+            if constexpr (!STATES) {
+#pragma unroll
+                for (int it = 2 * s; it < IT; ++it) {
+                    const int i = 16 * it + l16;
+#pragma unroll
+                    for (int q = 0; q < PP; ++q) {
+                        const bf16x8 fp = *reinterpret_cast<const bf16x8*>(ldsP + (q * C + i) * C + swizzle<C / 8>(i, 4 * s + g4) * 8);
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+#pragma unroll
+                            for (int m = 0; m < NT; ++m)
+                                if (p + q <= ORD) O[it][m] = mfma(fc[m][p], fp, O[it][m]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TA; ++t) {
+                const int row = 16 * t + l16;
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const bf16x8 fb = *reinterpret_cast<const bf16x8*>(ldsBT + (p * DA + row) * C + swizzle<C / 8>(row, 4 * s + g4) * 8);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+#pragma unroll
+                        for (int m = 0; m < NT; ++m)
+                            if (p + q <= 2) S[t][m] = mfma(fb, as_frag(ww[m][q]), S[t][m]);
+                }
+            }
+        }
+        if constexpr (!STATES) {
+            // ---- outputs: a lane has four columns of a row
+            const int64_t tokens = args.batch * args.seqlen, t0 = row0 * args.seqlen + p0;
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
+                const int i = 16 * it + l16;
+                const int64_t tok = t0 + dir * (r + i);
+                float dot = 0.0f;
+#pragma unroll
+                for (int m = 0; m < NT; ++m) {
+                    const int col = wave * 16 * NT + 16 * m + 4 * g4;
+                    if (job.dots != nullptr)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[it][m][e], dot);
+                    if (i >= n || col >= dc) continue;
+                    const int64_t at = (tok * args.heads + h) * dc + col;
+                    const int some = dc - col;
+                    if (job.out_f32 || sizeof(T) == 4) {
+                        float* o = static_cast<float*>(job.out) + at;
+                        if (some >= 4) *reinterpret_cast<AnyAddr<4>::v4*>(o) = __builtin_bit_cast(u32x4, O[it][m]);
+                        else
+                            for (int e = 0; e < some; ++e) o[e] = O[it][m][e];
+                    } else {
+                        T* o = static_cast<T*>(job.out) + at;
+                        if (some >= 4) {
+                            typedef typename AnyAddr<sizeof(T)>::v2 any2;
+                            if constexpr (sizeof(T) == 2)
+                                *reinterpret_cast<any2*>(o) = u32x2{pack2<T>(O[it][m][0], O[it][m][1]), pack2<T>(O[it][m][2], O[it][m][3])};
+                        } else {
+                            for (int e = 0; e < some; ++e) o[e] = from_f32<T>(O[it][m][e]);
+                        }
+                    }
+                }
+                if (job.dots != nullptr) {
+                    dot += __shfl_xor(dot, 16);
+                    dot += __shfl_xor(dot, 32);
+                    if (g4 == 0) dot_lds[wave][i] = dot;
+                }
+            }
+            if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
+            __syncthreads();
+            if (job.dots != nullptr && tid < n)
+                job.dots[h * tokens + t0 + dir * (r + tid)] = (dot_lds[0][tid] + dot_lds[1][tid]) + (dot_lds[2][tid] + dot_lds[3][tid]);
+        } else {
+            if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
+            __syncthreads();
+        }
+        buf ^= 1;
+        r = r_next;
+        n = n_next;
+    }
+
+    // ---- the state at the segment's end
+    const bool ends = sp.index + 1 == sp.segs;
+    const AttnState& st = STATES ? job.seg : job.last;
+    if (st.p != nullptr && (STATES || ends)) {
+        float* at = st.p + (STATES ? (int64_t)slot : sp.seq) * st.s[0] + h * st.s[1];
+        float by = 1.0f;
+        // backwards, the state before the sequence has its first decay too
+        if (!STATES && reverse && sp.len > 0) by = (float)exp(log_decay(to_f32(pg[sp.first * args.g_stride[1]])));
+#pragma unroll
+        for (int t = 0; t < TA; ++t)
+#pragma unroll
+            for (int m = 0; m < NT; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 16 * t + 4 * g4 + e, col = col0 + 16 * m;
+                    if (row < da && col < dc) at[row * st.s[2] + col * st.s[3]] = by * S[t][m][e];
+                }
+    }
+    if (STATES && tid == 3 * 64) job.decay[(int64_t)slot * args.heads + h] = (float)exp2(total);
+    // positions that no sequence covers
+    if (!STATES && args.cu != nullptr) {
+        auto zero = [&](int64_t from, int64_t to) {
+            for (int64_t i = tid; i < (to - from) * dc; i += 256) {
+                const int64_t at = ((from + i / dc) * args.heads + h) * dc + i % dc;
+                if (job.out_f32) static_cast<float*>(job.out)[at] = 0.0f;
+                else static_cast<T*>(job.out)[at] = from_f32<T>(0.0f);
+            }
+        };
+        if (sp.seq == 0 && sp.index == 0) zero(0, sp.first);
+        if (sp.seq == args.num_seqs - 1 && ends) zero(sp.first + sp.len, args.seqlen);
+    }
+}
+
+template <typename T, bool STATES> int launch_attn_sizes(const AttnArgs& a, int da, int dc, hipStream_t stream) {
+    const dim3 grid(a.blocks), block(256);
+    if (da <= 64 && dc <= 64) return launch(attn_kernel<T, 64, 64, STATES>, grid, block, stream, a);
+    if (da <= 64) return launch(attn_kernel<T, 64, 128, STATES>, grid, block, stream, a);
+    if (dc <= 64) return launch(attn_kernel<T, 128, 64, STATES>, grid, block, stream, a);
+    return launch(attn_kernel<T, 128, 128, STATES>, grid, block, stream, a);
+}
+
+// All jobs of `a` have rows of da and values of dc (explicitly instantiated in cc1d_attn_<dtype>.hip).
+template <typename T> int launch_attn_jobs(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream);
+
+}  // namespace cc1d

@@ -1,0 +1,135 @@
+// cc1d_attn_update.hip -- decode step of linear attention with a decay for
+// each head.
+//
+// Per (batch entry, head) the state's dk x dv values are read, moved by one
+// step per new token (S = exp(g) S + k v^T), multiplied with q, and written
+// back: 8 bytes of state a value, everything else is shared by its rows or
+// columns, so HBM bounds it.
+#include "cc1d_scan_device.hpp"
+
+namespace cc1d {
+namespace {
+
+struct AttnUpdateArgs {
+    cc1d_attn_update_params p;
+    FastDiv heads, group, quads;  // of quads: a row's groups of four columns
+    int32_t row_groups;           // rows that a block's threads take at once
+};
+
+// A block holds one state in registers, four columns of R rows a thread (all
+// loads in flight at once), and takes the tokens one after the other: the sum
+// over its own rows, then over the threads that share columns through LDS.
+template <typename T, int R, bool VEC> __global__ void __launch_bounds__(256) attn_update_kernel(const AttnUpdateArgs arg) {
+    const cc1d_attn_update_params& p = arg.p;
+    __shared__ float ql[2][CC1D_MAX_ATTN_DIM], kl[2][CC1D_MAX_ATTN_DIM];
+    __shared__ __attribute__((aligned(16))) float vl[2][CC1D_MAX_ATTN_DIM + 4], part[256 * 4];
+    __shared__ float decay[2];
+    const int tid = threadIdx.x, dk = (int)p.dk, dv = (int)p.dv, tokens = (int)p.tokens;
+    const uint32_t b = arg.heads.div(blockIdx.x), h = blockIdx.x - b * (uint32_t)p.heads;
+    T* const out = static_cast<T*>(p.out) + ((int64_t)b * tokens * p.heads + h) * dv;
+    const int64_t step = p.heads * dv;
+    const int64_t row = p.attn_state_indices ? ld_uniform(p.attn_state_indices + b) : b;
+    if (row < 0 || row >= p.state_rows) {
+        for (int i = tid; i < tokens * dv; i += 256) out[i / dv * step + i % dv] = T{};
+        return;
+    }
+    const int rg = (int)arg.quads.div((uint32_t)tid), quad = tid - rg * (int)arg.quads.d, col = 4 * quad;
+    const bool mine = rg < arg.row_groups;
+    float* const state = p.attn_state + row * p.attn_state_stride[0] + (int64_t)h * p.attn_state_stride[1] + col * p.attn_state_stride[3];
+    float S[R][4];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = rg + i * arg.row_groups;
+        const float* at = state + r * p.attn_state_stride[2];
+        const bool here = mine && r < dk;
+        if constexpr (VEC) {
+            u32x4 w = vzero();
+            if (here) w = vload_any_nt(at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][e] = __uint_as_float(w[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][e] = here && col + e < dv ? at[e * p.attn_state_stride[3]] : 0.0f;
+        }
+    }
+    const uint32_t kh = arg.group.div(h);
+    const T* const q = static_cast<const T*>(p.q) + b * p.q_stride[0] + kh * p.q_stride[2];
+    const T* const k = static_cast<const T*>(p.k) + b * p.k_stride[0] + kh * p.k_stride[2];
+    const T* const v = static_cast<const T*>(p.v) + b * p.v_stride[0] + h * p.v_stride[2];
+    const T* const g = static_cast<const T*>(p.g) + b * p.g_stride[0] + h * p.g_stride[2];
+    const float scale = (float)p.scale;
+    auto fetch = [&](int t, int buf) {  // one wavefront each for q, k and v, and the decay
+        const int lane = tid & 63, w = tid >> 6;
+        for (int i = lane; i < CC1D_MAX_ATTN_DIM; i += 64) {
+            if (w == 0 && i < dk) ql[buf][i] = to_f32(q[t * p.q_stride[1] + i * p.q_stride[3]]) * scale;
+            if (w == 1 && i < dk) kl[buf][i] = to_f32(k[t * p.k_stride[1] + i * p.k_stride[3]]);
+            if (w == 2) vl[buf][i] = i < dv ? to_f32(v[t * p.v_stride[1] + i * p.v_stride[3]]) : 0.0f;
+        }
+        if (tid == 192) decay[buf] = __builtin_amdgcn_exp2f(to_f32(g[t * p.g_stride[1]]) * 1.4426950408889634f);
+    };
+    fetch(0, 0);
+    __syncthreads();
+    for (int t = 0; t < tokens; ++t) {
+        const int buf = t & 1;
+        const float e = decay[buf];
+        float vq[4], acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vq[c] = vl[buf][(col < CC1D_MAX_ATTN_DIM ? col : 0) + c];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = rg + i * arg.row_groups;
+            const bool here = mine && r < dk;
+            const float kr = here ? kl[buf][r] : 0.0f, qr = here ? ql[buf][r] : 0.0f;
+            if (!here) continue;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                S[i][c] = __builtin_fmaf(e, S[i][c], kr * vq[c]);
+                acc[c] = __builtin_fmaf(qr, S[i][c], acc[c]);
+            }
+        }
+        if (mine) *reinterpret_cast<u32x4*>(part + 4 * tid) = u32x4{__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3])};
+        if (t + 1 < tokens) fetch(t + 1, buf ^ 1);
+        __syncthreads();
+        const int width = 4 * (int)arg.quads.d;  // part is (row_groups, width)
+        if (tid < dv) {
+            float y = 0.0f;
+            for (int r = 0; r < arg.row_groups; ++r) y += part[r * width + tid];
+            out[t * step + tid] = from_f32<T>(y);
+        }
+        if (t + 1 < tokens) __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = rg + i * arg.row_groups;
+        float* at = state + r * p.attn_state_stride[2];
+        if (!mine || r >= dk) continue;
+        if constexpr (VEC) {
+            vstore_any_nt(at, u32x4{__float_as_uint(S[i][0]), __float_as_uint(S[i][1]), __float_as_uint(S[i][2]), __float_as_uint(S[i][3])});
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < dv) at[e * p.attn_state_stride[3]] = S[i][e];
+        }
+    }
+}
+
+}  // namespace
+
+int launch_attn_update(const cc1d_attn_update_params& p, hipStream_t stream) {
+    AttnUpdateArgs a{p, FastDiv((uint32_t)p.heads), FastDiv((uint32_t)(p.heads / p.key_heads)), FastDiv((uint32_t)ceil_div(p.dv, 4)), 0};
+    a.row_groups = (int)(256 / a.quads.d);
+    const int rows = (int)ceil_div(p.dk, a.row_groups);
+    const dim3 grid((unsigned)(p.batch * p.heads));
+    const bool vec = p.dv % 4 == 0 && p.attn_state_stride[3] == 1;
+    return with_dtype(p.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        return with_flag(vec, [&](auto vv) {
+            constexpr bool VEC = decltype(vv)::value;
+            if (rows <= 4) return launch(attn_update_kernel<T, 4, VEC>, grid, dim3(256), stream, a);
+            if (rows <= 8) return launch(attn_update_kernel<T, 8, VEC>, grid, dim3(256), stream, a);
+            return launch(attn_update_kernel<T, 16, VEC>, grid, dim3(256), stream, a);
+        });
+    });
+}
+
+}  // namespace cc1d

@@ -41,6 +41,16 @@ int launch_norm_fwd(const cc1d_norm_params& p, hipStream_t stream);
 int launch_norm_bwd(const cc1d_norm_bwd_params& b, hipStream_t stream);
 int64_t norm_bwd_workspace_floats(const cc1d_norm_bwd_params& b);
 
+bool attn_fits(const cc1d_attn_params& p);  // its grids
+int launch_attn_fwd(const cc1d_attn_params& p, hipStream_t stream);
+int64_t attn_workspace_floats(const cc1d_attn_params& p);
+int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream);
+int64_t attn_bwd_workspace_floats(const cc1d_attn_bwd_params& b);
+int launch_attn_update(const cc1d_attn_update_params& p, hipStream_t stream);
+int launch_rotary_fwd(const cc1d_rotary_params& p, hipStream_t stream);
+int launch_rotary_bwd(const cc1d_rotary_bwd_params& b, hipStream_t stream);
+int64_t rotary_bwd_workspace_floats(const cc1d_rotary_bwd_params& b);
+
 // Compile-time dispatch over the runtime dtype code / width / flags.
 template <typename F> int with_dtype(int dtype, F&& f) {
     switch (dtype) {

@@ -331,5 +331,6 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "cc1d_host", "native host path of c
 PyMODINIT_FUNC PyInit_cc1d_host(void) {
     PyObject* m = PyModule_Create(&module);
     if (m != nullptr && PyModule_AddFunctions(m, ssm_methods) != 0) Py_CLEAR(m);
+    if (m != nullptr && PyModule_AddFunctions(m, attn_methods) != 0) Py_CLEAR(m);
     return m;
 }

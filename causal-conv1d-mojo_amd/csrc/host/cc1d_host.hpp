@@ -88,7 +88,8 @@ inline Tensor match_layout(const Tensor& t, const Tensor& like) {
 
 inline PyObject* not_implemented() { Py_RETURN_NOTIMPLEMENTED; }
 
-extern PyMethodDef ssm_methods[];  // cc1d_host_ssm.cpp
+extern PyMethodDef ssm_methods[];   // cc1d_host_ssm.cpp
+extern PyMethodDef attn_methods[];  // cc1d_host_attn.cpp
 
 #define CC1D_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
 

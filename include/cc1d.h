@@ -66,11 +66,16 @@ enum cc1d_status {
                                        CC1D_NOALLOC_WORKSPACE_FLOATS floats of workspace */
     CC1D_ERR_DSTATE = 10,           /* dstate outside 1..CC1D_MAX_DSTATE */
     CC1D_ERR_GROUPS = 11,           /* groups < 1, or dim not a multiple of it */
-    CC1D_ERR_NORM_DIM = 12          /* norm dim outside 1..CC1D_MAX_NORM_DIM */
+    CC1D_ERR_NORM_DIM = 12,         /* norm dim outside 1..CC1D_MAX_NORM_DIM */
+    CC1D_ERR_HEADS = 13,            /* key_heads < 1, or heads not a multiple of it */
+    CC1D_ERR_HEAD_DIM = 14,         /* a head's size outside 1..CC1D_MAX_ATTN_DIM (rotation: CC1D_MAX_ROTARY_DIM) */
+    CC1D_ERR_ROTATED = 15           /* rotated is odd, negative or more than the head's size */
 };
 
 #define CC1D_MAX_DSTATE 256
 #define CC1D_MAX_NORM_DIM 32768
+#define CC1D_MAX_ATTN_DIM 128
+#define CC1D_MAX_ROTARY_DIM 256
 
 /* Size (fp32 elements) of the static device scratch of cc1d_bwd_typed_noalloc: 8 MiB, reserved on
    every GPU where the library's kernels are loaded, whether or not cc1d_bwd_typed_noalloc is called
@@ -365,6 +370,131 @@ typedef struct cc1d_norm_bwd_params {
     int64_t dy_stride, dsum_stride, dx_stride, dresidual_stride;
 } cc1d_norm_bwd_params;
 
+/*
+ * Linear attention with a decay for each head, over prompts. Per sequence and
+ * head, with key head h / (heads / key_heads) for head h,
+ *     S[t] = exp(g[t]) S[t-1] + k[t] v[t]^T              (dk x dv values of state)
+ *     out[t] = scale * q[t]^T S[t].
+ * Sequences are the batch rows, or with cu_seqlens the runs [cu[i], cu[i+1])
+ * of the one batch row (its values are clamped to [0, seqlen] and have to be
+ * non-decreasing); S before the first position is initial_states, or 0.
+ * Positions that no sequence covers get 0. g is a log decay: any value up to
+ * 0, and -inf (nothing is kept), positive ones as far as the sums stay finite.
+ * q, k, v, g and out share dtype; states are fp32, sums of g run in 64 bits.
+ */
+typedef struct cc1d_attn_params {
+    const void* q;                 /* (batch, seqlen, key_heads, dk) */
+    const void* k;                 /* (batch, seqlen, key_heads, dk) */
+    const void* v;                 /* (batch, seqlen, heads, dv) */
+    const void* g;                 /* (batch, seqlen, heads) */
+    const int32_t* cu_seqlens;     /* (num_seqs + 1,) contiguous or NULL; batch is 1 */
+    const float* initial_states;   /* (sequences, heads, dk, dv) or NULL */
+    void* out;                     /* (batch, seqlen, heads, dv) contiguous */
+    float* final_states;           /* (sequences, heads, dk, dv) contiguous, or NULL */
+    float* workspace;              /* cc1d_attn_workspace_floats() floats, NULL if that is 0 */
+    int64_t workspace_floats;
+    int64_t batch, seqlen, heads, key_heads, dk, dv, num_seqs;
+    int64_t q_stride[4];
+    int64_t k_stride[4];
+    int64_t v_stride[4];
+    int64_t g_stride[3];
+    int64_t initial_states_stride[4];
+    double scale;
+    int32_t dtype;
+} cc1d_attn_params;
+
+/*
+ * Its backward: `fwd` as it was given to cc1d_attn_fwd (out, final_states and
+ * the workspace are not read), dout and dfinal_states the gradients of its
+ * results. Every sum runs in a fixed order. The gradients are contiguous, in
+ * the shapes of what they belong to; dinitial_states may be NULL.
+ */
+typedef struct cc1d_attn_bwd_params {
+    cc1d_attn_params fwd;
+    const void* dout;              /* (batch, seqlen, heads, dv) */
+    const float* dfinal_states;    /* (sequences, heads, dk, dv) or NULL */
+    void* dq;
+    void* dk;
+    void* dv;
+    void* dg;
+    float* dinitial_states;        /* or NULL */
+    float* workspace;              /* cc1d_attn_bwd_workspace_floats() floats */
+    int64_t workspace_floats;
+    int64_t dout_stride[4];
+    int64_t dfinal_states_stride[4];
+} cc1d_attn_bwd_params;
+
+/*
+ * The same for `tokens` new tokens (one or a few) per sequence of a decode
+ * batch, on a state pool updated in place. attn_state_indices redirects batch
+ * entry b to that row of the pool; an index < 0 (padding) or >= state_rows
+ * zeroes out[b] and leaves the pool untouched. Live entries name distinct rows.
+ */
+typedef struct cc1d_attn_update_params {
+    const void* q;                 /* (batch, tokens, key_heads, dk) */
+    const void* k;
+    const void* v;                 /* (batch, tokens, heads, dv) */
+    const void* g;                 /* (batch, tokens, heads) */
+    float* attn_state;             /* (state_rows, heads, dk, dv), updated */
+    const int32_t* attn_state_indices; /* (batch,) contiguous or NULL */
+    void* out;                     /* (batch, tokens, heads, dv) contiguous */
+    int64_t batch, tokens, heads, key_heads, dk, dv, state_rows;
+    int64_t q_stride[4];
+    int64_t k_stride[4];
+    int64_t v_stride[4];
+    int64_t g_stride[3];
+    int64_t attn_state_stride[4];
+    double scale;
+    int32_t dtype;
+} cc1d_attn_update_params;
+
+/*
+ * Norm of each query and key head, and rotation by position, in one pass:
+ *     x^ = x / sqrt(mean(x^2) + eps) * weight             (x without a weight)
+ * then the first `rotated` values of a head are turned in pairs,
+ *     (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq[i],
+ * pair i being values i and i + rotated / 2, or 2 i and 2 i + 1 when
+ * interleaved is set. The rest of a head is not turned and not scaled.
+ * Angles are formed in 64 bits; each output is rounded once.
+ */
+typedef struct cc1d_rotary_params {
+    const void* q;                 /* (batch, seqlen, q_heads, dim) */
+    const void* k;                 /* (batch, seqlen, k_heads, dim) */
+    const float* q_weight;         /* (dim,) contiguous, or NULL: no norm of q */
+    const float* k_weight;         /* (dim,) contiguous, or NULL: no norm of k */
+    const float* inv_freq;         /* (rotated / 2,) contiguous; not read when rotated is 0 */
+    const void* positions;         /* (batch, seqlen) int32 or int64, or NULL: 0 .. seqlen - 1 in every row */
+    void* q_out;                   /* contiguous */
+    void* k_out;                   /* contiguous */
+    int64_t batch, seqlen, q_heads, k_heads, dim, rotated;
+    int64_t q_stride[4];
+    int64_t k_stride[4];
+    int64_t positions_stride[2];
+    double eps, amplitude;
+    int32_t dtype;
+    int32_t positions_bytes;       /* 4 or 8 */
+    int32_t interleaved;
+} cc1d_rotary_params;
+
+/*
+ * Its backward: `fwd` as in the forward (q_out and k_out are not read; q and
+ * k only where they have a weight). The weights' gradients are summed in a
+ * fixed order over partial sums in the workspace.
+ */
+typedef struct cc1d_rotary_bwd_params {
+    cc1d_rotary_params fwd;
+    const void* dq_out;            /* (batch, seqlen, q_heads, dim) */
+    const void* dk_out;            /* (batch, seqlen, k_heads, dim) */
+    void* dq;                      /* contiguous */
+    void* dk;                      /* contiguous */
+    float* dq_weight;              /* (dim,); required when q_weight is given */
+    float* dk_weight;              /* (dim,); required when k_weight is given */
+    float* workspace;              /* cc1d_rotary_bwd_workspace_floats() floats */
+    int64_t workspace_floats;
+    int64_t dq_out_stride[4];
+    int64_t dk_out_stride[4];
+} cc1d_rotary_bwd_params;
+
 int cc1d_abi_version(void);
 const char* cc1d_strerror(int status);
 
@@ -419,6 +549,19 @@ int cc1d_scan_update(const cc1d_scan_update_params* params, void* stream);
 int cc1d_norm_fwd(const cc1d_norm_params* params, void* stream);
 int cc1d_norm_bwd(const cc1d_norm_bwd_params* params, void* stream);
 int64_t cc1d_norm_bwd_workspace_floats(const cc1d_norm_bwd_params* params);
+
+/*
+ * Linear attention, its decode step, and the head norm with rotation. The
+ * workspaces follow the rules above.
+ */
+int cc1d_attn_fwd(const cc1d_attn_params* params, void* stream);
+int64_t cc1d_attn_workspace_floats(const cc1d_attn_params* params);
+int cc1d_attn_bwd(const cc1d_attn_bwd_params* params, void* stream);
+int64_t cc1d_attn_bwd_workspace_floats(const cc1d_attn_bwd_params* params);
+int cc1d_attn_update(const cc1d_attn_update_params* params, void* stream);
+int cc1d_rotary_fwd(const cc1d_rotary_params* params, void* stream);
+int cc1d_rotary_bwd(const cc1d_rotary_bwd_params* params, void* stream);
+int64_t cc1d_rotary_bwd_workspace_floats(const cc1d_rotary_bwd_params* params);
 
 #ifdef __cplusplus
 }
