@@ -110,6 +110,19 @@ template <int BLKS> __device__ __forceinline__ int swizzle(int row, int blk) {
     else return blk ^ (((row >> 1) ^ (row >> 3)) & (BLKS - 1));
 }
 
+// Byte offsets of fragments: row 16 t + (lane & 15) of an image whose rows have
+// BLKS blocks, block b + (what the lane adds): a base of the lane's, xor a
+// constant of the tile's.
+template <int BLKS> __device__ __forceinline__ uint32_t frag_base(int l16, int blk, int half) {
+    return (uint32_t)(l16 * BLKS * 16 + swizzle<BLKS>(l16, blk) * 16 + half * 8);
+}
+template <int BLKS> __device__ __forceinline__ uint32_t frag_tile(int t, int blk) {
+    return (uint32_t)(t * 16 * BLKS * 16 | ((blk ^ (2 * t & (BLKS >= 8 ? 7 : BLKS - 1))) * 16));
+}
+template <typename V> __device__ __forceinline__ V lds_at(const uint16_t* image, uint32_t off) {
+    return *reinterpret_cast<const V*>(reinterpret_cast<const char*>(image) + off);
+}
+
 // exp2 of a sum held in two floats: the second is at most an ulp of the first
 __device__ __forceinline__ float exp2_sum(float hi, float lo) {
     return __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
@@ -184,10 +197,12 @@ template <typename T, int C, int D> struct AttnTile {
     static constexpr int P = AttnType<T>::planes;
     u32x4 v[N][4];
 
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d) {
+    // tid: the thread's index (not a loop invariant to the compiler: a register for every address would not leave
+    // enough for the state)
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, int tid) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int u = n * 256 + threadIdx.x, row = u / CGS * 4, col = u % CGS * EPV;
+            const int u = n * 256 + tid, row = u / CGS * 4, col = u % CGS * EPV;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 v[n][i] = vzero();
@@ -208,6 +223,12 @@ template <typename T, int C, int D> struct AttnTile {
         if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(to_f32(x));
         else w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, x) << (16 * (e & 1));
     }
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[n][i] = vzero();
+    }
     // whether anything is infinite or NaN
     __device__ __forceinline__ bool wild() const {
         constexpr uint32_t M = sizeof(T) == 4 ? 0x7f800000u : (std::is_same_v<T, bf16> ? 0x7f807f80u : 0x7c007c00u);
@@ -224,10 +245,10 @@ template <typename T, int C, int D> struct AttnTile {
         return w;
     }
     // rows[plane][position][column] and / or cols[plane][column][position]
-    template <bool ROWS, bool COLS> __device__ __forceinline__ void store(uint16_t* rows, uint16_t* cols) const {
+    template <bool ROWS, bool COLS> __device__ __forceinline__ void store(uint16_t* rows, uint16_t* cols, int tid) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int u = n * 256 + threadIdx.x, row = u / CGS * 4, col = u % CGS * EPV;
+            const int u = n * 256 + tid, row = u / CGS * 4, col = u % CGS * EPV;
             if (UNITS % 256 != 0 && u >= UNITS) continue;
             uint32_t w[4][P][EPV / 2];
 #pragma unroll
@@ -304,6 +325,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
     auto base = [&](const AttnOperand& o) {
         return static_cast<const T*>(o.p) + row0 * o.s[0] + p0 * o.s[1] + (int64_t)(h / o.div) * o.s[2];
     };
+    const T* const px = job.dots ? base(job.x) : nullptr;
     const T *const pa = base(job.a), *const pb = base(job.b), *const pc = base(job.c);
     const int64_t sa = dir * job.a.s[1], sb = dir * job.b.s[1], sc = dir * job.c.s[1];
     const T* const pg = static_cast<const T*>(args.g) + row0 * args.g_stride[0] + h * args.g_stride[2];
@@ -350,70 +372,64 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
 
     AttnTile<T, C, DA> ta, tb;
     AttnTile<T, C, DC> tc;
-    auto load = [&](int64_t r, int n) {
-        if constexpr (!STATES) ta.load(pa + r * sa, sa, job.a.s[3], n, da);
-        tb.load(pb + r * sb, sb, job.b.s[3], n, da);
-        tc.load(pc + r * sc, sc, job.c.s[3], n, dc);
+    auto load = [&](int64_t r, int n, int t) {
+        if constexpr (!STATES) ta.load(pa + r * sa, sa, job.a.s[3], n, da, t);
+        tb.load(pb + r * sb, sb, job.b.s[3], n, da, t);
+        tc.load(pc + r * sc, sc, job.c.s[3], n, dc, t);
     };
     auto rows_at = [&](int64_t r) { return (int)(r1_seg - r < C ? r1_seg - r : C); };
 
+    // The loop loads a chunk while it works on the one before; its first turn only loads.
     int64_t r = r0_seg, single = 0;  // rows before `single` go one by one
-    int n = rows_at(r), buf = 0;
-    float g_next = 0.0f;
+    int n = 0, buf = 1;
     if (tid == 0) wild_flag = 0;
-    if (n > 0) {
-        load(r, n);
-        if (wave == 3) decays(g_load(r, n), 0);
-    }
-    __syncthreads();
-    while (r < r1_seg) {
+    ta.none();
+    tb.none();
+    tc.none();
+    for (;;) {
+        const int otid = opaque(tid), l16 = otid & 15, g4 = (otid >> 4) & 3;
         // ---- the chunk into LDS
-        ta.template store<true, false>(ldsA, nullptr);
-        if constexpr (STATES) tb.template store<false, true>(nullptr, ldsBT);
-        else tb.template store<true, true>(ldsB, ldsBT);
-        tc.template store<false, true>(nullptr, ldsCT);
+        if constexpr (STATES) {
+            tb.template store<false, true>(nullptr, ldsBT, otid);
+        } else {
+            ta.template store<true, false>(ldsA, nullptr, otid);
+            tb.template store<true, true>(ldsB, ldsBT, otid);
+        }
+        tc.template store<false, true>(nullptr, ldsCT, otid);
         if constexpr (!STATES)
             if (tc.wild()) wild_flag = 1;
         __syncthreads();
         // An infinite or NaN value is multiplied with the zeros of the pairs that come before it: such a chunk goes
         // position by position, so that it reaches the later ones alone.
-        if (!STATES && wild_flag && n > 1) {
-            single = r + n;
-            n = 1;
-            load(r, 1);
-            const float g = wave == 3 ? g_load(r, 1) : 0.0f;
-            __syncthreads();
-            if (wave == 3) decays(g, buf);
-            if (tid == 0) wild_flag = 0;
-            __syncthreads();
-            continue;
-        }
-        const int64_t r_next = r + n;
+        const bool again = !STATES && wild_flag && n > 1;
+        if (again) single = r + n;
+        const int64_t r_next = again ? r : r + n;
         const int n_next = r_next >= r1_seg ? 0 : (r_next < single ? 1 : rows_at(r_next));
+        float g_next = 0.0f;
         if (n_next > 0) {
-            load(r_next, n_next);
+            load(r_next, n_next, otid);
             if (wave == 3) g_next = g_load(r_next, n_next);
         }
+        if (n == 0 || again) {
+            if (n_next == 0) break;
+            __syncthreads();  // everybody has seen the flag
+            if (tid == 0) wild_flag = 0;
+            buf ^= 1;
+            if (wave == 3) decays(g_next, buf);
+            r = r_next;
+            n = n_next;
+            continue;
+        }
 
+        const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0), halfD = frag_base<DA / 8>(l16, g4 >> 1, g4 & 1);
+        const uint32_t fragC = frag_base<C / 8>(l16, g4, 0), halfC = frag_base<C / 8>(l16, g4 >> 1, g4 & 1);
         f32x4 O[IT][NT];
-        float x[IT][NT][4];
         if constexpr (!STATES) {
-            if (job.dots != nullptr) {
-                const T* px = base(job.x);
-#pragma unroll
-                for (int it = 0; it < IT; ++it)
-#pragma unroll
-                    for (int m = 0; m < NT; ++m)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = 16 * it + l16, col = wave * 16 * NT + 16 * m + 4 * g4 + e;
-                            x[it][m][e] = i < n && col < dc ? to_f32(px[dir * (r + i) * job.x.s[1] + col * job.x.s[3]]) : 0.0f;
-                        }
-            }
             // ---- pairs: tile (rows it, columns jt) transposed, so that a lane gets four columns of a row
             uint32_t pw[TILES / 4][PP][2];
 #pragma unroll
             for (int k = 0; k < TILES / 4; ++k) {
+                __builtin_amdgcn_sched_barrier(0);
                 const int tile = k * 4 + wave;
                 int it, jt;
                 if constexpr (C == 64) {
@@ -429,11 +445,10 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
 #pragma unroll
                     for (int s = 0; s < SA; ++s) {
                         bf16x8 fa[P], fb[P];
-                        const int ia = 16 * it + l16, ib = 16 * jt + l16;
 #pragma unroll
                         for (int p = 0; p < P; ++p) {
-                            fa[p] = *reinterpret_cast<const bf16x8*>(ldsA + (p * C + ia) * DA + swizzle<DA / 8>(ia, 4 * s + g4) * 8);
-                            fb[p] = *reinterpret_cast<const bf16x8*>(ldsB + (p * C + ib) * DA + swizzle<DA / 8>(ib, 4 * s + g4) * 8);
+                            fa[p] = lds_at<bf16x8>(ldsA + p * C * DA, fragD ^ frag_tile<DA / 8>(it, 4 * s));
+                            fb[p] = lds_at<bf16x8>(ldsB + p * C * DA, fragD ^ frag_tile<DA / 8>(jt, 4 * s));
                         }
 #pragma unroll
                         for (int p = 0; p < P; ++p)
@@ -459,6 +474,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
                 for (int m = 0; m < NT; ++m) O[it][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < SA; ++s) {
+                __builtin_amdgcn_sched_barrier(0);
                 uint32_t sw[NT][PP][4];
 #pragma unroll
                 for (int m = 0; m < NT; ++m) {
@@ -472,12 +488,10 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
                 }
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
-                    const int i = 16 * it + l16;
 #pragma unroll
                     for (int q = 0; q < P; ++q) {
-                        const uint16_t* at = ldsA + (q * C + i) * DA + (g4 & 1) * 4;
-                        const u32x2 w0 = *reinterpret_cast<const u32x2*>(at + swizzle<DA / 8>(i, 4 * s + (g4 >> 1)) * 8);
-                        const u32x2 w1 = *reinterpret_cast<const u32x2*>(at + swizzle<DA / 8>(i, 4 * s + 2 + (g4 >> 1)) * 8);
+                        const u32x2 w0 = lds_at<u32x2>(ldsA + q * C * DA, halfD ^ frag_tile<DA / 8>(it, 4 * s));
+                        const u32x2 w1 = lds_at<u32x2>(ldsA + q * C * DA, halfD ^ frag_tile<DA / 8>(it, 4 * s + 2));
                         const uint32_t w[4] = {w0[0], w0[1], w1[0], w1[1]};
 #pragma unroll
                         for (int p = 0; p < PP; ++p)
@@ -507,10 +521,9 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
                     it = tile >> 1;
                     jt = tile & 1;
                 }
-                const int i = 16 * it + l16;
 #pragma unroll
                 for (int p = 0; p < PP; ++p)
-                    *reinterpret_cast<u32x2*>(ldsP + (p * C + i) * C + swizzle<C / 8>(i, 2 * jt + (g4 >> 1)) * 8 + (g4 & 1) * 4) =
+                    *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(it, 2 * jt))) =
                         u32x2{pw[k][p][0], pw[k][p][1]};
             }
             __syncthreads();
@@ -522,6 +535,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
             for (int m = 0; m < NT; ++m) S[t][m] *= decay;
 #pragma unroll
         for (int s = 0; s < SC; ++s) {
+            __builtin_amdgcn_sched_barrier(0);
             bf16x8 fc[NT][P];
             uint32_t ww[NT][3][4];
             float w8[8];
@@ -529,11 +543,10 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
             for (int e = 0; e < 8; ++e) w8[e] = left[buf][32 * s + 8 * g4 + e];
 #pragma unroll
             for (int m = 0; m < NT; ++m) {
-                const int col = col0 + 16 * m;
                 float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int p = P - 1; p >= 0; --p) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(ldsCT + (p * DC + col) * C + swizzle<C / 8>(col, 4 * s + g4) * 8);
+                    const u32x4 w = lds_at<u32x4>(ldsCT + p * DC * C, fragC ^ frag_tile<C / 8>(wave * NT + m, 4 * s));
                     fc[m][p] = __builtin_bit_cast(bf16x8, w);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] += vget<bf16>(w, e);
@@ -545,10 +558,9 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
             if constexpr (!STATES) {
 #pragma unroll
                 for (int it = 2 * s; it < IT; ++it) {
-                    const int i = 16 * it + l16;
 #pragma unroll
                     for (int q = 0; q < PP; ++q) {
-                        const bf16x8 fp = *reinterpret_cast<const bf16x8*>(ldsP + (q * C + i) * C + swizzle<C / 8>(i, 4 * s + g4) * 8);
+                        const bf16x8 fp = lds_at<bf16x8>(ldsP + q * C * C, fragC ^ frag_tile<C / 8>(it, 4 * s));
 #pragma unroll
                         for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -559,10 +571,9 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
             }
 #pragma unroll
             for (int t = 0; t < TA; ++t) {
-                const int row = 16 * t + l16;
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    const bf16x8 fb = *reinterpret_cast<const bf16x8*>(ldsBT + (p * DA + row) * C + swizzle<C / 8>(row, 4 * s + g4) * 8);
+                    const bf16x8 fb = lds_at<bf16x8>(ldsBT + p * DA * C, fragC ^ frag_tile<C / 8>(t, 4 * s));
 #pragma unroll
                     for (int q = 0; q < 3; ++q)
 #pragma unroll
@@ -582,10 +593,13 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
 #pragma unroll
                 for (int m = 0; m < NT; ++m) {
                     const int col = wave * 16 * NT + 16 * m + 4 * g4;
-                    if (job.dots != nullptr)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[it][m][e], dot);
                     if (i >= n || col >= dc) continue;
+                    if (px != nullptr) {
+                        const T* at = px + dir * (r + i) * job.x.s[1] + col * job.x.s[3];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (col + e < dc) dot = __builtin_fmaf(O[it][m][e], to_f32(at[e * job.x.s[3]]), dot);
+                    }
                     const int64_t at = (tok * args.heads + h) * dc + col;
                     const int some = dc - col;
                     if (job.out_f32 || sizeof(T) == 4) {
@@ -621,6 +635,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
         buf ^= 1;
         r = r_next;
         n = n_next;
+        if (n == 0) break;
     }
 
     // ---- the state at the segment's end
