@@ -297,6 +297,13 @@ def native_norm_bwd(x, weight, residual, stats, rms, dy, dsum, dx, dresidual, dw
     _lib.check(lib.cc1d_norm_bwd(ctypes.byref(b), _stream(dy)))
 
 
+def _near(t):
+    """States whose values lie within 2**31 of each other, as the kernels count them."""
+    if t is None or (t.shape[2] - 1) * t.stride(2) + (t.shape[3] - 1) * t.stride(3) < 2**31:
+        return t
+    return t.contiguous()
+
+
 def _attn_params(q, k, v, g, cu_seqlens, initial_states, scale):
     p = _lib.AttnParams()
     p.q, p.k, p.v, p.g = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr()
@@ -323,6 +330,7 @@ def _workspace(n, like):
 def native_attn_fwd(q, k, v, g, cu_seqlens, initial_states, scale, out, final_states) -> None:
     _require_device(q)
     lib = _lib.load()
+    initial_states = _near(initial_states)
     p = _attn_params(q, k, v, g, cu_seqlens, initial_states, scale)
     p.out, p.final_states = out.data_ptr(), _ptr(final_states)
     ws, p.workspace_floats = _workspace(lib.cc1d_attn_workspace_floats(ctypes.byref(p)), q)
@@ -336,6 +344,7 @@ def native_attn_bwd(q, k, v, g, cu_seqlens, initial_states, scale, dout, dfinal_
     _require_device(q)
     lib = _lib.load()
     b = _lib.AttnBwdParams()
+    initial_states, dfinal_states = _near(initial_states), _near(dfinal_states)
     b.fwd = _attn_params(q, k, v, g, cu_seqlens, initial_states, scale)
     b.dout, b.dfinal_states = dout.data_ptr(), _ptr(dfinal_states)
     b.dq, b.dk, b.dv, b.dg = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr()

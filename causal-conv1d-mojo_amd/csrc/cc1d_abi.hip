@@ -88,6 +88,11 @@ int check_norm(const cc1d_norm_params& p) {
 
 bool attn_dim(int64_t d) { return d >= 1 && d <= CC1D_MAX_ATTN_DIM; }
 
+// A state's values are found by 32-bit offsets from its first.
+bool state_fits(const float* p, const int64_t (&s)[4], int64_t dk, int64_t dv) {
+    return p == nullptr || (s[2] >= 0 && s[3] >= 0 && (double)(dk - 1) * (double)s[2] + (double)(dv - 1) * (double)s[3] < (double)((int64_t)1 << 31));
+}
+
 // Sizes of linear attention, before its pointers.
 int check_attn(const cc1d_attn_params& p) {
     if (!valid_dtype(p.dtype)) return CC1D_ERR_DTYPE;
@@ -95,6 +100,7 @@ int check_attn(const cc1d_attn_params& p) {
     if (p.batch < 0 || p.seqlen < 0 || p.heads < 0) return CC1D_ERR_SHAPE;
     if (p.key_heads < 1 || p.heads % p.key_heads != 0) return CC1D_ERR_HEADS;
     if (p.cu_seqlens != nullptr && (p.batch != 1 || p.num_seqs < 0 || (p.num_seqs == 0 && p.seqlen > 0))) return CC1D_ERR_SHAPE;
+    if (!state_fits(p.initial_states, p.initial_states_stride, p.dk, p.dv)) return CC1D_ERR_SHAPE;
     return attn_fits(p) ? CC1D_OK : CC1D_ERR_SHAPE;
 }
 
@@ -347,6 +353,7 @@ int cc1d_attn_bwd(const cc1d_attn_bwd_params* b, void* stream) {
     const cc1d_attn_params& p = b->fwd;
     const int st = check_attn(p);
     if (st != CC1D_OK) return st;
+    if (!state_fits(b->dfinal_states, b->dfinal_states_stride, p.dk, p.dv)) return CC1D_ERR_SHAPE;
     if (attn_empty(p)) {
         // no head adds to the gradients of q and k
         const int64_t n = p.batch * p.seqlen * p.key_heads, strides[3] = {p.dk, 0, 1};

@@ -259,9 +259,10 @@ Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
 }  // namespace
 
 bool attn_fits(const cc1d_attn_params& p) {
+    // inside a state, and from row to row of a chunk of outputs, the kernels count in 32 bits; so do launches:
     // blocks of 256 threads, 32-bit thread counts: one a slot, head and job, or one a piece of 256 values of a state
     const double seqs = p.cu_seqlens ? (double)p.num_seqs : (double)p.batch;
-    if ((double)p.heads >= (double)(1 << 20) || seqs * (double)p.heads * kAttnJobs >= (double)(1 << 23)) return false;
+    if ((double)p.heads >= (double)(1 << 15) || seqs * (double)p.heads * kAttnJobs >= (double)(1 << 23)) return false;
     if ((double)p.batch * (double)p.seqlen >= (double)((int64_t)1 << 40) || p.seqlen >= ((int64_t)1 << 31) - 4096) return false;
     return (double)plan_of(p, kAttnJobs).slots * (double)p.heads * kAttnJobs < (double)(1 << 24) &&
            (double)plan_of(p, 1).slots * (double)p.heads < (double)(1 << 24) && (double)p.heads * 2 * 64 < (double)(1 << 24);

@@ -4,7 +4,7 @@
 namespace cc1d {
 
 template <> int launch_attn_jobs<bf16>(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
-    return states ? launch_attn_sizes<bf16, true>(a, da, dc, stream) : launch_attn_sizes<bf16, false>(a, da, dc, stream);
+    return launch_attn_modes<bf16>(a, da, dc, states, stream);
 }
 
 }  // namespace cc1d

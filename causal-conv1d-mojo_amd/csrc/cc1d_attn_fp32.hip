@@ -4,7 +4,7 @@
 namespace cc1d {
 
 template <> int launch_attn_jobs<float>(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
-    return states ? launch_attn_sizes<float, true>(a, da, dc, stream) : launch_attn_sizes<float, false>(a, da, dc, stream);
+    return launch_attn_modes<float>(a, da, dc, states, stream);
 }
 
 }  // namespace cc1d

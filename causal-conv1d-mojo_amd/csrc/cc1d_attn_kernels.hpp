@@ -197,9 +197,24 @@ template <typename T, int C, int D> struct AttnTile {
     static constexpr int P = AttnType<T>::planes;
     u32x4 v[N][4];
 
-    // tid: the thread's index (not a loop invariant to the compiler: a register for every address would not leave
-    // enough for the state)
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, int tid) {
+    // rows positions from base on, row_stride apart. tid: the thread's index (not a loop invariant to the compiler: a
+    // register for every address would not leave enough for the state). whole: the head has all D columns, next to
+    // each other, and a chunk spans less than 2 GiB, so that full chunks go by a uniform base and 32-bit offsets.
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, bool whole, int tid) {
+        if (whole && rows == C) {
+            const bool down = row_stride < 0;
+            const char* const low = reinterpret_cast<const char*>(down ? base + (C - 1) * row_stride : base);
+            const uint32_t pitch = (uint32_t)((down ? -row_stride : row_stride) * (int64_t)sizeof(T));
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int u = n * 256 + tid, row = u / CGS * 4, col = u % CGS * EPV;
+                // (idle threads read the first unit's positions and store nothing)
+                const uint32_t at = UNITS % 256 == 0 || u < UNITS ? (uint32_t)(down ? C - 4 - row : row) * pitch + col * (uint32_t)sizeof(T) : 0u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[n][i] = vload_any(reinterpret_cast<const T*>(low + (uint64_t)((down ? 3 - i : i) * pitch) + at));
+            }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int u = n * 256 + tid, row = u / CGS * 4, col = u % CGS * EPV;
@@ -219,6 +234,10 @@ template <typename T, int C, int D> struct AttnTile {
             }
         }
     }
+    static __device__ __forceinline__ bool whole(int64_t row_stride, int64_t elem_stride, int d) {
+        const int64_t r = row_stride < 0 ? -row_stride : row_stride;
+        return elem_stride == 1 && d == D && r < ((int64_t)1 << 31) / (C * (int64_t)sizeof(T));
+    }
     static __device__ __forceinline__ void put(u32x4& w, int e, T x) {
         if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(to_f32(x));
         else w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, x) << (16 * (e & 1));
@@ -231,18 +250,27 @@ template <typename T, int C, int D> struct AttnTile {
     }
     // whether anything is infinite or NaN
     __device__ __forceinline__ bool wild() const {
-        constexpr uint32_t M = sizeof(T) == 4 ? 0x7f800000u : (std::is_same_v<T, bf16> ? 0x7f807f80u : 0x7c007c00u);
-        bool w = false;
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m = 0;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+            for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint32_t x = v[n][i][d] & M;
-                    w = w || (x >> 16) == (M >> 16) || (sizeof(T) == 2 && (x & 0xffffu) == (M & 0xffffu));
-                }
-        return w;
+                    for (int d = 0; d < 4; ++d) m = max(m, v[n][i][d] & 0x7f800000u);
+            return m == 0x7f800000u;
+        } else {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            constexpr uint32_t M = std::is_same_v<T, bf16> ? 0x7f807f80u : 0x7c007c00u;
+            u16x2 m = {0, 0};
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[n][i][d] & M));
+            return m[0] == (M & 0xffffu) || m[1] == (M & 0xffffu);
+        }
     }
     // rows[plane][position][column] and / or cols[plane][column][position]
     template <bool ROWS, bool COLS> __device__ __forceinline__ void store(uint16_t* rows, uint16_t* cols, int tid) const {
@@ -294,9 +322,13 @@ template <typename T, int C, int D> struct AttnTile {
 // runs over its inner index is free, so Q's fragments are read in that order.
 // The pairs' products are shared: each wavefront forms a quarter of their
 // tiles and passes them through LDS.
-// STATES: the state alone, of the segments that another one follows.
-template <typename T, int DA, int DC, bool STATES> __global__ void __launch_bounds__(256, 2) attn_kernel(const AttnArgs args) {
+// MODE: outputs; outputs and exact states, where somebody wants the last one (the third plane of what the state
+// takes); or the state alone, of the segments that another one follows.
+enum { kAttnOut = 0, kAttnExact = 1, kAttnStates = 2 };
+template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds__(256, 2) attn_kernel(const AttnArgs args) {
     typedef AttnType<T> Ty;
+    constexpr bool STATES = MODE == kAttnStates;
+    constexpr int SORD = MODE == kAttnOut ? AttnType<T>::order : 2, SP = SORD + 1;  // planes of what the state takes
     constexpr int C = Ty::chunk, P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
     constexpr int NT = DC / 64, TA = DA / 16, SC = C / 32, SA = DA / 32, IT = C / 16;
     constexpr int TILES = C == 64 ? 12 : 4;  // of the pairs, with the empty ones that a product reads
@@ -305,7 +337,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
     __shared__ __attribute__((aligned(16))) uint16_t lds[kA + kB + P * DA * C + P * DC * C];
     __shared__ __attribute__((aligned(16))) float sums_hi[2][C], sums_lo[2][C], into[2][C], left[2][C], whole[2];
     __shared__ float dot_lds[4][C];
-    __shared__ int wild_flag;
+    __shared__ int wild_flag[2];
     uint16_t *const ldsA = lds, *const ldsB = lds + kA, *const ldsBT = lds + kA + kB, *const ldsCT = ldsBT + P * DA * C;
     uint16_t* const ldsP = ldsB;  // the columns are dead once the pairs' products are formed
 
@@ -333,18 +365,24 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
     // ---- the state at the segment's start
     const int col0 = wave * 16 * NT + l16;  // this lane's column (of its first tile)
     f32x4 S[TA][NT];
-    {
-        const bool from_seg = sp.index > 0;
-        const AttnState& st = from_seg ? job.seg : job.first;
-        const float* at = st.p == nullptr || STATES ? nullptr : st.p + (from_seg ? (int64_t)slot : sp.seq) * st.s[0] + h * st.s[1];
+#pragma unroll
+    for (int t = 0; t < TA; ++t)
+#pragma unroll
+        for (int m = 0; m < NT; ++m) S[t][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const AttnState first = sp.index > 0 ? job.seg : job.first;
+    if (!STATES && first.p != nullptr) {
+        const float* const at = first.p + (sp.index > 0 ? (int64_t)slot : sp.seq) * first.s[0] + h * first.s[1];
+        const int s2 = (int)first.s[2], s3 = (int)first.s[3];
 #pragma unroll
         for (int t = 0; t < TA; ++t)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int m = 0; m < NT; ++m)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * t + 4 * g4 + r, col = col0 + 16 * n;
-                    S[t][n][r] = at != nullptr && row < da && col < dc ? at[row * st.s[2] + col * st.s[3]] : 0.0f;
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 16 * t + 4 * g4 + e, col = col0 + 16 * m;
+                    const bool in = row < da && col < dc;
+                    const float v = at[in ? (uint32_t)(row * s2 + col * s3) : 0u];
+                    S[t][m][e] = in ? v : 0.0f;
                 }
     }
 
@@ -372,17 +410,43 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
 
     AttnTile<T, C, DA> ta, tb;
     AttnTile<T, C, DC> tc;
+    const bool wa = ta.whole(sa, job.a.s[3], da), wb = tb.whole(sb, job.b.s[3], da), wc = tc.whole(sc, job.c.s[3], dc);
     auto load = [&](int64_t r, int n, int t) {
-        if constexpr (!STATES) ta.load(pa + r * sa, sa, job.a.s[3], n, da, t);
-        tb.load(pb + r * sb, sb, job.b.s[3], n, da, t);
-        tc.load(pc + r * sc, sc, job.c.s[3], n, dc, t);
+        if constexpr (!STATES) ta.load(pa + r * sa, sa, job.a.s[3], n, da, wa, t);
+        tb.load(pb + r * sb, sb, job.b.s[3], n, da, wb, t);
+        tc.load(pc + r * sc, sc, job.c.s[3], n, dc, wc, t);
     };
     auto rows_at = [&](int64_t r) { return (int)(r1_seg - r < C ? r1_seg - r : C); };
 
+    // four columns of the operand that the outputs are multiplied with
+    const int64_t xs = dir * job.x.s[1], xe = job.x.s[3];
+    const bool x_quick = xe == 1 && dc % 4 == 0 && (xs < 0 ? -xs : xs) < ((int64_t)1 << 24);
+    auto x_load = [&](const T* at, int i, int col, float (&x)[4]) {
+        if (x_quick) {
+            at += i * (int)xs + col;
+            if constexpr (sizeof(T) == 4) {
+                const u32x4 w = vload_any(at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(w[e]);
+            } else {
+                const u32x2 w = *reinterpret_cast<const typename AnyAddr<2>::v2*>(at);
+                const u32x4 w4 = {w[0], w[1], 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = vget<T>(w4, e);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = col + e < dc ? to_f32(at[i * xs + (col + e) * xe]) : 0.0f;
+        }
+    };
+    const int64_t tokens = args.batch * args.seqlen, t0 = row0 * args.seqlen + p0;
+    auto dots_out = [&](int64_t r) {
+        job.dots[h * tokens + t0 + dir * (r + tid)] = (dot_lds[0][tid] + dot_lds[1][tid]) + (dot_lds[2][tid] + dot_lds[3][tid]);
+    };
     // The loop loads a chunk while it works on the one before; its first turn only loads.
     int64_t r = r0_seg, single = 0;  // rows before `single` go one by one
     int n = 0, buf = 1;
-    if (tid == 0) wild_flag = 0;
+    if (tid < 2) wild_flag[tid] = 0;
     ta.none();
     tb.none();
     tc.none();
@@ -397,30 +461,22 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
         }
         tc.template store<false, true>(nullptr, ldsCT, otid);
         if constexpr (!STATES)
-            if (tc.wild()) wild_flag = 1;
+            if (tc.wild()) wild_flag[buf] = 1;
         __syncthreads();
         // An infinite or NaN value is multiplied with the zeros of the pairs that come before it: such a chunk goes
         // position by position, so that it reaches the later ones alone.
-        const bool again = !STATES && wild_flag && n > 1;
+        const bool again = !STATES && n > 1 && wild_flag[buf];
+        if (tid == 0) wild_flag[buf ^ 1] = 0;
         if (again) single = r + n;
         const int64_t r_next = again ? r : r + n;
         const int n_next = r_next >= r1_seg ? 0 : (r_next < single ? 1 : rows_at(r_next));
+        const bool work = n > 0 && !again;
         float g_next = 0.0f;
         if (n_next > 0) {
             load(r_next, n_next, otid);
             if (wave == 3) g_next = g_load(r_next, n_next);
         }
-        if (n == 0 || again) {
-            if (n_next == 0) break;
-            __syncthreads();  // everybody has seen the flag
-            if (tid == 0) wild_flag = 0;
-            buf ^= 1;
-            if (wave == 3) decays(g_next, buf);
-            r = r_next;
-            n = n_next;
-            continue;
-        }
-
+        if (work) {
         const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0), halfD = frag_base<DA / 8>(l16, g4 >> 1, g4 & 1);
         const uint32_t fragC = frag_base<C / 8>(l16, g4, 0), halfC = frag_base<C / 8>(l16, g4 >> 1, g4 & 1);
         f32x4 O[IT][NT];
@@ -508,7 +564,6 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
                 for (int m = 0; m < NT; ++m) O[it][m] *= e;
             }
             __syncthreads();
-            if (tid == 0) wild_flag = 0;
             // ---- the pairs to everybody
 #pragma unroll
             for (int k = 0; k < TILES / 4; ++k) {
@@ -537,7 +592,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
         for (int s = 0; s < SC; ++s) {
             __builtin_amdgcn_sched_barrier(0);
             bf16x8 fc[NT][P];
-            uint32_t ww[NT][3][4];
+            uint32_t ww[NT][SP][4];
             float w8[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w8[e] = left[buf][32 * s + 8 * g4 + e];
@@ -553,7 +608,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] *= w8[e];
-                to_planes<3, 4>(f, ww[m]);
+                to_planes<SP, 4>(f, ww[m]);
             }
             if constexpr (!STATES) {
 #pragma unroll
@@ -575,40 +630,39 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
                 for (int p = 0; p < P; ++p) {
                     const bf16x8 fb = lds_at<bf16x8>(ldsBT + p * DA * C, fragC ^ frag_tile<C / 8>(t, 4 * s));
 #pragma unroll
-                    for (int q = 0; q < 3; ++q)
+                    for (int q = 0; q < SP; ++q)
 #pragma unroll
                         for (int m = 0; m < NT; ++m)
-                            if (p + q <= 2) S[t][m] = mfma(fb, as_frag(ww[m][q]), S[t][m]);
+                            if (p + q <= SORD) S[t][m] = mfma(fb, as_frag(ww[m][q]), S[t][m]);
                 }
             }
         }
         if constexpr (!STATES) {
             // ---- outputs: a lane has four columns of a row
-            const int64_t tokens = args.batch * args.seqlen, t0 = row0 * args.seqlen + p0;
+            const int64_t tok = t0 + dir * r;
+            const int pitch = (int)dir * (int)args.heads * dc;  // from a row to the next
 #pragma unroll
             for (int it = 0; it < IT; ++it) {
                 const int i = 16 * it + l16;
-                const int64_t tok = t0 + dir * (r + i);
                 float dot = 0.0f;
 #pragma unroll
                 for (int m = 0; m < NT; ++m) {
                     const int col = wave * 16 * NT + 16 * m + 4 * g4;
                     if (i >= n || col >= dc) continue;
                     if (px != nullptr) {
-                        const T* at = px + dir * (r + i) * job.x.s[1] + col * job.x.s[3];
+                        float x[4];
+                        x_load(px + r * xs, i, col, x);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (col + e < dc) dot = __builtin_fmaf(O[it][m][e], to_f32(at[e * job.x.s[3]]), dot);
+                        for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[e], dot);
                     }
-                    const int64_t at = (tok * args.heads + h) * dc + col;
-                    const int some = dc - col;
+                    const int at = i * pitch + col, some = dc - col;
                     if (job.out_f32 || sizeof(T) == 4) {
-                        float* o = static_cast<float*>(job.out) + at;
+                        float* o = static_cast<float*>(job.out) + (tok * args.heads + h) * dc + at;
                         if (some >= 4) *reinterpret_cast<AnyAddr<4>::v4*>(o) = __builtin_bit_cast(u32x4, O[it][m]);
                         else
                             for (int e = 0; e < some; ++e) o[e] = O[it][m][e];
                     } else {
-                        T* o = static_cast<T*>(job.out) + at;
+                        T* o = static_cast<T*>(job.out) + (tok * args.heads + h) * dc + at;
                         if (some >= 4) {
                             typedef typename AnyAddr<sizeof(T)>::v2 any2;
                             if constexpr (sizeof(T) == 2)
@@ -618,31 +672,34 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
                         }
                     }
                 }
-                if (job.dots != nullptr) {
+                if (px != nullptr) {
                     dot += __shfl_xor(dot, 16);
                     dot += __shfl_xor(dot, 32);
                     if (g4 == 0) dot_lds[wave][i] = dot;
                 }
             }
-            if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
-            __syncthreads();
-            if (job.dots != nullptr && tid < n)
-                job.dots[h * tokens + t0 + dir * (r + tid)] = (dot_lds[0][tid] + dot_lds[1][tid]) + (dot_lds[2][tid] + dot_lds[3][tid]);
-        } else {
-            if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
-            __syncthreads();
         }
+        }
+        if (n_next == 0) break;
+        if (wave == 3) decays(g_next, buf ^ 1);
+        __syncthreads();
+        if constexpr (!STATES)
+            if (px != nullptr && work && tid < n) dots_out(r);
         buf ^= 1;
         r = r_next;
         n = n_next;
-        if (n == 0) break;
+    }
+    if constexpr (!STATES) {
+        __syncthreads();
+        if (px != nullptr && tid < n) dots_out(r);
     }
 
     // ---- the state at the segment's end
     const bool ends = sp.index + 1 == sp.segs;
-    const AttnState& st = STATES ? job.seg : job.last;
-    if (st.p != nullptr && (STATES || ends)) {
-        float* at = st.p + (STATES ? (int64_t)slot : sp.seq) * st.s[0] + h * st.s[1];
+    const AttnState last = STATES ? job.seg : job.last;
+    if (last.p != nullptr && (STATES || ends)) {
+        float* const at = last.p + (STATES ? (int64_t)slot : sp.seq) * last.s[0] + h * last.s[1];
+        const int s2 = (int)last.s[2], s3 = (int)last.s[3];
         float by = 1.0f;
         // backwards, the state before the sequence has its first decay too
         if (!STATES && reverse && sp.len > 0) by = (float)exp(log_decay(to_f32(pg[sp.first * args.g_stride[1]])));
@@ -653,7 +710,7 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int row = 16 * t + 4 * g4 + e, col = col0 + 16 * m;
-                    if (row < da && col < dc) at[row * st.s[2] + col * st.s[3]] = by * S[t][m][e];
+                    if (row < da && col < dc) at[(uint32_t)(row * s2 + col * s3)] = by * S[t][m][e];
                 }
     }
     if (STATES && tid == 3 * 64) job.decay[(int64_t)slot * args.heads + h] = (float)exp2(total);
@@ -671,15 +728,24 @@ template <typename T, int DA, int DC, bool STATES> __global__ void __launch_boun
     }
 }
 
-template <typename T, bool STATES> int launch_attn_sizes(const AttnArgs& a, int da, int dc, hipStream_t stream) {
+template <typename T, int MODE> int launch_attn_sizes(const AttnArgs& a, int da, int dc, hipStream_t stream) {
     const dim3 grid(a.blocks), block(256);
-    if (da <= 64 && dc <= 64) return launch(attn_kernel<T, 64, 64, STATES>, grid, block, stream, a);
-    if (da <= 64) return launch(attn_kernel<T, 64, 128, STATES>, grid, block, stream, a);
-    if (dc <= 64) return launch(attn_kernel<T, 128, 64, STATES>, grid, block, stream, a);
-    return launch(attn_kernel<T, 128, 128, STATES>, grid, block, stream, a);
+    if (da <= 64 && dc <= 64) return launch(attn_kernel<T, 64, 64, MODE>, grid, block, stream, a);
+    if (da <= 64) return launch(attn_kernel<T, 64, 128, MODE>, grid, block, stream, a);
+    if (dc <= 64) return launch(attn_kernel<T, 128, 64, MODE>, grid, block, stream, a);
+    return launch(attn_kernel<T, 128, 128, MODE>, grid, block, stream, a);
 }
 
 // All jobs of `a` have rows of da and values of dc (explicitly instantiated in cc1d_attn_<dtype>.hip).
 template <typename T> int launch_attn_jobs(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream);
+template <typename T> int launch_attn_modes(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
+    if (states) return launch_attn_sizes<T, kAttnStates>(a, da, dc, stream);
+    if constexpr (AttnType<T>::order < 2) {
+        bool exact = false;
+        for (uint32_t j = 0; j < a.jobs; ++j) exact = exact || a.job[j].last.p != nullptr;
+        if (!exact) return launch_attn_sizes<T, kAttnOut>(a, da, dc, stream);
+    }
+    return launch_attn_sizes<T, kAttnExact>(a, da, dc, stream);
+}
 
 }  // namespace cc1d

@@ -62,6 +62,12 @@ bool heads_fit(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& 
 
 // ---- linear attention ----
 
+// states whose values lie within 2**31 of each other, as the kernels count them
+Tensor near(const Tensor& t) {
+    if (!t.defined() || (t.size(2) - 1) * t.stride(2) + (t.size(3) - 1) * t.stride(3) < ((int64_t)1 << 31)) return t;
+    return t.contiguous();
+}
+
 struct Attn {
     Tensor q, k, v, g, cu, init;
     double scale;
@@ -127,7 +133,7 @@ struct AttnFn : public torch::autograd::Function<AttnFn> {
         const Tensor none;
         const auto s = ctx->get_saved_variables();
         const Attn a{s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble()};
-        const Tensor dfinal = grads.size() > 1 ? grads[1] : none;
+        const Tensor dfinal = grads.size() > 1 ? near(grads[1]) : none;
         if (!grads[0].defined() && !dfinal.defined()) return {none, none, none, none, none, none, none, none};
         const c10::OptionalDeviceGuard device(a.q.device());
         const Tensor dout = grads[0].defined() ? grads[0] : at::zeros(a.v.sizes(), a.v.options());
@@ -174,7 +180,7 @@ PyObject* py_attn(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const bool fin_wanted = o[7] == Py_True;
     if (a.q.dim() != 4 || !heads_fit(a.q, a.k, a.v, a.g) || !indices(a.cu, a.q)) return not_implemented();
     if (a.cu.defined() && (a.q.size(0) != 1 || a.cu.size(0) < 2)) return not_implemented();
-    if (!states(a.init, a.q, a.state_shape())) return not_implemented();
+    if (!states(a.init, a.q, a.state_shape()) || !near(a.init).is_same(a.init)) return not_implemented();
     a.scale = scale_of(o[4], a.q.size(3));
     if (std::isnan(a.scale)) return not_implemented();
 
