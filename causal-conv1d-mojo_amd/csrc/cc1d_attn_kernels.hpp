@@ -119,6 +119,24 @@ template <int BLKS> __device__ __forceinline__ uint32_t frag_base(int l16, int b
 template <int BLKS> __device__ __forceinline__ uint32_t frag_tile(int t, int blk) {
     return (uint32_t)(t * 16 * BLKS * 16 | ((blk ^ (2 * t & (BLKS >= 8 ? 7 : BLKS - 1))) * 16));
 }
+
+// Transposed images (columns of operands and values, positions next to each
+// other). Two neighbouring tiles share 32 of them in turns of four: lane
+// l & 15 of tile t has 32 (t / 2) + 8 (l / 4) + 4 (t % 2) + l % 4, so that the
+// accumulators of the two tiles hold eight neighbours in each lane, which is
+// what a fragment of the next product (or a 16-byte store) wants.
+template <int BLKS> __device__ __forceinline__ int swizzle_t(int row, int blk) {
+    if constexpr (BLKS >= 8) return blk ^ (((row & 3) ^ ((row >> 4) & 3)) | ((row >> 1) & 4));
+    else return blk ^ ((((row >> 1) ^ (row >> 4)) & 1) | ((row >> 2) & 2));
+}
+__device__ __forceinline__ int tile_col(int t, int l16) { return 32 * (t >> 1) + 4 * (t & 1) + 8 * (l16 >> 2) + (l16 & 3); }
+template <int BLKS> __device__ __forceinline__ uint32_t turn_base(int l16, int blk) {
+    const int row = tile_col(0, l16);
+    return (uint32_t)(row * BLKS * 16 + swizzle_t<BLKS>(row, blk) * 16);
+}
+template <int BLKS> __device__ __forceinline__ uint32_t turn_tile(int t, int blk) {
+    return (uint32_t)((32 * (t >> 1) + 4 * (t & 1)) * BLKS * 16 | ((BLKS >= 8 ? blk ^ (2 * ((t >> 1) & 1)) : blk) * 16));
+}
 template <typename V> __device__ __forceinline__ V lds_at(const uint16_t* image, uint32_t off) {
     return *reinterpret_cast<const V*>(reinterpret_cast<const char*>(image) + off);
 }
@@ -307,7 +325,7 @@ template <typename T, int C, int D> struct AttnTile {
                         const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;  // the high or the low halves of two dwords
                         const u32x2 q = {__builtin_amdgcn_perm(w[1][p][e >> 1], w[0][p][e >> 1], sel),
                                          __builtin_amdgcn_perm(w[3][p][e >> 1], w[2][p][e >> 1], sel)};
-                        *reinterpret_cast<u32x2*>(cols + (p * D + col + e) * C + swizzle<C / 8>(col + e, row >> 3) * 8 + (row & 7)) = q;
+                        *reinterpret_cast<u32x2*>(cols + (p * D + col + e) * C + swizzle_t<C / 8>(col + e, row >> 3) * 8 + (row & 7)) = q;
                     }
                 }
             }
@@ -315,55 +333,86 @@ template <typename T, int C, int D> struct AttnTile {
     }
 };
 
+// 4 * NT neighbouring values, widened.
+template <typename T, int NT> __device__ __forceinline__ void four_of(const T* p, float (&x)[4 * NT]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+            const u32x4 w = vload_any(p + 4 * m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * m + e] = __uint_as_float(w[e]);
+        }
+    } else if constexpr (NT == 2) {
+        const u32x4 w = vload_any(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = vget<T>(w, e);
+    } else {
+        const u32x2 w = *reinterpret_cast<const typename AnyAddr<2>::v2*>(p);
+        const u32x4 w4 = {w[0], w[1], 0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = vget<T>(w4, e);
+    }
+}
+template <typename T, int NT> __device__ __forceinline__ void store_outputs(char* o, const f32x4 (&O)[NT], bool f32) {
+    if (sizeof(T) == 4 || f32) {
+#pragma unroll
+        for (int m = 0; m < NT; ++m) *reinterpret_cast<AnyAddr<4>::v4*>(o + 16 * m) = __builtin_bit_cast(u32x4, O[m]);
+    } else if constexpr (sizeof(T) == 2) {
+        if constexpr (NT == 2) {
+            *reinterpret_cast<AnyAddr<2>::v4*>(o) = u32x4{pack2<T>(O[0][0], O[0][1]), pack2<T>(O[0][2], O[0][3]),
+                                                          pack2<T>(O[1][0], O[1][1]), pack2<T>(O[1][2], O[1][3])};
+        } else {
+            *reinterpret_cast<AnyAddr<2>::v2*>(o) = u32x2{pack2<T>(O[0][0], O[0][1]), pack2<T>(O[0][2], O[0][3])};
+        }
+    }
+}
+
 // One job of one segment of one head. Four wavefronts; each holds 16 * NT of
 // the state's columns with all its rows in registers (the accumulators of
-// S += K^T V), where they are at once the left operand of Q S: an accumulator
-// has four neighbouring rows of a column, and the order in which a product
-// runs over its inner index is free, so Q's fragments are read in that order.
-// The pairs' products are shared: each wavefront forms a quarter of their
-// tiles and passes them through LDS.
+// S += K^T V), where they are at once the left operand of Q S. The pairs'
+// products are shared: each wavefront forms those of 16 columns and passes
+// them through LDS.
 // MODE: outputs; outputs and exact states, where somebody wants the last one (the third plane of what the state
 // takes); or the state alone, of the segments that another one follows.
 enum { kAttnOut = 0, kAttnExact = 1, kAttnStates = 2 };
 template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds__(256, 2) attn_kernel(const AttnArgs args) {
     typedef AttnType<T> Ty;
     constexpr bool STATES = MODE == kAttnStates;
-    constexpr int SORD = MODE == kAttnOut ? AttnType<T>::order : 2, SP = SORD + 1;  // planes of what the state takes
+    constexpr int SORD = MODE == kAttnOut ? Ty::order : 2, SP = SORD + 1;  // planes of what the state takes
     constexpr int C = Ty::chunk, P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
     constexpr int NT = DC / 64, TA = DA / 16, SC = C / 32, SA = DA / 32, IT = C / 16;
-    constexpr int TILES = C == 64 ? 12 : 4;  // of the pairs, with the empty ones that a product reads
+    constexpr int PT = C == 64 ? 4 : 1;  // tiles of the pairs that a wavefront forms
     constexpr int kA = STATES ? 0 : P * C * DA, kPairs = PP * C * C;
     constexpr int kB = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
     __shared__ __attribute__((aligned(16))) uint16_t lds[kA + kB + P * DA * C + P * DC * C];
-    __shared__ __attribute__((aligned(16))) float sums_hi[2][C], sums_lo[2][C], into[2][C], left[2][C], whole[2];
-    __shared__ float dot_lds[4][C];
+    __shared__ __attribute__((aligned(16))) float sums_hi[2][C], sums_lo[2][C], into[2][C], left[2][C];
+    __shared__ float whole[2], dot_lds[4][C];
     __shared__ int wild_flag[2];
     uint16_t *const ldsA = lds, *const ldsB = lds + kA, *const ldsBT = lds + kA + kB, *const ldsCT = ldsBT + P * DA * C;
     uint16_t* const ldsP = ldsB;  // the columns are dead once the pairs' products are formed
 
-    const int tid = threadIdx.x, wave = uniform32(tid >> 6), lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+    const int tid = threadIdx.x, wave = uniform32(tid >> 6), lane = tid & 63;
     const uint32_t id = xcd_block(blockIdx.x, args.blocks);
     const uint32_t rest = args.jobs_div.div(id), jn = id - rest * args.jobs;
     const uint32_t slot = args.heads_div.div(rest), h = rest - slot * args.heads;
     const AttnJob& job = args.job[jn];
     const AttnSpan sp = attn_span(args, slot);
     if (!sp.live || (STATES && sp.index + 1 == sp.segs)) return;
-    const int64_t r0_seg = sp.index * args.seg, r1_seg = r0_seg + args.seg < sp.len ? r0_seg + args.seg : sp.len;
+    const int r_first = (int)(sp.index * args.seg);  // positions of the sequence, in the order of the walk
+    const int r_end = r_first + args.seg < sp.len ? r_first + (int)args.seg : (int)sp.len;
     const int64_t row0 = args.cu ? 0 : sp.seq;  // batch row
     const int da = job.da, dc = job.dc;
     const bool reverse = job.reverse;
     const int64_t dir = reverse ? -1 : 1, p0 = reverse ? sp.first + sp.len - 1 : sp.first;
 
-    auto base = [&](const AttnOperand& o) {
-        return static_cast<const T*>(o.p) + row0 * o.s[0] + p0 * o.s[1] + (int64_t)(h / o.div) * o.s[2];
+    // position r of the walk
+    auto base = [&](const AttnOperand& o, int r) {
+        return static_cast<const T*>(o.p) + row0 * o.s[0] + (p0 + dir * r) * o.s[1] + (int64_t)(h / o.div) * o.s[2];
     };
-    const T* const px = job.dots ? base(job.x) : nullptr;
-    const T *const pa = base(job.a), *const pb = base(job.b), *const pc = base(job.c);
-    const int64_t sa = dir * job.a.s[1], sb = dir * job.b.s[1], sc = dir * job.c.s[1];
+    const bool dots = job.dots != nullptr;
     const T* const pg = static_cast<const T*>(args.g) + row0 * args.g_stride[0] + h * args.g_stride[2];
 
     // ---- the state at the segment's start
-    const int col0 = wave * 16 * NT + l16;  // this lane's column (of its first tile)
     f32x4 S[TA][NT];
 #pragma unroll
     for (int t = 0; t < TA; ++t)
@@ -379,7 +428,7 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
             for (int m = 0; m < NT; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int row = 16 * t + 4 * g4 + e, col = col0 + 16 * m;
+                    const int row = tile_col(t, 4 * (lane >> 4) + e), col = tile_col(wave * NT + m, lane & 15);
                     const bool in = row < da && col < dc;
                     const float v = at[in ? (uint32_t)(row * s2 + col * s3) : 0u];
                     S[t][m][e] = in ? v : 0.0f;
@@ -388,10 +437,10 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
 
     // ---- decays of the rows from r on (by one wavefront)
     double total = 0.0;
-    auto g_load = [&](int64_t r, int n) {
+    auto g_load = [&](int r, int n) {
         if (lane >= n) return 0.0f;
         // backwards, a position's decay is the one of the position after it, and the sequence's last has none
-        const int64_t at = reverse ? p0 - (r + lane) + 1 : p0 + r + lane;
+        const int64_t at = p0 + dir * (r + lane) + (reverse ? 1 : 0);
         return reverse && r + lane == 0 ? 0.0f : to_f32(pg[at * args.g_stride[1]]);
     };
     auto decays = [&](float g, int buf) {
@@ -408,43 +457,38 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
         if (lane == 0) whole[buf] = exp2_sum(ehi, elo);
     };
 
+    // ---- operands: where the next chunk starts, and the step from row to row
     AttnTile<T, C, DA> ta, tb;
     AttnTile<T, C, DC> tc;
+    int pos = r_first;
+    const T *pa = base(job.a, pos), *pb = base(job.b, pos), *pc = base(job.c, pos), *px = dots ? base(job.x, pos) : nullptr;
+    const int64_t sa = dir * job.a.s[1], sb = dir * job.b.s[1], sc = dir * job.c.s[1], sx = dir * job.x.s[1];
     const bool wa = ta.whole(sa, job.a.s[3], da), wb = tb.whole(sb, job.b.s[3], da), wc = tc.whole(sc, job.c.s[3], dc);
-    auto load = [&](int64_t r, int n, int t) {
-        if constexpr (!STATES) ta.load(pa + r * sa, sa, job.a.s[3], n, da, wa, t);
-        tb.load(pb + r * sb, sb, job.b.s[3], n, da, wb, t);
-        tc.load(pc + r * sc, sc, job.c.s[3], n, dc, wc, t);
+    const bool wx = dots && tc.whole(sx, job.x.s[3], dc);
+    auto load = [&](int n, int t) {
+        if constexpr (!STATES) ta.load(pa, sa, job.a.s[3], n, da, wa, t);
+        tb.load(pb, sb, job.b.s[3], n, da, wb, t);
+        tc.load(pc, sc, job.c.s[3], n, dc, wc, t);
     };
-    auto rows_at = [&](int64_t r) { return (int)(r1_seg - r < C ? r1_seg - r : C); };
+    auto move = [&](int by) {
+        pa += by * sa;
+        pb += by * sb;
+        pc += by * sc;
+        pos += by;
+    };
+    auto rows_at = [&](int r) { return r_end - r < C ? r_end - r : C; };
 
-    // four columns of the operand that the outputs are multiplied with
-    const int64_t xs = dir * job.x.s[1], xe = job.x.s[3];
-    const bool x_quick = xe == 1 && dc % 4 == 0 && (xs < 0 ? -xs : xs) < ((int64_t)1 << 24);
-    auto x_load = [&](const T* at, int i, int col, float (&x)[4]) {
-        if (x_quick) {
-            at += i * (int)xs + col;
-            if constexpr (sizeof(T) == 4) {
-                const u32x4 w = vload_any(at);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(w[e]);
-            } else {
-                const u32x2 w = *reinterpret_cast<const typename AnyAddr<2>::v2*>(at);
-                const u32x4 w4 = {w[0], w[1], 0u, 0u};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = vget<T>(w4, e);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = col + e < dc ? to_f32(at[i * xs + (col + e) * xe]) : 0.0f;
-        }
-    };
+    // ---- outputs: a lane has NT * 4 neighbouring columns of row 16 it + (lane & 15)
     const int64_t tokens = args.batch * args.seqlen, t0 = row0 * args.seqlen + p0;
-    auto dots_out = [&](int64_t r) {
+    const int osize = job.out_f32 ? 4 : (int)sizeof(T);
+    const int64_t opitch = (int64_t)args.heads * dc * osize;  // bytes from token to token
+    char* out = static_cast<char*>(job.out) + (t0 + dir * r_first) * opitch + (int64_t)h * dc * osize;
+    auto dots_out = [&](int r) {
         job.dots[h * tokens + t0 + dir * (r + tid)] = (dot_lds[0][tid] + dot_lds[1][tid]) + (dot_lds[2][tid] + dot_lds[3][tid]);
     };
+
     // The loop loads a chunk while it works on the one before; its first turn only loads.
-    int64_t r = r0_seg, single = 0;  // rows before `single` go one by one
+    int r = r_first, single = 0;  // rows before `single` go one by one
     int n = 0, buf = 1;
     if (tid < 2) wild_flag[tid] = 0;
     ta.none();
@@ -452,6 +496,10 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
     tc.none();
     for (;;) {
         const int otid = opaque(tid), l16 = otid & 15, g4 = (otid >> 4) & 3;
+        // the decays of the next chunk, unless this one has to be gone through again
+        const int n_plan = r + n >= r_end ? 0 : (r + n < single ? 1 : rows_at(r + n));
+        float g_next = 0.0f;
+        if (wave == 3 && n_plan > 0) g_next = g_load(r + n, n_plan);
         // ---- the chunk into LDS
         if constexpr (STATES) {
             tb.template store<false, true>(nullptr, ldsBT, otid);
@@ -468,230 +516,238 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
         const bool again = !STATES && n > 1 && wild_flag[buf];
         if (tid == 0) wild_flag[buf ^ 1] = 0;
         if (again) single = r + n;
-        const int64_t r_next = again ? r : r + n;
-        const int n_next = r_next >= r1_seg ? 0 : (r_next < single ? 1 : rows_at(r_next));
+        const int r_next = again ? r : r + n, n_next = again ? 1 : n_plan;
         const bool work = n > 0 && !again;
-        float g_next = 0.0f;
+        if (again) move(r - pos);
         if (n_next > 0) {
-            load(r_next, n_next, otid);
-            if (wave == 3) g_next = g_load(r_next, n_next);
+            load(n_next, otid);
+            move(n_next);
         }
         if (work) {
-        const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0), halfD = frag_base<DA / 8>(l16, g4 >> 1, g4 & 1);
-        const uint32_t fragC = frag_base<C / 8>(l16, g4, 0), halfC = frag_base<C / 8>(l16, g4 >> 1, g4 & 1);
-        f32x4 O[IT][NT];
-        if constexpr (!STATES) {
-            // ---- pairs: tile (rows it, columns jt) transposed, so that a lane gets four columns of a row
-            uint32_t pw[TILES / 4][PP][2];
+            const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0);
+            const uint32_t fragC = frag_base<C / 8>(l16, g4, 0), halfC = frag_base<C / 8>(l16, g4 >> 1, g4 & 1);
+            const uint32_t fragT = turn_base<C / 8>(l16, g4);
+            f32x4 O[IT][NT];
+            if constexpr (!STATES) {
+                // ---- pairs, transposed (columns x rows), so that a lane gets four columns of a row
+                uint32_t pw[PT][PP][2];
+                auto pairs = [&](auto count, int it0, int k0) {
+                    constexpr int N = decltype(count)::value;
+                    const int jt = C == 64 ? wave : wave & 1;
+                    f32x4 acc[N];
 #pragma unroll
-            for (int k = 0; k < TILES / 4; ++k) {
-                __builtin_amdgcn_sched_barrier(0);
-                const int tile = k * 4 + wave;
-                int it, jt;
-                if constexpr (C == 64) {
-                    it = tile < 2 ? 0 : tile < 4 ? 1 : tile < 8 ? 2 : 3;
-                    jt = tile < 4 ? tile & 1 : tile & 3;
-                } else {
-                    it = tile >> 1;
-                    jt = tile & 1;
-                }
-                float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (jt <= it) {
-                    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int k = 0; k < N; ++k) acc[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int s = 0; s < SA; ++s) {
-                        bf16x8 fa[P], fb[P];
+                        bf16x8 fb[P];
 #pragma unroll
-                        for (int p = 0; p < P; ++p) {
-                            fa[p] = lds_at<bf16x8>(ldsA + p * C * DA, fragD ^ frag_tile<DA / 8>(it, 4 * s));
-                            fb[p] = lds_at<bf16x8>(ldsB + p * C * DA, fragD ^ frag_tile<DA / 8>(jt, 4 * s));
+                        for (int p = 0; p < P; ++p) fb[p] = lds_at<bf16x8>(ldsB + p * C * DA, fragD ^ frag_tile<DA / 8>(jt, 4 * s));
+#pragma unroll
+                        for (int k = 0; k < N; ++k) {
+                            bf16x8 fa[P];
+#pragma unroll
+                            for (int p = 0; p < P; ++p) fa[p] = lds_at<bf16x8>(ldsA + p * C * DA, fragD ^ frag_tile<DA / 8>(it0 + k, 4 * s));
+#pragma unroll
+                            for (int p = 0; p < P; ++p)
+#pragma unroll
+                                for (int q = 0; q < P; ++q)
+                                    if (p + q <= ORD) acc[k] = mfma(fb[p], fa[q], acc[k]);
                         }
-#pragma unroll
-                        for (int p = 0; p < P; ++p)
-#pragma unroll
-                            for (int q = 0; q < P; ++q)
-                                if (p + q <= ORD) acc = mfma(fb[p], fa[q], acc);
                     }
-                    const int i = 16 * it + l16;
-                    const float hi = sums_hi[buf][i], lo = sums_lo[buf][i];
+                    const int j = 16 * jt + 4 * g4;
+                    const f32x4 jhi = *reinterpret_cast<const f32x4*>(&sums_hi[buf][j]), jlo = *reinterpret_cast<const f32x4*>(&sums_lo[buf][j]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = 16 * jt + 4 * g4 + e;
-                        const float m = __builtin_amdgcn_exp2f((hi - sums_hi[buf][j]) + (lo - sums_lo[buf][j])) * job.p_scale;
-                        f[e] = j <= i ? acc[e] * m : 0.0f;
+                    for (int k = 0; k < N; ++k) {
+                        const int i = 16 * (it0 + k) + l16;
+                        const float hi = sums_hi[buf][i], lo = sums_lo[buf][i];
+                        float f[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float m = __builtin_amdgcn_exp2f((hi - jhi[e]) + (lo - jlo[e])) * job.p_scale;
+                            f[e] = j + e <= i ? acc[k][e] * m : 0.0f;
+                        }
+                        to_planes<PP, 2>(f, pw[k0 + k]);
                     }
+                };
+                if constexpr (C == 64) {
+                    // rows before 48 have no pairs with the last 16 columns: their wavefront forms the decays instead
+                    if (wave != 3) pairs(std::integral_constant<int, 3>{}, 0, 0);
+                    else if (n_plan > 0) decays(g_next, buf ^ 1);
+                    pairs(std::integral_constant<int, 1>{}, 3, 3);
+                } else {
+                    pairs(std::integral_constant<int, 1>{}, wave >> 1, 0);
+                    if (wave == 3 && n_plan > 0) decays(g_next, buf ^ 1);
                 }
-                to_planes<PP, 2>(f, pw[k]);
-            }
-            // ---- what the state gives
+                // ---- what the state gives
 #pragma unroll
-            for (int it = 0; it < IT; ++it)
+                for (int it = 0; it < IT; ++it)
 #pragma unroll
-                for (int m = 0; m < NT; ++m) O[it][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int m = 0; m < NT; ++m) O[it][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int s = 0; s < SA; ++s) {
-                __builtin_amdgcn_sched_barrier(0);
-                uint32_t sw[NT][PP][4];
+                for (int s = 0; s < SA; ++s) {
+                    uint32_t sw[NT][PP][4];
 #pragma unroll
-                for (int m = 0; m < NT; ++m) {
-                    float f[8];
+                    for (int m = 0; m < NT; ++m) {
+                        float f[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f[e] = S[2 * s][m][e];
-                        f[4 + e] = S[2 * s + 1][m][e];
+                        for (int e = 0; e < 4; ++e) {
+                            f[e] = S[2 * s][m][e];
+                            f[4 + e] = S[2 * s + 1][m][e];
+                        }
+                        to_planes<PP, 4>(f, sw[m]);
                     }
-                    to_planes<PP, 4>(f, sw[m]);
+#pragma unroll
+                    for (int it = 0; it < IT; ++it)
+#pragma unroll
+                        for (int q = 0; q < P; ++q) {
+                            const bf16x8 fq = lds_at<bf16x8>(ldsA + q * C * DA, fragD ^ frag_tile<DA / 8>(it, 4 * s));
+#pragma unroll
+                            for (int p = 0; p < PP; ++p)
+#pragma unroll
+                                for (int m = 0; m < NT; ++m)
+                                    if (p + q <= ORD) O[it][m] = mfma(as_frag(sw[m][p]), fq, O[it][m]);
+                        }
                 }
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
+                    const float e = into[buf][16 * it + l16];
 #pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        const u32x2 w0 = lds_at<u32x2>(ldsA + q * C * DA, halfD ^ frag_tile<DA / 8>(it, 4 * s));
-                        const u32x2 w1 = lds_at<u32x2>(ldsA + q * C * DA, halfD ^ frag_tile<DA / 8>(it, 4 * s + 2));
-                        const uint32_t w[4] = {w0[0], w0[1], w1[0], w1[1]};
-#pragma unroll
-                        for (int p = 0; p < PP; ++p)
-#pragma unroll
-                            for (int m = 0; m < NT; ++m)
-                                if (p + q <= ORD) O[it][m] = mfma(as_frag(sw[m][p]), as_frag(w), O[it][m]);
-                    }
+                    for (int m = 0; m < NT; ++m) O[it][m] *= e;
                 }
-            }
+                __syncthreads();
+                // ---- the pairs to everybody
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
-                const float e = into[buf][16 * it + l16];
+                for (int k = 0; k < PT; ++k) {
+                    if (C == 64 && k < 3 && wave == 3) continue;  // (read by nobody, but for the next to the last 16 rows)
+                    const int it = C == 64 ? k : wave >> 1, jt = C == 64 ? wave : wave & 1;
 #pragma unroll
-                for (int m = 0; m < NT; ++m) O[it][m] *= e;
-            }
-            __syncthreads();
-            // ---- the pairs to everybody
-#pragma unroll
-            for (int k = 0; k < TILES / 4; ++k) {
-                const int tile = k * 4 + wave;
-                int it, jt;
-                if constexpr (C == 64) {
-                    it = tile < 2 ? 0 : tile < 4 ? 1 : tile < 8 ? 2 : 3;
-                    jt = tile < 4 ? tile & 1 : tile & 3;
-                } else {
-                    it = tile >> 1;
-                    jt = tile & 1;
+                    for (int p = 0; p < PP; ++p)
+                        *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(it, 2 * jt))) =
+                            u32x2{pw[k][p][0], pw[k][p][1]};
                 }
+                if (C == 64 && wave == 3)
 #pragma unroll
-                for (int p = 0; p < PP; ++p)
-                    *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(it, 2 * jt))) =
-                        u32x2{pw[k][p][0], pw[k][p][1]};
+                    for (int p = 0; p < PP; ++p)
+                        *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(2, 6))) = u32x2{0u, 0u};
+                __syncthreads();
             }
-            __syncthreads();
-        }
-        const float decay = whole[buf];
+            const float decay = whole[buf];
 #pragma unroll
-        for (int t = 0; t < TA; ++t)
+            for (int t = 0; t < TA; ++t)
 #pragma unroll
-            for (int m = 0; m < NT; ++m) S[t][m] *= decay;
+                for (int m = 0; m < NT; ++m) S[t][m] *= decay;
 #pragma unroll
-        for (int s = 0; s < SC; ++s) {
-            __builtin_amdgcn_sched_barrier(0);
-            bf16x8 fc[NT][P];
-            uint32_t ww[NT][SP][4];
-            float w8[8];
+            for (int s = 0; s < SC; ++s) {
+                bf16x8 fc[NT][P];
+                uint32_t ww[NT][SP][4];
+                float w8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w8[e] = left[buf][32 * s + 8 * g4 + e];
-#pragma unroll
-            for (int m = 0; m < NT; ++m) {
-                float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int p = P - 1; p >= 0; --p) {
-                    const u32x4 w = lds_at<u32x4>(ldsCT + p * DC * C, fragC ^ frag_tile<C / 8>(wave * NT + m, 4 * s));
-                    fc[m][p] = __builtin_bit_cast(bf16x8, w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] += vget<bf16>(w, e);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] *= w8[e];
-                to_planes<SP, 4>(f, ww[m]);
-            }
-            if constexpr (!STATES) {
-#pragma unroll
-                for (int it = 2 * s; it < IT; ++it) {
-#pragma unroll
-                    for (int q = 0; q < PP; ++q) {
-                        const bf16x8 fp = lds_at<bf16x8>(ldsP + q * C * C, fragC ^ frag_tile<C / 8>(it, 4 * s));
-#pragma unroll
-                        for (int p = 0; p < P; ++p)
-#pragma unroll
-                            for (int m = 0; m < NT; ++m)
-                                if (p + q <= ORD) O[it][m] = mfma(fc[m][p], fp, O[it][m]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < TA; ++t) {
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const bf16x8 fb = lds_at<bf16x8>(ldsBT + p * DA * C, fragC ^ frag_tile<C / 8>(t, 4 * s));
-#pragma unroll
-                    for (int q = 0; q < SP; ++q)
-#pragma unroll
-                        for (int m = 0; m < NT; ++m)
-                            if (p + q <= SORD) S[t][m] = mfma(fb, as_frag(ww[m][q]), S[t][m]);
-                }
-            }
-        }
-        if constexpr (!STATES) {
-            // ---- outputs: a lane has four columns of a row
-            const int64_t tok = t0 + dir * r;
-            const int pitch = (int)dir * (int)args.heads * dc;  // from a row to the next
-#pragma unroll
-            for (int it = 0; it < IT; ++it) {
-                const int i = 16 * it + l16;
-                float dot = 0.0f;
+                for (int e = 0; e < 8; ++e) w8[e] = left[buf][32 * s + 8 * g4 + e];
 #pragma unroll
                 for (int m = 0; m < NT; ++m) {
-                    const int col = wave * 16 * NT + 16 * m + 4 * g4;
-                    if (i >= n || col >= dc) continue;
-                    if (px != nullptr) {
-                        float x[4];
-                        x_load(px + r * xs, i, col, x);
+                    float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[e], dot);
+                    for (int p = P - 1; p >= 0; --p) {
+                        const u32x4 w = lds_at<u32x4>(ldsCT + p * DC * C, fragT ^ turn_tile<C / 8>(wave * NT + m, 4 * s));
+                        fc[m][p] = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = p == P - 1 ? vget<bf16>(w, e) : f[e] + vget<bf16>(w, e);
                     }
-                    const int at = i * pitch + col, some = dc - col;
-                    if (job.out_f32 || sizeof(T) == 4) {
-                        float* o = static_cast<float*>(job.out) + (tok * args.heads + h) * dc + at;
-                        if (some >= 4) *reinterpret_cast<AnyAddr<4>::v4*>(o) = __builtin_bit_cast(u32x4, O[it][m]);
-                        else
-                            for (int e = 0; e < some; ++e) o[e] = O[it][m][e];
-                    } else {
-                        T* o = static_cast<T*>(job.out) + (tok * args.heads + h) * dc + at;
-                        if (some >= 4) {
-                            typedef typename AnyAddr<sizeof(T)>::v2 any2;
-                            if constexpr (sizeof(T) == 2)
-                                *reinterpret_cast<any2*>(o) = u32x2{pack2<T>(O[it][m][0], O[it][m][1]), pack2<T>(O[it][m][2], O[it][m][3])};
-                        } else {
-                            for (int e = 0; e < some; ++e) o[e] = from_f32<T>(O[it][m][e]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= w8[e];
+                    to_planes<SP, 4>(f, ww[m]);
+                }
+                if constexpr (!STATES) {
+#pragma unroll
+                    for (int it = 2 * s; it < IT; ++it) {
+#pragma unroll
+                        for (int q = 0; q < PP; ++q) {
+                            const bf16x8 fp = lds_at<bf16x8>(ldsP + q * C * C, fragC ^ frag_tile<C / 8>(it, 4 * s));
+#pragma unroll
+                            for (int p = 0; p < P; ++p)
+#pragma unroll
+                                for (int m = 0; m < NT; ++m)
+                                    if (p + q <= ORD) O[it][m] = mfma(fc[m][p], fp, O[it][m]);
                         }
                     }
                 }
-                if (px != nullptr) {
-                    dot += __shfl_xor(dot, 16);
-                    dot += __shfl_xor(dot, 32);
-                    if (g4 == 0) dot_lds[wave][i] = dot;
+#pragma unroll
+                for (int t = 0; t < TA; ++t) {
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const bf16x8 fb = lds_at<bf16x8>(ldsBT + p * DA * C, fragT ^ turn_tile<C / 8>(t, 4 * s));
+#pragma unroll
+                        for (int q = 0; q < SP; ++q)
+#pragma unroll
+                            for (int m = 0; m < NT; ++m)
+                                if (p + q <= SORD) S[t][m] = mfma(fb, as_frag(ww[m][q]), S[t][m]);
+                    }
                 }
             }
-        }
+            if constexpr (!STATES) {
+                const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
+                // from the lowest address of the chunk, so that offsets count up in 32 bits
+                char* const low = out + (reverse ? -(C - 1) * opitch : 0);
+                const char* const xlow = reinterpret_cast<const char*>(px) + (reverse ? (C - 1) * sx * (int64_t)sizeof(T) : 0);
+                const uint32_t pitch = (uint32_t)opitch, xpitch = (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T));
+                const uint32_t row = (uint32_t)(reverse ? 15 - l16 : l16);
+                const uint32_t at = row * pitch + (uint32_t)(col * osize), xat = row * xpitch + (uint32_t)(col * (int)sizeof(T));
+                const bool full = n == C && dc == DC;
+                if (dots) {
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        const int i = 16 * it + l16;
+                        float x[4 * NT], dot = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4 * NT; ++e) x[e] = 0.0f;
+                        if (full && wx) {
+                            const T* const p = reinterpret_cast<const T*>(xlow + (uint64_t)(uint32_t)((reverse ? C - 16 - 16 * it : 16 * it) * xpitch) + xat);
+                            four_of<T, NT>(p, x);
+                        } else if (i < n) {
+#pragma unroll
+                            for (int e = 0; e < 4 * NT; ++e)
+                                if (col + e < dc) x[e] = to_f32(px[i * sx + (col + e) * job.x.s[3]]);
+                        }
+#pragma unroll
+                        for (int m = 0; m < NT; ++m)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[4 * m + e], dot);
+                        dot += __shfl_xor(dot, 16);
+                        dot += __shfl_xor(dot, 32);
+                        if (g4 == 0) dot_lds[wave][i] = dot;
+                    }
+                }
+#pragma unroll
+                for (int it = 0; it < IT; ++it) {
+                    char* const o = low + (uint64_t)(uint32_t)((reverse ? C - 16 - 16 * it : 16 * it) * pitch) + at;
+                    if (full) store_outputs<T, NT>(o, O[it], job.out_f32);
+                    else if (16 * it + l16 < n) {
+#pragma unroll
+                        for (int m = 0; m < NT; ++m)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (col + 4 * m + e < dc) {
+                                    if (job.out_f32) reinterpret_cast<float*>(o)[4 * m + e] = O[it][m][e];
+                                    else reinterpret_cast<T*>(o)[4 * m + e] = from_f32<T>(O[it][m][e]);
+                                }
+                    }
+                }
+                out += n * dir * opitch;
+                if (dots) px += n * sx;
+            }
         }
         if (n_next == 0) break;
-        if (wave == 3) decays(g_next, buf ^ 1);
+        if (wave == 3 && (STATES || !work)) decays(again ? g_load(r_next, n_next) : g_next, buf ^ 1);
         __syncthreads();
         if constexpr (!STATES)
-            if (px != nullptr && work && tid < n) dots_out(r);
+            if (dots && work && tid < n) dots_out(r);
         buf ^= 1;
         r = r_next;
         n = n_next;
     }
     if constexpr (!STATES) {
         __syncthreads();
-        if (px != nullptr && tid < n) dots_out(r);
+        if (dots && tid < n) dots_out(r);
     }
 
     // ---- the state at the segment's end
@@ -709,7 +765,7 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
             for (int m = 0; m < NT; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int row = 16 * t + 4 * g4 + e, col = col0 + 16 * m;
+                    const int row = tile_col(t, 4 * (lane >> 4) + e), col = tile_col(wave * NT + m, lane & 15);
                     if (row < da && col < dc) at[(uint32_t)(row * s2 + col * s3)] = by * S[t][m][e];
                 }
     }
