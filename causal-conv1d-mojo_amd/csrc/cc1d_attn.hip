@@ -79,7 +79,10 @@ AttnState turned(AttnState s) {
 }
 
 int launch_jobs(int dtype, const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
-    return with_dtype(dtype, [&](auto t) { return launch_attn_jobs<decltype(t)>(a, da, dc, states, stream); });
+    return with_dtype(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        return attn_quick<T>(a) ? launch_attn_modes<T, true>(a, da, dc, states, stream) : launch_attn_modes<T, false>(a, da, dc, states, stream);
+    });
 }
 
 // ---- states from segment to segment

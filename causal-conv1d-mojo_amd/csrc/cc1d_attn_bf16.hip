@@ -1,10 +1,10 @@
-// cc1d_attn_bf16.hip -- linear attention's kernels for bf16.
+// cc1d_attn_bf16.hip -- linear attention's kernels for bf16, of whole vectors.
 #include "cc1d_attn_kernels.hpp"
 
 namespace cc1d {
 
-template <> int launch_attn_jobs<bf16>(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
-    return launch_attn_modes<bf16>(a, da, dc, states, stream);
+template <> int launch_attn_modes<bf16, true>(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
+    return launch_attn_modes_impl<bf16, true>(a, da, dc, states, stream);
 }
 
 }  // namespace cc1d

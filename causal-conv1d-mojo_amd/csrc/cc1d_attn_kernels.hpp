@@ -215,35 +215,57 @@ template <typename T, int C, int D> struct AttnTile {
     static constexpr int P = AttnType<T>::planes;
     u32x4 v[N][4];
 
-    // rows positions from base on, row_stride apart. tid: the thread's index (not a loop invariant to the compiler: a
-    // register for every address would not leave enough for the state). whole: the head has all D columns, next to
-    // each other, and a chunk spans less than 2 GiB, so that full chunks go by a uniform base and 32-bit offsets.
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, bool whole, int tid) {
-        if (whole && rows == C) {
+    // Unit n of a thread: 8 neighbours take a row's neighbouring vectors, 16 two neighbouring groups of rows (a
+    // transposing store then fills whole blocks of LDS).
+    static __device__ __forceinline__ bool unit(int n, int tid, int& row, int& col) {
+        const int u = n * 256 + tid;
+        row = (u >> 4) / (CGS / 8) * 8 + ((u >> 3) & 1) * 4;
+        col = ((u >> 4) % (CGS / 8) * 8 + (u & 7)) * EPV;
+        return UNITS % 256 == 0 || u < UNITS;
+    }
+    // `rows` positions from base on, row_stride apart. tid: the thread's index (not a loop invariant to the compiler: a
+    // register for every address would not leave enough for the state).
+    // QUICK: heads of whole vectors, next to each other, and chunks that span less than 2 GiB, so that a uniform base
+    // and 32-bit offsets do; what lies outside is read as something inside and dropped.
+    template <bool QUICK> __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, int tid) {
+        if constexpr (QUICK) {
             const bool down = row_stride < 0;
+            const int last = down ? C - rows : rows - 1;  // of the rows there are, counted from the lowest address
             const char* const low = reinterpret_cast<const char*>(down ? base + (C - 1) * row_stride : base);
             const uint32_t pitch = (uint32_t)((down ? -row_stride : row_stride) * (int64_t)sizeof(T));
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int u = n * 256 + tid, row = u / CGS * 4, col = u % CGS * EPV;
-                // (idle threads read the first unit's positions and store nothing)
-                const uint32_t at = UNITS % 256 == 0 || u < UNITS ? (uint32_t)(down ? C - 4 - row : row) * pitch + col * (uint32_t)sizeof(T) : 0u;
+                int row, col;
+                const bool mine = unit(n, tid, row, col);
+                const uint32_t cb = mine && (d == D || col < d) ? col * (uint32_t)sizeof(T) : 0u;
+                if (rows == C) {
+                    const uint32_t at = (mine ? (uint32_t)(down ? C - 4 - row : row) * pitch : 0u) + cb;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[n][i] = vload_any(reinterpret_cast<const T*>(low + (uint64_t)((down ? 3 - i : i) * pitch) + at));
+                    for (int i = 0; i < 4; ++i) v[n][i] = vload_any(reinterpret_cast<const T*>(low + (uint64_t)((down ? 3 - i : i) * pitch) + at));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = down ? C - 1 - row - i : row + i;
+                        const bool in = mine && row + i < rows;
+                        v[n][i] = vload_any(reinterpret_cast<const T*>(low + (uint32_t)(in ? r : last) * (uint64_t)pitch + cb));
+                        if (!in) v[n][i] = vzero();
+                    }
+                }
+                if (d < D && col >= d) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[n][i] = vzero();
+                }
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int u = n * 256 + tid, row = u / CGS * 4, col = u % CGS * EPV;
+            for (int n = 0; n < N; ++n) {
+                int row, col;
+                const bool mine = unit(n, tid, row, col);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[n][i] = vzero();
-                if ((UNITS % 256 == 0 || u < UNITS) && row + i < rows && col < d) {
-                    const T* at = base + (row + i) * row_stride + col * elem_stride;
-                    if (elem_stride == 1 && col + EPV <= d) {
-                        v[n][i] = vload_any(at);
-                    } else {
+                for (int i = 0; i < 4; ++i) {
+                    v[n][i] = vzero();
+                    if (mine && row + i < rows) {
+                        const T* at = base + (row + i) * row_stride + col * elem_stride;
 #pragma unroll
                         for (int e = 0; e < EPV; ++e)
                             if (col + e < d) put(v[n][i], e, at[e * elem_stride]);
@@ -251,10 +273,6 @@ template <typename T, int C, int D> struct AttnTile {
                 }
             }
         }
-    }
-    static __device__ __forceinline__ bool whole(int64_t row_stride, int64_t elem_stride, int d) {
-        const int64_t r = row_stride < 0 ? -row_stride : row_stride;
-        return elem_stride == 1 && d == D && r < ((int64_t)1 << 31) / (C * (int64_t)sizeof(T));
     }
     static __device__ __forceinline__ void put(u32x4& w, int e, T x) {
         if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(to_f32(x));
@@ -294,8 +312,8 @@ template <typename T, int C, int D> struct AttnTile {
     template <bool ROWS, bool COLS> __device__ __forceinline__ void store(uint16_t* rows, uint16_t* cols, int tid) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int u = n * 256 + tid, row = u / CGS * 4, col = u % CGS * EPV;
-            if (UNITS % 256 != 0 && u >= UNITS) continue;
+            int row, col;
+            if (!unit(n, tid, row, col)) continue;
             uint32_t w[4][P][EPV / 2];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -333,19 +351,12 @@ template <typename T, int C, int D> struct AttnTile {
     }
 };
 
-// 4 * NT neighbouring values, widened.
-template <typename T, int NT> __device__ __forceinline__ void four_of(const T* p, float (&x)[4 * NT]) {
+// Four neighbouring values, widened.
+template <typename T> __device__ __forceinline__ void four_of(const T* p, float (&x)[4]) {
     if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int m = 0; m < NT; ++m) {
-            const u32x4 w = vload_any(p + 4 * m);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * m + e] = __uint_as_float(w[e]);
-        }
-    } else if constexpr (NT == 2) {
         const u32x4 w = vload_any(p);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = vget<T>(w, e);
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(w[e]);
     } else {
         const u32x2 w = *reinterpret_cast<const typename AnyAddr<2>::v2*>(p);
         const u32x4 w4 = {w[0], w[1], 0u, 0u};
@@ -373,9 +384,10 @@ template <typename T, int NT> __device__ __forceinline__ void store_outputs(char
 // products are shared: each wavefront forms those of 16 columns and passes
 // them through LDS.
 // MODE: outputs; outputs and exact states, where somebody wants the last one (the third plane of what the state
-// takes); or the state alone, of the segments that another one follows.
+// takes); or the state alone, of the segments that another one follows. QUICK: whole vectors (attn_quick()); else
+// operands are read element by element.
 enum { kAttnOut = 0, kAttnExact = 1, kAttnStates = 2 };
-template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds__(256, 2) attn_kernel(const AttnArgs args) {
+template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, 2) attn_kernel(const AttnArgs args) {
     typedef AttnType<T> Ty;
     constexpr bool STATES = MODE == kAttnStates;
     constexpr int SORD = MODE == kAttnOut ? Ty::order : 2, SP = SORD + 1;  // planes of what the state takes
@@ -463,12 +475,11 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
     int pos = r_first;
     const T *pa = base(job.a, pos), *pb = base(job.b, pos), *pc = base(job.c, pos), *px = dots ? base(job.x, pos) : nullptr;
     const int64_t sa = dir * job.a.s[1], sb = dir * job.b.s[1], sc = dir * job.c.s[1], sx = dir * job.x.s[1];
-    const bool wa = ta.whole(sa, job.a.s[3], da), wb = tb.whole(sb, job.b.s[3], da), wc = tc.whole(sc, job.c.s[3], dc);
-    const bool wx = dots && tc.whole(sx, job.x.s[3], dc);
+    const int64_t ea = job.a.s[3], eb = job.b.s[3], ec = job.c.s[3], ex = job.x.s[3];
     auto load = [&](int n, int t) {
-        if constexpr (!STATES) ta.load(pa, sa, job.a.s[3], n, da, wa, t);
-        tb.load(pb, sb, job.b.s[3], n, da, wb, t);
-        tc.load(pc, sc, job.c.s[3], n, dc, wc, t);
+        if constexpr (!STATES) ta.template load<QUICK>(pa, sa, ea, n, da, t);
+        tb.template load<QUICK>(pb, sb, eb, n, da, t);
+        tc.template load<QUICK>(pc, sc, ec, n, dc, t);
     };
     auto move = [&](int by) {
         pa += by * sa;
@@ -529,62 +540,21 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
             const uint32_t fragT = turn_base<C / 8>(l16, g4);
             f32x4 O[IT][NT];
             if constexpr (!STATES) {
-                // ---- pairs, transposed (columns x rows), so that a lane gets four columns of a row
-                uint32_t pw[PT][PP][2];
-                auto pairs = [&](auto count, int it0, int k0) {
-                    constexpr int N = decltype(count)::value;
-                    const int jt = C == 64 ? wave : wave & 1;
-                    f32x4 acc[N];
+                // ---- what the state gives, and the pairs, transposed (columns x rows), so that a lane gets four columns
+                // of a row: both from one reading of the rows
+                const int jt = C == 64 ? wave : wave & 1, it0 = C == 64 ? 0 : wave >> 1;  // this wavefront's columns; its first rows
+                f32x4 acc[PT];
 #pragma unroll
-                    for (int k = 0; k < N; ++k) acc[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int s = 0; s < SA; ++s) {
-                        bf16x8 fb[P];
-#pragma unroll
-                        for (int p = 0; p < P; ++p) fb[p] = lds_at<bf16x8>(ldsB + p * C * DA, fragD ^ frag_tile<DA / 8>(jt, 4 * s));
-#pragma unroll
-                        for (int k = 0; k < N; ++k) {
-                            bf16x8 fa[P];
-#pragma unroll
-                            for (int p = 0; p < P; ++p) fa[p] = lds_at<bf16x8>(ldsA + p * C * DA, fragD ^ frag_tile<DA / 8>(it0 + k, 4 * s));
-#pragma unroll
-                            for (int p = 0; p < P; ++p)
-#pragma unroll
-                                for (int q = 0; q < P; ++q)
-                                    if (p + q <= ORD) acc[k] = mfma(fb[p], fa[q], acc[k]);
-                        }
-                    }
-                    const int j = 16 * jt + 4 * g4;
-                    const f32x4 jhi = *reinterpret_cast<const f32x4*>(&sums_hi[buf][j]), jlo = *reinterpret_cast<const f32x4*>(&sums_lo[buf][j]);
-#pragma unroll
-                    for (int k = 0; k < N; ++k) {
-                        const int i = 16 * (it0 + k) + l16;
-                        const float hi = sums_hi[buf][i], lo = sums_lo[buf][i];
-                        float f[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float m = __builtin_amdgcn_exp2f((hi - jhi[e]) + (lo - jlo[e])) * job.p_scale;
-                            f[e] = j + e <= i ? acc[k][e] * m : 0.0f;
-                        }
-                        to_planes<PP, 2>(f, pw[k0 + k]);
-                    }
-                };
-                if constexpr (C == 64) {
-                    // rows before 48 have no pairs with the last 16 columns: their wavefront forms the decays instead
-                    if (wave != 3) pairs(std::integral_constant<int, 3>{}, 0, 0);
-                    else if (n_plan > 0) decays(g_next, buf ^ 1);
-                    pairs(std::integral_constant<int, 1>{}, 3, 3);
-                } else {
-                    pairs(std::integral_constant<int, 1>{}, wave >> 1, 0);
-                    if (wave == 3 && n_plan > 0) decays(g_next, buf ^ 1);
-                }
-                // ---- what the state gives
+                for (int k = 0; k < PT; ++k) acc[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int it = 0; it < IT; ++it)
 #pragma unroll
                     for (int m = 0; m < NT; ++m) O[it][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int s = 0; s < SA; ++s) {
+                    bf16x8 fb[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) fb[p] = lds_at<bf16x8>(ldsB + p * C * DA, fragD ^ frag_tile<DA / 8>(jt, 4 * s));
                     uint32_t sw[NT][PP][4];
 #pragma unroll
                     for (int m = 0; m < NT; ++m) {
@@ -606,6 +576,10 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
 #pragma unroll
                                 for (int m = 0; m < NT; ++m)
                                     if (p + q <= ORD) O[it][m] = mfma(as_frag(sw[m][p]), fq, O[it][m]);
+                            if (C == 64 || it == it0)
+#pragma unroll
+                                for (int p = 0; p < P; ++p)
+                                    if (p + q <= ORD) acc[C == 64 ? it : 0] = mfma(fb[p], fq, acc[C == 64 ? it : 0]);
                         }
                 }
 #pragma unroll
@@ -614,12 +588,32 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
 #pragma unroll
                     for (int m = 0; m < NT; ++m) O[it][m] *= e;
                 }
+                uint32_t pw[PT][PP][2];
+                const int j = 16 * jt + 4 * g4;
+                const f32x4 jhi = *reinterpret_cast<const f32x4*>(&sums_hi[buf][j]), jlo = *reinterpret_cast<const f32x4*>(&sums_lo[buf][j]);
+                auto pairs = [&](int it, const f32x4& a, uint32_t (&w)[PP][2]) {
+                    const int i = 16 * it + l16;
+                    const float hi = sums_hi[buf][i], lo = sums_lo[buf][i];
+                    float f[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float m = __builtin_amdgcn_exp2f((hi - jhi[e]) + (lo - jlo[e])) * job.p_scale;
+                        f[e] = j + e <= i ? a[e] * m : 0.0f;
+                    }
+                    to_planes<PP, 2>(f, w);
+                };
+                // rows before 48 have no pairs with the last 16 columns: their wavefront forms the decays instead
+                if (C == 64 && wave != 3)
+#pragma unroll
+                    for (int k = 0; k < PT - 1; ++k) pairs(k, acc[k], pw[k]);
+                if (wave == 3 && n_plan > 0) decays(g_next, buf ^ 1);
+                pairs(C == 64 ? 3 : it0, acc[PT - 1], pw[PT - 1]);
                 __syncthreads();
                 // ---- the pairs to everybody
 #pragma unroll
                 for (int k = 0; k < PT; ++k) {
                     if (C == 64 && k < 3 && wave == 3) continue;  // (read by nobody, but for the next to the last 16 rows)
-                    const int it = C == 64 ? k : wave >> 1, jt = C == 64 ? wave : wave & 1;
+                    const int it = it0 + k;
 #pragma unroll
                     for (int p = 0; p < PP; ++p)
                         *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(it, 2 * jt))) =
@@ -685,6 +679,7 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
                 }
             }
             if constexpr (!STATES) {
+                if constexpr (!QUICK) __builtin_amdgcn_sched_barrier(0);
                 const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
                 // from the lowest address of the chunk, so that offsets count up in 32 bits
                 char* const low = out + (reverse ? -(C - 1) * opitch : 0);
@@ -697,21 +692,21 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
 #pragma unroll
                     for (int it = 0; it < IT; ++it) {
                         const int i = 16 * it + l16;
-                        float x[4 * NT], dot = 0.0f;
+                        const T* const p = reinterpret_cast<const T*>(xlow + (uint64_t)(uint32_t)((reverse ? C - 16 - 16 * it : 16 * it) * xpitch) + xat);
+                        float dot = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 4 * NT; ++e) x[e] = 0.0f;
-                        if (full && wx) {
-                            const T* const p = reinterpret_cast<const T*>(xlow + (uint64_t)(uint32_t)((reverse ? C - 16 - 16 * it : 16 * it) * xpitch) + xat);
-                            four_of<T, NT>(p, x);
-                        } else if (i < n) {
+                        for (int m = 0; m < NT; ++m) {
+                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            if constexpr (QUICK) {
+                                if (full || (i < n && col + 4 * m < dc)) four_of<T>(p + 4 * m, x);
+                            } else {
 #pragma unroll
-                            for (int e = 0; e < 4 * NT; ++e)
-                                if (col + e < dc) x[e] = to_f32(px[i * sx + (col + e) * job.x.s[3]]);
+                                for (int e = 0; e < 4; ++e)
+                                    if (i < n && col + 4 * m + e < dc) x[e] = to_f32(px[i * sx + (col + 4 * m + e) * ex]);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[e], dot);
                         }
-#pragma unroll
-                        for (int m = 0; m < NT; ++m)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[4 * m + e], dot);
                         dot += __shfl_xor(dot, 16);
                         dot += __shfl_xor(dot, 32);
                         if (g4 == 0) dot_lds[wave][i] = dot;
@@ -720,16 +715,22 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
                     char* const o = low + (uint64_t)(uint32_t)((reverse ? C - 16 - 16 * it : 16 * it) * pitch) + at;
-                    if (full) store_outputs<T, NT>(o, O[it], job.out_f32);
-                    else if (16 * it + l16 < n) {
+                    if (full) {
+                        store_outputs<T, NT>(o, O[it], job.out_f32);
+                    } else if (16 * it + l16 < n) {
 #pragma unroll
-                        for (int m = 0; m < NT; ++m)
+                        for (int m = 0; m < NT; ++m) {
+                            if (QUICK && col + 4 * m + 4 <= dc) {
+                                store_outputs<T, 1>(o + 4 * m * osize, {O[it][m]}, job.out_f32);
+                                continue;
+                            }
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 if (col + 4 * m + e < dc) {
                                     if (job.out_f32) reinterpret_cast<float*>(o)[4 * m + e] = O[it][m][e];
                                     else reinterpret_cast<T*>(o)[4 * m + e] = from_f32<T>(O[it][m][e]);
                                 }
+                        }
                     }
                 }
                 out += n * dir * opitch;
@@ -784,24 +785,39 @@ template <typename T, int DA, int DC, int MODE> __global__ void __launch_bounds_
     }
 }
 
-template <typename T, int MODE> int launch_attn_sizes(const AttnArgs& a, int da, int dc, hipStream_t stream) {
-    const dim3 grid(a.blocks), block(256);
-    if (da <= 64 && dc <= 64) return launch(attn_kernel<T, 64, 64, MODE>, grid, block, stream, a);
-    if (da <= 64) return launch(attn_kernel<T, 64, 128, MODE>, grid, block, stream, a);
-    if (dc <= 64) return launch(attn_kernel<T, 128, 64, MODE>, grid, block, stream, a);
-    return launch(attn_kernel<T, 128, 128, MODE>, grid, block, stream, a);
+// Whether every operand of every job is made of whole 16-byte vectors, and a chunk of it spans less than 2 GiB.
+template <typename T> bool attn_quick(const AttnArgs& a) {
+    constexpr int64_t EPV = elems16<T>::value;
+    auto fits = [&](const AttnOperand& o, int d) {
+        const int64_t r = o.s[1] < 0 ? -o.s[1] : o.s[1];
+        return o.p == nullptr || (o.s[3] == 1 && d % EPV == 0 && r < ((int64_t)1 << 31) / (64 * (int64_t)sizeof(T)));
+    };
+    bool quick = true;
+    for (uint32_t j = 0; j < a.jobs; ++j) {
+        const AttnJob& b = a.job[j];
+        quick = quick && fits(b.a, b.da) && fits(b.b, b.da) && fits(b.c, b.dc) && fits(b.x, b.dc);
+    }
+    return quick;
 }
 
-// All jobs of `a` have rows of da and values of dc (explicitly instantiated in cc1d_attn_<dtype>.hip).
-template <typename T> int launch_attn_jobs(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream);
-template <typename T> int launch_attn_modes(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
-    if (states) return launch_attn_sizes<T, kAttnStates>(a, da, dc, stream);
+template <typename T, int MODE, bool QUICK> int launch_attn_sizes(const AttnArgs& a, int da, int dc, hipStream_t stream) {
+    const dim3 grid(a.blocks), block(256);
+    if (da <= 64 && dc <= 64) return launch(attn_kernel<T, 64, 64, MODE, QUICK>, grid, block, stream, a);
+    if (da <= 64) return launch(attn_kernel<T, 64, 128, MODE, QUICK>, grid, block, stream, a);
+    if (dc <= 64) return launch(attn_kernel<T, 128, 64, MODE, QUICK>, grid, block, stream, a);
+    return launch(attn_kernel<T, 128, 128, MODE, QUICK>, grid, block, stream, a);
+}
+
+// All jobs of `a` have rows of da and values of dc (explicitly instantiated in cc1d_attn_<dtype>[_any].hip).
+template <typename T, bool QUICK> int launch_attn_modes(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream);
+template <typename T, bool QUICK> int launch_attn_modes_impl(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
+    if (states) return launch_attn_sizes<T, kAttnStates, QUICK>(a, da, dc, stream);
     if constexpr (AttnType<T>::order < 2) {
         bool exact = false;
         for (uint32_t j = 0; j < a.jobs; ++j) exact = exact || a.job[j].last.p != nullptr;
-        if (!exact) return launch_attn_sizes<T, kAttnOut>(a, da, dc, stream);
+        if (!exact) return launch_attn_sizes<T, kAttnOut, QUICK>(a, da, dc, stream);
     }
-    return launch_attn_sizes<T, kAttnExact>(a, da, dc, stream);
+    return launch_attn_sizes<T, kAttnExact, QUICK>(a, da, dc, stream);
 }
 
 }  // namespace cc1d
