@@ -80,6 +80,7 @@ template <> struct AttnType<float> { static constexpr int planes = 3, chunk = 32
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t uint16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -103,42 +104,49 @@ template <int P, int N> __device__ __forceinline__ void to_planes(const float (&
 }
 __device__ __forceinline__ bf16x8 as_frag(const uint32_t (&w)[4]) { return __builtin_bit_cast(bf16x8, w); }
 
-// 16-byte block `blk` of an LDS row, permuted so that neither the rows that a
-// fragment takes nor the columns that a transposing store takes share banks
+// LDS images: rows of BLKS 16-byte blocks, block `blk` of a row permuted so
+// that the 16 rows of a fragment lie in 16 different places of the 64 banks,
+// and the four rows by four blocks of a transposing read as well.
 template <int BLKS> __device__ __forceinline__ int swizzle(int row, int blk) {
-    if constexpr (BLKS >= 8) return blk ^ ((row ^ (row >> 3)) & 7);
-    else return blk ^ (((row >> 1) ^ (row >> 3)) & (BLKS - 1));
+    if constexpr (BLKS == 16) return blk ^ (4 * (row & 3) + ((row >> 2) & 3));
+    else if constexpr (BLKS == 8) return blk ^ (4 * ((row >> 1) & 1) + ((row >> 2) & 3));
+    else return blk ^ ((row >> 2) & 3);
 }
-
-// Byte offsets of fragments: row 16 t + (lane & 15) of an image whose rows have
-// BLKS blocks, block b + (what the lane adds): a base of the lane's, xor a
-// constant of the tile's.
+// Byte offsets: row 16 t + (lane & 15), block b + (what the lane adds) is a base of the lane's, xor a constant of the
+// tile's (b a multiple of what the lane adds at most).
 template <int BLKS> __device__ __forceinline__ uint32_t frag_base(int l16, int blk, int half) {
     return (uint32_t)(l16 * BLKS * 16 + swizzle<BLKS>(l16, blk) * 16 + half * 8);
 }
-template <int BLKS> __device__ __forceinline__ uint32_t frag_tile(int t, int blk) {
-    return (uint32_t)(t * 16 * BLKS * 16 | ((blk ^ (2 * t & (BLKS >= 8 ? 7 : BLKS - 1))) * 16));
-}
-
-// Transposed images (columns of operands and values, positions next to each
-// other). Two neighbouring tiles share 32 of them in turns of four: lane
-// l & 15 of tile t has 32 (t / 2) + 8 (l / 4) + 4 (t % 2) + l % 4, so that the
-// accumulators of the two tiles hold eight neighbours in each lane, which is
-// what a fragment of the next product (or a 16-byte store) wants.
-template <int BLKS> __device__ __forceinline__ int swizzle_t(int row, int blk) {
-    if constexpr (BLKS >= 8) return blk ^ (((row & 3) ^ ((row >> 4) & 3)) | ((row >> 1) & 4));
-    else return blk ^ ((((row >> 1) ^ (row >> 4)) & 1) | ((row >> 2) & 2));
-}
-__device__ __forceinline__ int tile_col(int t, int l16) { return 32 * (t >> 1) + 4 * (t & 1) + 8 * (l16 >> 2) + (l16 & 3); }
-template <int BLKS> __device__ __forceinline__ uint32_t turn_base(int l16, int blk) {
-    const int row = tile_col(0, l16);
-    return (uint32_t)(row * BLKS * 16 + swizzle_t<BLKS>(row, blk) * 16);
-}
-template <int BLKS> __device__ __forceinline__ uint32_t turn_tile(int t, int blk) {
-    return (uint32_t)((32 * (t >> 1) + 4 * (t & 1)) * BLKS * 16 | ((BLKS >= 8 ? blk ^ (2 * ((t >> 1) & 1)) : blk) * 16));
-}
+template <int BLKS> __device__ __forceinline__ uint32_t frag_tile(int t, int blk) { return (uint32_t)(t * 16 * BLKS * 16 | blk * 16); }
+typedef __attribute__((address_space(3))) char lds_char;
 template <typename V> __device__ __forceinline__ V lds_at(const uint16_t* image, uint32_t off) {
     return *reinterpret_cast<const V*>(reinterpret_cast<const char*>(image) + off);
+}
+
+// Fragments across an image's rows (its positions are the inner index of the
+// product): ds_read_b64_tr_b16 gives lane l of 16 the l-th of the 16 columns
+// that lanes 4 r .. 4 r + 3 name in row r, for four rows. Two neighbouring
+// tiles share 32 columns in turns of four, lane l of tile t has
+// tile_col(t, l), so that the accumulators of the two tiles hold eight
+// neighbours in each lane, which is what a fragment of the next product (or a
+// 16-byte store) wants.
+__device__ __forceinline__ int tile_col(int t, int l16) { return 32 * (t >> 1) + 4 * (t & 1) + 8 * (l16 >> 2) + (l16 & 3); }
+template <int BLKS> __device__ __forceinline__ uint32_t turn_base(int l16, int g4) {
+    const int row = 8 * g4 + (l16 >> 2);
+    return (uint32_t)(row * BLKS * 16 + swizzle<BLKS>(row, l16 & 3) * 16);
+}
+// positions 32 s .. of tile t, as a fragment
+template <int BLKS> __device__ __forceinline__ u32x4 turn_at(const uint16_t* image, uint32_t base, int t, int s) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    lds_char* const at = (lds_char*)image;
+    u32x2 w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t off = base ^ (uint32_t)((32 * s + 4 * h) * BLKS * 16 | ((4 * (t >> 1)) ^ h) * 16 | (t & 1) * 8);
+        w[h] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + off)));
+    }
+    return u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
 }
 
 // exp2 of a sum held in two floats: the second is at most an ulp of the first
@@ -207,70 +215,58 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, uint32_t slot) 
     return s;
 }
 
-// What one thread carries of a chunk of one operand from HBM to LDS: units of
-// 4 positions x one 16-byte vector, so that four positions of a column leave
-// for the transposed image in one store.
-template <typename T, int C, int D> struct AttnTile {
-    static constexpr int EPV = elems16<T>::value, CGS = D / EPV, UNITS = C / 4 * CGS, N = (UNITS + 255) / 256;
-    static constexpr int P = AttnType<T>::planes;
-    u32x4 v[N][4];
+// A chunk of one operand, from HBM into its image: bf16 of whole vectors goes
+// straight there (global_load_lds), else through registers, where a value
+// becomes its planes.
+template <typename T, int C, int D, bool QUICK> struct AttnTile {
+    static constexpr int EPV = elems16<T>::value, CGS = D / EPV, UNITS = C * CGS, N = UNITS / 256, P = AttnType<T>::planes;
+    static constexpr bool DIRECT = QUICK && std::is_same_v<T, bf16>;
+    static_assert(UNITS % 256 == 0, "whole turns of a block");
+    u32x4 v[DIRECT ? 1 : N];
 
-    // Unit n of a thread: 8 neighbours take a row's neighbouring vectors, 16 two neighbouring groups of rows (a
-    // transposing store then fills whole blocks of LDS).
-    static __device__ __forceinline__ bool unit(int n, int tid, int& row, int& col) {
+    // Vector n of a thread: its row and column; neighbouring lanes take neighbouring places of the image. tid: the
+    // thread's index (not a loop invariant to the compiler: a register for every address would not leave enough for the
+    // state).
+    static __device__ __forceinline__ void unit(int n, int tid, int& row, int& col) {
         const int u = n * 256 + tid;
-        row = (u >> 4) / (CGS / 8) * 8 + ((u >> 3) & 1) * 4;
-        col = ((u >> 4) % (CGS / 8) * 8 + (u & 7)) * EPV;
-        return UNITS % 256 == 0 || u < UNITS;
+        row = u / CGS;
+        col = u % CGS * EPV;
+        if constexpr (DIRECT) col = swizzle<CGS>(row, u % CGS) * EPV;
     }
-    // `rows` positions from base on, row_stride apart. tid: the thread's index (not a loop invariant to the compiler: a
-    // register for every address would not leave enough for the state).
-    // QUICK: heads of whole vectors, next to each other, and chunks that span less than 2 GiB, so that a uniform base
-    // and 32-bit offsets do; what lies outside is read as something inside and dropped.
-    template <bool QUICK> __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, int tid) {
+    // `rows` positions from base on, row_stride apart. QUICK: heads of whole vectors, next to each other, and chunks
+    // that span less than 2 GiB, so that a uniform base and 32-bit offsets do.
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, uint16_t* image, int tid) {
         if constexpr (QUICK) {
             const bool down = row_stride < 0;
-            const int last = down ? C - rows : rows - 1;  // of the rows there are, counted from the lowest address
             const char* const low = reinterpret_cast<const char*>(down ? base + (C - 1) * row_stride : base);
             const uint32_t pitch = (uint32_t)((down ? -row_stride : row_stride) * (int64_t)sizeof(T));
+            const bool all = rows == C && d == D;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 int row, col;
-                const bool mine = unit(n, tid, row, col);
-                const uint32_t cb = mine && (d == D || col < d) ? col * (uint32_t)sizeof(T) : 0u;
-                if (rows == C) {
-                    const uint32_t at = (mine ? (uint32_t)(down ? C - 4 - row : row) * pitch : 0u) + cb;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[n][i] = vload_any(reinterpret_cast<const T*>(low + (uint64_t)((down ? 3 - i : i) * pitch) + at));
+                unit(n, tid, row, col);
+                const bool in = all || (row < rows && col < d);
+                const char* const at = low + (uint32_t)((uint32_t)(down ? C - 1 - row : row) * pitch + col * (uint32_t)sizeof(T));
+                if constexpr (DIRECT) {
+                    uint16_t* const to = image + (n * 256 + uniform32(tid & ~63)) * 8;  // of the wavefront; its lanes follow
+                    if (in) __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+                    else *reinterpret_cast<u32x4*>(to + (tid & 63) * 8) = vzero();
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = down ? C - 1 - row - i : row + i;
-                        const bool in = mine && row + i < rows;
-                        v[n][i] = vload_any(reinterpret_cast<const T*>(low + (uint32_t)(in ? r : last) * (uint64_t)pitch + cb));
-                        if (!in) v[n][i] = vzero();
-                    }
-                }
-                if (d < D && col >= d) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[n][i] = vzero();
+                    v[n] = vzero();
+                    if (in) v[n] = vload_any(reinterpret_cast<const T*>(at));
                 }
             }
         } else {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 int row, col;
-                const bool mine = unit(n, tid, row, col);
+                unit(n, tid, row, col);
+                v[n] = vzero();
+                if (row >= rows) continue;
+                const T* const at = base + row * row_stride + col * elem_stride;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[n][i] = vzero();
-                    if (mine && row + i < rows) {
-                        const T* at = base + (row + i) * row_stride + col * elem_stride;
-#pragma unroll
-                        for (int e = 0; e < EPV; ++e)
-                            if (col + e < d) put(v[n][i], e, at[e * elem_stride]);
-                    }
-                }
+                for (int e = 0; e < EPV; ++e)
+                    if (col + e < d) put(v[n], e, at[e * elem_stride]);
             }
         }
     }
@@ -279,73 +275,31 @@ template <typename T, int C, int D> struct AttnTile {
         else w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, x) << (16 * (e & 1));
     }
     __device__ __forceinline__ void none() {
+        if constexpr (!DIRECT)
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[n][i] = vzero();
+            for (int n = 0; n < N; ++n) v[n] = vzero();
     }
-    // whether anything is infinite or NaN
-    __device__ __forceinline__ bool wild() const {
-        if constexpr (sizeof(T) == 4) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) m = max(m, v[n][i][d] & 0x7f800000u);
-            return m == 0x7f800000u;
-        } else {
-            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-            constexpr uint32_t M = std::is_same_v<T, bf16> ? 0x7f807f80u : 0x7c007c00u;
-            u16x2 m = {0, 0};
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[n][i][d] & M));
-            return m[0] == (M & 0xffffu) || m[1] == (M & 0xffffu);
-        }
-    }
-    // rows[plane][position][column] and / or cols[plane][column][position]
-    template <bool ROWS, bool COLS> __device__ __forceinline__ void store(uint16_t* rows, uint16_t* cols, int tid) const {
+    // image[plane][position][column]
+    __device__ __forceinline__ void store(uint16_t* image, int tid) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             int row, col;
-            if (!unit(n, tid, row, col)) continue;
-            uint32_t w[4][P][EPV / 2];
+            unit(n, tid, row, col);
+            uint32_t w[P][EPV / 2];
+            if constexpr (std::is_same_v<T, bf16>) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (std::is_same_v<T, bf16>) {
+                for (int i = 0; i < 4; ++i) w[0][i] = v[n][i];
+            } else {
+                float f[EPV];
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) w[i][0][d] = v[n][i][d];
-                } else {
-                    float f[EPV];
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) f[e] = vget<T>(v[n][i], e);
-                    to_planes<P, EPV / 2>(f, w[i]);
-                }
+                for (int e = 0; e < EPV; ++e) f[e] = vget<T>(v[n], e);
+                to_planes<P, EPV / 2>(f, w);
             }
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                if constexpr (ROWS) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint16_t* at = rows + (p * C + row + i) * D + swizzle<D / 8>(row + i, col >> 3) * 8 + (col & 7);
-                        if constexpr (EPV == 8) *reinterpret_cast<u32x4*>(at) = u32x4{w[i][p][0], w[i][p][1], w[i][p][2], w[i][p][3]};
-                        else *reinterpret_cast<u32x2*>(at) = u32x2{w[i][p][0], w[i][p][1]};
-                    }
-                }
-                if constexpr (COLS) {
-#pragma unroll
-                    for (int e = 0; e < EPV; ++e) {
-                        const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;  // the high or the low halves of two dwords
-                        const u32x2 q = {__builtin_amdgcn_perm(w[1][p][e >> 1], w[0][p][e >> 1], sel),
-                                         __builtin_amdgcn_perm(w[3][p][e >> 1], w[2][p][e >> 1], sel)};
-                        *reinterpret_cast<u32x2*>(cols + (p * D + col + e) * C + swizzle_t<C / 8>(col + e, row >> 3) * 8 + (row & 7)) = q;
-                    }
-                }
+                uint16_t* const at = image + (p * C + row) * D + swizzle<D / 8>(row, col >> 3) * 8 + (col & 7);
+                if constexpr (EPV == 8) *reinterpret_cast<u32x4*>(at) = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+                else *reinterpret_cast<u32x2*>(at) = u32x2{w[p][0], w[p][1]};
             }
         }
     }
@@ -387,21 +341,19 @@ template <typename T, int NT> __device__ __forceinline__ void store_outputs(char
 // takes); or the state alone, of the segments that another one follows. QUICK: whole vectors (attn_quick()); else
 // operands are read element by element.
 enum { kAttnOut = 0, kAttnExact = 1, kAttnStates = 2 };
-template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, 2) attn_kernel(const AttnArgs args) {
+template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 ? 3 : 2) attn_kernel(const AttnArgs args) {
     typedef AttnType<T> Ty;
     constexpr bool STATES = MODE == kAttnStates;
     constexpr int SORD = MODE == kAttnOut ? Ty::order : 2, SP = SORD + 1;  // planes of what the state takes
     constexpr int C = Ty::chunk, P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
     constexpr int NT = DC / 64, TA = DA / 16, SC = C / 32, SA = DA / 32, IT = C / 16;
     constexpr int PT = C == 64 ? 4 : 1;  // tiles of the pairs that a wavefront forms
-    constexpr int kA = STATES ? 0 : P * C * DA, kPairs = PP * C * C;
-    constexpr int kB = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
-    __shared__ __attribute__((aligned(16))) uint16_t lds[kA + kB + P * DA * C + P * DC * C];
+    constexpr int kPairs = PP * C * C, kA = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
+    __shared__ __attribute__((aligned(16))) uint16_t lds[kA + P * C * DA + P * C * DC];
     __shared__ __attribute__((aligned(16))) float sums_hi[2][C], sums_lo[2][C], into[2][C], left[2][C];
     __shared__ float whole[2], dot_lds[4][C];
-    __shared__ int wild_flag[2];
-    uint16_t *const ldsA = lds, *const ldsB = lds + kA, *const ldsBT = lds + kA + kB, *const ldsCT = ldsBT + P * DA * C;
-    uint16_t* const ldsP = ldsB;  // the columns are dead once the pairs' products are formed
+    uint16_t *const ldsA = lds, *const ldsB = lds + kA, *const ldsC = ldsB + P * C * DA;
+    uint16_t* const ldsP = ldsA;  // the rows are dead once their products are formed
 
     const int tid = threadIdx.x, wave = uniform32(tid >> 6), lane = tid & 63;
     const uint32_t id = xcd_block(blockIdx.x, args.blocks);
@@ -470,22 +422,20 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     };
 
     // ---- operands: where the next chunk starts, and the step from row to row
-    AttnTile<T, C, DA> ta, tb;
-    AttnTile<T, C, DC> tc;
-    int pos = r_first;
-    const T *pa = base(job.a, pos), *pb = base(job.b, pos), *pc = base(job.c, pos), *px = dots ? base(job.x, pos) : nullptr;
+    AttnTile<T, C, DA, QUICK> ta, tb;
+    AttnTile<T, C, DC, QUICK> tc;
+    constexpr bool DIRECT = decltype(ta)::DIRECT;
+    const T *pa = base(job.a, r_first), *pb = base(job.b, r_first), *pc = base(job.c, r_first), *px = dots ? base(job.x, r_first) : nullptr;
     const int64_t sa = dir * job.a.s[1], sb = dir * job.b.s[1], sc = dir * job.c.s[1], sx = dir * job.x.s[1];
     const int64_t ea = job.a.s[3], eb = job.b.s[3], ec = job.c.s[3], ex = job.x.s[3];
+    // the next n rows, and on past them
     auto load = [&](int n, int t) {
-        if constexpr (!STATES) ta.template load<QUICK>(pa, sa, ea, n, da, t);
-        tb.template load<QUICK>(pb, sb, eb, n, da, t);
-        tc.template load<QUICK>(pc, sc, ec, n, dc, t);
-    };
-    auto move = [&](int by) {
-        pa += by * sa;
-        pb += by * sb;
-        pc += by * sc;
-        pos += by;
+        if constexpr (!STATES) ta.load(pa, sa, ea, n, da, ldsA, t);
+        tb.load(pb, sb, eb, n, da, ldsB, t);
+        tc.load(pc, sc, ec, n, dc, ldsC, t);
+        pa += n * sa;
+        pb += n * sb;
+        pc += n * sc;
     };
     auto rows_at = [&](int r) { return r_end - r < C ? r_end - r : C; };
 
@@ -498,46 +448,33 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
         job.dots[h * tokens + t0 + dir * (r + tid)] = (dot_lds[0][tid] + dot_lds[1][tid]) + (dot_lds[2][tid] + dot_lds[3][tid]);
     };
 
-    // The loop loads a chunk while it works on the one before; its first turn only loads.
-    int r = r_first, single = 0;  // rows before `single` go one by one
-    int n = 0, buf = 1;
-    if (tid < 2) wild_flag[tid] = 0;
+    // Registers load a chunk while the block works on the one before; what goes straight into its image is waited for
+    // while the CU's other blocks work. The first turn only loads (or only forms the decays).
+    int r = r_first, n = 0, buf = 1;
     ta.none();
     tb.none();
     tc.none();
     for (;;) {
         const int otid = opaque(tid), l16 = otid & 15, g4 = (otid >> 4) & 3;
-        // the decays of the next chunk, unless this one has to be gone through again
-        const int n_plan = r + n >= r_end ? 0 : (r + n < single ? 1 : rows_at(r + n));
+        const int n_next = rows_at(r + n);
         float g_next = 0.0f;
-        if (wave == 3 && n_plan > 0) g_next = g_load(r + n, n_plan);
+        if (wave == 3 && n_next > 0) g_next = g_load(r + n, n_next);
         // ---- the chunk into LDS
-        if constexpr (STATES) {
-            tb.template store<false, true>(nullptr, ldsBT, otid);
+        if constexpr (DIRECT) {
+            if (n > 0) load(n, otid);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         } else {
-            ta.template store<true, false>(ldsA, nullptr, otid);
-            tb.template store<true, true>(ldsB, ldsBT, otid);
+            if constexpr (!STATES) ta.store(ldsA, otid);
+            tb.store(ldsB, otid);
+            tc.store(ldsC, otid);
         }
-        tc.template store<false, true>(nullptr, ldsCT, otid);
-        if constexpr (!STATES)
-            if (tc.wild()) wild_flag[buf] = 1;
         __syncthreads();
-        // An infinite or NaN value is multiplied with the zeros of the pairs that come before it: such a chunk goes
-        // position by position, so that it reaches the later ones alone.
-        const bool again = !STATES && n > 1 && wild_flag[buf];
-        if (tid == 0) wild_flag[buf ^ 1] = 0;
-        if (again) single = r + n;
-        const int r_next = again ? r : r + n, n_next = again ? 1 : n_plan;
-        const bool work = n > 0 && !again;
-        if (again) move(r - pos);
-        if (n_next > 0) {
-            load(n_next, otid);
-            move(n_next);
-        }
-        if (work) {
+        if constexpr (!DIRECT)
+            if (n_next > 0) load(n_next, otid);
+        if (n > 0) {
             const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0);
             const uint32_t fragC = frag_base<C / 8>(l16, g4, 0), halfC = frag_base<C / 8>(l16, g4 >> 1, g4 & 1);
-            const uint32_t fragT = turn_base<C / 8>(l16, g4);
+            const uint32_t turnB = turn_base<DA / 8>(l16, g4), turnC = turn_base<DC / 8>(l16, g4);
             f32x4 O[IT][NT];
             if constexpr (!STATES) {
                 // ---- what the state gives, and the pairs, transposed (columns x rows), so that a lane gets four columns
@@ -606,7 +543,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 if (C == 64 && wave != 3)
 #pragma unroll
                     for (int k = 0; k < PT - 1; ++k) pairs(k, acc[k], pw[k]);
-                if (wave == 3 && n_plan > 0) decays(g_next, buf ^ 1);
+                if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
                 pairs(C == 64 ? 3 : it0, acc[PT - 1], pw[PT - 1]);
                 __syncthreads();
                 // ---- the pairs to everybody
@@ -626,13 +563,14 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 __syncthreads();
             }
             const float decay = whole[buf];
+            bool wild = false;
 #pragma unroll
             for (int t = 0; t < TA; ++t)
 #pragma unroll
                 for (int m = 0; m < NT; ++m) S[t][m] *= decay;
 #pragma unroll
             for (int s = 0; s < SC; ++s) {
-                bf16x8 fc[NT][P];
+                u32x4 fc[NT][P];
                 uint32_t ww[NT][SP][4];
                 float w8[8];
 #pragma unroll
@@ -642,14 +580,34 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                     float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int p = P - 1; p >= 0; --p) {
-                        const u32x4 w = lds_at<u32x4>(ldsCT + p * DC * C, fragT ^ turn_tile<C / 8>(wave * NT + m, 4 * s));
-                        fc[m][p] = __builtin_bit_cast(bf16x8, w);
+                        fc[m][p] = turn_at<DC / 8>(ldsC + p * C * DC, turnC, wave * NT + m, s);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = p == P - 1 ? vget<bf16>(w, e) : f[e] + vget<bf16>(w, e);
+                        for (int e = 0; e < 8; ++e) f[e] = p == P - 1 ? vget<bf16>(fc[m][p], e) : f[e] + vget<bf16>(fc[m][p], e);
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] *= w8[e];
                     to_planes<SP, 4>(f, ww[m]);
+                }
+                if constexpr (!STATES) {
+                    // An infinite or NaN value must not meet the zeros of the pairs that come before it: it is left out
+                    // here, and put on its own and the later rows below.
+                    uint16x2 top = {0, 0};
+#pragma unroll
+                    for (int m = 0; m < NT; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(uint16x2, fc[m][0][i] & 0x7f807f80u));
+                    if (__any(top[0] == 0x7f80 || top[1] == 0x7f80)) {
+                        wild = true;
+#pragma unroll
+                        for (int m = 0; m < NT; ++m)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t x = fc[m][0][i];
+                                const uint32_t keep = ((x & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+#pragma unroll
+                                for (int p = 0; p < P; ++p) fc[m][p][i] &= keep;
+                            }
+                    }
                 }
                 if constexpr (!STATES) {
 #pragma unroll
@@ -661,7 +619,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                             for (int p = 0; p < P; ++p)
 #pragma unroll
                                 for (int m = 0; m < NT; ++m)
-                                    if (p + q <= ORD) O[it][m] = mfma(fc[m][p], fp, O[it][m]);
+                                    if (p + q <= ORD) O[it][m] = mfma(__builtin_bit_cast(bf16x8, fc[m][p]), fp, O[it][m]);
                         }
                     }
                 }
@@ -669,7 +627,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 for (int t = 0; t < TA; ++t) {
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
-                        const bf16x8 fb = lds_at<bf16x8>(ldsBT + p * DA * C, fragT ^ turn_tile<C / 8>(t, 4 * s));
+                        const bf16x8 fb = __builtin_bit_cast(bf16x8, turn_at<DA / 8>(ldsB + p * C * DA, turnB, t, s));
 #pragma unroll
                         for (int q = 0; q < SP; ++q)
 #pragma unroll
@@ -679,7 +637,20 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 }
             }
             if constexpr (!STATES) {
-                if constexpr (!QUICK) __builtin_amdgcn_sched_barrier(0);
+                if (wild)
+                    for (int j = 0; j < n; ++j) {
+#pragma unroll
+                        for (int m = 0; m < NT; ++m)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int c = tile_col(wave * NT + m, 4 * g4 + e);
+                                const uint32_t b = ldsC[j * DC + swizzle<DC / 8>(j, c >> 3) * 8 + (c & 7)];
+                                const float nan = __uint_as_float(b << 16) * 0.0f;  // or 0
+#pragma unroll
+                                for (int it = 0; it < IT; ++it)
+                                    if (16 * it + l16 >= j) O[it][m][e] += nan;
+                            }
+                    }
                 const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
                 // from the lowest address of the chunk, so that offsets count up in 32 bits
                 char* const low = out + (reverse ? -(C - 1) * opitch : 0);
@@ -737,13 +708,13 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 if (dots) px += n * sx;
             }
         }
-        if (n_next == 0) break;
-        if (wave == 3 && (STATES || !work)) decays(again ? g_load(r_next, n_next) : g_next, buf ^ 1);
+        if (n_next <= 0) break;
+        if (wave == 3 && (STATES || n == 0)) decays(g_next, buf ^ 1);
         __syncthreads();
         if constexpr (!STATES)
-            if (dots && work && tid < n) dots_out(r);
+            if (dots && tid < n) dots_out(r);
         buf ^= 1;
-        r = r_next;
+        r += n;
         n = n_next;
     }
     if constexpr (!STATES) {
