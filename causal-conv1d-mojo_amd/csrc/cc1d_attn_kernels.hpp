@@ -149,6 +149,8 @@ template <int BLKS> __device__ __forceinline__ u32x4 turn_at(const uint16_t* ima
     return u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
 }
 
+__device__ __forceinline__ float opaque_f32(float v) { return __int_as_float(opaque(__float_as_int(v))); }
+
 // exp2 of a sum held in two floats: the second is at most an ulp of the first
 __device__ __forceinline__ float exp2_sum(float hi, float lo) {
     return __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
@@ -341,7 +343,7 @@ template <typename T, int NT> __device__ __forceinline__ void store_outputs(char
 // takes); or the state alone, of the segments that another one follows. QUICK: whole vectors (attn_quick()); else
 // operands are read element by element.
 enum { kAttnOut = 0, kAttnExact = 1, kAttnStates = 2 };
-template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 ? 3 : 2) attn_kernel(const AttnArgs args) {
+template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DA * DC < 16384 ? 3 : 2) attn_kernel(const AttnArgs args) {
     typedef AttnType<T> Ty;
     constexpr bool STATES = MODE == kAttnStates;
     constexpr int SORD = MODE == kAttnOut ? Ty::order : 2, SP = SORD + 1;  // planes of what the state takes
@@ -374,6 +376,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
         return static_cast<const T*>(o.p) + row0 * o.s[0] + (p0 + dir * r) * o.s[1] + (int64_t)(h / o.div) * o.s[2];
     };
     const bool dots = job.dots != nullptr;
+    const float p_scale = opaque_f32(job.p_scale);
     const T* const pg = static_cast<const T*>(args.g) + row0 * args.g_stride[0] + h * args.g_stride[2];
 
     // ---- the state at the segment's start
@@ -503,21 +506,22 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                         }
                         to_planes<PP, 4>(f, sw[m]);
                     }
+                    // (products that follow each other add to different sums)
 #pragma unroll
-                    for (int it = 0; it < IT; ++it)
+                    for (int q = 0; q < P; ++q) {
+                        bf16x8 fq[IT];
 #pragma unroll
-                        for (int q = 0; q < P; ++q) {
-                            const bf16x8 fq = lds_at<bf16x8>(ldsA + q * C * DA, fragD ^ frag_tile<DA / 8>(it, 4 * s));
+                        for (int it = 0; it < IT; ++it) fq[it] = lds_at<bf16x8>(ldsA + q * C * DA, fragD ^ frag_tile<DA / 8>(it, 4 * s));
 #pragma unroll
-                            for (int p = 0; p < PP; ++p)
+                        for (int p = 0; p < PP; ++p)
+#pragma unroll
+                            for (int it = 0; it < IT; ++it) {
 #pragma unroll
                                 for (int m = 0; m < NT; ++m)
-                                    if (p + q <= ORD) O[it][m] = mfma(as_frag(sw[m][p]), fq, O[it][m]);
-                            if (C == 64 || it == it0)
-#pragma unroll
-                                for (int p = 0; p < P; ++p)
-                                    if (p + q <= ORD) acc[C == 64 ? it : 0] = mfma(fb[p], fq, acc[C == 64 ? it : 0]);
-                        }
+                                    if (p + q <= ORD) O[it][m] = mfma(as_frag(sw[m][p]), fq[it], O[it][m]);
+                                if (p < P && p + q <= ORD && (C == 64 || it == it0)) acc[C == 64 ? it : 0] = mfma(fb[p < P ? p : 0], fq[it], acc[C == 64 ? it : 0]);
+                            }
+                    }
                 }
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
@@ -534,8 +538,9 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                     float f[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float m = __builtin_amdgcn_exp2f((hi - jhi[e]) + (lo - jlo[e])) * job.p_scale;
-                        f[e] = j + e <= i ? a[e] * m : 0.0f;
+                        // (opaque: a select, not a branch around each exponential)
+                        const float m = opaque_f32(a[e] * (__builtin_amdgcn_exp2f((hi - jhi[e]) + (lo - jlo[e])) * p_scale));
+                        f[e] = j + e <= i ? m : 0.0f;
                     }
                     to_planes<PP, 2>(f, w);
                 };
@@ -611,30 +616,35 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 }
                 if constexpr (!STATES) {
 #pragma unroll
-                    for (int it = 2 * s; it < IT; ++it) {
+                    for (int q = 0; q < PP; ++q) {
+                        bf16x8 fp[IT];
 #pragma unroll
-                        for (int q = 0; q < PP; ++q) {
-                            const bf16x8 fp = lds_at<bf16x8>(ldsP + q * C * C, fragC ^ frag_tile<C / 8>(it, 4 * s));
+                        for (int it = 2 * s; it < IT; ++it) fp[it] = lds_at<bf16x8>(ldsP + q * C * C, fragC ^ frag_tile<C / 8>(it, 4 * s));
 #pragma unroll
-                            for (int p = 0; p < P; ++p)
+                        for (int p = 0; p < P; ++p)
+#pragma unroll
+                            for (int it = 2 * s; it < IT; ++it)
 #pragma unroll
                                 for (int m = 0; m < NT; ++m)
-                                    if (p + q <= ORD) O[it][m] = mfma(__builtin_bit_cast(bf16x8, fc[m][p]), fp, O[it][m]);
-                        }
+                                    if (p + q <= ORD) O[it][m] = mfma(__builtin_bit_cast(bf16x8, fc[m][p]), fp[it], O[it][m]);
                     }
                 }
+                constexpr int TG = TA < 4 ? TA : 4;  // tiles at once
 #pragma unroll
-                for (int t = 0; t < TA; ++t) {
+                for (int t0 = 0; t0 < TA; t0 += TG)
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
-                        const bf16x8 fb = __builtin_bit_cast(bf16x8, turn_at<DA / 8>(ldsB + p * C * DA, turnB, t, s));
+                        bf16x8 fb[TG];
+#pragma unroll
+                        for (int t = 0; t < TG; ++t) fb[t] = __builtin_bit_cast(bf16x8, turn_at<DA / 8>(ldsB + p * C * DA, turnB, t0 + t, s));
 #pragma unroll
                         for (int q = 0; q < SP; ++q)
 #pragma unroll
-                            for (int m = 0; m < NT; ++m)
-                                if (p + q <= SORD) S[t][m] = mfma(fb, as_frag(ww[m][q]), S[t][m]);
+                            for (int t = 0; t < TG; ++t)
+#pragma unroll
+                                for (int m = 0; m < NT; ++m)
+                                    if (p + q <= SORD) S[t0 + t][m] = mfma(fb[t], as_frag(ww[m][q]), S[t0 + t][m]);
                     }
-                }
             }
             if constexpr (!STATES) {
                 if (wild)
