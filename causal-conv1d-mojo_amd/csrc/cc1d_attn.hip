@@ -16,16 +16,28 @@ struct Plan {
     bool cut() const { return slots > seqs; }
 };
 
-// Sequences run as one block per head where those fill the chip; longer ones
-// are cut into segments that run side by side, from states that a first pass
-// over keys and values alone provides.
+// Sequences run as one block per head where those come near to filling the
+// chip (256 CUs, two or three blocks each); longer ones are cut into segments
+// that run side by side, from states that a first pass over keys and values
+// alone provides, which costs about half as much again. Measured, bf16 128 x 128,
+// both directions: batch 4 of 40 heads, 2048 positions 506 us whole and 602 in
+// three segments; fp32 80 x 72, 16 heads of 2048: 242 us in segments of 256,
+// about 205 with 128, 933 whole. Packed sequences are cut whatever their
+// number, as their lengths are not known here and one of them may be nearly
+// all: a block's share is then at most 1 / 768 of the work (8192 positions, 32
+// heads: 180 us, and 211 with segments of 256, 196 with 512, 264 whole).
 Plan plan_of(const cc1d_attn_params& p, int jobs) {
     Plan pl;
     pl.seqs = p.cu_seqlens ? p.num_seqs : p.batch;
-    const double work = (double)p.batch * (double)p.seqlen * (double)p.heads * jobs;
     const int64_t c = chunk_of(p.dtype);
-    int64_t seg = (int64_t)(work / 768.0);
-    seg = ceil_div(seg < 256 ? 256 : seg, c) * c;
+    int64_t seg;
+    if (p.cu_seqlens) {
+        seg = (int64_t)((double)p.seqlen * (double)p.heads / 768.0);
+    } else {
+        const double blocks = (double)p.batch * (double)p.heads * jobs;
+        seg = blocks >= 128.0 ? p.seqlen : (int64_t)((double)p.seqlen * blocks / 512.0);
+    }
+    seg = ceil_div(seg < 160 ? 160 : seg, c) * c;
     if (seg >= p.seqlen) {
         pl.seg = ceil_div(p.seqlen > 0 ? p.seqlen : 1, c) * c;
         pl.per_row = 1;
@@ -89,19 +101,25 @@ int launch_jobs(int dtype, const AttnArgs& a, int da, int dc, bool states, hipSt
 
 struct CombineArgs {
     AttnArgs a;  // the segments (jobs of the first pass)
-    uint32_t pieces;  // of 256 values
+    uint32_t pieces;  // of 256 vectors
 };
 
 // The first pass left in every slot what its segment adds to a state of 0;
 // afterwards a slot holds the state at its segment's start (a sequence's first
-// one is left out). A thread per value; the walk over the segments is serial.
-__global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg) {
+// one is left out). A thread for V values, in the order of memory; the walk
+// over the segments is serial, with four of them on their way. Bound by the
+// states, read and written once (170 MB for 8192 positions of 32 heads of
+// 128 x 128 in segments of 384: COMBINE_FIGURE).
+template <int V> __global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg) {
+    typedef float vec __attribute__((ext_vector_type(V)));
     const AttnArgs& a = arg.a;
     const uint32_t rest = blockIdx.x / arg.pieces, jn = rest / a.heads, h = rest - jn * a.heads;
     const AttnJob& job = a.job[jn];
-    const int64_t per = (int64_t)job.da * job.dc, e = (int64_t)(blockIdx.x - rest * arg.pieces) * 256 + threadIdx.x;
+    const int32_t per = job.da * job.dc, e = (int32_t)((blockIdx.x - rest * arg.pieces) * 256 + threadIdx.x) * V;
     if (e >= per) return;
-    const int64_t row = e / job.dc, col = e % job.dc;
+    const bool turned = job.seg.s[3] != 1;  // rows are next to each other
+    const int32_t inner = turned ? job.da : job.dc;
+    const float* const decay = job.decay + h;
     for (int64_t seq = blockIdx.y; seq < a.num_seqs; seq += gridDim.y) {
         int64_t slot, len;
         if (a.cu == nullptr) {
@@ -115,14 +133,33 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg
         int64_t segs = len <= a.seg ? 1 : (len + a.seg - 1) / a.seg;
         if (slot + segs > a.slots) segs = a.slots - slot;
         if (segs < 2) continue;
-        float* at = job.seg.p + slot * job.seg.s[0] + h * job.seg.s[1] + row * job.seg.s[2] + col * job.seg.s[3];
-        float cur = job.first.p ? job.first.p[seq * job.first.s[0] + h * job.first.s[1] + row * job.first.s[2] + col * job.first.s[3]] : 0.0f;
-        float adds = *at;
-        for (int64_t i = 0; i + 1 < segs; ++i) {
-            cur = __builtin_fmaf(job.decay[(slot + i) * a.heads + h], cur, adds);
-            at += job.seg.s[0];
-            if (i + 2 < segs) adds = *at;
-            *at = cur;
+        float* at = job.seg.p + slot * job.seg.s[0] + h * job.seg.s[1] + e;
+        vec cur = 0.0f;
+        if (job.first.p) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int32_t out = (e + i) / inner, in = (e + i) - out * inner;
+                cur[i] = job.first.p[seq * job.first.s[0] + h * job.first.s[1] + (turned ? in : out) * job.first.s[2] + (turned ? out : in) * job.first.s[3]];
+            }
+        }
+        constexpr int K = 4;
+        vec adds[K + 1];
+        adds[K] = *reinterpret_cast<const vec*>(at);
+        for (int64_t i = 0; i + 1 < segs; i += K, at += K * job.seg.s[0]) {
+            // (read before the turn writes: a slot turns from what it adds into its state)
+            float by[K];
+            adds[0] = adds[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (i + k + 1 < segs) by[k] = decay[(slot + i + k) * a.heads];
+                if (i + k + 2 < segs) adds[k + 1] = *reinterpret_cast<const vec*>(at + (k + 1) * job.seg.s[0]);
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (i + k + 1 < segs) {
+                    cur = by[k] * cur + adds[k];
+                    *reinterpret_cast<vec*>(at + (k + 1) * job.seg.s[0]) = cur;
+                }
         }
     }
 }
@@ -130,9 +167,11 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg
 int run_segments(const cc1d_attn_params& p, const Plan& pl, const AttnArgs& a, int da, int dc, hipStream_t stream) {
     const int st = launch_jobs(p.dtype, a, da, dc, true, stream);
     if (st != CC1D_OK) return st;
-    const uint32_t pieces = (uint32_t)ceil_div((int64_t)da * dc, 256);
+    bool whole = (int64_t)da * dc % 4 == 0;
+    for (uint32_t j = 0; j < a.jobs; ++j) whole = whole && reinterpret_cast<uintptr_t>(a.job[j].seg.p) % 16 == 0;
+    const uint32_t pieces = (uint32_t)ceil_div((int64_t)da * dc, whole ? 1024 : 256);
     const dim3 grid((unsigned)(pieces * p.heads * a.jobs), (unsigned)(pl.seqs < 1024 ? pl.seqs : 1024));
-    return launch(attn_combine_kernel, grid, dim3(256), stream, CombineArgs{a, pieces});
+    return launch(whole ? attn_combine_kernel<4> : attn_combine_kernel<1>, grid, dim3(256), stream, CombineArgs{a, pieces});
 }
 
 // ---- the gradient of the decays
@@ -230,15 +269,20 @@ struct GroupSumArgs {
     int32_t each, dk;      // heads to a key head
 };
 
-template <typename T> __global__ void __launch_bounds__(256) attn_group_sum_kernel(const GroupSumArgs a) {
+// A thread for V neighbours; each value is read and written once.
+template <typename T, int V> __global__ void __launch_bounds__(256) attn_group_sum_kernel(const GroupSumArgs a) {
+    typedef float vec __attribute__((ext_vector_type(V)));
     const float* const part = a.part[blockIdx.y];
     T* const out = static_cast<T*>(a.out[blockIdx.y]);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n; i += (int64_t)gridDim.x * 256) {
-        const int64_t head = i / a.dk, c = i - head * a.dk;
-        const float* at = part + head * a.each * a.dk + c;
-        float s = 0.0f;
-        for (int r = 0; r < a.each; ++r) s += at[(int64_t)r * a.dk];
-        out[i] = from_f32<T>(s);
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < a.n; i += (int64_t)gridDim.x * 256 * V) {
+        const float* const at = part + i / a.dk * (a.each - 1) * a.dk + i;
+        vec s = 0.0f;
+#pragma unroll 4
+        for (int r = 0; r < a.each; ++r) s += *reinterpret_cast<const vec*>(at + (int64_t)r * a.dk);
+        T w[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = from_f32<T>(s[e]);
+        __builtin_memcpy(__builtin_assume_aligned(out + i, V * sizeof(T)), w, sizeof(w));
     }
 }
 
@@ -399,9 +443,13 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     });
     if (st != CC1D_OK || !shared) return st;
     const GroupSumArgs gs{{dq_part, dk_part}, {b.dq, b.dk}, tokens * p.key_heads * p.dk, (int32_t)per, dk};
-    const int64_t blocks = ceil_div(gs.n, 256);
+    auto whole = [](const void* at, size_t bytes) { return reinterpret_cast<uintptr_t>(at) % bytes == 0; };
     return with_dtype(p.dtype, [&](auto t) {
-        return launch(attn_group_sum_kernel<decltype(t)>, dim3((unsigned)(blocks < 65536 ? blocks : 65536), 2), dim3(256), stream, gs);
+        typedef decltype(t) T;
+        const bool four = dk % 4 == 0 && whole(dq_part, 16) && whole(dk_part, 16) && whole(b.dq, 4 * sizeof(T)) && whole(b.dk, 4 * sizeof(T));
+        const int64_t blocks = ceil_div(gs.n, four ? 1024 : 256);
+        const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536), 2);
+        return launch(four ? attn_group_sum_kernel<T, 4> : attn_group_sum_kernel<T, 1>, grid, dim3(256), stream, gs);
     });
 }
 

@@ -237,25 +237,34 @@ template <typename T, int C, int D, bool QUICK> struct AttnTile {
     }
     // `rows` positions from base on, row_stride apart. QUICK: heads of whole vectors, next to each other, and chunks
     // that span less than 2 GiB, so that a uniform base and 32-bit offsets do.
-    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, uint16_t* image, int tid) {
+    __device__ __forceinline__ void load(const T* base, int64_t row_stride, int64_t elem_stride, int rows, int d, uint16_t* image, int tid, int wave) {
         if constexpr (QUICK) {
+            // (a whole turn of the block is R rows, and a thread's column the same in each)
+            constexpr int R = 256 / CGS;
+            int row, col;
+            unit(0, tid, row, col);
             const bool down = row_stride < 0;
-            const char* const low = reinterpret_cast<const char*>(down ? base + (C - 1) * row_stride : base);
             const uint32_t pitch = (uint32_t)((down ? -row_stride : row_stride) * (int64_t)sizeof(T));
-            const bool all = rows == C && d == D;
+            const uint32_t at = (uint32_t)(down ? R - 1 - row : row) * pitch + col * (uint32_t)sizeof(T);
+            const char* low = reinterpret_cast<const char*>(base) - (down ? (uint64_t)((R - 1) * pitch) : 0);
+            const int64_t turn = (int64_t)(R * sizeof(T)) * row_stride;
+            if (rows == C && d == D) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                int row, col;
-                unit(n, tid, row, col);
-                const bool in = all || (row < rows && col < d);
-                const char* const at = low + (uint32_t)((uint32_t)(down ? C - 1 - row : row) * pitch + col * (uint32_t)sizeof(T));
-                if constexpr (DIRECT) {
-                    uint16_t* const to = image + (n * 256 + uniform32(tid & ~63)) * 8;  // of the wavefront; its lanes follow
-                    if (in) __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-                    else *reinterpret_cast<u32x4*>(to + (tid & 63) * 8) = vzero();
-                } else {
-                    v[n] = vzero();
-                    if (in) v[n] = vload_any(reinterpret_cast<const T*>(at));
+                for (int n = 0; n < N; ++n, low += turn) {
+                    if constexpr (DIRECT) direct(low + at, image, n, wave);
+                    else v[n] = vload_any(reinterpret_cast<const T*>(low + at));
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n, low += turn) {
+                    const bool in = n * R + row < rows && col < d;
+                    if constexpr (DIRECT) {
+                        if (in) direct(low + at, image, n, wave);
+                        else *reinterpret_cast<u32x4*>(image + (n * 256 + tid) * 8) = vzero();
+                    } else {
+                        v[n] = vzero();
+                        if (in) v[n] = vload_any(reinterpret_cast<const T*>(low + at));
+                    }
                 }
             }
         } else {
@@ -271,6 +280,11 @@ template <typename T, int C, int D, bool QUICK> struct AttnTile {
                     if (col + e < d) put(v[n], e, at[e * elem_stride]);
             }
         }
+    }
+    // vector n of a wavefront's lanes
+    static __device__ __forceinline__ void direct(const char* at, uint16_t* image, int n, int wave) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at,
+                                         (__attribute__((address_space(3))) void*)(image + (n * 256 + wave * 64) * 8), 16, 0, 0);
     }
     static __device__ __forceinline__ void put(u32x4& w, int e, T x) {
         if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(to_f32(x));
@@ -308,18 +322,6 @@ template <typename T, int C, int D, bool QUICK> struct AttnTile {
 };
 
 // Four neighbouring values, widened.
-template <typename T> __device__ __forceinline__ void four_of(const T* p, float (&x)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        const u32x4 w = vload_any(p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(w[e]);
-    } else {
-        const u32x2 w = *reinterpret_cast<const typename AnyAddr<2>::v2*>(p);
-        const u32x4 w4 = {w[0], w[1], 0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = vget<T>(w4, e);
-    }
-}
 template <typename T, int NT> __device__ __forceinline__ void store_outputs(char* o, const f32x4 (&O)[NT], bool f32) {
     if (sizeof(T) == 4 || f32) {
 #pragma unroll
@@ -343,7 +345,7 @@ template <typename T, int NT> __device__ __forceinline__ void store_outputs(char
 // takes); or the state alone, of the segments that another one follows. QUICK: whole vectors (attn_quick()); else
 // operands are read element by element.
 enum { kAttnOut = 0, kAttnExact = 1, kAttnStates = 2 };
-template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DA * DC < 16384 ? 3 : 2) attn_kernel(const AttnArgs args) {
+template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 : 2) attn_kernel(const AttnArgs args) {
     typedef AttnType<T> Ty;
     constexpr bool STATES = MODE == kAttnStates;
     constexpr int SORD = MODE == kAttnOut ? Ty::order : 2, SP = SORD + 1;  // planes of what the state takes
@@ -403,14 +405,17 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     }
 
     // ---- decays of the rows from r on (by one wavefront)
+    typedef std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t> Bits;
     double total = 0.0;
     auto g_load = [&](int r, int n) {
-        if (lane >= n) return 0.0f;
         // backwards, a position's decay is the one of the position after it, and the sequence's last has none
-        const int64_t at = p0 + dir * (r + lane) + (reverse ? 1 : 0);
-        return reverse && r + lane == 0 ? 0.0f : to_f32(pg[at * args.g_stride[1]]);
+        const T* const at = pg + (p0 + dir * r + (reverse ? 1 : 0)) * args.g_stride[1];
+        uint32_t g = 0;  // (bits: converted where they are used, so that nothing waits for them here)
+        if (lane < n && !(reverse && r + lane == 0)) g = *reinterpret_cast<const Bits*>(at + lane * (dir * args.g_stride[1]));
+        return g;
     };
-    auto decays = [&](float g, int buf) {
+    auto decays = [&](uint32_t bits, int buf) {
+        const float g = to_f32(__builtin_bit_cast(T, (Bits)(uint32_t)opaque((int)bits)));
         const double c = wave_prefix_f64(log_decay(g) * 1.4426950408889634), end = lane63(c);
         total += end;
         const float hi = (float)c, lo = (float)(c - (double)hi);
@@ -433,14 +438,27 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     const int64_t ea = job.a.s[3], eb = job.b.s[3], ec = job.c.s[3], ex = job.x.s[3];
     // the next n rows, and on past them
     auto load = [&](int n, int t) {
-        if constexpr (!STATES) ta.load(pa, sa, ea, n, da, ldsA, t);
-        tb.load(pb, sb, eb, n, da, ldsB, t);
-        tc.load(pc, sc, ec, n, dc, ldsC, t);
+        if constexpr (!STATES) ta.load(pa, sa, ea, n, da, ldsA, t, wave);
+        tb.load(pb, sb, eb, n, da, ldsB, t, wave);
+        tc.load(pc, sc, ec, n, dc, ldsC, t, wave);
         pa += n * sa;
         pb += n * sb;
         pc += n * sc;
     };
     auto rows_at = [&](int r) { return r_end - r < C ? r_end - r : C; };
+    // A word of each 128 bytes of the next n rows, so that what goes straight into its image comes from the L2 cache when
+    // its turn has come (two wavefronts to an operand).
+    uint32_t ahead[2] = {0, 0};
+    auto fetch = [&](int n, const T* px_next, int t) {
+        auto word = [&](const T* p, int64_t s, int d, int lines, uint32_t& to) {
+            const int row = lines == 2 ? (t & 127) >> 1 : t & 63, at = lines == 2 ? (t & 1) * 64 : 0;
+            if (row < n && at < d) to = *reinterpret_cast<const uint32_t*>(p + row * s + at);
+        };
+        if (wave >= 2) word(pb, sb, da, DA / 64, ahead[0]);
+        else if (!STATES) word(pa, sa, da, DA / 64, ahead[0]);
+        if (wave < 2) word(pc, sc, dc, DC / 64, ahead[1]);
+        else if (!STATES && dots) word(px_next, sx, dc, DC / 64, ahead[1]);
+    };
 
     // ---- outputs: a lane has NT * 4 neighbouring columns of row 16 it + (lane & 15)
     const int64_t tokens = args.batch * args.seqlen, t0 = row0 * args.seqlen + p0;
@@ -460,25 +478,34 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     for (;;) {
         const int otid = opaque(tid), l16 = otid & 15, g4 = (otid >> 4) & 3;
         const int n_next = rows_at(r + n);
-        float g_next = 0.0f;
-        if (wave == 3 && n_next > 0) g_next = g_load(r + n, n_next);
+        uint32_t g_next = 0;
         // ---- the chunk into LDS
         if constexpr (DIRECT) {
             if (n > 0) load(n, otid);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (wave == 3 && n_next > 0) g_next = g_load(r + n, n_next);
+            asm volatile("s_waitcnt vmcnt(0)" ::"v"(ahead[0]), "v"(ahead[1]) : "memory");
         } else {
+            if (wave == 3 && n_next > 0) g_next = g_load(r + n, n_next);
             if constexpr (!STATES) ta.store(ldsA, otid);
             tb.store(ldsB, otid);
             tc.store(ldsC, otid);
         }
         __syncthreads();
-        if constexpr (!DIRECT)
-            if (n_next > 0) load(n_next, otid);
+        if (n_next > 0) {
+            if constexpr (DIRECT) {
+                if (n > 0) fetch(n_next, px + n * sx, otid);
+            } else {
+                load(n_next, otid);
+            }
+        }
         if (n > 0) {
             const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0);
             const uint32_t fragC = frag_base<C / 8>(l16, g4, 0), halfC = frag_base<C / 8>(l16, g4 >> 1, g4 & 1);
             const uint32_t turnB = turn_base<DA / 8>(l16, g4), turnC = turn_base<DC / 8>(l16, g4);
             f32x4 O[IT][NT];
+            const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
+            const bool full = n == C && dc == DC;
+            u32x4 x4[IT][sizeof(T) == 2 ? (NT + 1) / 2 : NT];  // what the outputs are dotted with
             if constexpr (!STATES) {
                 // ---- what the state gives, and the pairs, transposed (columns x rows), so that a lane gets four columns
                 // of a row: both from one reading of the rows
@@ -551,6 +578,25 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
                 pairs(C == 64 ? 3 : it0, acc[PT - 1], pw[PT - 1]);
                 __syncthreads();
+                if (QUICK && dots) {
+                    const char* const low = reinterpret_cast<const char*>(px) + (reverse ? 15 * sx * (int64_t)sizeof(T) : 0);
+                    const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(col * (int)sizeof(T));
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        const T* const p = reinterpret_cast<const T*>(low + 16 * it * sx * (int64_t)sizeof(T) + at);
+                        const bool in = full || 16 * it + l16 < n;
+#pragma unroll
+                        for (int m = 0; m < NT; m += 4 / (int)sizeof(T)) {
+                            u32x4 w = vzero();
+                            if constexpr (sizeof(T) == 2 && NT == 1) {
+                                if (in && col < dc) { const u32x2 v = *reinterpret_cast<const typename AnyAddr<2>::v2*>(p); w[0] = v[0]; w[1] = v[1]; }
+                            } else {
+                                if (in && col + 4 * m < dc) w = vload_any(p + 4 * m);
+                            }
+                            x4[it][sizeof(T) == 2 ? 0 : m] = w;
+                        }
+                    }
+                }
                 // ---- the pairs to everybody
 #pragma unroll
                 for (int k = 0; k < PT; ++k) {
@@ -661,25 +707,22 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                                     if (16 * it + l16 >= j) O[it][m][e] += nan;
                             }
                     }
-                const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
                 // from the lowest address of the chunk, so that offsets count up in 32 bits
                 char* const low = out + (reverse ? -(C - 1) * opitch : 0);
-                const char* const xlow = reinterpret_cast<const char*>(px) + (reverse ? (C - 1) * sx * (int64_t)sizeof(T) : 0);
-                const uint32_t pitch = (uint32_t)opitch, xpitch = (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T));
+                const uint32_t pitch = (uint32_t)opitch;
                 const uint32_t row = (uint32_t)(reverse ? 15 - l16 : l16);
-                const uint32_t at = row * pitch + (uint32_t)(col * osize), xat = row * xpitch + (uint32_t)(col * (int)sizeof(T));
-                const bool full = n == C && dc == DC;
+                const uint32_t at = row * pitch + (uint32_t)(col * osize);
                 if (dots) {
 #pragma unroll
                     for (int it = 0; it < IT; ++it) {
                         const int i = 16 * it + l16;
-                        const T* const p = reinterpret_cast<const T*>(xlow + (uint64_t)(uint32_t)((reverse ? C - 16 - 16 * it : 16 * it) * xpitch) + xat);
                         float dot = 0.0f;
 #pragma unroll
                         for (int m = 0; m < NT; ++m) {
                             float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                             if constexpr (QUICK) {
-                                if (full || (i < n && col + 4 * m < dc)) four_of<T>(p + 4 * m, x);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[e] = sizeof(T) == 2 ? vget<T>(x4[it][0], 4 * m + e) : vget<T>(x4[it][m % NT], e);
                             } else {
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
