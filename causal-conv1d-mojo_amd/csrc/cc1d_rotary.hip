@@ -5,7 +5,8 @@
 // shared by all its heads, so a wavefront takes one token, forms the sines
 // and cosines of the pairs that its lanes hold once, and walks over heads:
 // HBM bounds it. A lane holds eight values of a head: four pairs, or eight
-// values behind the rotated ones.
+// values behind the rotated ones. The walk goes on from queries to keys and
+// to the wavefront's next token, and loads one stop ahead of what it computes.
 //
 // Angles: position * inv_freq is formed and reduced to a quarter turn in 64
 // bits (at a position of a million 32 bits would be off by a few hundredths of
@@ -20,7 +21,7 @@ struct RotaryArgs {
     cc1d_rotary_params p;
     cc1d_rotary_bwd_params b;  // the backward's own fields (fwd is p)
     FastDiv seqlen;
-    int32_t share;             // wavefronts to a token: 1, 2 or 4
+    int32_t share;             // wavefronts to a token: 1 or 4
     uint32_t tokens, blocks;
 };
 
@@ -95,12 +96,24 @@ template <typename T> struct Four {
             else w[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, at[i * stride]) << (16 * (i & 1));
         }
     }
-    __device__ __forceinline__ void get(float* f) const {
+    // four neighbours, without a branch: the loads of a stop are counted, so that only those of the stop before are waited for
+    __device__ __forceinline__ void whole(const T* at) {
+        if constexpr (sizeof(T) == 4) {
+            const u32x4 x = vload_any(at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = x[i];
+        } else {
+            const u32x2 x = *reinterpret_cast<const typename AnyAddr<2>::v2*>(at);
+            w[0] = x[0];
+            w[1] = x[1];
+        }
+    }
+    __device__ __forceinline__ void get(float* f, bool some) const {
         u32x4 x = vzero();
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(w) / 4); ++i) x[i] = w[i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = vget<T>(x, i);
+        for (int i = 0; i < 4; ++i) f[i] = some ? vget<T>(x, i) : 0.0f;
     }
 };
 template <typename T> __device__ __forceinline__ void store_four(T* at, const float* f, int count) {
@@ -160,16 +173,34 @@ template <bool INTER, bool BACK> __device__ __forceinline__ void turn(float (&v)
     }
 }
 
-template <typename T, int LPH, bool INTER> __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs arg) {
+// A wavefront's walk: K heads a lane at each stop, from the queries (which 0) to the keys, from token to token.
+template <int STEP> struct Stop {
+    uint32_t token;
+    int32_t which, h;
+    __device__ __forceinline__ void settle(const RotaryArgs& a, int first, uint32_t tokens_a_turn) {
+        while (token < a.tokens && h >= (which ? (int)a.p.k_heads : (int)a.p.q_heads)) {
+            token += which ? tokens_a_turn : 0;
+            which ^= 1;
+            h = first;
+        }
+    }
+    __device__ __forceinline__ Stop next(const RotaryArgs& a, int first, uint32_t tokens_a_turn) const {
+        Stop s = {token, which, h + STEP * a.share};
+        s.settle(a, first, tokens_a_turn);
+        return s;
+    }
+};
+
+// WHOLE: unit strides and runs of four (whole_runs()).
+template <typename T, int LPH, bool INTER, bool WHOLE> __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs arg) {
     const cc1d_rotary_params& p = arg.p;
-    constexpr int HEADS = 64 / LPH, K = 4;  // heads a wavefront takes at once; of those, in flight
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, dim = (int)p.dim, rotated = (int)p.rotated;
-    const uint32_t token = blockIdx.x * (4 / arg.share) + wave / arg.share;
-    if (token >= arg.tokens) return;
-    const int part = wave % arg.share;
-    const uint32_t b = arg.seqlen.div(token), t = token - b * (uint32_t)p.seqlen;
+    constexpr int HEADS = 64 / LPH, K = sizeof(T) == 2 ? 4 : 2;  // heads a wavefront takes at once; of those, at a stop
+    typedef Stop<HEADS * K> Stop;
+    const int wave = uniform32(threadIdx.x >> 6), lane = threadIdx.x & 63, dim = (int)p.dim, rotated = (int)p.rotated;
+    const int first = wave % arg.share * HEADS;
+    const uint32_t per = 4 / arg.share, turns = arg.blocks * per;
     const Unit u = unit_of<INTER>(lane % LPH, dim, rotated);
-    const Angles a = angles_of(p, b, t, u);
+    Angles a;
     float wq[8], wk[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -178,55 +209,90 @@ template <typename T, int LPH, bool INTER> __global__ void __launch_bounds__(256
         wk[e] = p.k_weight && in ? p.k_weight[u.at[e >> 2] + (e & 3)] : 1.0f;
     }
     const float inv = 1.0f / (float)dim, eps = (float)p.eps;
-    auto heads = [&](const void* src, const int64_t (&stride)[4], void* dst, int64_t count, bool norm, const float (&w)[8]) {
-        const T* const base = static_cast<const T*>(src) + b * stride[0] + t * stride[1];
-        T* const out = static_cast<T*>(dst) + (int64_t)token * count * dim;
-        for (int64_t h0 = part * HEADS + lane / LPH; h0 < count; h0 += K * arg.share * HEADS) {
-            Four<T> raw[K][2];
+    struct Raw {
+        Four<T> v[K][2];
+    };
+    auto load = [&](const Stop& s, Raw& r) {
+        const uint32_t b = arg.seqlen.div(s.token), t = s.token - b * (uint32_t)p.seqlen;
+        const int64_t (&stride)[4] = s.which ? p.k_stride : p.q_stride;
+        const T* const base = static_cast<const T*>(s.which ? p.k : p.q) + b * stride[0] + t * stride[1];
+        const int count = s.which ? (int)p.k_heads : (int)p.q_heads;
 #pragma unroll
-            for (int j = 0; j < K; ++j) {
-                const int64_t h = h0 + j * arg.share * HEADS;
-                if (h >= count) continue;
+        for (int j = 0; j < K; ++j) {
+            const int h = s.h + j * arg.share * HEADS + lane / LPH;
+            if constexpr (WHOLE) {
+                const T* const at = base + (h < count ? h : count - 1) * stride[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) raw[j][i].load(base + h * stride[2] + u.at[i] * stride[3], stride[3], u.count[i]);
+                for (int i = 0; i < 2; ++i) r.v[j][i].whole(at + (u.count[i] ? u.at[i] : 0));
+                continue;
             }
+            if (h >= count) continue;
 #pragma unroll
-            for (int j = 0; j < K; ++j) {
-                const int64_t h = h0 + j * arg.share * HEADS;
-                if (h >= count) continue;  // (the lanes of a head together)
-                float v[8];
-                raw[j][0].get(v);
-                raw[j][1].get(v + 4);
-                if (norm) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
-                    const float rstd = 1.0f / sqrtf(__builtin_fmaf(group_sum<LPH>(sum), inv, eps));
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = v[e] * rstd * w[e];
-                }
-                turn<INTER, false>(v, a, u, rotated >> 1);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) store_four(out + h * dim + u.at[i], v + 4 * i, u.count[i]);
-            }
+            for (int i = 0; i < 2; ++i) r.v[j][i].load(base + h * stride[2] + u.at[i] * stride[3], stride[3], u.count[i]);
         }
     };
-    heads(p.q, p.q_stride, p.q_out, p.q_heads, p.q_weight != nullptr, wq);
-    heads(p.k, p.k_stride, p.k_out, p.k_heads, p.k_weight != nullptr, wk);
+    auto work = [&](const Stop& s, const Raw& r, T* dst, int count, bool norm, const float (&w)[8]) {
+        T* const out = dst + (int64_t)s.token * count * dim;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const int h = s.h + j * arg.share * HEADS + lane / LPH;
+            if (h >= count) continue;  // (the lanes of a head together)
+            float v[8];
+            r.v[j][0].get(v, !WHOLE || u.count[0]);
+            r.v[j][1].get(v + 4, !WHOLE || u.count[1]);
+            if (norm) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
+                const float rstd = 1.0f / sqrtf(__builtin_fmaf(group_sum<LPH>(sum), inv, eps));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = v[e] * rstd * w[e];
+            }
+            turn<INTER, false>(v, a, u, rotated >> 1);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) store_four(out + (int64_t)h * dim + u.at[i], v + 4 * i, u.count[i]);
+        }
+    };
+    Stop here = {blockIdx.x * per + wave / arg.share, 0, first};
+    here.settle(arg, first, turns);
+    uint32_t angles_at = ~0u;
+    // the work of a stop, with the loads of the one after it on their way
+    auto at = [&](const Stop& s, const Raw& now, Raw& ahead) {
+        const Stop after = s.next(arg, first, turns);
+        if (WHOLE || after.token < arg.tokens) load(after.token < arg.tokens ? after : s, ahead);
+        if (s.token != angles_at) {
+            angles_at = s.token;
+            const uint32_t b = arg.seqlen.div(s.token);
+            a = angles_of(p, b, s.token - b * (uint32_t)p.seqlen, u);
+        }
+        if (s.which == 0) work(s, now, static_cast<T*>(p.q_out), (int)p.q_heads, p.q_weight != nullptr, wq);
+        else work(s, now, static_cast<T*>(p.k_out), (int)p.k_heads, p.k_weight != nullptr, wk);
+        return after;
+    };
+    Raw even, odd;  // (in turns: a copy would wait for the loads)
+    if (here.token < arg.tokens) load(here, even);
+    while (here.token < arg.tokens) {
+        const Stop there = at(here, even, odd);
+        if (there.token >= arg.tokens) break;
+        here = at(there, odd, even);
+    }
 }
 
 // Backward: with d = the gradient turned back, dweight += d x^, and dx = rstd
 // (d w - x^ mean(d w x^)), x^ = x rstd. A block walks over tokens and keeps
 // its lanes' shares of the weights' gradients; they are added over the block's
 // heads and wavefronts at its end, and over the blocks by a second kernel.
-template <typename T, int LPH, bool INTER> __global__ void __launch_bounds__(256) rotary_bwd_kernel(const RotaryArgs arg) {
+template <typename T, int LPH, bool INTER, bool WHOLE> __global__ void __launch_bounds__(256) rotary_bwd_kernel(const RotaryArgs arg) {
     const cc1d_rotary_params& p = arg.p;
     const cc1d_rotary_bwd_params& g = arg.b;
-    constexpr int HEADS = 64 / LPH, K = 2;
+    constexpr int HEADS = 64 / LPH, K = sizeof(T) == 2 ? 2 : 1;
+    typedef Stop<HEADS * K> Stop;
     __shared__ float share_lds[2][4][LPH * 8];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, dim = (int)p.dim, rotated = (int)p.rotated;
-    const int part = wave % arg.share;
+    const int wave = uniform32(threadIdx.x >> 6), lane = threadIdx.x & 63, dim = (int)p.dim, rotated = (int)p.rotated;
+    const int first = wave % arg.share * HEADS;
+    const uint32_t per = 4 / arg.share, turns = arg.blocks * per;
     const Unit u = unit_of<INTER>(lane % LPH, dim, rotated);
+    Angles a;
     float wq[8], wk[8], dwq[8], dwk[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -236,60 +302,94 @@ template <typename T, int LPH, bool INTER> __global__ void __launch_bounds__(256
         dwq[e] = dwk[e] = 0.0f;
     }
     const float inv = 1.0f / (float)dim, eps = (float)p.eps;
-    const uint32_t per = 4 / arg.share;
-    for (uint32_t token = blockIdx.x * per + wave / arg.share; token < arg.tokens; token += arg.blocks * per) {
-        const uint32_t b = arg.seqlen.div(token), t = token - b * (uint32_t)p.seqlen;
-        const Angles a = angles_of(p, b, t, u);
-        auto heads = [&](const void* src, const int64_t (&stride)[4], const void* grad, const int64_t (&gstride)[4], void* dst, int64_t count,
-                         bool norm, const float (&w)[8], float (&dw)[8]) {
-            const T* const base = static_cast<const T*>(src) + b * stride[0] + t * stride[1];
-            const T* const gbase = static_cast<const T*>(grad) + b * gstride[0] + t * gstride[1];
-            T* const out = static_cast<T*>(dst) + (int64_t)token * count * dim;
-            for (int64_t h0 = part * HEADS + lane / LPH; h0 < count; h0 += K * arg.share * HEADS) {
-                Four<T> raw[K][2], graw[K][2];
+    struct Raw {
+        Four<T> v[K][2], d[K][2];
+    };
+    auto load = [&](const Stop& s, Raw& r) {
+        const uint32_t b = arg.seqlen.div(s.token), t = s.token - b * (uint32_t)p.seqlen;
+        const int64_t (&stride)[4] = s.which ? p.k_stride : p.q_stride;
+        const int64_t (&gstride)[4] = s.which ? g.dk_out_stride : g.dq_out_stride;
+        const T* const base = static_cast<const T*>(s.which ? p.k : p.q) + b * stride[0] + t * stride[1];
+        const T* const gbase = static_cast<const T*>(s.which ? g.dk_out : g.dq_out) + b * gstride[0] + t * gstride[1];
+        const int count = s.which ? (int)p.k_heads : (int)p.q_heads;
+        const bool norm = (s.which ? p.k_weight : p.q_weight) != nullptr;
 #pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    const int64_t h = h0 + j * arg.share * HEADS;
-                    if (h >= count) continue;
+        for (int j = 0; j < K; ++j) {
+            const int h = s.h + j * arg.share * HEADS + lane / LPH;
+            if constexpr (WHOLE) {
+                const int64_t hc = h < count ? h : count - 1;
+                const T* const gat = gbase + hc * gstride[2];
+                const T* const at = norm ? base + hc * stride[2] : gat;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        graw[j][i].load(gbase + h * gstride[2] + u.at[i] * gstride[3], gstride[3], u.count[i]);
-                        if (norm) raw[j][i].load(base + h * stride[2] + u.at[i] * stride[3], stride[3], u.count[i]);
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    const int e = u.count[i] ? u.at[i] : 0;
+                    r.d[j][i].whole(gat + e);
+                    r.v[j][i].whole(at + e);
                 }
+                continue;
+            }
+            if (h >= count) continue;
 #pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    const int64_t h = h0 + j * arg.share * HEADS;
-                    if (h >= count) continue;
-                    float d[8];
-                    graw[j][0].get(d);
-                    graw[j][1].get(d + 4);
-                    turn<INTER, true>(d, a, u, rotated >> 1);
-                    if (norm) {
-                        float x[8], sum = 0.0f, along = 0.0f;
-                        raw[j][0].get(x);
-                        raw[j][1].get(x + 4);
+            for (int i = 0; i < 2; ++i) {
+                r.d[j][i].load(gbase + h * gstride[2] + u.at[i] * gstride[3], gstride[3], u.count[i]);
+                if (norm) r.v[j][i].load(base + h * stride[2] + u.at[i] * stride[3], stride[3], u.count[i]);
+            }
+        }
+    };
+    auto work = [&](const Stop& s, const Raw& r, T* dst, int count, bool norm, const float (&w)[8], float (&dw)[8]) {
+        T* const out = dst + (int64_t)s.token * count * dim;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            sum = __builtin_fmaf(x[e], x[e], sum);
-                            along = __builtin_fmaf(d[e] * w[e], x[e], along);
-                        }
-                        const float rstd = 1.0f / sqrtf(__builtin_fmaf(group_sum<LPH>(sum), inv, eps));
-                        along = group_sum<LPH>(along) * inv * rstd;
+        for (int j = 0; j < K; ++j) {
+            const int h = s.h + j * arg.share * HEADS + lane / LPH;
+            if (h >= count) continue;
+            float d[8];
+            r.d[j][0].get(d, !WHOLE || u.count[0]);
+            r.d[j][1].get(d + 4, !WHOLE || u.count[1]);
+            turn<INTER, true>(d, a, u, rotated >> 1);
+            if (norm) {
+                float x[8], sum = 0.0f, along = 0.0f;
+                r.v[j][0].get(x, !WHOLE || u.count[0]);
+                r.v[j][1].get(x + 4, !WHOLE || u.count[1]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float xh = x[e] * rstd;
-                            dw[e] = __builtin_fmaf(d[e], xh, dw[e]);
-                            d[e] = rstd * __builtin_fmaf(-xh, along, d[e] * w[e]);
-                        }
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    sum = __builtin_fmaf(x[e], x[e], sum);
+                    along = __builtin_fmaf(d[e] * w[e], x[e], along);
+                }
+                const float rstd = 1.0f / sqrtf(__builtin_fmaf(group_sum<LPH>(sum), inv, eps));
+                along = group_sum<LPH>(along) * inv * rstd;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) store_four(out + h * dim + u.at[i], d + 4 * i, u.count[i]);
+                for (int e = 0; e < 8; ++e) {
+                    const float xh = x[e] * rstd;
+                    dw[e] = __builtin_fmaf(d[e], xh, dw[e]);
+                    d[e] = rstd * __builtin_fmaf(-xh, along, d[e] * w[e]);
                 }
             }
-        };
-        heads(p.q, p.q_stride, g.dq_out, g.dq_out_stride, g.dq, p.q_heads, p.q_weight != nullptr, wq, dwq);
-        heads(p.k, p.k_stride, g.dk_out, g.dk_out_stride, g.dk, p.k_heads, p.k_weight != nullptr, wk, dwk);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) store_four(out + (int64_t)h * dim + u.at[i], d + 4 * i, u.count[i]);
+        }
+    };
+    Stop here = {blockIdx.x * per + wave / arg.share, 0, first};
+    here.settle(arg, first, turns);
+    uint32_t angles_at = ~0u;
+    // the work of a stop, with the loads of the one after it on their way
+    auto at = [&](const Stop& s, const Raw& now, Raw& ahead) {
+        const Stop after = s.next(arg, first, turns);
+        if (WHOLE || after.token < arg.tokens) load(after.token < arg.tokens ? after : s, ahead);
+        if (s.token != angles_at) {
+            angles_at = s.token;
+            const uint32_t b = arg.seqlen.div(s.token);
+            a = angles_of(p, b, s.token - b * (uint32_t)p.seqlen, u);
+        }
+        if (s.which == 0) work(s, now, static_cast<T*>(g.dq), (int)p.q_heads, p.q_weight != nullptr, wq, dwq);
+        else work(s, now, static_cast<T*>(g.dk), (int)p.k_heads, p.k_weight != nullptr, wk, dwk);
+        return after;
+    };
+    Raw even, odd;  // (in turns: a copy would wait for the loads)
+    if (here.token < arg.tokens) load(here, even);
+    while (here.token < arg.tokens) {
+        const Stop there = at(here, even, odd);
+        if (there.token >= arg.tokens) break;
+        here = at(there, odd, even);
     }
     if (p.q_weight == nullptr && p.k_weight == nullptr) return;
     for (int e = 0; e < 8; ++e) {
@@ -315,22 +415,28 @@ template <typename T, int LPH, bool INTER> __global__ void __launch_bounds__(256
     }
 }
 
-// Sums of a column of the blocks' shares, in a fixed order: 16 columns a block.
+// Sums of a column of the blocks' shares, in a fixed order: eight columns (32 bytes) a block, 32 rows at a time, eight
+// of them on their way.
 __global__ void __launch_bounds__(256) rotary_weights_kernel(const RotaryArgs arg) {
-    __shared__ float sums[16][17];
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, dim = (int)arg.p.dim;
+    __shared__ float sums[32][9];
+    const int c = threadIdx.x & 7, r = threadIdx.x >> 3, dim = (int)arg.p.dim;
     float* const out = blockIdx.y ? arg.b.dk_weight : arg.b.dq_weight;
     if ((blockIdx.y ? arg.p.k_weight : arg.p.q_weight) == nullptr) return;
-    const int col = blockIdx.x * 16 + c;
+    const int col = blockIdx.x * 8 + c;
     float s = 0.0f;
     if (col < dim) {
-        const float* at = arg.b.workspace + (int64_t)blockIdx.y * arg.blocks * dim + col;
-        for (uint32_t i = r; i < arg.blocks; i += 16) s += at[(int64_t)i * dim];
+        const float* const at = arg.b.workspace + (int64_t)blockIdx.y * arg.blocks * dim + col;
+        for (uint32_t i = r; i < arg.blocks; i += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = i + 32 * k < arg.blocks ? at[(int64_t)(i + 32 * k) * dim] : 0.0f;
+            s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
     }
     sums[r][c] = s;
     __syncthreads();
     if (r == 0 && col < dim) {
-        for (int i = 1; i < 16; ++i) s += sums[i][c];
+        for (int i = 1; i < 32; ++i) s += sums[i][c];
         out[col] = s;
     }
 }
@@ -343,20 +449,34 @@ int head_lanes(const cc1d_rotary_params& p) {
     return n;
 }
 
-template <typename F> int with_lanes(const cc1d_rotary_params& p, F&& f) {
+template <typename F> int with_lanes(const cc1d_rotary_params& p, bool whole, F&& f) {
     return with_flag(p.interleaved != 0, [&](auto inter) {
-        switch (head_lanes(p)) {
-        case 8: return f(std::integral_constant<int, 8>{}, inter);
-        case 16: return f(std::integral_constant<int, 16>{}, inter);
-        case 32: return f(std::integral_constant<int, 32>{}, inter);
-        default: return f(std::integral_constant<int, 64>{}, inter);
-        }
+        return with_flag(whole, [&](auto w) {
+            switch (head_lanes(p)) {
+            case 8: return f(std::integral_constant<int, 8>{}, inter, w);
+            case 16: return f(std::integral_constant<int, 16>{}, inter, w);
+            case 32: return f(std::integral_constant<int, 32>{}, inter, w);
+            default: return f(std::integral_constant<int, 64>{}, inter, w);
+            }
+        });
     });
 }
 
-int64_t bwd_blocks(const cc1d_rotary_params& p) {
-    const int64_t tokens = p.batch * p.seqlen;
-    return tokens < 1024 ? (tokens > 0 ? tokens : 1) : 1024;
+// Whether every run of a lane is four neighbours or none.
+bool whole_runs(const cc1d_rotary_params& p) {
+    const bool fours = p.dim % 4 == 0 && (p.interleaved || p.rotated % 8 == 0);
+    return fours && (p.q_heads == 0 || p.q_stride[3] == 1) && (p.k_heads == 0 || p.k_stride[3] == 1);
+}
+
+// Several wavefronts share a token where there are too few tokens to fill the chip, and heads enough for each.
+int share_of(const cc1d_rotary_params& p) {
+    const int64_t heads = p.q_heads > p.k_heads ? p.q_heads : p.k_heads;
+    return p.batch * p.seqlen < 8192 && heads * head_lanes(p) > 2 * 64 ? 4 : 1;
+}
+
+int64_t blocks_of(const cc1d_rotary_params& p, int64_t most) {
+    const int64_t n = ceil_div(p.batch * p.seqlen, 4 / share_of(p));
+    return n < 1 ? 1 : n < most ? n : most;
 }
 
 RotaryArgs args_of(const cc1d_rotary_params& p, int64_t most) {
@@ -364,39 +484,41 @@ RotaryArgs args_of(const cc1d_rotary_params& p, int64_t most) {
     a.p = p;
     a.tokens = (uint32_t)(p.batch * p.seqlen);
     a.seqlen = FastDiv((uint32_t)(p.seqlen > 0 ? p.seqlen : 1));
-    // several wavefronts share a token where there are too few tokens to fill the chip
-    a.share = p.batch * p.seqlen >= most ? 1 : 4;
+    a.share = share_of(p);
+    a.blocks = (uint32_t)blocks_of(p, most);
     return a;
 }
+
+constexpr int64_t kFwdBlocks = 1024, kBwdBlocks = 768;
 
 }  // namespace
 
 int launch_rotary_fwd(const cc1d_rotary_params& p, hipStream_t stream) {
-    const RotaryArgs a = args_of(p, 8192);
-    const dim3 grid((unsigned)ceil_div(a.tokens, 4 / a.share));
+    const RotaryArgs a = args_of(p, kFwdBlocks);
+    const dim3 grid(a.blocks);
     return with_dtype(p.dtype, [&](auto t) {
-        return with_lanes(p, [&](auto l, auto inter) {
-            return launch(rotary_kernel<decltype(t), decltype(l)::value, decltype(inter)::value>, grid, dim3(256), stream, a);
+        return with_lanes(p, whole_runs(p), [&](auto l, auto inter, auto w) {
+            return launch(rotary_kernel<decltype(t), decltype(l)::value, decltype(inter)::value, decltype(w)::value>, grid, dim3(256), stream, a);
         });
     });
 }
 
 int64_t rotary_bwd_workspace_floats(const cc1d_rotary_bwd_params& b) {
-    return b.fwd.q_weight || b.fwd.k_weight ? 2 * bwd_blocks(b.fwd) * b.fwd.dim : 0;
+    return b.fwd.q_weight || b.fwd.k_weight ? 2 * blocks_of(b.fwd, kBwdBlocks) * b.fwd.dim : 0;
 }
 
 int launch_rotary_bwd(const cc1d_rotary_bwd_params& b, hipStream_t stream) {
     const cc1d_rotary_params& p = b.fwd;
-    RotaryArgs a = args_of(p, 8192);
+    RotaryArgs a = args_of(p, kBwdBlocks);
     a.b = b;
-    a.blocks = (uint32_t)bwd_blocks(p);
+    const bool whole = whole_runs(p) && (p.q_heads == 0 || b.dq_out_stride[3] == 1) && (p.k_heads == 0 || b.dk_out_stride[3] == 1);
     const int st = with_dtype(p.dtype, [&](auto t) {
-        return with_lanes(p, [&](auto l, auto inter) {
-            return launch(rotary_bwd_kernel<decltype(t), decltype(l)::value, decltype(inter)::value>, dim3(a.blocks), dim3(256), stream, a);
+        return with_lanes(p, whole, [&](auto l, auto inter, auto w) {
+            return launch(rotary_bwd_kernel<decltype(t), decltype(l)::value, decltype(inter)::value, decltype(w)::value>, dim3(a.blocks), dim3(256), stream, a);
         });
     });
     if (st != CC1D_OK || (!p.q_weight && !p.k_weight)) return st;
-    return launch(rotary_weights_kernel, dim3((unsigned)ceil_div(p.dim, 16), 2), dim3(256), stream, a);
+    return launch(rotary_weights_kernel, dim3((unsigned)ceil_div(p.dim, 8), 2), dim3(256), stream, a);
 }
 
 }  // namespace cc1d
