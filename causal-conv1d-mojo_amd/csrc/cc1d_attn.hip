@@ -242,7 +242,8 @@ template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_ker
         __syncthreads();
         if (lane == 63) part[wave] = incl;
         __syncthreads();
-        double before = carry + incl - sum;
+        const double later = __shfl_up(incl, 1);  // (not incl - sum, where one that is not finite would reach later positions)
+        double before = carry + (lane ? later : 0.0);
         for (int w = 0; w < wave; ++w) before += part[w];
 #pragma unroll
         for (int i = 0; i < K; ++i) {
