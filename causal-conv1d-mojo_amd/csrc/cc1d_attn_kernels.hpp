@@ -447,9 +447,12 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     };
     auto rows_at = [&](int r) { return r_end - r < C ? r_end - r : C; };
     // A word of each 128 bytes of the next n rows, so that what goes straight into its image comes from the L2 cache when
-    // its turn has come (two wavefronts to an operand).
+    // its turn has come (two wavefronts to an operand). Not long before: the blocks of an XCD work on about as much as
+    // its L2 holds, and lines fetched a whole chunk ahead were gone when they were wanted. Backward of 4 x 2048, 40 heads
+    // of 128 x 128, bf16: 0.80 GB read and 310 us without, 1.32 GB and 275 us from the chunk's start, 0.95 GB and the
+    // same 275 us from its middle.
     uint32_t ahead[2] = {0, 0};
-    auto fetch = [&](int n, const T* px_next, int t) {
+    auto fetch = [&](int n, int t) {
         auto word = [&](const T* p, int64_t s, int d, int lines, uint32_t& to) {
             const int row = lines == 2 ? (t & 127) >> 1 : t & 63, at = lines == 2 ? (t & 1) * 64 : 0;
             if (row < n && at < d) to = *reinterpret_cast<const uint32_t*>(p + row * s + at);
@@ -457,7 +460,6 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
         if (wave >= 2) word(pb, sb, da, DA / 64, ahead[0]);
         else if (!STATES) word(pa, sa, da, DA / 64, ahead[0]);
         if (wave < 2) word(pc, sc, dc, DC / 64, ahead[1]);
-        else if (!STATES && dots) word(px_next, sx, dc, DC / 64, ahead[1]);
     };
 
     // ---- outputs: a lane has NT * 4 neighbouring columns of row 16 it + (lane & 15)
@@ -492,11 +494,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
         }
         __syncthreads();
         if (n_next > 0) {
-            if constexpr (DIRECT) {
-                if (n > 0) fetch(n_next, px + n * sx, otid);
-            } else {
-                load(n_next, otid);
-            }
+            if constexpr (!DIRECT) load(n_next, otid);
         }
         if (n > 0) {
             const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0);
@@ -613,6 +611,8 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                         *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(2, 6))) = u32x2{0u, 0u};
                 __syncthreads();
             }
+            if constexpr (DIRECT)
+                if (n_next > 0) fetch(n_next, otid);
             const float decay = whole[buf];
             bool wild = false;
 #pragma unroll
