@@ -216,9 +216,19 @@ template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_ker
         const float* x = a.dfinal.p + seq * a.dfinal.s[0] + h * a.dfinal.s[1];
         const float* y = a.fin.p + seq * a.fin.s[0] + h * a.fin.s[1];
         double s = 0.0;
-        for (int i = tid; i < a.dk * a.dv; i += 256) {
-            const int64_t r = i / a.dv, c = i % a.dv;
-            s += (double)x[r * a.dfinal.s[2] + c * a.dfinal.s[3]] * (double)y[r * a.fin.s[2] + c * a.fin.s[3]];
+        for (int i0 = tid; i0 < a.dk * a.dv; i0 += 8 * 256) {  // eight loads of each on their way
+            float xs[8], ys[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = i0 + 256 * k, r = i / a.dv, c = i - r * a.dv;
+                xs[k] = ys[k] = 0.0f;
+                if (i < a.dk * a.dv) {
+                    xs[k] = x[r * a.dfinal.s[2] + c * a.dfinal.s[3]];
+                    ys[k] = y[r * a.fin.s[2] + c * a.fin.s[3]];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += (double)xs[k] * (double)ys[k];
         }
         carry = block_sum(s);
     }

@@ -35,6 +35,36 @@ template <typename T, int R, bool VEC> __global__ void __launch_bounds__(256) at
     }
     const int rg = (int)arg.quads.div((uint32_t)tid), quad = tid - rg * (int)arg.quads.d, col = 4 * quad;
     const bool mine = rg < arg.row_groups;
+    const uint32_t kh = arg.group.div(h);
+    const T* const q = static_cast<const T*>(p.q) + b * p.q_stride[0] + kh * p.q_stride[2];
+    const T* const k = static_cast<const T*>(p.k) + b * p.k_stride[0] + kh * p.k_stride[2];
+    const T* const v = static_cast<const T*>(p.v) + b * p.v_stride[0] + h * p.v_stride[2];
+    const T* const g = static_cast<const T*>(p.g) + b * p.g_stride[0] + h * p.g_stride[2];
+    const float scale = (float)p.scale;
+    // One wavefront each for q, k and v, and the decay: two values a lane, asked for before and put into LDS after
+    // whatever else the block asks for.
+    const int lane = tid & 63, w = tid >> 6, size = w < 2 ? dk : dv;
+    const T* const mine_at = w == 0 ? q : w == 1 ? k : w == 2 ? v : g;
+    const int64_t by_token = w == 0 ? p.q_stride[1] : w == 1 ? p.k_stride[1] : w == 2 ? p.v_stride[1] : p.g_stride[1];
+    const int64_t by_element = w == 0 ? p.q_stride[3] : w == 1 ? p.k_stride[3] : w == 2 ? p.v_stride[3] : 0;
+    T next[2];
+    auto ask = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) next[i] = mine_at[t * by_token + (lane + 64 * i < size ? lane + 64 * i : 0) * by_element];
+    };
+    auto put = [&](int buf) {
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) f[i] = lane + 64 * i < size ? to_f32(next[i]) : 0.0f;
+        if (w == 3) {
+            if (lane == 0) decay[buf] = __builtin_amdgcn_exp2f(f[0] * 1.4426950408889634f);
+            return;
+        }
+        float* const to = w == 0 ? ql[buf] : w == 1 ? kl[buf] : vl[buf];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) to[lane + 64 * i] = w == 0 ? f[i] * scale : f[i];
+    };
+    ask(0);
     float* const state = p.attn_state + row * p.attn_state_stride[0] + (int64_t)h * p.attn_state_stride[1] + col * p.attn_state_stride[3];
     float S[R][4];
 #pragma unroll
@@ -52,25 +82,26 @@ template <typename T, int R, bool VEC> __global__ void __launch_bounds__(256) at
             for (int e = 0; e < 4; ++e) S[i][e] = here && col + e < dv ? at[e * p.attn_state_stride[3]] : 0.0f;
         }
     }
-    const uint32_t kh = arg.group.div(h);
-    const T* const q = static_cast<const T*>(p.q) + b * p.q_stride[0] + kh * p.q_stride[2];
-    const T* const k = static_cast<const T*>(p.k) + b * p.k_stride[0] + kh * p.k_stride[2];
-    const T* const v = static_cast<const T*>(p.v) + b * p.v_stride[0] + h * p.v_stride[2];
-    const T* const g = static_cast<const T*>(p.g) + b * p.g_stride[0] + h * p.g_stride[2];
-    const float scale = (float)p.scale;
-    auto fetch = [&](int t, int buf) {  // one wavefront each for q, k and v, and the decay
-        const int lane = tid & 63, w = tid >> 6;
-        for (int i = lane; i < CC1D_MAX_ATTN_DIM; i += 64) {
-            if (w == 0 && i < dk) ql[buf][i] = to_f32(q[t * p.q_stride[1] + i * p.q_stride[3]]) * scale;
-            if (w == 1 && i < dk) kl[buf][i] = to_f32(k[t * p.k_stride[1] + i * p.k_stride[3]]);
-            if (w == 2) vl[buf][i] = i < dv ? to_f32(v[t * p.v_stride[1] + i * p.v_stride[3]]) : 0.0f;
-        }
-        if (tid == 192) decay[buf] = __builtin_amdgcn_exp2f(to_f32(g[t * p.g_stride[1]]) * 1.4426950408889634f);
-    };
-    fetch(0, 0);
+    put(0);
     __syncthreads();
+    auto store = [&]() {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = rg + i * arg.row_groups;
+            float* at = state + r * p.attn_state_stride[2];
+            if (!mine || r >= dk) continue;
+            if constexpr (VEC) {
+                vstore_any_nt(at, u32x4{__float_as_uint(S[i][0]), __float_as_uint(S[i][1]), __float_as_uint(S[i][2]), __float_as_uint(S[i][3])});
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < dv) at[e * p.attn_state_stride[3]] = S[i][e];
+            }
+        }
+    };
     for (int t = 0; t < tokens; ++t) {
         const int buf = t & 1;
+        if (t + 1 < tokens) ask(t + 1);
         const float e = decay[buf];
         float vq[4], acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -88,7 +119,8 @@ template <typename T, int R, bool VEC> __global__ void __launch_bounds__(256) at
             }
         }
         if (mine) *reinterpret_cast<u32x4*>(part + 4 * tid) = u32x4{__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3])};
-        if (t + 1 < tokens) fetch(t + 1, buf ^ 1);
+        if (t + 1 < tokens) put(buf ^ 1);
+        else store();
         __syncthreads();
         const int width = 4 * (int)arg.quads.d;  // part is (row_groups, width)
         if (tid < dv) {
@@ -97,19 +129,6 @@ template <typename T, int R, bool VEC> __global__ void __launch_bounds__(256) at
             out[t * step + tid] = from_f32<T>(y);
         }
         if (t + 1 < tokens) __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int r = rg + i * arg.row_groups;
-        float* at = state + r * p.attn_state_stride[2];
-        if (!mine || r >= dk) continue;
-        if constexpr (VEC) {
-            vstore_any_nt(at, u32x4{__float_as_uint(S[i][0]), __float_as_uint(S[i][1]), __float_as_uint(S[i][2]), __float_as_uint(S[i][3])});
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (col + e < dv) at[e * p.attn_state_stride[3]] = S[i][e];
-        }
     }
 }
 
