@@ -9,8 +9,6 @@ namespace {
 
 constexpr int64_t kAlign = 4;  // floats
 
-int chunk_of(int dtype) { return dtype == CC1D_DTYPE_BF16 ? AttnType<bf16>::chunk : AttnType<float>::chunk; }
-
 struct Plan {
     int64_t seqs, seg, slots, per_row;
     bool cut() const { return slots > seqs; }
@@ -26,10 +24,13 @@ struct Plan {
 // number, as their lengths are not known here and one of them may be nearly
 // all: a block's share is then at most 1 / 768 of the work (8192 positions, 32
 // heads: 180 us, and 211 with segments of 256, 196 with 512, 264 whole).
+// Below 384 positions two more launches cost more than they save (16 heads of
+// 128 x 128, bf16, 256 positions: 22 us whole, 34 in two segments; 448: 40 and
+// 37 in three; 1024: 81 and 42 in six).
 Plan plan_of(const cc1d_attn_params& p, int jobs) {
     Plan pl;
     pl.seqs = p.cu_seqlens ? p.num_seqs : p.batch;
-    const int64_t c = chunk_of(p.dtype);
+    constexpr int64_t c = kMaxChunk;
     int64_t seg;
     if (p.cu_seqlens) {
         seg = (int64_t)((double)p.seqlen * (double)p.heads / 768.0);
@@ -37,7 +38,7 @@ Plan plan_of(const cc1d_attn_params& p, int jobs) {
         const double blocks = (double)p.batch * (double)p.heads * jobs;
         seg = blocks >= 128.0 ? p.seqlen : (int64_t)((double)p.seqlen * blocks / 512.0);
     }
-    seg = ceil_div(seg < 160 ? 160 : seg, c) * c;
+    seg = p.seqlen < 384 ? p.seqlen : ceil_div(seg < 160 ? 160 : seg, c) * c;
     if (seg >= p.seqlen) {
         pl.seg = ceil_div(p.seqlen > 0 ? p.seqlen : 1, c) * c;
         pl.per_row = 1;
@@ -109,7 +110,7 @@ struct CombineArgs {
 // one is left out). A thread for V values, in the order of memory; the walk
 // over the segments is serial, with four of them on their way. Bound by the
 // states, read and written once (170 MB for 8192 positions of 32 heads of
-// 128 x 128 in segments of 384: COMBINE_FIGURE).
+// 128 x 128 in segments of 384: 22 us, from the last-level cache in part).
 template <int V> __global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg) {
     typedef float vec __attribute__((ext_vector_type(V)));
     const AttnArgs& a = arg.a;

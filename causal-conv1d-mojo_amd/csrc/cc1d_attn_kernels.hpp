@@ -74,9 +74,15 @@ struct AttnArgs {
 };
 
 template <typename T> struct AttnType;
-template <> struct AttnType<bf16> { static constexpr int planes = 1, chunk = 64, order = 1; };
-template <> struct AttnType<f16> { static constexpr int planes = 2, chunk = 32, order = 1; };
-template <> struct AttnType<float> { static constexpr int planes = 3, chunk = 32, order = 2; };
+template <> struct AttnType<bf16> { static constexpr int planes = 1, order = 1; };
+template <> struct AttnType<f16> { static constexpr int planes = 2, order = 1; };
+template <> struct AttnType<float> { static constexpr int planes = 3, order = 2; };
+
+// Positions of a chunk: 64 where the images of that many leave two blocks and more to a CU (both directions of 4 x 2048,
+// 32 heads of 64 x 64, fp16: 330 us, with 32 positions 405; but 8164 packed positions of 128 x 64, where the backward's
+// 64 x 128 would have 64 as well: 561, with 32 535).
+constexpr int kMaxChunk = 64;
+template <typename T, int DA, int DC> constexpr int chunk_of() { return AttnType<T>::planes * (2 * DA + DC) <= 384 ? kMaxChunk : 32; }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -349,7 +355,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     typedef AttnType<T> Ty;
     constexpr bool STATES = MODE == kAttnStates;
     constexpr int SORD = MODE == kAttnOut ? Ty::order : 2, SP = SORD + 1;  // planes of what the state takes
-    constexpr int C = Ty::chunk, P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
+    constexpr int C = chunk_of<T, DA, DC>(), P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
     constexpr int NT = DC / 64, TA = DA / 16, SC = C / 32, SA = DA / 32, IT = C / 16;
     constexpr int PT = C == 64 ? 4 : 1;  // tiles of the pairs that a wavefront forms
     constexpr int kPairs = PP * C * C, kA = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
