@@ -14,6 +14,26 @@ struct Plan {
     bool cut() const { return slots > seqs; }
 };
 
+// Segments of about `seg` positions, or whole sequences.
+Plan cut_of(const cc1d_attn_params& p, int64_t seg) {
+    Plan pl;
+    pl.seqs = p.cu_seqlens ? p.num_seqs : p.batch;
+    constexpr int64_t c = kMaxChunk;
+    seg = ceil_div(seg > 0 ? seg : 1, c) * c;
+    if (seg >= p.seqlen) {
+        pl.seg = seg;
+        pl.per_row = 1;
+        // (with cu_seqlens a slot starts at cu[i] / seg + i: seg has to be more than the last start)
+        if (p.cu_seqlens) pl.seg += c;
+        pl.slots = pl.seqs;
+    } else {
+        pl.seg = seg;
+        pl.per_row = ceil_div(p.seqlen, seg);
+        pl.slots = p.cu_seqlens ? p.seqlen / seg + p.num_seqs : p.batch * pl.per_row;
+    }
+    return pl;
+}
+
 // Sequences run as one block per head where those come near to filling the
 // chip (256 CUs, two or three blocks each); longer ones are cut into segments
 // that run side by side, from states that a first pass over keys and values
@@ -28,9 +48,6 @@ struct Plan {
 // 128 x 128, bf16, 256 positions: 22 us whole, 34 in two segments; 448: 40 and
 // 37 in three; 1024: 81 and 42 in six).
 Plan plan_of(const cc1d_attn_params& p, int jobs) {
-    Plan pl;
-    pl.seqs = p.cu_seqlens ? p.num_seqs : p.batch;
-    constexpr int64_t c = kMaxChunk;
     int64_t seg;
     if (p.cu_seqlens) {
         seg = (int64_t)((double)p.seqlen * (double)p.heads / 768.0);
@@ -38,20 +55,12 @@ Plan plan_of(const cc1d_attn_params& p, int jobs) {
         const double blocks = (double)p.batch * (double)p.heads * jobs;
         seg = blocks >= 128.0 ? p.seqlen : (int64_t)((double)p.seqlen * blocks / 512.0);
     }
-    seg = p.seqlen < 384 ? p.seqlen : ceil_div(seg < 160 ? 160 : seg, c) * c;
-    if (seg >= p.seqlen) {
-        pl.seg = ceil_div(p.seqlen > 0 ? p.seqlen : 1, c) * c;
-        pl.per_row = 1;
-        // (with cu_seqlens a slot starts at cu[i] / seg + i: seg has to be more than the last start)
-        if (p.cu_seqlens) pl.seg += c;
-        pl.slots = pl.seqs;
-    } else {
-        pl.seg = seg;
-        pl.per_row = ceil_div(p.seqlen, seg);
-        pl.slots = p.cu_seqlens ? p.seqlen / seg + p.num_seqs : p.batch * pl.per_row;
-    }
-    return pl;
+    return cut_of(p, p.seqlen < 384 ? p.seqlen : seg < 160 ? 160 : seg);
 }
+
+// Pieces of the walk over a decay's gradient.
+constexpr int64_t kPiece = 4096;
+Plan pieces_of(const cc1d_attn_params& p) { return cut_of(p, p.seqlen > 2 * kPiece ? kPiece : p.seqlen); }
 
 int64_t aligned(int64_t n) { return ceil_div(n, kAlign) * kAlign; }
 
@@ -184,66 +193,99 @@ struct DecayGradArgs {
     void* dg;               // (tokens, heads)
     AttnState dfinal, fin;  // p null: the final states are not used
     int64_t g_stride[3];
-    const int32_t* cu;
-    int64_t seqlen, num_seqs, tokens, heads;
+    int64_t tokens;
     int32_t dk, dv;
+    AttnArgs at;  // the pieces (as a sequence's segments), heads
+    float* sums;  // of pieces and final states, two floats a double: (slots + sequences, heads); null: one piece a sequence
 };
+
+typedef uint32_t double_bits __attribute__((ext_vector_type(2), aligned(4)));
+
+// The sum over a block of 256, in everybody, in a fixed order. (NaN and infinities of one wavefront reach all.)
+__device__ __forceinline__ double block_sum_f64(double v, double (&part)[4]) {
+    const double s = lane63(wave_prefix_f64(v));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__device__ __forceinline__ double final_states_dot(const DecayGradArgs& a, int64_t seq, uint32_t h, double (&part)[4]) {
+    if (a.dfinal.p == nullptr) return 0.0;
+    const float* x = a.dfinal.p + seq * a.dfinal.s[0] + h * a.dfinal.s[1];
+    const float* y = a.fin.p + seq * a.fin.s[0] + h * a.fin.s[1];
+    double s = 0.0;
+    for (int i0 = threadIdx.x; i0 < a.dk * a.dv; i0 += 8 * 256) {  // eight loads of each on their way
+        float xs[8], ys[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + 256 * k, r = i / a.dv, c = i - r * a.dv;
+            xs[k] = ys[k] = 0.0f;
+            if (i < a.dk * a.dv) {
+                xs[k] = x[r * a.dfinal.s[2] + c * a.dfinal.s[3]];
+                ys[k] = y[r * a.fin.s[2] + c * a.fin.s[3]];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += (double)xs[k] * (double)ys[k];
+    }
+    return block_sum_f64(s, part);
+}
+
+// Each piece's sum, and by the block of a sequence's last one <G, S> after it.
+__global__ void __launch_bounds__(256) attn_dots_sum_kernel(const DecayGradArgs a) {
+    __shared__ double part[4];
+    const uint32_t slot = a.at.heads_div.div(blockIdx.x), h = blockIdx.x - slot * a.at.heads;
+    const AttnSpan sp = attn_span(a.at, slot);
+    if (!sp.live) return;
+    const int64_t base = h * a.tokens + (a.at.cu ? 0 : sp.seq * a.at.seqlen) + sp.first;
+    const int64_t begin = sp.index * a.at.seg, end = begin + a.at.seg < sp.len ? begin + a.at.seg : sp.len;
+    double s = 0.0;
+    for (int64_t t = begin + threadIdx.x; t < end; t += 256) s += (double)a.row_dots[base + t] - (double)a.col_dots[base + t];
+    s = block_sum_f64(s, part);
+    double_bits* const sums = reinterpret_cast<double_bits*>(a.sums);
+    if (threadIdx.x == 0) sums[(int64_t)slot * a.at.heads + h] = __builtin_bit_cast(u32x2, s);
+    if (sp.index + 1 != sp.segs) return;
+    s = final_states_dot(a, sp.seq, h, part);
+    if (threadIdx.x == 0) sums[((int64_t)a.at.slots + sp.seq) * a.at.heads + h] = __builtin_bit_cast(u32x2, s);
+}
 
 // dg[t] = <G, S> after the sequence's last position + sum over s >= t of
 // (q . dq - k . dk)[s]: a position's decay carries all that is written before
 // it and read from it on, and what is written and read on one side cancels.
-// The sums run in 64 bits. A block per sequence and head; 4 bytes twice a
-// position, read once.
+// The sums run in 64 bits. A block per sequence and head walks from the last
+// position to the first, 2 us for 1024 of them; sequences of more than
+// 2 kPiece positions go by pieces, from their sums (1048576 positions of one
+// head: 2033 us as one walk, 23 in pieces).
 template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_kernel(const DecayGradArgs a) {
     __shared__ double part[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int64_t seq = blockIdx.x / (uint32_t)a.heads, h = blockIdx.x - (uint32_t)seq * (uint32_t)a.heads;
-    int64_t first = 0, len = a.seqlen, row = seq;
-    if (a.cu) {
-        row = 0;
-        first = clamp_pos(ld_uniform(a.cu + seq), a.seqlen);
-        len = clamp_pos(ld_uniform(a.cu + seq + 1), a.seqlen) - first;
-        if (len < 0) len = 0;
-    }
-    auto block_sum = [&](double v) {  // of everybody's
-        const double s = lane63(wave_prefix_f64(v));
-        __syncthreads();
-        if (lane == 0) part[wave] = s;
-        __syncthreads();
-        return (part[0] + part[1]) + (part[2] + part[3]);
-    };
+    const int64_t heads = a.at.heads;
+    const uint32_t slot = a.at.heads_div.div(blockIdx.x), h = blockIdx.x - slot * a.at.heads;
+    const AttnSpan sp = attn_span(a.at, slot);
+    if (!sp.live) return;
+    const int64_t row = a.at.cu ? 0 : sp.seq;
     double carry = 0.0;
-    if (a.dfinal.p) {
-        const float* x = a.dfinal.p + seq * a.dfinal.s[0] + h * a.dfinal.s[1];
-        const float* y = a.fin.p + seq * a.fin.s[0] + h * a.fin.s[1];
-        double s = 0.0;
-        for (int i0 = tid; i0 < a.dk * a.dv; i0 += 8 * 256) {  // eight loads of each on their way
-            float xs[8], ys[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int i = i0 + 256 * k, r = i / a.dv, c = i - r * a.dv;
-                xs[k] = ys[k] = 0.0f;
-                if (i < a.dk * a.dv) {
-                    xs[k] = x[r * a.dfinal.s[2] + c * a.dfinal.s[3]];
-                    ys[k] = y[r * a.fin.s[2] + c * a.fin.s[3]];
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) s += (double)xs[k] * (double)ys[k];
-        }
-        carry = block_sum(s);
+    if (a.sums == nullptr) {
+        carry = final_states_dot(a, sp.seq, h, part);
+    } else {
+        const double_bits* const sums = reinterpret_cast<const double_bits*>(a.sums);
+        auto sum = [&](int64_t i) { return __builtin_bit_cast(double, (u32x2)sums[i * heads + h]); };
+        for (int64_t i = sp.index + 1 + tid; i < sp.segs; i += 256) carry += sum(sp.slot + i);
+        carry = block_sum_f64(carry, part) + sum((int64_t)a.at.slots + sp.seq);
     }
-    const int64_t base = row * a.seqlen;
+    const int64_t base = row * a.at.seqlen;
     T* const dg = static_cast<T*>(a.dg);
     const T* const g = static_cast<const T*>(a.g) + row * a.g_stride[0] + h * a.g_stride[2];
     constexpr int K = 4;  // positions a thread
-    for (int64_t end = first + len; end > first; end -= 256 * K) {
+    const int64_t begin = sp.first + sp.index * a.at.seg, last = begin + a.at.seg < sp.first + sp.len ? begin + a.at.seg : sp.first + sp.len;
+    for (int64_t end = last; end > begin; end -= 256 * K) {
         // thread t has positions end - 1 - K t - i
         double v[K], sum = 0.0;
 #pragma unroll
         for (int i = 0; i < K; ++i) {
             const int64_t t = end - 1 - K * tid - i;
-            if (t >= first) {
+            if (t >= begin) {
                 const int64_t at = h * a.tokens + base + t;
                 sum += (double)a.row_dots[at] - (double)a.col_dots[at];
             }
@@ -260,15 +302,15 @@ template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_ker
         for (int i = 0; i < K; ++i) {
             const int64_t t = end - 1 - K * tid - i;
             // nothing is carried over a decay of 0
-            if (t >= first) dg[(base + t) * a.heads + h] = from_f32<T>(to_f32(g[t * a.g_stride[1]]) < -1e5f ? 0.0f : (float)(before + v[i]));
+            if (t >= begin) dg[(base + t) * heads + h] = from_f32<T>(to_f32(g[t * a.g_stride[1]]) < -1e5f ? 0.0f : (float)(before + v[i]));
         }
         carry += (part[0] + part[1]) + (part[2] + part[3]);
     }
-    if (a.cu) {
-        if (seq == 0)
-            for (int64_t t = tid; t < first; t += 256) dg[t * a.heads + h] = from_f32<T>(0.0f);
-        if (seq == a.num_seqs - 1)
-            for (int64_t t = first + len + tid; t < a.seqlen; t += 256) dg[t * a.heads + h] = from_f32<T>(0.0f);
+    if (a.at.cu) {
+        if (sp.seq == 0 && sp.index == 0)
+            for (int64_t t = tid; t < sp.first; t += 256) dg[t * heads + h] = from_f32<T>(0.0f);
+        if (sp.seq == a.at.num_seqs - 1 && sp.index + 1 == sp.segs)
+            for (int64_t t = last + tid; t < a.at.seqlen; t += 256) dg[t * heads + h] = from_f32<T>(0.0f);
     }
 }
 
@@ -300,7 +342,7 @@ template <typename T, int V> __global__ void __launch_bounds__(256) attn_group_s
 
 // The backward's workspace, in floats.
 struct Room {
-    int64_t dots, part, seg, decay, fin, total;
+    int64_t dots, part, seg, decay, fin, sums, total;
 };
 Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
     const cc1d_attn_params& p = b.fwd;
@@ -311,7 +353,9 @@ Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
     r.seg = pl.cut() ? aligned(pl.slots * per) : 0;
     r.decay = pl.cut() ? aligned(pl.slots * p.heads) : 0;
     r.fin = b.dfinal_states ? aligned(pl.seqs * per) : 0;
-    r.total = 2 * r.dots + 2 * r.part + 2 * r.seg + 2 * r.decay + r.fin;
+    const Plan pieces = pieces_of(p);
+    r.sums = pieces.cut() ? aligned(2 * (pieces.slots + pieces.seqs) * p.heads) : 0;
+    r.total = r.sums + 2 * r.dots + 2 * r.part + 2 * r.seg + 2 * r.decay + r.fin;
     return r;
 }
 
@@ -324,7 +368,8 @@ bool attn_fits(const cc1d_attn_params& p) {
     if ((double)p.heads >= (double)(1 << 15) || seqs * (double)p.heads * kAttnJobs >= (double)(1 << 23)) return false;
     if ((double)p.batch * (double)p.seqlen >= (double)((int64_t)1 << 40) || p.seqlen >= ((int64_t)1 << 31) - 4096) return false;
     return (double)plan_of(p, kAttnJobs).slots * (double)p.heads * kAttnJobs < (double)(1 << 24) &&
-           (double)plan_of(p, 1).slots * (double)p.heads < (double)(1 << 24) && (double)p.heads * 2 * 64 < (double)(1 << 24);
+           (double)plan_of(p, 1).slots * (double)p.heads < (double)(1 << 24) &&
+           (double)pieces_of(p).slots * (double)p.heads < (double)(1 << 24) && (double)p.heads * 2 * 64 < (double)(1 << 24);
 }
 
 int64_t attn_workspace_floats(const cc1d_attn_params& p) {
@@ -375,7 +420,7 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     float *const dq_part = take(room.part), *const dk_part = take(room.part);
     float *const seg_s = take(room.seg), *const seg_g = take(room.seg);
     float *const decay_s = take(room.decay), *const decay_g = take(room.decay);
-    float* const fin = take(room.fin);
+    float *const fin = take(room.fin), *const sums = take(room.sums);
 
     const AttnOperand q = operand(p.q, p.q_stride, per), k = operand(p.k, p.k_stride, per), v = operand(p.v, p.v_stride, 1);
     const AttnOperand d = operand(b.dout, b.dout_stride, 1);
@@ -447,11 +492,15 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     }
     if (st != CC1D_OK) return st;
     if (tokens == 0) return CC1D_OK;
-    DecayGradArgs dg{row_dots, col_dots, p.g, b.dg, last_grad, state(fin, p.heads, dk, dv), {}, p.cu_seqlens,
-                     p.seqlen, pl.seqs, tokens, p.heads, dk, dv};
+    const Plan pieces = pieces_of(p);
+    DecayGradArgs dg{row_dots, col_dots, p.g, b.dg, last_grad, state(fin, p.heads, dk, dv), {}, tokens, dk, dv, args_of(p, pieces, 1), sums};
     for (int i = 0; i < 3; ++i) dg.g_stride[i] = p.g_stride[i];
+    if (sums != nullptr) {
+        st = launch(attn_dots_sum_kernel, dim3(dg.at.blocks), dim3(256), stream, dg);
+        if (st != CC1D_OK) return st;
+    }
     st = with_dtype(p.dtype, [&](auto t) {
-        return launch(attn_decay_grad_kernel<decltype(t)>, dim3((unsigned)(p.heads * pl.seqs)), dim3(256), stream, dg);
+        return launch(attn_decay_grad_kernel<decltype(t)>, dim3(dg.at.blocks), dim3(256), stream, dg);
     });
     if (st != CC1D_OK || !shared) return st;
     const GroupSumArgs gs{{dq_part, dk_part}, {b.dq, b.dk}, tokens * p.key_heads * p.dk, (int32_t)per, dk};

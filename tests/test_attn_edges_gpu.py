@@ -10,7 +10,7 @@ import torch
 
 import causal_conv1d_amd as cc
 from _attn import attn64, close
-from test_attn_gpu import BF16, DEV, FP16, FP32, GRADS, TYPES, check, compare, make, own
+from test_attn_gpu import BF16, DEV, FP16, FP32, GRADS, TYPES, check, check_packed, compare, make, own
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -179,6 +179,19 @@ def test_many_short_sequences():
     got = own(p, torch.tensor(ends, dtype=torch.int32, device=DEV))
     one = {n: None if t is None else (t if n in ("init", "dfinal") else t.view(200, 3, *t.shape[2:])) for n, t in p.items()}
     compare({n: t if n in ("final", "dinit") else t.view(200, 3, *t.shape[2:]) for n, t in got.items()}, one)
+
+
+@TYPES
+def test_long_sequences(dtype):
+    """Sequences whose decays' gradients are summed by pieces; a gradient that is not finite stays before its position."""
+    p = make(2, 8200, 2, 1, 16, 16, dtype, states=True, train=True)
+    check(p)
+    want = own(p)
+    p["dout"][0, 5000, 1, 3] = NAN
+    got = own(p)
+    assert torch.equal(got["dg"][:, 5001:], want["dg"][:, 5001:]) and torch.equal(got["dg"][:, :, 0], want["dg"][:, :, 0])
+    assert not got["dg"][0, :5000, 1].isfinite().any()
+    check_packed(make(1, 9000, 2, 2, 16, 16, dtype, True, True, seqs=4), [3, 5000, 5001, 5001, 8999])
 
 
 def test_values_past_32_bits():
