@@ -117,7 +117,7 @@ struct CombineArgs {
 // The first pass left in every slot what its segment adds to a state of 0;
 // afterwards a slot holds the state at its segment's start (a sequence's first
 // one is left out). A thread for V values, in the order of memory; the walk
-// over the segments is serial, with four of them on their way. Bound by the
+// over the segments is serial, with eight of them on their way. Bound by the
 // states, read and written once (170 MB for 8192 positions of 32 heads of
 // 128 x 128 in segments of 384: 22 us, from the last-level cache in part).
 template <int V> __global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg) {
@@ -152,7 +152,7 @@ template <int V> __global__ void __launch_bounds__(256) attn_combine_kernel(cons
                 cur[i] = job.first.p[seq * job.first.s[0] + h * job.first.s[1] + (turned ? in : out) * job.first.s[2] + (turned ? out : in) * job.first.s[3]];
             }
         }
-        constexpr int K = 4;
+        constexpr int K = 8;
         vec adds[K + 1];
         adds[K] = *reinterpret_cast<const vec*>(at);
         for (int64_t i = 0; i + 1 < segs; i += K, at += K * job.seg.s[0]) {
