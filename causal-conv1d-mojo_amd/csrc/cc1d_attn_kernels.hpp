@@ -204,12 +204,17 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, uint32_t slot) 
         s.len = a.seqlen;
         s.slot = s.seq * a.per_row;
     } else {
-        // sequence i has the slots from cu[i] / seg + i on: the last that starts at or before this one
-        int64_t lo = 0, hi = a.num_seqs - 1;
+        // Sequence i has the slots from cu[i] / seg + i on: the last that starts at or before this one. As many sequences
+        // come before it as slots, less one for each segment that may have come in between; a lane looks at every step-th.
+        int64_t lo = (int64_t)slot - ((int64_t)a.slots - a.num_seqs), hi = slot < a.num_seqs ? (int64_t)slot : a.num_seqs - 1;
+        lo = lo < 0 ? 0 : lo;
         while (lo < hi) {
-            const int64_t mid = (lo + hi + 1) >> 1;
-            if (clamp_pos(ld_uniform(a.cu + mid), a.seqlen) / a.seg + mid <= slot) lo = mid;
-            else hi = mid - 1;
+            const int64_t step = (hi - lo + 64) >> 6, at = lo + (int64_t)(threadIdx.x & 63) * step;
+            const bool before = at <= hi && (uint32_t)clamp_pos(a.cu[at < hi ? at : hi], a.seqlen) / (uint32_t)a.seg + at <= slot;
+            const uint64_t all = __ballot(before);
+            const int last = all ? 63 - __builtin_clzll(all) : 0;
+            lo += last * step;
+            hi = hi < lo + step - 1 ? hi : lo + step - 1;
         }
         s.seq = lo;
         s.first = clamp_pos(ld_uniform(a.cu + lo), a.seqlen);
@@ -501,6 +506,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
         __syncthreads();
         if (n_next > 0) {
             if constexpr (!DIRECT) load(n_next, otid);
+            else if (n == 0) fetch(n_next, otid);
         }
         if (n > 0) {
             const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0);
