@@ -286,6 +286,10 @@ template <typename T, int C, int D, bool QUICK> struct AttnTile {
                 v[n] = vzero();
                 if (row >= rows) continue;
                 const T* const at = base + row * row_stride + col * elem_stride;
+                if (elem_stride == 1 && col + EPV <= d) {
+                    v[n] = vload_any(at);
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < EPV; ++e)
                     if (col + e < d) put(v[n], e, at[e * elem_stride]);
@@ -332,7 +336,7 @@ template <typename T, int C, int D, bool QUICK> struct AttnTile {
     }
 };
 
-// Four neighbouring values, widened.
+// A row's 4 NT neighbouring outputs.
 template <typename T, int NT> __device__ __forceinline__ void store_outputs(char* o, const f32x4 (&O)[NT], bool f32) {
     if (sizeof(T) == 4 || f32) {
 #pragma unroll
@@ -736,9 +740,17 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) x[e] = sizeof(T) == 2 ? vget<T>(x4[it][0], 4 * m + e) : vget<T>(x4[it][m % NT], e);
                             } else {
+                                const T* const at = px + i * sx + (col + 4 * m) * ex;
+                                if (ex == 1 && i < n && col + 4 * m + 4 <= dc) {
+                                    T w[4];
+                                    __builtin_memcpy(w, at, sizeof(w));
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (i < n && col + 4 * m + e < dc) x[e] = to_f32(px[i * sx + (col + 4 * m + e) * ex]);
+                                    for (int e = 0; e < 4; ++e) x[e] = to_f32(w[e]);
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (i < n && col + 4 * m + e < dc) x[e] = to_f32(at[e * ex]);
+                                }
                             }
 #pragma unroll
                             for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[e], dot);
@@ -756,7 +768,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                     } else if (16 * it + l16 < n) {
 #pragma unroll
                         for (int m = 0; m < NT; ++m) {
-                            if (QUICK && col + 4 * m + 4 <= dc) {
+                            if (col + 4 * m + 4 <= dc) {
                                 store_outputs<T, 1>(o + 4 * m * osize, {O[it][m]}, job.out_f32);
                                 continue;
                             }
