@@ -196,6 +196,8 @@ struct DecayGradArgs {
     int64_t tokens;
     int32_t dk, dv;
     AttnArgs at;  // the pieces (as a sequence's segments), heads
+    // states at the segments' starts, forwards and backwards; null: not cut
+    const float *seg_s, *seg_g;
     float* sums;  // of pieces and final states, two floats a double: (slots + sequences, heads); null: one piece a sequence
 };
 
@@ -253,9 +255,13 @@ __global__ void __launch_bounds__(256) attn_dots_sum_kernel(const DecayGradArgs 
 // dg[t] = <G, S> after the sequence's last position + sum over s >= t of
 // (q . dq - k . dk)[s]: a position's decay carries all that is written before
 // it and read from it on, and what is written and read on one side cancels.
-// The sums run in 64 bits. A block per sequence and head walks from the last
-// position to the first, 2 us for 1024 of them; sequences of more than
-// 2 kPiece positions go by pieces, from their sums (1048576 positions of one
+// The sums run in 64 bits, but of values that are fp32 products' sums, whose
+// errors add up over a walk: where sequences are cut, each segment's begins
+// anew from the states at its end, exp(g) <G, S> (16 heads of 80 x 72, 2048
+// positions, fp32: off by 5e-7 to 1.4e-6 in one walk, 4e-7 to 6e-7 in segments).
+// A block per sequence and head walks from the last position to the first, 2 us
+// for 1024 of them; uncut sequences of more than 2 kPiece positions go by
+// pieces, from their sums (1048576 positions of one
 // head: 2033 us as one walk, 23 in pieces).
 template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_kernel(const DecayGradArgs a) {
     __shared__ double part[4];
@@ -265,8 +271,21 @@ template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_ker
     const AttnSpan sp = attn_span(a.at, slot);
     if (!sp.live) return;
     const int64_t row = a.at.cu ? 0 : sp.seq;
+    const T* const g = static_cast<const T*>(a.g) + row * a.g_stride[0] + h * a.g_stride[2];
+    const int64_t begin = sp.first + sp.index * a.at.seg, last = begin + a.at.seg < sp.first + sp.len ? begin + a.at.seg : sp.first + sp.len;
     double carry = 0.0;
-    if (a.sums == nullptr) {
+    if (a.seg_s != nullptr && sp.index + 1 < sp.segs) {
+        // the gradient at the next segment's first position
+        const float decay = to_f32(g[last * a.g_stride[1]]);
+        const int64_t per = (int64_t)a.dk * a.dv;
+        const float* const x = a.seg_s + ((sp.slot + sp.index + 1) * heads + h) * per;
+        const float* const y = a.seg_g + ((sp.slot + sp.segs - 1 - sp.index) * heads + h) * per;
+        double s = 0.0;
+#pragma unroll 8
+        for (int i = tid; i < (int)per; i += 256) s += (double)x[i] * (double)y[i];
+        s = block_sum_f64(s, part);
+        carry = decay < -1e5f ? 0.0 : exp((double)decay) * s;
+    } else if (a.sums == nullptr) {
         carry = final_states_dot(a, sp.seq, h, part);
     } else {
         const double_bits* const sums = reinterpret_cast<const double_bits*>(a.sums);
@@ -276,9 +295,7 @@ template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_ker
     }
     const int64_t base = row * a.at.seqlen;
     T* const dg = static_cast<T*>(a.dg);
-    const T* const g = static_cast<const T*>(a.g) + row * a.g_stride[0] + h * a.g_stride[2];
     constexpr int K = 4;  // positions a thread
-    const int64_t begin = sp.first + sp.index * a.at.seg, last = begin + a.at.seg < sp.first + sp.len ? begin + a.at.seg : sp.first + sp.len;
     for (int64_t end = last; end > begin; end -= 256 * K) {
         // thread t has positions end - 1 - K t - i
         double v[K], sum = 0.0;
@@ -354,7 +371,7 @@ Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
     r.decay = pl.cut() ? aligned(pl.slots * p.heads) : 0;
     r.fin = b.dfinal_states ? aligned(pl.seqs * per) : 0;
     const Plan pieces = pieces_of(p);
-    r.sums = pieces.cut() ? aligned(2 * (pieces.slots + pieces.seqs) * p.heads) : 0;
+    r.sums = !pl.cut() && pieces.cut() ? aligned(2 * (pieces.slots + pieces.seqs) * p.heads) : 0;
     r.total = r.sums + 2 * r.dots + 2 * r.part + 2 * r.seg + 2 * r.decay + r.fin;
     return r;
 }
@@ -492,8 +509,8 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     }
     if (st != CC1D_OK) return st;
     if (tokens == 0) return CC1D_OK;
-    const Plan pieces = pieces_of(p);
-    DecayGradArgs dg{row_dots, col_dots, p.g, b.dg, last_grad, state(fin, p.heads, dk, dv), {}, tokens, dk, dv, args_of(p, pieces, 1), sums};
+    const Plan walk = pl.cut() ? pl : pieces_of(p);
+    DecayGradArgs dg{row_dots, col_dots, p.g, b.dg, last_grad, state(fin, p.heads, dk, dv), {}, tokens, dk, dv, args_of(p, walk, 1), seg_s, seg_g, sums};
     for (int i = 0; i < 3; ++i) dg.g_stride[i] = p.g_stride[i];
     if (sums != nullptr) {
         st = launch(attn_dots_sum_kernel, dim3(dg.at.blocks), dim3(256), stream, dg);

@@ -381,11 +381,12 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     const AttnJob& job = args.job[jn];
     const AttnSpan sp = attn_span(args, slot);
     if (!sp.live || (STATES && sp.index + 1 == sp.segs)) return;
-    const int r_first = (int)(sp.index * args.seg);  // positions of the sequence, in the order of the walk
-    const int r_end = r_first + args.seg < sp.len ? r_first + (int)args.seg : (int)sp.len;
     const int64_t row0 = args.cu ? 0 : sp.seq;  // batch row
     const int da = job.da, dc = job.dc;
     const bool reverse = job.reverse;
+    // positions of the sequence, in the order of the walk; segments begin and end at the same ones either way
+    const int64_t early = reverse ? sp.segs * args.seg - sp.len : 0, from = sp.index * args.seg - early, to = from + args.seg;
+    const int r_first = from > 0 ? (int)from : 0, r_end = (int)(to < sp.len ? to : sp.len);
     const int64_t dir = reverse ? -1 : 1, p0 = reverse ? sp.first + sp.len - 1 : sp.first;
 
     // position r of the walk
