@@ -367,6 +367,13 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     constexpr int C = chunk_of<T, DA, DC>(), P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
     constexpr int NT = DC / 64, TA = DA / 16, SC = C / 32, SA = DA / 32, IT = C / 16;
     constexpr int PT = C == 64 ? 4 : 1;  // tiles of the pairs that a wavefront forms
+    // In fp32 the products of lesser planes have sums of their own, so that a large sum is rounded once for a product of
+    // the first planes and once for the rest, not by each of six. 2 x 2048, 40 heads of 128 x 128: outputs and gradients
+    // off by 1.7e-7 to 1.9e-7 instead of 3.4e-7 to 3.8e-7, dg of sequences that are not cut by 5e-7 to 7e-7 instead of
+    // 1.2e-6 to 1.5e-6. Free in heads of 64; in those of 128 x 128 registers are short (TIGHT: what the outputs are
+    // dotted with is read when it is wanted) and both directions take 14 % longer.
+    constexpr bool LESSER = std::is_same_v<T, float>, TIGHT = LESSER && DA * DC >= 128 * 128;
+    constexpr int LI = LESSER ? C / 16 : 0, LP = LESSER ? PT : 0;
     constexpr int kPairs = PP * C * C, kA = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
     __shared__ __attribute__((aligned(16))) uint16_t lds[kA + P * C * DA + P * C * DC];
     __shared__ __attribute__((aligned(16))) float sums_hi[2][C], sums_lo[2][C], into[2][C], left[2][C];
@@ -532,6 +539,13 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 for (int it = 0; it < IT; ++it)
 #pragma unroll
                     for (int m = 0; m < NT; ++m) O[it][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                f32x4 lesser[LI + 1][NT], few[LP + 1];
+#pragma unroll
+                for (int it = 0; it < LI; ++it)
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) lesser[it][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < LP; ++k) few[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int s = 0; s < SA; ++s) {
                     bf16x8 fb[P];
@@ -559,9 +573,12 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
 #pragma unroll
                             for (int it = 0; it < IT; ++it) {
 #pragma unroll
-                                for (int m = 0; m < NT; ++m)
-                                    if (p + q <= ORD) O[it][m] = mfma(as_frag(sw[m][p]), fq[it], O[it][m]);
-                                if (p < P && p + q <= ORD && (C == 64 || it == it0)) acc[C == 64 ? it : 0] = mfma(fb[p < P ? p : 0], fq[it], acc[C == 64 ? it : 0]);
+                                for (int m = 0; m < NT; ++m) {
+                                    f32x4& to = LESSER && p + q > 0 ? lesser[LESSER ? it : 0][m] : O[it][m];
+                                    if (p + q <= ORD) to = mfma(as_frag(sw[m][p]), fq[it], to);
+                                }
+                                f32x4& to = LESSER && p + q > 0 ? few[0] : acc[C == 64 ? it : 0];
+                                if (p < P && p + q <= ORD && (C == 64 || it == it0)) to = mfma(fb[p < P ? p : 0], fq[it], to);
                             }
                     }
                 }
@@ -569,8 +586,12 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 for (int it = 0; it < IT; ++it) {
                     const float e = into[buf][16 * it + l16];
 #pragma unroll
-                    for (int m = 0; m < NT; ++m) O[it][m] *= e;
+                    for (int m = 0; m < NT; ++m) {
+                        if constexpr (LESSER) O[it][m] += lesser[it][m];
+                        O[it][m] *= e;
+                    }
                 }
+                if constexpr (LESSER) acc[0] += few[0];
                 uint32_t pw[PT][PP][2];
                 const int j = 16 * jt + 4 * g4;
                 const f32x4 jhi = *reinterpret_cast<const f32x4*>(&sums_hi[buf][j]), jlo = *reinterpret_cast<const f32x4*>(&sums_lo[buf][j]);
@@ -593,7 +614,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
                 pairs(C == 64 ? 3 : it0, acc[PT - 1], pw[PT - 1]);
                 __syncthreads();
-                if (QUICK && dots) {
+                if (QUICK && !TIGHT && dots) {
                     const char* const low = reinterpret_cast<const char*>(px) + (reverse ? 15 * sx * (int64_t)sizeof(T) : 0);
                     const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(col * (int)sizeof(T));
 #pragma unroll
@@ -692,9 +713,15 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                                     if (p + q <= ORD) O[it][m] = mfma(__builtin_bit_cast(bf16x8, fc[m][p]), fp[it], O[it][m]);
                     }
                 }
-                constexpr int TG = TA < 4 ? TA : 4;  // tiles at once
+                constexpr int TG = LESSER ? 2 : TA < 4 ? TA : 4;  // tiles at once
 #pragma unroll
-                for (int t0 = 0; t0 < TA; t0 += TG)
+                for (int t0 = 0; t0 < TA; t0 += TG) {
+                    f32x4 lesser[LESSER ? TG : 1][NT];
+                    if constexpr (LESSER)
+#pragma unroll
+                        for (int t = 0; t < TG; ++t)
+#pragma unroll
+                            for (int m = 0; m < NT; ++m) lesser[t][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
                         bf16x8 fb[TG];
@@ -705,9 +732,18 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
 #pragma unroll
                             for (int t = 0; t < TG; ++t)
 #pragma unroll
-                                for (int m = 0; m < NT; ++m)
-                                    if (p + q <= SORD) S[t0 + t][m] = mfma(fb[t], as_frag(ww[m][q]), S[t0 + t][m]);
+                                for (int m = 0; m < NT; ++m) {
+                                    f32x4& to = LESSER && p + q > 0 ? lesser[LESSER ? t : 0][m] : S[t0 + t][m];
+                                    if (p + q <= SORD) to = mfma(fb[t], as_frag(ww[m][q]), to);
+                                }
                     }
+                    if constexpr (LESSER)
+#pragma unroll
+                        for (int t = 0; t < TG; ++t)
+#pragma unroll
+                            for (int m = 0; m < NT; ++m) S[t0 + t][m] += lesser[t][m];
+                    if constexpr (LESSER) __builtin_amdgcn_sched_barrier(0);  // (one group's sums at a time)
+                }
             }
             if constexpr (!STATES) {
                 if (wild)
@@ -729,6 +765,25 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 const uint32_t pitch = (uint32_t)opitch;
                 const uint32_t row = (uint32_t)(reverse ? 15 - l16 : l16);
                 const uint32_t at = row * pitch + (uint32_t)(col * osize);
+                if (QUICK && TIGHT && dots) {
+                    const char* const low = reinterpret_cast<const char*>(px) + (reverse ? 15 * sx * (int64_t)sizeof(T) : 0);
+                    const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(col * (int)sizeof(T));
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        const T* const p = reinterpret_cast<const T*>(low + 16 * it * sx * (int64_t)sizeof(T) + at);
+                        const bool in = full || 16 * it + l16 < n;
+#pragma unroll
+                        for (int m = 0; m < NT; m += 4 / (int)sizeof(T)) {
+                            u32x4 w = vzero();
+                            if constexpr (sizeof(T) == 2 && NT == 1) {
+                                if (in && col < dc) { const u32x2 v = *reinterpret_cast<const typename AnyAddr<2>::v2*>(p); w[0] = v[0]; w[1] = v[1]; }
+                            } else {
+                                if (in && col + 4 * m < dc) w = vload_any(p + 4 * m);
+                            }
+                            x4[it][sizeof(T) == 2 ? 0 : m] = w;
+                        }
+                    }
+                }
                 if (dots) {
 #pragma unroll
                     for (int it = 0; it < IT; ++it) {
