@@ -24,7 +24,8 @@ def linear_attn_update(
 ) -> torch.Tensor:
     """
     q, k: (batch, key_heads, dk) or (batch, tokens, key_heads, dk) -- the new tokens, fp16 / bf16 / fp32
-    attn_state: (batch_or_pool_size, heads, dk, dv) fp32; mutated in place
+    attn_state: (batch_or_pool_size, heads, dk, dv) fp32; mutated in place, as autograd is told: a backward of
+        ``linear_attn_fn`` that went on from this buffer before raises
     v: (batch, [tokens,] heads, dv), g: (batch, [tokens,] heads), as in ``linear_attn_fn``
     scale: on the outputs; dk ** -0.5 if None
     attn_state_indices: (batch,) int32 or None -- state row per batch entry, distinct; < 0 marks padding

@@ -72,6 +72,12 @@ inline bool shaped(const Tensor& t, at::IntArrayRef s) { return t.sizes() == s; 
 inline const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 inline void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
+// Tells autograd that a kernel wrote to a caller's tensor, so that a backward which saved it earlier refuses to read it
+// (a tensor made in inference mode has no version, and no backward).
+inline void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 template <int N> void strides(int64_t (&dst)[N], const Tensor& t) {
     for (int i = 0; i < N; ++i) dst[i] = t.defined() ? t.stride(i) : 0;
 }

@@ -256,6 +256,7 @@ PyObject* py_update(PyObject*, PyObject* const* o, Py_ssize_t n) {
     p.scale = scale;
     p.dtype = dtype_code(q);
     check(api.update(&p, stream_of(q)));
+    written(state);
     unlocked.reset();
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
