@@ -9,7 +9,7 @@ import torch
 
 from causal_conv1d_amd import _host
 from causal_conv1d_amd._attn import _check_heads, _flat
-from causal_conv1d_amd._native import native_attn_update
+from causal_conv1d_amd._native import native_attn_update, written
 from causal_conv1d_amd._scan import _check_int32, _check_like
 
 
@@ -54,4 +54,5 @@ def linear_attn_update(
         parts = (q, k, v, g, out) if q.dim() == 4 else tuple(t.unsqueeze(1) for t in (q, k, v, g, out))
         native_attn_update(parts[0], attn_state, *parts[1:4], dk**-0.5 if scale is None else float(scale),
                            attn_state_indices, parts[4])
+        written(attn_state)
         return out

@@ -25,7 +25,7 @@ def _require_device(x: torch.Tensor) -> None:
         )
 
 
-def _written(t: torch.Tensor) -> None:
+def written(t: torch.Tensor) -> None:
     """Tells autograd that a kernel wrote to a caller's tensor: a backward that saved it earlier refuses to read it."""
     torch.autograd.graph.increment_version(t)
 
@@ -380,7 +380,6 @@ def native_attn_update(q, attn_state, k, v, g, scale, attn_state_indices, out) -
     p.scale, p.dtype = scale, _DTYPE_CODE[q.dtype]
     with torch.cuda.device(q.device):
         _lib.check(lib.cc1d_attn_update(ctypes.byref(p), _stream(q)))
-    _written(attn_state)
 
 
 def _rotary_params(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved, amplitude):

@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from causal_conv1d_amd import _host
-from causal_conv1d_amd._native import native_scan_update
+from causal_conv1d_amd._native import native_scan_update, written
 from causal_conv1d_amd._scan import _check_int32, _check_like, _check_parameters
 
 
@@ -27,7 +27,8 @@ def ssm_scan_update(
 ) -> torch.Tensor:
     """
     u, delta, z: (batch, dim) or (batch, dim, seqlen) -- the new tokens, fp16 / bf16 / fp32
-    ssm_state: (batch_or_pool_size, dim, dstate) fp32; mutated in place
+    ssm_state: (batch_or_pool_size, dim, dstate) fp32; mutated in place, as autograd is told: a backward of
+        ``ssm_scan_fn`` that went on from this buffer before raises
     A: (dim, dstate) fp32; D, delta_bias: (dim,) fp32
     B, C: (batch, [groups,] dstate) for u (batch, dim), (batch, [groups,] dstate, seqlen) otherwise, dtype of u
     ssm_state_indices: (batch,) int32 or None -- state row per batch entry, distinct; < 0 marks padding
@@ -73,4 +74,5 @@ def ssm_scan_update(
             z = None if z is None else z.unsqueeze(-1)
         out = torch.empty_like(u)
         native_scan_update(u, ssm_state, delta, A, B, C, D, z, delta_bias, bool(delta_softplus), ssm_state_indices, out)
+        written(ssm_state)
         return out.squeeze(-1) if unsqueeze else out

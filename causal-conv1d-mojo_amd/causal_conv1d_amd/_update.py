@@ -17,7 +17,7 @@ import torch
 
 from causal_conv1d_amd import _host
 from causal_conv1d_amd._dtype import _DTYPE_CODE
-from causal_conv1d_amd._native import native_update
+from causal_conv1d_amd._native import native_update, written
 
 
 def causal_conv1d_update(
@@ -31,7 +31,8 @@ def causal_conv1d_update(
 ) -> torch.Tensor:
     """
     x: (batch, dim) or (batch, dim, seqlen) -- the new tokens
-    conv_state: (batch_or_pool_size, dim, state_len), state_len >= width - 1; mutated in place
+    conv_state: (batch_or_pool_size, dim, state_len), state_len >= width - 1; mutated in place,
+        as autograd is told: a backward of ``causal_conv1d_fn`` that went on from this buffer before raises
     weight: (dim, width)
     bias: (dim,) or None
     activation: None | "silu" | "swish"
@@ -123,6 +124,7 @@ def causal_conv1d_update(
     out = torch.empty_like(x)
     apply_silu = activation in ("silu", "swish")
     native_update(x, weight, bias, conv_state, conv_state_indices, cache_seqlens, out, apply_silu)
+    written(conv_state)
     if unsqueeze:
         out = out.squeeze(-1)
     return out

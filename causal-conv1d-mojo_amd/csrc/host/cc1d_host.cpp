@@ -258,6 +258,7 @@ PyObject* py_update(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.dtype = dtype_code(x);
     p.apply_silu = act;
     check(api.update(&p, stream_of(x)));
+    written(state);
     unlocked.reset();
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS

@@ -304,6 +304,7 @@ PyObject* py_scan_update(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.dtype = dtype_code(u);
     p.delta_softplus = a[9] == Py_True;
     check(api.scan_update(&p, stream_of(u)));
+    written(state);
     unlocked.reset();
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
