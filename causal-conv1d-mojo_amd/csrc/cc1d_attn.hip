@@ -10,7 +10,7 @@ namespace {
 constexpr int64_t kAlign = 4;  // floats
 
 struct Plan {
-    int64_t seqs, seg, slots, per_row;
+    int64_t seqs, seg, slots, per_row, states;  // states: between segments
     bool cut() const { return slots > seqs; }
 };
 
@@ -26,10 +26,12 @@ Plan cut_of(const cc1d_attn_params& p, int64_t seg) {
         // (with cu_seqlens a slot starts at cu[i] / seg + i: seg has to be more than the last start)
         if (p.cu_seqlens) pl.seg += c;
         pl.slots = pl.seqs;
+        pl.states = 0;
     } else {
         pl.seg = seg;
         pl.per_row = ceil_div(p.seqlen, seg);
         pl.slots = p.cu_seqlens ? p.seqlen / seg + p.num_seqs : p.batch * pl.per_row;
+        pl.states = p.cu_seqlens ? (p.seqlen - 1) / seg : p.batch * (pl.per_row - 1);
     }
     return pl;
 }
@@ -42,8 +44,9 @@ Plan cut_of(const cc1d_attn_params& p, int64_t seg) {
 // three segments; fp32 80 x 72, 16 heads of 2048: 242 us in segments of 256,
 // about 205 with 128, 933 whole. Packed sequences are cut whatever their
 // number, as their lengths are not known here and one of them may be nearly
-// all: a block's share is then at most 1 / 768 of the work (8192 positions, 32
-// heads: 180 us, and 211 with segments of 256, 196 with 512, 264 whole).
+// all: a block's share is then 1 / 768 of the work or 192 positions, whichever
+// is more (8192 positions, 32 heads: 180 us, and 211 with segments of 256, 196
+// with 512, 264 whole).
 // Below 384 positions two more launches cost more than they save (16 heads of
 // 128 x 128, bf16, 256 positions: 22 us whole, 34 in two segments; 448: 40 and
 // 37 in three; 1024: 81 and 42 in six).
@@ -114,12 +117,12 @@ struct CombineArgs {
     uint32_t pieces;  // of 256 vectors
 };
 
-// The first pass left in every slot what its segment adds to a state of 0;
-// afterwards a slot holds the state at its segment's start (a sequence's first
-// one is left out). A thread for V values, in the order of memory; the walk
-// over the segments is serial, with eight of them on their way. Bound by the
-// states, read and written once (170 MB for 8192 positions of 32 heads of
-// 128 x 128 in segments of 384: 22 us, from the last-level cache in part).
+// The first pass left after every segment but a sequence's last what that
+// segment adds to a state of 0; afterwards the state itself is there. A thread
+// for V values, in the order of memory; the walk over the segments is serial,
+// with eight of them on their way. Bound by the states, read and written once
+// (170 MB for 8192 positions of 32 heads of 128 x 128 in segments of 384:
+// 22 us, from the last-level cache in part).
 template <int V> __global__ void __launch_bounds__(256) attn_combine_kernel(const CombineArgs arg) {
     typedef float vec __attribute__((ext_vector_type(V)));
     const AttnArgs& a = arg.a;
@@ -131,19 +134,19 @@ template <int V> __global__ void __launch_bounds__(256) attn_combine_kernel(cons
     const int32_t inner = turned ? job.da : job.dc;
     const float* const decay = job.decay + h;
     for (int64_t seq = blockIdx.y; seq < a.num_seqs; seq += gridDim.y) {
-        int64_t slot, len;
+        AttnSpan s;
         if (a.cu == nullptr) {
-            slot = seq * a.per_row;
-            len = a.seqlen;
+            s.states = seq * (a.per_row - 1);
+            s.len = a.seqlen;
         } else {
             const int64_t first = clamp_pos(a.cu[seq], a.seqlen);
-            len = clamp_pos(a.cu[seq + 1], a.seqlen) - first;
-            slot = first / a.seg + seq;
+            s.len = clamp_pos(a.cu[seq + 1], a.seqlen) - first;
+            s.states = first / a.seg;
         }
-        int64_t segs = len <= a.seg ? 1 : (len + a.seg - 1) / a.seg;
-        if (slot + segs > a.slots) segs = a.slots - slot;
-        if (segs < 2) continue;
-        float* at = job.seg.p + slot * job.seg.s[0] + h * job.seg.s[1] + e;
+        if (s.len <= a.seg) continue;
+        s.segs = (s.len + a.seg - 1) / a.seg;
+        s.index = 0;
+        const int64_t n = s.segs - 1, start = s.after(job.reverse), dir = job.reverse ? -1 : 1;
         vec cur = 0.0f;
         if (job.first.p) {
 #pragma unroll
@@ -153,22 +156,23 @@ template <int V> __global__ void __launch_bounds__(256) attn_combine_kernel(cons
             }
         }
         constexpr int K = 8;
-        vec adds[K + 1];
-        adds[K] = *reinterpret_cast<const vec*>(at);
-        for (int64_t i = 0; i + 1 < segs; i += K, at += K * job.seg.s[0]) {
-            // (read before the turn writes: a slot turns from what it adds into its state)
+        float* at = job.seg.p + start * job.seg.s[0] + h * job.seg.s[1] + e;
+        const float* by_at = decay + start * a.heads;
+        const int64_t step = dir * job.seg.s[0], by_step = dir * (int64_t)a.heads;
+        for (int64_t i = 0; i < n; i += K, at += K * step, by_at += K * by_step) {
+            vec adds[K];
             float by[K];
-            adds[0] = adds[K];
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (i + k + 1 < segs) by[k] = decay[(slot + i + k) * a.heads];
-                if (i + k + 2 < segs) adds[k + 1] = *reinterpret_cast<const vec*>(at + (k + 1) * job.seg.s[0]);
-            }
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (i + k + 1 < segs) {
+                if (i + k < n) {
+                    by[k] = by_at[k * by_step];
+                    adds[k] = *reinterpret_cast<const vec*>(at + k * step);
+                }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (i + k < n) {
                     cur = by[k] * cur + adds[k];
-                    *reinterpret_cast<vec*>(at + (k + 1) * job.seg.s[0]) = cur;
+                    *reinterpret_cast<vec*>(at + k * step) = cur;
                 }
         }
     }
@@ -196,7 +200,7 @@ struct DecayGradArgs {
     int64_t tokens;
     int32_t dk, dv;
     AttnArgs at;  // the pieces (as a sequence's segments), heads
-    // states at the segments' starts, forwards and backwards; null: not cut
+    // states between segments, forwards and backwards; null: not cut
     const float *seg_s, *seg_g;
     float* sums;  // of pieces and final states, two floats a double: (slots + sequences, heads); null: one piece a sequence
 };
@@ -278,8 +282,8 @@ template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_ker
         // the gradient at the next segment's first position
         const float decay = to_f32(g[last * a.g_stride[1]]);
         const int64_t per = (int64_t)a.dk * a.dv;
-        const float* const x = a.seg_s + ((sp.slot + sp.index + 1) * heads + h) * per;
-        const float* const y = a.seg_g + ((sp.slot + sp.segs - 1 - sp.index) * heads + h) * per;
+        const int64_t at = (sp.after(false) * heads + h) * per;
+        const float *const x = a.seg_s + at, *const y = a.seg_g + at;
         double s = 0.0;
 #pragma unroll 8
         for (int i = tid; i < (int)per; i += 256) s += (double)x[i] * (double)y[i];
@@ -367,8 +371,8 @@ Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
     Room r;
     r.dots = aligned(tokens * p.heads);
     r.part = p.heads == p.key_heads ? 0 : aligned(tokens * p.heads * p.dk);
-    r.seg = pl.cut() ? aligned(pl.slots * per) : 0;
-    r.decay = pl.cut() ? aligned(pl.slots * p.heads) : 0;
+    r.seg = aligned(pl.states * per);
+    r.decay = aligned(pl.states * p.heads);
     r.fin = b.dfinal_states ? aligned(pl.seqs * per) : 0;
     const Plan pieces = pieces_of(p);
     r.sums = !pl.cut() && pieces.cut() ? aligned(2 * (pieces.slots + pieces.seqs) * p.heads) : 0;
@@ -391,7 +395,7 @@ bool attn_fits(const cc1d_attn_params& p) {
 
 int64_t attn_workspace_floats(const cc1d_attn_params& p) {
     const Plan pl = plan_of(p, 1);
-    return pl.cut() ? aligned(pl.slots * p.heads * p.dk * p.dv) + aligned(pl.slots * p.heads) : 0;
+    return aligned(pl.states * p.heads * p.dk * p.dv) + aligned(pl.states * p.heads);
 }
 
 int launch_attn_fwd(const cc1d_attn_params& p, hipStream_t stream) {
@@ -411,7 +415,7 @@ int launch_attn_fwd(const cc1d_attn_params& p, hipStream_t stream) {
     j.w_scale = 1.0f;
     if (pl.cut()) {
         j.seg = state(p.workspace, p.heads, p.dk, p.dv);
-        j.decay = p.workspace + aligned(pl.slots * p.heads * p.dk * p.dv);
+        j.decay = p.workspace + aligned(pl.states * p.heads * p.dk * p.dv);
         const int st = run_segments(p, pl, a, (int)p.dk, (int)p.dv, stream);
         if (st != CC1D_OK) return st;
     }

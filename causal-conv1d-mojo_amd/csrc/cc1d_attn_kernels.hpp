@@ -50,8 +50,8 @@ struct AttnJob {
     AttnOperand x;        // dotted with the outputs; p null: no dots
     AttnState first;      // state before the first position; p null: 0
     AttnState last;       // state after the last; p null: not wanted
-    AttnState seg;        // state at the start of each segment but a sequence's first; p null: whole sequences
-    float* decay;         // (slots, heads): a segment's decay
+    AttnState seg;        // states between segments, by AttnSpan::between(); p null: whole sequences
+    float* decay;         // (the same, heads): the decay of the segment walked before it
     void* out;            // (batch * seqlen, heads, dc) contiguous
     float* dots;          // (heads, batch * seqlen)
     int32_t da, dc;       // sizes of rows and columns, of values
@@ -193,7 +193,16 @@ struct AttnSpan {
     int64_t seq, first, len;  // the sequence; its first position and length
     int64_t slot;             // of its first segment
     int64_t segs, index;      // its segments, and which of them this is
+    int64_t states;           // where its states begin
     bool live;
+
+    // Where the state between segments p - 1 and p of the sequence lies, 1 <= p < segs. A segment that another one
+    // follows has `seg` whole positions and so holds one multiple of `seg` (of the packed row, or of its own), which
+    // numbers it: (seqlen - 1) / seg states at most however many sequences there are, and none for those of one segment.
+    __device__ __forceinline__ int64_t between(int64_t p) const { return states + p - 1; }
+    // of the state before (after) this segment in its walk
+    __device__ __forceinline__ int64_t before(bool reverse) const { return between(reverse ? segs - index : index); }
+    __device__ __forceinline__ int64_t after(bool reverse) const { return between(reverse ? segs - 1 - index : index + 1); }
 };
 
 __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, uint32_t slot) {
@@ -203,6 +212,7 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, uint32_t slot) 
         s.first = 0;
         s.len = a.seqlen;
         s.slot = s.seq * a.per_row;
+        s.states = s.seq * (a.per_row - 1);
     } else {
         // Sequence i has the slots from cu[i] / seg + i on: the last that starts at or before this one. As many sequences
         // come before it as slots, less one for each segment that may have come in between; a lane looks at every step-th.
@@ -220,7 +230,8 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, uint32_t slot) 
         s.first = clamp_pos(ld_uniform(a.cu + lo), a.seqlen);
         s.len = clamp_pos(ld_uniform(a.cu + lo + 1), a.seqlen) - s.first;
         if (s.len < 0) s.len = 0;
-        s.slot = s.first / a.seg + lo;
+        s.states = s.first / a.seg;
+        s.slot = s.states + lo;
     }
     s.segs = s.len <= a.seg ? 1 : (s.len + a.seg - 1) / a.seg;
     s.index = (int64_t)slot - s.slot;
@@ -412,7 +423,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
         for (int m = 0; m < NT; ++m) S[t][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const AttnState first = sp.index > 0 ? job.seg : job.first;
     if (!STATES && first.p != nullptr) {
-        const float* const at = first.p + (sp.index > 0 ? (int64_t)slot : sp.seq) * first.s[0] + h * first.s[1];
+        const float* const at = first.p + (sp.index > 0 ? sp.before(reverse) : sp.seq) * first.s[0] + h * first.s[1];
         const int s2 = (int)first.s[2], s3 = (int)first.s[3];
 #pragma unroll
         for (int t = 0; t < TA; ++t)
@@ -859,7 +870,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     const bool ends = sp.index + 1 == sp.segs;
     const AttnState last = STATES ? job.seg : job.last;
     if (last.p != nullptr && (STATES || ends)) {
-        float* const at = last.p + (STATES ? (int64_t)slot : sp.seq) * last.s[0] + h * last.s[1];
+        float* const at = last.p + (STATES ? sp.after(reverse) : sp.seq) * last.s[0] + h * last.s[1];
         const int s2 = (int)last.s[2], s3 = (int)last.s[3];
         float by = 1.0f;
         // backwards, the state before the sequence has its first decay too
@@ -874,7 +885,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                     if (row < da && col < dc) at[(uint32_t)(row * s2 + col * s3)] = by * S[t][m][e];
                 }
     }
-    if (STATES && tid == 3 * 64) job.decay[(int64_t)slot * args.heads + h] = (float)exp2(total);
+    if (STATES && tid == 3 * 64) job.decay[sp.after(reverse) * args.heads + h] = (float)exp2(total);
     // positions that no sequence covers
     if (!STATES && args.cu != nullptr) {
         auto zero = [&](int64_t from, int64_t to) {
