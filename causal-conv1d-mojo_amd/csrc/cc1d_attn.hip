@@ -36,6 +36,13 @@ Plan cut_of(const cc1d_attn_params& p, int64_t seg) {
     return pl;
 }
 
+// Positions after which the decays' gradient begins anew from the states (attn_decay_grad_kernel), which the backward
+// writes on the way. In fp32 512: its error over 2048 positions of 48 heads of 64 x 64 is 3.3e-7 to 3.9e-7 of it where
+// heads remember 2 to 1000 positions, with 1024 4.1e-7 to 6.8e-7 (and 1e-7 where they forget faster, either way); no
+// difference in time (2048 x 16 heads of 80 x 72). 16 bits round far above that (2e-4), and their states are larger
+// beside what else is moved (4 x 2048, 40 heads of 128 x 128: 459 us, with 1024 470, with 512 493).
+int64_t piece_of(const cc1d_attn_params& p) { return p.dtype == CC1D_DTYPE_FP32 ? 512 : 2048; }
+
 // Sequences run as one block per head where those come near to filling the
 // chip (256 CUs, two or three blocks each); longer ones are cut into segments
 // that run side by side, from states that a first pass over keys and values
@@ -58,12 +65,15 @@ Plan plan_of(const cc1d_attn_params& p, int jobs) {
         const double blocks = (double)p.batch * (double)p.heads * jobs;
         seg = blocks >= 128.0 ? p.seqlen : (int64_t)((double)p.seqlen * blocks / 512.0);
     }
+    if (jobs > 1 && p.dtype == CC1D_DTYPE_FP32 && seg < p.seqlen && seg > piece_of(p)) seg = piece_of(p);  // (16 bits need it less than the states' room)
     return cut_of(p, p.seqlen < 384 ? p.seqlen : seg < 160 ? 160 : seg);
 }
 
-// Pieces of the walk over a decay's gradient.
-constexpr int64_t kPiece = 4096;
-Plan pieces_of(const cc1d_attn_params& p) { return cut_of(p, p.seqlen > 2 * kPiece ? kPiece : p.seqlen); }
+// Pieces of the walk over a decay's gradient: where sequences are cut, their segments.
+Plan pieces_of(const cc1d_attn_params& p) {
+    const Plan pl = plan_of(p, kAttnJobs);
+    return pl.cut() ? pl : cut_of(p, piece_of(p));
+}
 
 int64_t aligned(int64_t n) { return ceil_div(n, kAlign) * kAlign; }
 
@@ -191,21 +201,19 @@ int run_segments(const cc1d_attn_params& p, const Plan& pl, const AttnArgs& a, i
 // ---- the gradient of the decays
 
 struct DecayGradArgs {
-    const float* row_dots;  // q . dq, (heads, tokens)
-    const float* col_dots;  // k . dk
+    const float* row_dots;  // q . (what dq gets from the state before its chunk), (heads, tokens)
+    const float* col_dots;  // k . (what dk gets from the gradient of the state after its chunk)
+    const float* over;      // the chunk's pairs over each position
     const void* g;
     void* dg;               // (tokens, heads)
-    AttnState dfinal, fin;  // p null: the final states are not used
+    AttnState dfinal, tail;  // gradients of the final states, and the states before the last chunks; p null: not used
     int64_t g_stride[3];
     int64_t tokens;
     int32_t dk, dv;
     AttnArgs at;  // the pieces (as a sequence's segments), heads
-    // states between segments, forwards and backwards; null: not cut
-    const float *seg_s, *seg_g;
-    float* sums;  // of pieces and final states, two floats a double: (slots + sequences, heads); null: one piece a sequence
+    // states between pieces, forwards and backwards: (places, heads, dk, dv)
+    const float *states, *grads;
 };
-
-typedef uint32_t double_bits __attribute__((ext_vector_type(2), aligned(4)));
 
 // The sum over a block of 256, in everybody, in a fixed order. (NaN and infinities of one wavefront reach all.)
 __device__ __forceinline__ double block_sum_f64(double v, double (&part)[4]) {
@@ -216,10 +224,10 @@ __device__ __forceinline__ double block_sum_f64(double v, double (&part)[4]) {
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-__device__ __forceinline__ double final_states_dot(const DecayGradArgs& a, int64_t seq, uint32_t h, double (&part)[4]) {
+__device__ __forceinline__ double tail_dot(const DecayGradArgs& a, int64_t seq, uint32_t h, double (&part)[4]) {
     if (a.dfinal.p == nullptr) return 0.0;
     const float* x = a.dfinal.p + seq * a.dfinal.s[0] + h * a.dfinal.s[1];
-    const float* y = a.fin.p + seq * a.fin.s[0] + h * a.fin.s[1];
+    const float* y = a.tail.p + seq * a.tail.s[0] + h * a.tail.s[1];
     double s = 0.0;
     for (int i0 = threadIdx.x; i0 < a.dk * a.dv; i0 += 8 * 256) {  // eight loads of each on their way
         float xs[8], ys[8];
@@ -229,7 +237,7 @@ __device__ __forceinline__ double final_states_dot(const DecayGradArgs& a, int64
             xs[k] = ys[k] = 0.0f;
             if (i < a.dk * a.dv) {
                 xs[k] = x[r * a.dfinal.s[2] + c * a.dfinal.s[3]];
-                ys[k] = y[r * a.fin.s[2] + c * a.fin.s[3]];
+                ys[k] = y[r * a.tail.s[2] + c * a.tail.s[3]];
             }
         }
 #pragma unroll
@@ -238,38 +246,35 @@ __device__ __forceinline__ double final_states_dot(const DecayGradArgs& a, int64
     return block_sum_f64(s, part);
 }
 
-// Each piece's sum, and by the block of a sequence's last one <G, S> after it.
-__global__ void __launch_bounds__(256) attn_dots_sum_kernel(const DecayGradArgs a) {
-    __shared__ double part[4];
-    const uint32_t slot = a.at.heads_div.div(blockIdx.x), h = blockIdx.x - slot * a.at.heads;
-    const AttnSpan sp = attn_span(a.at, slot);
-    if (!sp.live) return;
-    const int64_t base = h * a.tokens + (a.at.cu ? 0 : sp.seq * a.at.seqlen) + sp.first;
-    const int64_t begin = sp.index * a.at.seg, end = begin + a.at.seg < sp.len ? begin + a.at.seg : sp.len;
-    double s = 0.0;
-    for (int64_t t = begin + threadIdx.x; t < end; t += 256) s += (double)a.row_dots[base + t] - (double)a.col_dots[base + t];
-    s = block_sum_f64(s, part);
-    double_bits* const sums = reinterpret_cast<double_bits*>(a.sums);
-    if (threadIdx.x == 0) sums[(int64_t)slot * a.at.heads + h] = __builtin_bit_cast(u32x2, s);
-    if (sp.index + 1 != sp.segs) return;
-    s = final_states_dot(a, sp.seq, h, part);
-    if (threadIdx.x == 0) sums[((int64_t)a.at.slots + sp.seq) * a.at.heads + h] = __builtin_bit_cast(u32x2, s);
-}
-
-// dg[t] = <G, S> after the sequence's last position + sum over s >= t of
-// (q . dq - k . dk)[s]: a position's decay carries all that is written before
-// it and read from it on, and what is written and read on one side cancels.
-// The sums run in 64 bits, but of values that are fp32 products' sums, whose
-// errors add up over a walk: where sequences are cut, each segment's begins
-// anew from the states at its end, exp(g) <G, S> (16 heads of 80 x 72, 2048
-// positions, fp32: off by 2e-7 to 3e-7; 2 x 2048 of 40 heads, uncut, 5e-7 to 7e-7).
-// A block per sequence and head walks from the last position to the first, 2 us
-// for 1024 of them; uncut sequences of more than 2 kPiece positions go by
-// pieces, from their sums (1048576 positions of one
-// head: 2033 us as one walk, 23 in pieces).
-template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_kernel(const DecayGradArgs a) {
-    __shared__ double part[4];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+// dg[t] = exp(g[t]) <G[t], S[t-1]>, G the gradient of the state: all that a
+// decay carries from the positions before it to itself and the ones behind. By
+// chunks, the kernel that forms dq and dk leaves three shares of that, none of
+// which holds anything that does not pass over the position:
+//     dg[t] = over[t]                      pairs of the chunk, on its two sides
+//           + sum of row_dots from t on    out of the chunk's first state
+//           + sum of col_dots before t     into the gradient after the chunk
+//           + X                            from before the chunk to behind it.
+// X is the same for a chunk's positions. With D the whole at a boundary between
+// chunks, X = D[end] - sum col_dots and D[start] = X + sum row_dots, from the
+// sequence's last chunk on, whose X is exp(its g) <dfinal, S before it>. These
+// are differences, and errors of D's size add up from chunk to chunk, as the
+// square root of their number: D is formed anew, exp(g) <G, S>, after each
+// piece (piece_of()), and X is 0 where the chunk's decay is less than 2^-24, as
+// it then is below those errors. What is left is an error of D's size at a
+// position that forgets far more than the ones around it.
+// (A running sum of q . dq - k . dk alone takes back all that does not pass
+// over a position, and where heads forget at once dg is far less than that.
+// 2048 positions of 64 x 64, fp32, exp(g) = exp(-4), exp(-10): off by 4e-4 and
+// 0.1 of dg, root mean square, this by 1e-7.)
+// A block per piece and head walks over 1024 positions at a time, four to a
+// thread, GL threads to a chunk, sums in 64 bits. Latency bounds it (17 us for
+// 4 x 2048, 40 heads of 128 x 128), and for many short pieces their states.
+template <typename T, int GL> __global__ void __launch_bounds__(256) attn_decay_grad_kernel(const DecayGradArgs a) {
+    constexpr int K = 4, TILE = 256 * K, NG = 256 / GL;  // positions a thread, of a turn; chunks of a turn
+    __shared__ double part[4], rows_of[NG], cols_of[NG];
+    __shared__ float passes[NG];
+    __shared__ double whole_of;
+    const int tid = threadIdx.x, lane = tid & 63, gl = tid % GL, group = tid / GL;
     const int64_t heads = a.at.heads;
     const uint32_t slot = a.at.heads_div.div(blockIdx.x), h = blockIdx.x - slot * a.at.heads;
     const AttnSpan sp = attn_span(a.at, slot);
@@ -277,55 +282,92 @@ template <typename T> __global__ void __launch_bounds__(256) attn_decay_grad_ker
     const int64_t row = a.at.cu ? 0 : sp.seq;
     const T* const g = static_cast<const T*>(a.g) + row * a.g_stride[0] + h * a.g_stride[2];
     const int64_t begin = sp.first + sp.index * a.at.seg, last = begin + a.at.seg < sp.first + sp.len ? begin + a.at.seg : sp.first + sp.len;
+    // D at the piece's end; at the sequence's, <dfinal, S before the last chunk>
     double carry = 0.0;
-    if (a.seg_s != nullptr && sp.index + 1 < sp.segs) {
-        // the gradient at the next segment's first position
+    const bool tail = sp.index + 1 == sp.segs;
+    if (!tail) {
         const float decay = to_f32(g[last * a.g_stride[1]]);
-        const int64_t per = (int64_t)a.dk * a.dv;
-        const int64_t at = (sp.after(false) * heads + h) * per;
-        const float *const x = a.seg_s + at, *const y = a.seg_g + at;
+        const int64_t per = (int64_t)a.dk * a.dv, at = (sp.after(false) * heads + h) * per;
+        const float *const x = a.states + at, *const y = a.grads + at;
         double s = 0.0;
 #pragma unroll 8
         for (int i = tid; i < (int)per; i += 256) s += (double)x[i] * (double)y[i];
         s = block_sum_f64(s, part);
-        carry = decay < -1e5f ? 0.0 : exp((double)decay) * s;
-    } else if (a.sums == nullptr) {
-        carry = final_states_dot(a, sp.seq, h, part);
+        carry = decay < kNoDecay ? 0.0 : exp((double)decay) * s;
     } else {
-        const double_bits* const sums = reinterpret_cast<const double_bits*>(a.sums);
-        auto sum = [&](int64_t i) { return __builtin_bit_cast(double, (u32x2)sums[i * heads + h]); };
-        for (int64_t i = sp.index + 1 + tid; i < sp.segs; i += 256) carry += sum(sp.slot + i);
-        carry = block_sum_f64(carry, part) + sum((int64_t)a.at.slots + sp.seq);
+        carry = tail_dot(a, sp.seq, h, part);
     }
     const int64_t base = row * a.at.seqlen;
     T* const dg = static_cast<T*>(a.dg);
-    constexpr int K = 4;  // positions a thread
-    for (int64_t end = last; end > begin; end -= 256 * K) {
-        // thread t has positions end - 1 - K t - i
-        double v[K], sum = 0.0;
+    bool first = true;
+    const int last_group = (int)((last - begin - 1) % TILE) / (K * GL);  // of the first turn
+    for (int64_t from = begin + (last - begin - 1) / TILE * TILE; from >= begin && from < last; from -= TILE) {
+        // thread t has positions from + K t + i
+        double u[K], v[K], us = 0.0, vs = 0.0, gs = 0.0;
+        float w[K], decay[K];
 #pragma unroll
         for (int i = 0; i < K; ++i) {
-            const int64_t t = end - 1 - K * tid - i;
-            if (t >= begin) {
-                const int64_t at = h * a.tokens + base + t;
-                sum += (double)a.row_dots[at] - (double)a.col_dots[at];
+            const int64_t t = from + K * tid + i, at = h * a.tokens + base + t;
+            const bool in = t < last;
+            u[i] = in ? (double)a.row_dots[at] : 0.0;
+            v[i] = in ? (double)a.col_dots[at] : 0.0;
+            w[i] = in ? a.over[at] : 0.0f;
+            decay[i] = in ? to_f32(g[t * a.g_stride[1]]) : 0.0f;
+            us += u[i];
+            vs += v[i];
+            gs += log_decay(decay[i]);
+        }
+        // rows from this thread's on, columns up to its, the decays of the chunk. (No difference of sums: one that is
+        // not finite stays on its side.)
+#pragma unroll
+        for (int d = 1; d < GL; d *= 2) {
+            const double later = __shfl_down(us, d, GL), earlier = __shfl_up(vs, d, GL);
+            if (gl + d < GL) us += later;
+            if (gl >= d) vs += earlier;
+            gs += __shfl_xor(gs, d);
+        }
+        const double later = __shfl_down(us, 1, GL), earlier = __shfl_up(vs, 1, GL);
+        double behind = gl + 1 < GL ? later : 0.0, before = gl > 0 ? earlier : 0.0;
+        __syncthreads();  // (of the turn before)
+        if (gl == 0) rows_of[group] = us;
+        if (gl == GL - 1) {
+            cols_of[group] = vs;
+            passes[group] = gs < -24.0 * 0.6931471805599453 ? 0.0f : 1.0f;
+            if (first && tail && group == last_group) {
+                passes[group] = 0.0f;
+                whole_of = carry == 0.0 ? 0.0 : exp(gs) * carry;
             }
-            v[i] = sum;
         }
-        const double incl = wave_prefix_f64(sum);
         __syncthreads();
-        if (lane == 63) part[wave] = incl;
-        __syncthreads();
-        const double later = __shfl_up(incl, 1);  // (not incl - sum, where one that is not finite would reach later positions)
-        double before = carry + (lane ? later : 0.0);
-        for (int w = 0; w < wave; ++w) before += part[w];
+        // D at a chunk's start is p D[end] + (rows - p cols): a lane a chunk, from the last one back
+        const int n = lane % NG;
+        const double rows = rows_of[n], cols = cols_of[n], p = (double)passes[n], own = first && tail && n == last_group ? whole_of : 0.0;
+        double all = p, add = own + (rows - p * cols);
+#pragma unroll
+        for (int d = 1; d < NG; d *= 2) {
+            const double all_later = __shfl_down(all, d, NG), add_later = __shfl_down(add, d, NG);
+            if (n + d < NG) {
+                add += all * add_later;
+                all *= all_later;
+            }
+        }
+        const double start = add + all * carry, next = __shfl_down(start, 1, NG);
+        const double x = __shfl(own + p * ((n + 1 < NG ? next : carry) - cols), group);
+        carry = __shfl(start, 0);
+        first = false;
+        double lower[K];
 #pragma unroll
         for (int i = 0; i < K; ++i) {
-            const int64_t t = end - 1 - K * tid - i;
-            // nothing is carried over a decay of 0
-            if (t >= begin) dg[(base + t) * heads + h] = from_f32<T>(to_f32(g[t * a.g_stride[1]]) < -1e5f ? 0.0f : (float)(before + v[i]));
+            lower[i] = before;
+            before += v[i];
         }
-        carry += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int i = K - 1; i >= 0; --i) {
+            const int64_t t = from + K * tid + i;
+            behind += u[i];
+            // nothing is carried over a decay of 0
+            if (t < last) dg[(base + t) * heads + h] = from_f32<T>(decay[i] < kNoDecay ? 0.0f : (float)(((double)w[i] + x) + (lower[i] + behind)));
+        }
     }
     if (a.at.cu) {
         if (sp.seq == 0 && sp.index == 0)
@@ -363,7 +405,7 @@ template <typename T, int V> __global__ void __launch_bounds__(256) attn_group_s
 
 // The backward's workspace, in floats.
 struct Room {
-    int64_t dots, part, seg, decay, fin, sums, total;
+    int64_t dots, part, between, decay, tail, total;
 };
 Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
     const cc1d_attn_params& p = b.fwd;
@@ -371,12 +413,10 @@ Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
     Room r;
     r.dots = aligned(tokens * p.heads);
     r.part = p.heads == p.key_heads ? 0 : aligned(tokens * p.heads * p.dk);
-    r.seg = aligned(pl.states * per);
+    r.between = aligned(pieces_of(p).states * per);
     r.decay = aligned(pl.states * p.heads);
-    r.fin = b.dfinal_states ? aligned(pl.seqs * per) : 0;
-    const Plan pieces = pieces_of(p);
-    r.sums = !pl.cut() && pieces.cut() ? aligned(2 * (pieces.slots + pieces.seqs) * p.heads) : 0;
-    r.total = r.sums + 2 * r.dots + 2 * r.part + 2 * r.seg + 2 * r.decay + r.fin;
+    r.tail = b.dfinal_states ? aligned(pl.seqs * per) : 0;
+    r.total = 3 * r.dots + 2 * r.part + 2 * r.between + 2 * r.decay + r.tail;
     return r;
 }
 
@@ -437,11 +477,11 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
         ws += n;
         return at;
     };
-    float *const row_dots = take(room.dots), *const col_dots = take(room.dots);
+    float *const row_dots = take(room.dots), *const col_dots = take(room.dots), *const over = take(room.dots);
     float *const dq_part = take(room.part), *const dk_part = take(room.part);
-    float *const seg_s = take(room.seg), *const seg_g = take(room.seg);
+    float *const states = take(room.between), *const grads = take(room.between);
     float *const decay_s = take(room.decay), *const decay_g = take(room.decay);
-    float *const fin = take(room.fin), *const sums = take(room.sums);
+    float* const tail = take(room.tail);
 
     const AttnOperand q = operand(p.q, p.q_stride, per), k = operand(p.k, p.k_stride, per), v = operand(p.v, p.v_stride, 1);
     const AttnOperand d = operand(b.dout, b.dout_stride, 1);
@@ -452,8 +492,8 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     AttnJob jq{}, jk{}, jv{};
     jq.a = d; jq.b = v; jq.c = k; jq.x = q;
     jq.first = turned(first);
-    jq.last = turned(state(fin, p.heads, dk, dv));
-    jq.seg = turned(state(seg_s, p.heads, dk, dv));
+    jq.tail = turned(state(tail, p.heads, dk, dv));
+    jq.seg = turned(state(states, p.heads, dk, dv));
     jq.decay = decay_s;
     jq.out = shared ? dq_part : b.dq;
     jq.dots = row_dots;
@@ -463,7 +503,7 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
 
     jk.a = v; jk.b = d; jk.c = q; jk.x = k;
     jk.first = turned(last_grad);
-    jk.seg = turned(state(seg_g, p.heads, dk, dv));
+    jk.seg = turned(state(grads, p.heads, dk, dv));
     jk.decay = decay_g;
     jk.out = shared ? dk_part : b.dk;
     jk.dots = col_dots;
@@ -472,12 +512,13 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     jk.reverse = 1;
     jk.out_f32 = shared;
 
-    jv.a = k; jv.b = q; jv.c = d;
+    jv.a = k; jv.b = q; jv.c = d; jv.x = v;
     jv.first = last_grad;
     jv.last = state(b.dinitial_states, p.heads, dk, dv);
-    jv.seg = state(seg_g, p.heads, dk, dv);
+    jv.seg = state(grads, p.heads, dk, dv);
     jv.decay = decay_g;
     jv.out = b.dv;
+    jv.over = over;
     jv.da = dk; jv.dc = dv;
     jv.p_scale = jv.w_scale = scale; jv.in_scale = 1.0f;
     jv.reverse = 1;
@@ -488,7 +529,7 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
         s.job[0] = jv;
         s.job[0].b = k; s.job[0].c = v;
         s.job[0].first = first;
-        s.job[0].seg = state(seg_s, p.heads, dk, dv);
+        s.job[0].seg = state(states, p.heads, dk, dv);
         s.job[0].decay = decay_s;
         s.job[0].w_scale = 1.0f;
         s.job[0].reverse = 0;
@@ -496,32 +537,42 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
         const int st = run_segments(p, pl, s, dk, dv, stream);
         if (st != CC1D_OK) return st;
     }
+    // where sequences are not cut, the walks leave states for the decays' gradient as they go
+    const Plan pieces = pieces_of(p);
+    if (!pl.cut() && pieces.cut()) {
+        jq.mark = jq.seg;
+        jk.mark = jk.seg;
+    }
+    auto jobs_of = [&](int jobs) {
+        AttnArgs a = args_of(p, pl, jobs);
+        a.piece = pieces.seg;
+        a.pieces = pieces.per_row;
+        return a;
+    };
     int st;
     const bool alike = (dk <= 64) == (dv <= 64);  // one kernel for all
     if (alike) {
-        AttnArgs a = args_of(p, pl, 3);
+        AttnArgs a = jobs_of(3);
         a.job[0] = jq; a.job[1] = jk; a.job[2] = jv;
         st = launch_jobs(p.dtype, a, dk, dv, false, stream);
     } else {
-        AttnArgs a = args_of(p, pl, 2);
+        AttnArgs a = jobs_of(2);
         a.job[0] = jq; a.job[1] = jk;
         st = launch_jobs(p.dtype, a, dv, dk, false, stream);
         if (st != CC1D_OK) return st;
-        AttnArgs c = args_of(p, pl, 1);
+        AttnArgs c = jobs_of(1);
         c.job[0] = jv;
         st = launch_jobs(p.dtype, c, dk, dv, false, stream);
     }
     if (st != CC1D_OK) return st;
     if (tokens == 0) return CC1D_OK;
-    const Plan walk = pl.cut() ? pl : pieces_of(p);
-    DecayGradArgs dg{row_dots, col_dots, p.g, b.dg, last_grad, state(fin, p.heads, dk, dv), {}, tokens, dk, dv, args_of(p, walk, 1), seg_s, seg_g, sums};
+    DecayGradArgs dg{row_dots, col_dots, over, p.g, b.dg, last_grad, state(tail, p.heads, dk, dv), {}, tokens, dk, dv, args_of(p, pieces, 1), states, grads};
     for (int i = 0; i < 3; ++i) dg.g_stride[i] = p.g_stride[i];
-    if (sums != nullptr) {
-        st = launch(attn_dots_sum_kernel, dim3(dg.at.blocks), dim3(256), stream, dg);
-        if (st != CC1D_OK) return st;
-    }
     st = with_dtype(p.dtype, [&](auto t) {
-        return launch(attn_decay_grad_kernel<decltype(t)>, dim3(dg.at.blocks), dim3(256), stream, dg);
+        typedef decltype(t) T;
+        static_assert(chunk_of<T>(64, 128) == chunk_of<T>(128, 64), "dq, dk and dv in the same chunks");
+        const bool wide = chunk_of<T>(attn_dim_of(dv), attn_dim_of(dk)) == 64;
+        return launch(wide ? attn_decay_grad_kernel<T, 16> : attn_decay_grad_kernel<T, 8>, dim3(dg.at.blocks), dim3(256), stream, dg);
     });
     if (st != CC1D_OK || !shared) return st;
     const GroupSumArgs gs{{dq_part, dk_part}, {b.dq, b.dk}, tokens * p.key_heads * p.dk, (int32_t)per, dk};

@@ -47,13 +47,16 @@ struct AttnState {
 
 struct AttnJob {
     AttnOperand a, b, c;  // rows, columns, values
-    AttnOperand x;        // dotted with the outputs; p null: no dots
+    AttnOperand x;        // beside the outputs, for `dots` and `over`; p null: neither
     AttnState first;      // state before the first position; p null: 0
     AttnState last;       // state after the last; p null: not wanted
     AttnState seg;        // states between segments, by AttnSpan::between(); p null: whole sequences
     float* decay;         // (the same, heads): the decay of the segment walked before it
     void* out;            // (batch * seqlen, heads, dc) contiguous
-    float* dots;          // (heads, batch * seqlen)
+    AttnState mark;       // states on the way, at multiples of AttnArgs::piece, by AttnSpan::between(); p null: none
+    AttnState tail;       // state before the sequence's last chunk (forwards); p null: not wanted
+    float* dots;          // (heads, batch * seqlen): x with what the state gives the outputs; null: not wanted
+    float* over;          // the same: the chunk's pairs over each position; null: not wanted
     int32_t da, dc;       // sizes of rows and columns, of values
     float p_scale, in_scale, w_scale;  // on the pairs, on what the state gives, on what it takes
     int32_t reverse, out_f32;
@@ -68,6 +71,7 @@ struct AttnArgs {
     const int32_t* cu;
     int64_t batch, seqlen, num_seqs;
     int64_t seg;  // positions of a segment, a multiple of the chunk
+    int64_t piece, pieces;  // of marks, the same; of a row (without cu)
     uint32_t heads, jobs, slots, per_row;  // slots of all sequences; of one (without cu)
     FastDiv heads_div, jobs_div, row_div;
     uint32_t blocks;
@@ -82,7 +86,8 @@ template <> struct AttnType<float> { static constexpr int planes = 3, order = 2;
 // 32 heads of 64 x 64, fp16: 330 us, with 32 positions 405; but 8164 packed positions of 128 x 64, where the backward's
 // 64 x 128 would have 64 as well: 561, with 32 535).
 constexpr int kMaxChunk = 64;
-template <typename T, int DA, int DC> constexpr int chunk_of() { return AttnType<T>::planes * (2 * DA + DC) <= 384 ? kMaxChunk : 32; }
+template <typename T> constexpr int chunk_of(int da, int dc) { return AttnType<T>::planes * (2 * da + dc) <= 384 ? kMaxChunk : 32; }
+constexpr int attn_dim_of(int64_t d) { return d <= 64 ? 64 : 128; }  // a head of d is computed as one of this
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -184,9 +189,20 @@ __device__ __forceinline__ double lane63(double v) {
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
+// Sum over 16 neighbouring lanes, in every one of them.
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp_f32<kDppQuadSwap1, 0xf>(v);
+    v += dpp_f32<kDppQuadSwap2, 0xf>(v);
+    v += dpp_f32<kDppRowRor4, 0xf>(v);
+    v += dpp_f32<kDppRowRor8, 0xf>(v);
+    return v;
+}
+
 // A log decay as the sums take it: -1e5 stands for everything below (its
 // exponential is 0), so that sums of -inf have differences.
 __device__ __forceinline__ double log_decay(float g) { return g < -1e5f ? -1e5 : (double)g; }
+// Below this a decay is 0: its exponential is less than the least normal number, 2^-126.
+constexpr float kNoDecay = -87.33655f;
 
 // Where a block works: a sequence's segment.
 struct AttnSpan {
@@ -370,25 +386,27 @@ template <typename T, int NT> __device__ __forceinline__ void store_outputs(char
 // MODE: outputs; outputs and exact states, where somebody wants the last one (the third plane of what the state
 // takes); or the state alone, of the segments that another one follows. QUICK: whole vectors (attn_quick()); else
 // operands are read element by element.
+// GRADS: jobs of a backward, with x.
 enum { kAttnOut = 0, kAttnExact = 1, kAttnStates = 2 };
-template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 : 2) attn_kernel(const AttnArgs args) {
+template <typename T, int DA, int DC, int MODE, bool QUICK, bool GRADS>
+__global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 : 2) attn_kernel(const AttnArgs args) {
     typedef AttnType<T> Ty;
     constexpr bool STATES = MODE == kAttnStates;
     constexpr int SORD = MODE == kAttnOut ? Ty::order : 2, SP = SORD + 1;  // planes of what the state takes
-    constexpr int C = chunk_of<T, DA, DC>(), P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
+    constexpr int C = chunk_of<T>(DA, DC), P = Ty::planes, ORD = Ty::order, PP = ORD + 1;  // PP: planes of computed operands
     constexpr int NT = DC / 64, TA = DA / 16, SC = C / 32, SA = DA / 32, IT = C / 16;
     constexpr int PT = C == 64 ? 4 : 1;  // tiles of the pairs that a wavefront forms
     // In fp32 the products of lesser planes have sums of their own, so that a large sum is rounded once for a product of
     // the first planes and once for the rest, not by each of six. 2 x 2048, 40 heads of 128 x 128: outputs and gradients
-    // off by 1.7e-7 to 1.9e-7 instead of 3.4e-7 to 3.8e-7, dg of sequences that are not cut by 5e-7 to 7e-7 instead of
-    // 1.2e-6 to 1.5e-6. Free in heads of 64; in those of 128 x 128 registers are short (TIGHT: what the outputs are
-    // dotted with is read when it is wanted) and both directions take 14 % longer.
+    // off by 1.7e-7 to 1.9e-7 instead of 3.4e-7 to 3.8e-7. Free in heads of 64; in those of 128 x 128 registers are
+    // short (TIGHT: x is read when it is wanted) and both directions take 14 % longer.
     constexpr bool LESSER = std::is_same_v<T, float>, TIGHT = LESSER && DA * DC >= 128 * 128;
     constexpr int LI = LESSER ? C / 16 : 0, LP = LESSER ? PT : 0;
     constexpr int kPairs = PP * C * C, kA = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
     __shared__ __attribute__((aligned(16))) uint16_t lds[kA + P * C * DA + P * C * DC];
     __shared__ __attribute__((aligned(16))) float sums_hi[2][C], sums_lo[2][C], into[2][C], left[2][C];
-    __shared__ float whole[2], dot_lds[4][C];
+    __shared__ float whole[2];
+    __shared__ __attribute__((aligned(16))) float dot_lds[GRADS ? 4 : 1][GRADS ? C : 1], over_lds[GRADS ? 4 : 1][GRADS ? C : 4];
     uint16_t *const ldsA = lds, *const ldsB = lds + kA, *const ldsC = ldsB + P * C * DA;
     uint16_t* const ldsP = ldsA;  // the rows are dead once their products are formed
 
@@ -411,7 +429,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     auto base = [&](const AttnOperand& o, int r) {
         return static_cast<const T*>(o.p) + row0 * o.s[0] + (p0 + dir * r) * o.s[1] + (int64_t)(h / o.div) * o.s[2];
     };
-    const bool dots = job.dots != nullptr;
+    const bool dots = GRADS && job.dots != nullptr, over = GRADS && job.over != nullptr, beside = dots || over;
     const float p_scale = opaque_f32(job.p_scale);
     const T* const pg = static_cast<const T*>(args.g) + row0 * args.g_stride[0] + h * args.g_stride[2];
 
@@ -467,7 +485,7 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     AttnTile<T, C, DA, QUICK> ta, tb;
     AttnTile<T, C, DC, QUICK> tc;
     constexpr bool DIRECT = decltype(ta)::DIRECT;
-    const T *pa = base(job.a, r_first), *pb = base(job.b, r_first), *pc = base(job.c, r_first), *px = dots ? base(job.x, r_first) : nullptr;
+    const T *pa = base(job.a, r_first), *pb = base(job.b, r_first), *pc = base(job.c, r_first), *px = beside ? base(job.x, r_first) : nullptr;
     const int64_t sa = dir * job.a.s[1], sb = dir * job.b.s[1], sc = dir * job.c.s[1], sx = dir * job.x.s[1];
     const int64_t ea = job.a.s[3], eb = job.b.s[3], ec = job.c.s[3], ex = job.x.s[3];
     // the next n rows, and on past them
@@ -479,7 +497,9 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
         pb += n * sb;
         pc += n * sc;
     };
-    auto rows_at = [&](int r) { return r_end - r < C ? r_end - r : C; };
+    // Chunks begin at multiples of C from the segment's first position either way: backwards, the partial one comes first.
+    const int head = reverse ? (r_end - r_first) % C : 0;
+    auto rows_at = [&](int r) { return r == r_first && head > 0 ? head : r_end - r < C ? r_end - r : C; };
     // A word of each 128 bytes of the next n rows, so that what goes straight into its image comes from the L2 cache when
     // its turn has come (two wavefronts to an operand). Not long before: the blocks of an XCD work on about as much as
     // its L2 holds, and lines fetched a whole chunk ahead were gone when they were wanted. Backward of 4 x 2048, 40 heads
@@ -502,8 +522,28 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
     const int64_t opitch = (int64_t)args.heads * dc * osize;  // bytes from token to token
     char* out = static_cast<char*>(job.out) + (t0 + dir * r_first) * opitch + (int64_t)h * dc * osize;
     auto dots_out = [&](int r) {
-        job.dots[h * tokens + t0 + dir * (r + tid)] = (dot_lds[0][tid] + dot_lds[1][tid]) + (dot_lds[2][tid] + dot_lds[3][tid]);
+        const int64_t at = h * tokens + t0 + dir * (r + tid);
+        if constexpr (GRADS) {
+            if (dots) job.dots[at] = (dot_lds[0][tid] + dot_lds[1][tid]) + (dot_lds[2][tid] + dot_lds[3][tid]);
+            if (over) job.over[at] = (over_lds[0][tid] + over_lds[1][tid]) + (over_lds[2][tid] + over_lds[3][tid]);
+        }
     };
+    auto put_state = [&](const AttnState& to, int64_t place, float by, int lane) {
+        float* const at = to.p + place * to.s[0] + h * to.s[1];
+        const int s2 = (int)to.s[2], s3 = (int)to.s[3];
+#pragma unroll
+        for (int t = 0; t < TA; ++t)
+#pragma unroll
+            for (int m = 0; m < NT; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = tile_col(t, 4 * (lane >> 4) + e), col = tile_col(wave * NT + m, lane & 15);
+                    if (row < da && col < dc) at[(uint32_t)(row * s2 + col * s3)] = by * S[t][m][e];
+                }
+    };
+    // the position of the walk where the state is wanted next
+    int mark = 0x7fffffff;
+    if (GRADS && job.mark.p != nullptr) mark = reverse && sp.len % args.piece ? (int)(sp.len % args.piece) : (int)args.piece;
 
     // Registers load a chunk while the block works on the one before; what goes straight into its image is waited for
     // while the CU's other blocks work. The first turn only loads (or only forms the decays).
@@ -538,7 +578,50 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
             f32x4 O[IT][NT];
             const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
             const bool full = n == C && dc == DC;
-            u32x4 x4[IT][sizeof(T) == 2 ? (NT + 1) / 2 : NT];  // what the outputs are dotted with
+            // x, in vectors of 16 bytes: for `dots` beside the outputs, a row's NT * 4 neighbours; for `over` as a left
+            // operand of NS products of 32 columns, 16 rows of x a wavefront (in chunks of 32 half of their columns)
+            constexpr int XV = sizeof(T) == 2 ? 1 : 2, NS = C == 64 ? DC / 32 : DC / 64;
+            constexpr int XD = sizeof(T) == 2 ? IT : IT * NT, XN = XD > NS * XV ? XD : NS * XV;
+            u32x4 x4[GRADS ? XN : 1];
+            const int xt = C == 64 ? wave : wave & 1, xs = C == 64 ? 0 : (wave >> 1) * NS;
+            auto load_x = [&]() {
+                constexpr int EPV = elems16<T>::value;
+                auto get = [&](u32x4& w, int tile, int c) {  // of the row of tile that is the lane's
+                    constexpr bool TWO = sizeof(T) == 2 && NT == 1;  // (for `dots`: half a vector)
+                    const bool part = TWO && dots;
+                    w = vzero();
+                    if (!(full || 16 * tile + l16 < n)) return;
+                    if constexpr (QUICK) {
+                        const char* const low = reinterpret_cast<const char*>(px) + ((reverse ? 15 : 0) + 16 * tile) * sx * (int64_t)sizeof(T);
+                        const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(c * (int)sizeof(T));
+                        if (c >= dc) return;
+                        if (part) {
+                            const u32x2 v = *reinterpret_cast<const typename AnyAddr<2>::v2*>(reinterpret_cast<const T*>(low + at));
+                            w[0] = v[0];
+                            w[1] = v[1];
+                        } else {
+                            w = vload_any(reinterpret_cast<const T*>(low + at));
+                        }
+                    } else {
+                        const T* const p = px + (16 * tile + l16) * sx + c * ex;
+                        const int count = part ? 4 : EPV;
+                        if (ex == 1 && !part && c + EPV <= dc) {
+                            w = vload_any(p);
+                            return;
+                        }
+#pragma unroll
+                        for (int e = 0; e < EPV; ++e)
+                            if (e < count && c + e < dc) decltype(ta)::put(w, e, p[e * ex]);
+                    }
+                };
+                if (dots) {
+#pragma unroll
+                    for (int i = 0; i < XD; ++i) get(x4[i], i / (XD / IT), col + 4 * (i % (XD / IT)));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NS * XV; ++i) get(x4[i], xt, 32 * (xs + i / XV) + 8 * g4 + 4 * (i % XV));
+                }
+            };
             if constexpr (!STATES) {
                 // ---- what the state gives, and the pairs, transposed (columns x rows), so that a lane gets four columns
                 // of a row: both from one reading of the rows
@@ -603,6 +686,8 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                     }
                 }
                 if constexpr (LESSER) acc[0] += few[0];
+                if constexpr (GRADS && !TIGHT)
+                    if (beside) load_x();
                 uint32_t pw[PT][PP][2];
                 const int j = 16 * jt + 4 * g4;
                 const f32x4 jhi = *reinterpret_cast<const f32x4*>(&sums_hi[buf][j]), jlo = *reinterpret_cast<const f32x4*>(&sums_lo[buf][j]);
@@ -625,25 +710,6 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 if (wave == 3 && n_next > 0) decays(g_next, buf ^ 1);
                 pairs(C == 64 ? 3 : it0, acc[PT - 1], pw[PT - 1]);
                 __syncthreads();
-                if (QUICK && !TIGHT && dots) {
-                    const char* const low = reinterpret_cast<const char*>(px) + (reverse ? 15 * sx * (int64_t)sizeof(T) : 0);
-                    const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(col * (int)sizeof(T));
-#pragma unroll
-                    for (int it = 0; it < IT; ++it) {
-                        const T* const p = reinterpret_cast<const T*>(low + 16 * it * sx * (int64_t)sizeof(T) + at);
-                        const bool in = full || 16 * it + l16 < n;
-#pragma unroll
-                        for (int m = 0; m < NT; m += 4 / (int)sizeof(T)) {
-                            u32x4 w = vzero();
-                            if constexpr (sizeof(T) == 2 && NT == 1) {
-                                if (in && col < dc) { const u32x2 v = *reinterpret_cast<const typename AnyAddr<2>::v2*>(p); w[0] = v[0]; w[1] = v[1]; }
-                            } else {
-                                if (in && col + 4 * m < dc) w = vload_any(p + 4 * m);
-                            }
-                            x4[it][sizeof(T) == 2 ? 0 : m] = w;
-                        }
-                    }
-                }
                 // ---- the pairs to everybody
 #pragma unroll
                 for (int k = 0; k < PT; ++k) {
@@ -659,6 +725,88 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                     for (int p = 0; p < PP; ++p)
                         *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(2, 6))) = u32x2{0u, 0u};
                 __syncthreads();
+                if constexpr (GRADS && TIGHT)
+                    if (beside) load_x();
+                if constexpr (GRADS) if (dots) {
+                    // ---- what the state gives, dotted
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        float dot = 0.0f;
+#pragma unroll
+                        for (int m = 0; m < NT; ++m)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float x = sizeof(T) == 2 ? vget<T>(x4[it], 4 * m + e) : vget<T>(x4[it * (XD / IT) + (sizeof(T) == 2 ? 0 : m)], e);
+                                dot = __builtin_fmaf(O[it][m][e], x, dot);
+                            }
+                        dot += __shfl_xor(dot, 16);
+                        dot += __shfl_xor(dot, 32);
+                        if (g4 == 0) dot_lds[wave][16 * it + l16] = dot;
+                    }
+                }
+                if constexpr (GRADS) if (over) {
+                    // ---- The chunk's pairs over a position: of its rows on one side and its columns on the other, the pair
+                    // times the product of the row of x and the column's values. A wavefront takes 16 rows (in chunks of 32
+                    // half of each product: shares add up in the end). Sums along a row run up to each position, rows add
+                    // up: forwards of the columns before it and the rows from it on, backwards of the columns up to it
+                    // (which are the positions from it on) and the rows after it.
+                    const uint32_t fragX = frag_base<DC / 8>(l16, g4, 0);
+                    uint32_t xw[NS][P][4];
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) {
+                        if constexpr (std::is_same_v<T, bf16>) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) xw[s][0][i] = x4[s][i];
+                        } else {
+                            float f[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) f[i] = sizeof(T) == 2 ? vget<T>(x4[s], i) : vget<T>(x4[XV * s + i / 4 % XV], i & 3);
+                            to_planes<P, 4>(f, xw[s]);
+                        }
+                    }
+                    // (every tile without a branch, so that they wait side by side; what is not the position's is dropped in
+                    // the end, by a select, as it need not be finite)
+                    f32x4 w[IT];
+#pragma unroll
+                    for (int jt = 0; jt < IT; ++jt) {
+                        f32x4 less = {0.0f, 0.0f, 0.0f, 0.0f};
+                        w[jt] = less;
+#pragma unroll
+                        for (int s = 0; s < NS; ++s)
+#pragma unroll
+                            for (int p = 0; p < P; ++p) {
+                                const bf16x8 fk = lds_at<bf16x8>(ldsC + p * C * DC, fragX ^ frag_tile<DC / 8>(jt, 4 * (xs + s)));
+#pragma unroll
+                                for (int q = 0; q < P; ++q) {
+                                    f32x4& to = LESSER && p + q > 0 ? less : w[jt];
+                                    if (p + q <= ORD) to = mfma(fk, as_frag(xw[s][q]), to);
+                                }
+                            }
+                        if constexpr (LESSER) w[jt] += less;
+                        f32x4 pair = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int q = PP - 1; q >= 0; --q) {
+                            const u32x2 b = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(ldsP + q * C * C) + (halfC ^ frag_tile<C / 8>(xt, 2 * jt)));
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) pair[e] += __uint_as_float(e & 1 ? b[e >> 1] & 0xffff0000u : b[e >> 1] << 16);
+                        }
+                        w[jt] *= pair;
+                    }
+                    float tiles = 0.0f;  // of the tiles before
+#pragma unroll
+                    for (int jt = 0; jt < IT; ++jt) {
+                        const float w01 = w[jt][0] + w[jt][1], w012 = w01 + w[jt][2], all = w012 + w[jt][3];
+                        const float one = __shfl_up(all, 16), near = g4 >= 1 ? one : 0.0f, two = __shfl_up(all + near, 32);
+                        const float lanes = near + (g4 >= 2 ? two : 0.0f), base = tiles + lanes;
+                        const float upto[5] = {base, base + w[jt][0], base + w01, base + w012, base + all};
+                        if (jt + 1 < IT) tiles += __shfl(lanes + all, 48 + l16);
+                        const int most = !(full || 16 * xt + l16 < n) || jt > xt ? -1 : jt < xt ? C : l16 - 4 * g4 - (reverse ? 1 : 0);
+                        f32x4 sums;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sums[e] = sum16(e <= most ? (reverse ? upto[e + 1] : upto[e]) : 0.0f);
+                        if (l16 == 0) *reinterpret_cast<f32x4*>(&over_lds[wave][16 * jt + 4 * g4]) = sums;
+                    }
+                }
             }
             if constexpr (DIRECT)
                 if (n_next > 0) fetch(n_next, otid);
@@ -776,57 +924,6 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                 const uint32_t pitch = (uint32_t)opitch;
                 const uint32_t row = (uint32_t)(reverse ? 15 - l16 : l16);
                 const uint32_t at = row * pitch + (uint32_t)(col * osize);
-                if (QUICK && TIGHT && dots) {
-                    const char* const low = reinterpret_cast<const char*>(px) + (reverse ? 15 * sx * (int64_t)sizeof(T) : 0);
-                    const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(col * (int)sizeof(T));
-#pragma unroll
-                    for (int it = 0; it < IT; ++it) {
-                        const T* const p = reinterpret_cast<const T*>(low + 16 * it * sx * (int64_t)sizeof(T) + at);
-                        const bool in = full || 16 * it + l16 < n;
-#pragma unroll
-                        for (int m = 0; m < NT; m += 4 / (int)sizeof(T)) {
-                            u32x4 w = vzero();
-                            if constexpr (sizeof(T) == 2 && NT == 1) {
-                                if (in && col < dc) { const u32x2 v = *reinterpret_cast<const typename AnyAddr<2>::v2*>(p); w[0] = v[0]; w[1] = v[1]; }
-                            } else {
-                                if (in && col + 4 * m < dc) w = vload_any(p + 4 * m);
-                            }
-                            x4[it][sizeof(T) == 2 ? 0 : m] = w;
-                        }
-                    }
-                }
-                if (dots) {
-#pragma unroll
-                    for (int it = 0; it < IT; ++it) {
-                        const int i = 16 * it + l16;
-                        float dot = 0.0f;
-#pragma unroll
-                        for (int m = 0; m < NT; ++m) {
-                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            if constexpr (QUICK) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) x[e] = sizeof(T) == 2 ? vget<T>(x4[it][0], 4 * m + e) : vget<T>(x4[it][m % NT], e);
-                            } else {
-                                const T* const at = px + i * sx + (col + 4 * m) * ex;
-                                if (ex == 1 && i < n && col + 4 * m + 4 <= dc) {
-                                    T w[4];
-                                    __builtin_memcpy(w, at, sizeof(w));
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) x[e] = to_f32(w[e]);
-                                } else {
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e)
-                                        if (i < n && col + 4 * m + e < dc) x[e] = to_f32(at[e * ex]);
-                                }
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(O[it][m][e], x[e], dot);
-                        }
-                        dot += __shfl_xor(dot, 16);
-                        dot += __shfl_xor(dot, 32);
-                        if (g4 == 0) dot_lds[wave][i] = dot;
-                    }
-                }
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
                     char* const o = low + (uint64_t)(uint32_t)((reverse ? C - 16 - 16 * it : 16 * it) * pitch) + at;
@@ -849,42 +946,46 @@ template <typename T, int DA, int DC, int MODE, bool QUICK> __global__ void __la
                     }
                 }
                 out += n * dir * opitch;
-                if (dots) px += n * sx;
+                if (beside) px += n * sx;
             }
         }
         if (n_next <= 0) break;
+        if constexpr (GRADS)
+#pragma unroll 1
+            for (int want = 0; want < 2; ++want) {
+                const bool tail = want == 1;
+                if (tail ? job.tail.p == nullptr || r + n + n_next != (int)sp.len : r + n != mark) continue;
+                int64_t place = sp.seq;
+                if (!tail) {
+                    const int64_t p = (reverse ? sp.len - mark : (int64_t)mark) / args.piece;
+                    place = (args.cu ? sp.first / args.piece : sp.seq * (args.pieces - 1)) + p - 1;
+                    mark += (int)args.piece;
+                }
+                put_state(tail ? job.tail : job.mark, place, 1.0f, opaque(lane));
+            }
         if (wave == 3 && (STATES || n == 0)) decays(g_next, buf ^ 1);
         __syncthreads();
-        if constexpr (!STATES)
-            if (dots && tid < n) dots_out(r);
+        if constexpr (GRADS)
+            if (beside && tid < n) dots_out(r);
         buf ^= 1;
         r += n;
         n = n_next;
     }
-    if constexpr (!STATES) {
+    if constexpr (GRADS) {
         __syncthreads();
-        if (dots && tid < n) dots_out(r);
+        if (beside && tid < n) dots_out(r);
     }
 
     // ---- the state at the segment's end
     const bool ends = sp.index + 1 == sp.segs;
     const AttnState last = STATES ? job.seg : job.last;
     if (last.p != nullptr && (STATES || ends)) {
-        float* const at = last.p + (STATES ? sp.after(reverse) : sp.seq) * last.s[0] + h * last.s[1];
-        const int s2 = (int)last.s[2], s3 = (int)last.s[3];
         float by = 1.0f;
         // backwards, the state before the sequence has its first decay too
         if (!STATES && reverse && sp.len > 0) by = (float)exp(log_decay(to_f32(pg[sp.first * args.g_stride[1]])));
-#pragma unroll
-        for (int t = 0; t < TA; ++t)
-#pragma unroll
-            for (int m = 0; m < NT; ++m)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = tile_col(t, 4 * (lane >> 4) + e), col = tile_col(wave * NT + m, lane & 15);
-                    if (row < da && col < dc) at[(uint32_t)(row * s2 + col * s3)] = by * S[t][m][e];
-                }
+        put_state(last, STATES ? sp.after(reverse) : sp.seq, by, lane);
     }
+
     if (STATES && tid == 3 * 64) job.decay[sp.after(reverse) * args.heads + h] = (float)exp2(total);
     // positions that no sequence covers
     if (!STATES && args.cu != nullptr) {
@@ -915,24 +1016,29 @@ template <typename T> bool attn_quick(const AttnArgs& a) {
     return quick;
 }
 
-template <typename T, int MODE, bool QUICK> int launch_attn_sizes(const AttnArgs& a, int da, int dc, hipStream_t stream) {
+template <typename T, int MODE, bool QUICK, bool GRADS> int launch_attn_sizes(const AttnArgs& a, int da, int dc, hipStream_t stream) {
     const dim3 grid(a.blocks), block(256);
-    if (da <= 64 && dc <= 64) return launch(attn_kernel<T, 64, 64, MODE, QUICK>, grid, block, stream, a);
-    if (da <= 64) return launch(attn_kernel<T, 64, 128, MODE, QUICK>, grid, block, stream, a);
-    if (dc <= 64) return launch(attn_kernel<T, 128, 64, MODE, QUICK>, grid, block, stream, a);
-    return launch(attn_kernel<T, 128, 128, MODE, QUICK>, grid, block, stream, a);
+    if (da <= 64 && dc <= 64) return launch(attn_kernel<T, 64, 64, MODE, QUICK, GRADS>, grid, block, stream, a);
+    if (da <= 64) return launch(attn_kernel<T, 64, 128, MODE, QUICK, GRADS>, grid, block, stream, a);
+    if (dc <= 64) return launch(attn_kernel<T, 128, 64, MODE, QUICK, GRADS>, grid, block, stream, a);
+    return launch(attn_kernel<T, 128, 128, MODE, QUICK, GRADS>, grid, block, stream, a);
 }
 
 // All jobs of `a` have rows of da and values of dc (explicitly instantiated in cc1d_attn_<dtype>[_any].hip).
 template <typename T, bool QUICK> int launch_attn_modes(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream);
 template <typename T, bool QUICK> int launch_attn_modes_impl(const AttnArgs& a, int da, int dc, bool states, hipStream_t stream) {
-    if (states) return launch_attn_sizes<T, kAttnStates, QUICK>(a, da, dc, stream);
-    if constexpr (AttnType<T>::order < 2) {
-        bool exact = false;
-        for (uint32_t j = 0; j < a.jobs; ++j) exact = exact || a.job[j].last.p != nullptr;
-        if (!exact) return launch_attn_sizes<T, kAttnOut, QUICK>(a, da, dc, stream);
+    if (states) return launch_attn_sizes<T, kAttnStates, QUICK, false>(a, da, dc, stream);
+    bool exact = AttnType<T>::order == 2, grads = false;
+    for (uint32_t j = 0; j < a.jobs; ++j) {
+        exact = exact || a.job[j].last.p != nullptr;
+        grads = grads || a.job[j].x.p != nullptr;
     }
-    return launch_attn_sizes<T, kAttnExact, QUICK>(a, da, dc, stream);
+    return with_flag(grads, [&](auto gr) {
+        constexpr bool GRADS = decltype(gr)::value;
+        if constexpr (AttnType<T>::order < 2)
+            if (!exact) return launch_attn_sizes<T, kAttnOut, QUICK, GRADS>(a, da, dc, stream);
+        return launch_attn_sizes<T, kAttnExact, QUICK, GRADS>(a, da, dc, stream);
+    });
 }
 
 }  // namespace cc1d
