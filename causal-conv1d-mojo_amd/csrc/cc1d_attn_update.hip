@@ -10,6 +10,14 @@
 namespace cc1d {
 namespace {
 
+// exp(g), by a product with log2(e) in two floats: rounded to one, an exponent of -16 would cost 8 * 2^-24 of the decay.
+// (-1e5 stands for everything below, as 1e5 for everything above: their second float would not be a number.)
+__device__ __forceinline__ float decay_of(float g) {
+    const float x = g < -1e5f ? -1e5f : g > 1e5f ? 1e5f : g, hi = x * 1.44269502f;
+    const float lo = __builtin_fmaf(x, 1.44269502f, -hi) + x * 1.92596299e-8f;
+    return __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
+}
+
 struct AttnUpdateArgs {
     cc1d_attn_update_params p;
     FastDiv heads, group, quads;  // of quads: a row's groups of four columns
@@ -57,7 +65,7 @@ template <typename T, int R, bool VEC> __global__ void __launch_bounds__(256) at
 #pragma unroll
         for (int i = 0; i < 2; ++i) f[i] = lane + 64 * i < size ? to_f32(next[i]) : 0.0f;
         if (w == 3) {
-            if (lane == 0) decay[buf] = __builtin_amdgcn_exp2f(f[0] * 1.4426950408889634f);
+            if (lane == 0) decay[buf] = decay_of(f[0]);
             return;
         }
         float* const to = w == 0 ? ql[buf] : w == 1 ? kl[buf] : vl[buf];
