@@ -9,8 +9,41 @@ import torch
 
 from causal_conv1d_amd import _host
 from causal_conv1d_amd._attn import _check_heads, _flat
-from causal_conv1d_amd._native import native_attn_update, written
+from causal_conv1d_amd._native import native_attn_update
 from causal_conv1d_amd._scan import _check_int32, _check_like
+
+
+def _attn_update_impl(
+    q: torch.Tensor,
+    attn_state: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    g: torch.Tensor,
+    scale: float,
+    attn_state_indices: torch.Tensor | None,
+    out: torch.Tensor,
+) -> None:
+    native_attn_update(q, attn_state, k, v, g, scale, attn_state_indices, out)
+
+
+def _attn_update_fake(
+    q: torch.Tensor,
+    attn_state: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    g: torch.Tensor,
+    scale: float,
+    attn_state_indices: torch.Tensor | None,
+    out: torch.Tensor,
+) -> None:
+    return None
+
+
+_attn_update_inplace = torch.library.custom_op(
+    "causal_conv1d_amd::_attn_update_inplace",
+    mutates_args=("attn_state", "out"),
+)(_attn_update_impl)
+_attn_update_inplace.register_fake(_attn_update_fake)
 
 
 def linear_attn_update(
@@ -52,7 +85,6 @@ def linear_attn_update(
     with torch.no_grad():
         out = _flat(v)
         parts = (q, k, v, g, out) if q.dim() == 4 else tuple(t.unsqueeze(1) for t in (q, k, v, g, out))
-        native_attn_update(parts[0], attn_state, *parts[1:4], dk**-0.5 if scale is None else float(scale),
-                           attn_state_indices, parts[4])
-        written(attn_state)
+        torch.ops.causal_conv1d_amd._attn_update_inplace(
+            parts[0], attn_state, *parts[1:4], dk**-0.5 if scale is None else float(scale), attn_state_indices, parts[4])
         return out
