@@ -25,11 +25,6 @@ def _require_device(x: torch.Tensor) -> None:
         )
 
 
-def written(t: torch.Tensor) -> None:
-    """Tells autograd that a kernel wrote to a caller's tensor: a backward that saved it earlier refuses to read it."""
-    torch.autograd.graph.increment_version(t)
-
-
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

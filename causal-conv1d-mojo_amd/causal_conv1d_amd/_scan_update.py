@@ -8,8 +8,49 @@ from __future__ import annotations
 import torch
 
 from causal_conv1d_amd import _host
-from causal_conv1d_amd._native import native_scan_update, written
+from causal_conv1d_amd._native import native_scan_update
 from causal_conv1d_amd._scan import _check_int32, _check_like, _check_parameters
+
+
+def _scan_update_impl(
+    u: torch.Tensor,
+    ssm_state: torch.Tensor,
+    delta: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None,
+    z: torch.Tensor | None,
+    delta_bias: torch.Tensor | None,
+    delta_softplus: bool,
+    ssm_state_indices: torch.Tensor | None,
+    out: torch.Tensor,
+) -> None:
+    native_scan_update(u, ssm_state, delta, A, B, C, D, z, delta_bias, delta_softplus, ssm_state_indices, out)
+
+
+def _scan_update_fake(
+    u: torch.Tensor,
+    ssm_state: torch.Tensor,
+    delta: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None,
+    z: torch.Tensor | None,
+    delta_bias: torch.Tensor | None,
+    delta_softplus: bool,
+    ssm_state_indices: torch.Tensor | None,
+    out: torch.Tensor,
+) -> None:
+    return None
+
+
+_scan_update_inplace = torch.library.custom_op(
+    "causal_conv1d_amd::_scan_update_inplace",
+    mutates_args=("ssm_state", "out"),
+)(_scan_update_impl)
+_scan_update_inplace.register_fake(_scan_update_fake)
 
 
 def ssm_scan_update(
@@ -73,6 +114,6 @@ def ssm_scan_update(
             u, delta, B, C = (t.unsqueeze(-1) for t in (u, delta, B, C))
             z = None if z is None else z.unsqueeze(-1)
         out = torch.empty_like(u)
-        native_scan_update(u, ssm_state, delta, A, B, C, D, z, delta_bias, bool(delta_softplus), ssm_state_indices, out)
-        written(ssm_state)
+        torch.ops.causal_conv1d_amd._scan_update_inplace(u, ssm_state, delta, A, B, C, D, z, delta_bias,
+                                                         bool(delta_softplus), ssm_state_indices, out)
         return out.squeeze(-1) if unsqueeze else out

@@ -17,7 +17,40 @@ import torch
 
 from causal_conv1d_amd import _host
 from causal_conv1d_amd._dtype import _DTYPE_CODE
-from causal_conv1d_amd._native import native_update, written
+from causal_conv1d_amd._native import native_update
+
+
+def _update_impl(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None,
+    conv_state: torch.Tensor,
+    conv_state_indices: torch.Tensor | None,
+    cache_seqlens: torch.Tensor | None,
+    out: torch.Tensor,
+    apply_silu: bool,
+) -> None:
+    native_update(x, weight, bias, conv_state, conv_state_indices, cache_seqlens, out, apply_silu)
+
+
+def _update_fake(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None,
+    conv_state: torch.Tensor,
+    conv_state_indices: torch.Tensor | None,
+    cache_seqlens: torch.Tensor | None,
+    out: torch.Tensor,
+    apply_silu: bool,
+) -> None:
+    return None
+
+
+_update_inplace = torch.library.custom_op(
+    "causal_conv1d_amd::_update_inplace",
+    mutates_args=("conv_state", "out"),
+)(_update_impl)
+_update_inplace.register_fake(_update_fake)
 
 
 def causal_conv1d_update(
@@ -121,10 +154,8 @@ def causal_conv1d_update(
         if not conv_state_indices.is_contiguous():
             conv_state_indices = conv_state_indices.contiguous()
 
-    out = torch.empty_like(x)
-    apply_silu = activation in ("silu", "swish")
-    native_update(x, weight, bias, conv_state, conv_state_indices, cache_seqlens, out, apply_silu)
-    written(conv_state)
-    if unsqueeze:
-        out = out.squeeze(-1)
-    return out
+    with torch.no_grad():
+        out = torch.empty_like(x)
+        torch.ops.causal_conv1d_amd._update_inplace(x, weight, bias, conv_state, conv_state_indices, cache_seqlens, out,
+                                                    activation in ("silu", "swish"))
+        return out.squeeze(-1) if unsqueeze else out

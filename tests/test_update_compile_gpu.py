@@ -7,6 +7,7 @@ import torch
 
 import causal_conv1d_amd as cc
 from test_attn_update_gpu import call, make
+from test_scan_update_gpu import make as scan_make
 
 pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore:.*torch.jit.script.*:DeprecationWarning")]
 DEV = "cuda"
@@ -55,3 +56,40 @@ def test_linear_attn_update_of_tensors_that_want_gradients():
     big = torch.stack((p["state"], p["state"]))  # a view, which is written through
     out = call({**p, "q": q, "state": big[1]})
     assert torch.equal(out, want) and torch.equal(big[0], p["state"]) and not torch.equal(big[1], p["state"])
+
+
+@pytest.mark.parametrize("T", [None, 3])
+@pytest.mark.parametrize("softplus", [False, True])
+def test_ssm_scan_update(softplus, T):
+    p = scan_make(4, 24, 16, 2, T, BF16, rows=6)
+    idx = torch.tensor([5, -1, 0, 2], dtype=torch.int32, device=DEV)
+
+    def f(u, state, delta, A, B, C, z):
+        return cc.ssm_scan_update(u, state, delta, A, B, C, D=p["D"], z=z, delta_bias=p["bias"], delta_softplus=softplus,
+                                  ssm_state_indices=idx) * 2.0
+
+    compiled(f, [p[n] for n in ("u", "state", "delta", "A", "B", "C", "z")], 1)
+
+
+@pytest.mark.parametrize("T", [None, 3])
+@pytest.mark.parametrize("ring", [False, True])
+def test_causal_conv1d_update(ring, T):
+    x = torch.randn(2, 24, *(() if T is None else (T,)), device=DEV)
+    w, bias, state = torch.randn(24, 4, device=DEV), torch.randn(24, device=DEV), torch.randn(2, 24, 5, device=DEV)
+    heads = torch.tensor([0, 2], dtype=torch.int32, device=DEV) if ring else None
+
+    def f(x, state, w):
+        return cc.causal_conv1d_update(x, state, w, bias, activation="silu", cache_seqlens=heads) * 2.0
+
+    compiled(f, [x, state, w], 1)
+
+
+def test_opchecks():
+    ops = torch.ops.causal_conv1d_amd
+    x, w, state = torch.randn(2, 24, 2, device=DEV), torch.randn(24, 4, device=DEV), torch.randn(2, 24, 5, device=DEV)
+    torch.library.opcheck(ops._update_inplace.default, (x, w, None, state, None, None, torch.empty_like(x), True))
+    p = scan_make(3, 8, 16, 1, 2, BF16, rows=5)
+    idx = torch.tensor([4, -1, 0], dtype=torch.int32, device=DEV)
+    torch.library.opcheck(ops._scan_update_inplace.default,
+                          (p["u"], p["state"], p["delta"], p["A"], p["B"], p["C"], p["D"], p["z"], p["bias"], True, idx,
+                           torch.empty_like(p["u"])))
