@@ -37,26 +37,27 @@ Plan cut_of(const cc1d_attn_params& p, int64_t seg) {
 }
 
 // Positions after which the decays' gradient begins anew from the states (attn_decay_grad_kernel), which the backward
-// writes on the way. In fp32 512: its error over 2048 positions of 48 heads of 64 x 64 is 3.3e-7 to 3.9e-7 of it where
-// heads remember 2 to 1000 positions, with 1024 4.1e-7 to 6.8e-7 (and 1e-7 where they forget faster, either way); no
-// difference in time (2048 x 16 heads of 80 x 72). 16 bits round far above that (2e-4), and their states are larger
-// beside what else is moved (4 x 2048, 40 heads of 128 x 128: 459 us, with 1024 470, with 512 493).
+// leaves on the way. In fp32 512: its error over 2048 positions of 48 heads of 64 x 64 is 3.3e-7 to 3.9e-7 of it where
+// heads remember 2 to 1000 positions, with 1024 4.1e-7 to 6.8e-7, with 2048 4.9e-7 to 8.6e-7 (1e-7 where they forget
+// faster, with any); 4 x 2048, 40 heads of 128 x 128, both directions: 1211, 1209 and 1206 us. 16 bits round far above
+// that (2e-4), and their states are larger beside what else is moved: 482, 460 and 448 us for the same in bf16.
 int64_t piece_of(const cc1d_attn_params& p) { return p.dtype == CC1D_DTYPE_FP32 ? 512 : 2048; }
 
 // Sequences run as one block per head where those come near to filling the
 // chip (256 CUs, two or three blocks each); longer ones are cut into segments
 // that run side by side, from states that a first pass over keys and values
 // alone provides, which costs about half as much again. Measured, bf16 128 x 128,
-// both directions: batch 4 of 40 heads, 2048 positions 506 us whole and 602 in
-// three segments; fp32 80 x 72, 16 heads of 2048: 242 us in segments of 256,
-// about 205 with 128, 933 whole. Packed sequences are cut whatever their
-// number, as their lengths are not known here and one of them may be nearly
+// both directions: batch 4 of 40 heads, 2048 positions 450 us whole and 552 in
+// three segments; fp32 80 x 72, 16 heads of 2048: 248 us in segments of 192 (this
+// rule's) or 256, 193 with 128, 1006 whole. Packed sequences are cut whatever
+// their number, as their lengths are not known here and one of them may be nearly
 // all: a block's share is then 1 / 768 of the work or 192 positions, whichever
-// is more (8192 positions, 32 heads: 180 us, and 211 with segments of 256, 196
-// with 512, 264 whole).
+// is more (8192 ragged positions, 32 heads, forward: 166 us, and 188 with segments
+// of 256, 183 with 512, 225 whole).
 // Below 384 positions two more launches cost more than they save (16 heads of
-// 128 x 128, bf16, 256 positions: 22 us whole, 34 in two segments; 448: 40 and
-// 37 in three; 1024: 81 and 42 in six).
+// 128 x 128, bf16, forward: 256 positions 22 us whole, 30 in two segments; 448: 35
+// and 38 in three; 1024: 73 and 43 in six; both directions 71 and 86, 86 and 99,
+// 179 and 116).
 Plan plan_of(const cc1d_attn_params& p, int jobs) {
     int64_t seg;
     if (p.cu_seqlens) {
@@ -206,13 +207,16 @@ struct DecayGradArgs {
     const float* over;      // the chunk's pairs over each position
     const void* g;
     void* dg;               // (tokens, heads)
-    AttnState dfinal, tail;  // gradients of the final states, and the states before the last chunks; p null: not used
+    AttnState dfinal;       // gradients of the final states; p null: not used
+    const float* tail;      // and the states before the last chunks, as `states`
     int64_t g_stride[3];
     int64_t tokens;
     int32_t dk, dv;
     AttnArgs at;  // the pieces (as a sequence's segments), heads
-    // states between pieces, forwards and backwards: (places, heads, dk, dv)
+    // states between pieces, forwards and backwards: (places, heads, dk, dv), dv rounded up to whole vectors where the
+    // walks left them (`pitch`); null: one piece a sequence
     const float *states, *grads;
+    int32_t pitch;
 };
 
 // The sum over a block of 256, in everybody, in a fixed order. (NaN and infinities of one wavefront reach all.)
@@ -226,22 +230,13 @@ __device__ __forceinline__ double block_sum_f64(double v, double (&part)[4]) {
 
 __device__ __forceinline__ double tail_dot(const DecayGradArgs& a, int64_t seq, uint32_t h, double (&part)[4]) {
     if (a.dfinal.p == nullptr) return 0.0;
-    const float* x = a.dfinal.p + seq * a.dfinal.s[0] + h * a.dfinal.s[1];
-    const float* y = a.tail.p + seq * a.tail.s[0] + h * a.tail.s[1];
+    const float* const x = a.dfinal.p + seq * a.dfinal.s[0] + h * a.dfinal.s[1];
+    const int pitch = (int)kept_rows(a.dv);
+    const float* const y = a.tail + (seq * a.at.heads + h) * a.dk * pitch;
     double s = 0.0;
-    for (int i0 = threadIdx.x; i0 < a.dk * a.dv; i0 += 8 * 256) {  // eight loads of each on their way
-        float xs[8], ys[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int i = i0 + 256 * k, r = i / a.dv, c = i - r * a.dv;
-            xs[k] = ys[k] = 0.0f;
-            if (i < a.dk * a.dv) {
-                xs[k] = x[r * a.dfinal.s[2] + c * a.dfinal.s[3]];
-                ys[k] = y[r * a.tail.s[2] + c * a.tail.s[3]];
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s += (double)xs[k] * (double)ys[k];
+    for (int c = threadIdx.x & 63; c < a.dv; c += 64) {
+#pragma unroll 8
+        for (int r = threadIdx.x >> 6; r < a.dk; r += 4) s += (double)x[r * a.dfinal.s[2] + c * a.dfinal.s[3]] * (double)y[r * pitch + c];
     }
     return block_sum_f64(s, part);
 }
@@ -267,7 +262,7 @@ __device__ __forceinline__ double tail_dot(const DecayGradArgs& a, int64_t seq, 
 // 2048 positions of 64 x 64, fp32, exp(g) = exp(-4), exp(-10): off by 4e-4 and
 // 0.1 of dg, root mean square, this by 1e-7.)
 // A block per piece and head walks over 1024 positions at a time, four to a
-// thread, GL threads to a chunk, sums in 64 bits. Latency bounds it (17 us for
+// thread, GL threads to a chunk, sums in 64 bits. Latency bounds it (14 us for
 // 4 x 2048, 40 heads of 128 x 128), and for many short pieces their states.
 template <typename T, int GL> __global__ void __launch_bounds__(256) attn_decay_grad_kernel(const DecayGradArgs a) {
     constexpr int K = 4, TILE = 256 * K, NG = 256 / GL;  // positions a thread, of a turn; chunks of a turn
@@ -287,7 +282,7 @@ template <typename T, int GL> __global__ void __launch_bounds__(256) attn_decay_
     const bool tail = sp.index + 1 == sp.segs;
     if (!tail) {
         const float decay = to_f32(g[last * a.g_stride[1]]);
-        const int64_t per = (int64_t)a.dk * a.dv, at = (sp.after(false) * heads + h) * per;
+        const int64_t per = (int64_t)a.dk * a.pitch, at = (sp.after(false) * heads + h) * per;
         const float *const x = a.states + at, *const y = a.grads + at;
         double s = 0.0;
 #pragma unroll 8
@@ -413,9 +408,9 @@ Room room_of(const cc1d_attn_bwd_params& b, const Plan& pl) {
     Room r;
     r.dots = aligned(tokens * p.heads);
     r.part = p.heads == p.key_heads ? 0 : aligned(tokens * p.heads * p.dk);
-    r.between = aligned(pieces_of(p).states * per);
+    r.between = aligned(pieces_of(p).states * (pl.cut() ? per : p.heads * p.dk * kept_rows(p.dv)));
     r.decay = aligned(pl.states * p.heads);
-    r.tail = b.dfinal_states ? aligned(pl.seqs * per) : 0;
+    r.tail = b.dfinal_states ? aligned(pl.seqs * p.heads * p.dk * kept_rows(p.dv)) : 0;
     r.total = 3 * r.dots + 2 * r.part + 2 * r.between + 2 * r.decay + r.tail;
     return r;
 }
@@ -492,7 +487,7 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     AttnJob jq{}, jk{}, jv{};
     jq.a = d; jq.b = v; jq.c = k; jq.x = q;
     jq.first = turned(first);
-    jq.tail = turned(state(tail, p.heads, dk, dv));
+    jq.tail = tail;
     jq.seg = turned(state(states, p.heads, dk, dv));
     jq.decay = decay_s;
     jq.out = shared ? dq_part : b.dq;
@@ -540,33 +535,29 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     // where sequences are not cut, the walks leave states for the decays' gradient as they go
     const Plan pieces = pieces_of(p);
     if (!pl.cut() && pieces.cut()) {
-        jq.mark = jq.seg;
-        jk.mark = jk.seg;
+        jq.mark = states;
+        jk.mark = grads;
+        jq.piece = jk.piece = pieces.seg;
+        jq.pieces = jk.pieces = pieces.per_row;
     }
-    auto jobs_of = [&](int jobs) {
-        AttnArgs a = args_of(p, pl, jobs);
-        a.piece = pieces.seg;
-        a.pieces = pieces.per_row;
-        return a;
-    };
     int st;
     const bool alike = (dk <= 64) == (dv <= 64);  // one kernel for all
     if (alike) {
-        AttnArgs a = jobs_of(3);
+        AttnArgs a = args_of(p, pl, 3);
         a.job[0] = jq; a.job[1] = jk; a.job[2] = jv;
         st = launch_jobs(p.dtype, a, dk, dv, false, stream);
     } else {
-        AttnArgs a = jobs_of(2);
+        AttnArgs a = args_of(p, pl, 2);
         a.job[0] = jq; a.job[1] = jk;
         st = launch_jobs(p.dtype, a, dv, dk, false, stream);
         if (st != CC1D_OK) return st;
-        AttnArgs c = jobs_of(1);
+        AttnArgs c = args_of(p, pl, 1);
         c.job[0] = jv;
         st = launch_jobs(p.dtype, c, dk, dv, false, stream);
     }
     if (st != CC1D_OK) return st;
     if (tokens == 0) return CC1D_OK;
-    DecayGradArgs dg{row_dots, col_dots, over, p.g, b.dg, last_grad, state(tail, p.heads, dk, dv), {}, tokens, dk, dv, args_of(p, pieces, 1), states, grads};
+    DecayGradArgs dg{row_dots, col_dots, over, p.g, b.dg, last_grad, tail, {}, tokens, dk, dv, args_of(p, pieces, 1), states, grads, (int32_t)(pl.cut() ? dv : kept_rows(dv))};
     for (int i = 0; i < 3; ++i) dg.g_stride[i] = p.g_stride[i];
     st = with_dtype(p.dtype, [&](auto t) {
         typedef decltype(t) T;

@@ -53,8 +53,9 @@ struct AttnJob {
     AttnState seg;        // states between segments, by AttnSpan::between(); p null: whole sequences
     float* decay;         // (the same, heads): the decay of the segment walked before it
     void* out;            // (batch * seqlen, heads, dc) contiguous
-    AttnState mark;       // states on the way, at multiples of AttnArgs::piece, by AttnSpan::between(); p null: none
-    AttnState tail;       // state before the sequence's last chunk (forwards); p null: not wanted
+    float* mark;          // states on the way, at multiples of `piece`, by AttnSpan::between(); null: not wanted
+    float* tail;          // states before the sequences' last chunks (forwards); null: not wanted. Both: see kept_rows()
+    int64_t piece, pieces;  // of marks: positions, a multiple of the chunk; of a row (without cu)
     float* dots;          // (heads, batch * seqlen): x with what the state gives the outputs; null: not wanted
     float* over;          // the same: the chunk's pairs over each position; null: not wanted
     int32_t da, dc;       // sizes of rows and columns, of values
@@ -71,7 +72,6 @@ struct AttnArgs {
     const int32_t* cu;
     int64_t batch, seqlen, num_seqs;
     int64_t seg;  // positions of a segment, a multiple of the chunk
-    int64_t piece, pieces;  // of marks, the same; of a row (without cu)
     uint32_t heads, jobs, slots, per_row;  // slots of all sequences; of one (without cu)
     FastDiv heads_div, jobs_div, row_div;
     uint32_t blocks;
@@ -83,8 +83,8 @@ template <> struct AttnType<f16> { static constexpr int planes = 2, order = 1; }
 template <> struct AttnType<float> { static constexpr int planes = 3, order = 2; };
 
 // Positions of a chunk: 64 where the images of that many leave two blocks and more to a CU (both directions of 4 x 2048,
-// 32 heads of 64 x 64, fp16: 330 us, with 32 positions 405; but 8164 packed positions of 128 x 64, where the backward's
-// 64 x 128 would have 64 as well: 561, with 32 535).
+// 32 heads of 64 x 64, fp16: 350 us, with 32 positions 418; but 8164 packed positions of 128 x 64: 580, with 32 468).
+// Rows and columns may change places: dq, dk and dv need the same chunks.
 constexpr int kMaxChunk = 64;
 template <typename T> constexpr int chunk_of(int da, int dc) { return AttnType<T>::planes * (2 * da + dc) <= 384 ? kMaxChunk : 32; }
 constexpr int attn_dim_of(int64_t d) { return d <= 64 ? 64 : 128; }  // a head of d is computed as one of this
@@ -160,6 +160,9 @@ template <int BLKS> __device__ __forceinline__ u32x4 turn_at(const uint16_t* ima
     return u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
 }
 
+// States that the backward leaves for the decays' gradient: (places, heads, columns, rows rounded up to whole vectors).
+__host__ __device__ constexpr int64_t kept_rows(int64_t rows) { return (rows + 3) / 4 * 4; }
+
 __device__ __forceinline__ float opaque_f32(float v) { return __int_as_float(opaque(__float_as_int(v))); }
 
 // exp2 of a sum held in two floats: the second is at most an ulp of the first
@@ -196,6 +199,20 @@ __device__ __forceinline__ float sum16(float v) {
     v += dpp_f32<kDppRowRor4, 0xf>(v);
     v += dpp_f32<kDppRowRor8, 0xf>(v);
     return v;
+}
+
+// Sum over the four lanes that are 16 apart, in every one of them, and over those of them before this one. Swaps of rows
+// in the vector unit: a lane permutation through LDS takes as long as an access, and one waits for the other.
+__device__ __forceinline__ float sum_rows(float v, int row, float& before) {
+    typedef unsigned two __attribute__((ext_vector_type(2)));
+    const unsigned u = __float_as_uint(v);
+    const two a = __builtin_bit_cast(two, __builtin_amdgcn_permlane16_swap(u, u, false, false));  // rows 0 0 2 2, 1 1 3 3
+    const float even = __uint_as_float(a[0]), pair = even + __uint_as_float(a[1]);
+    const unsigned w = __float_as_uint(pair);
+    const two b = __builtin_bit_cast(two, __builtin_amdgcn_permlane32_swap(w, w, false, false));  // the lower pair, the upper
+    const float low = __uint_as_float(b[0]);
+    before = (row & 1 ? even : 0.0f) + (row & 2 ? low : 0.0f);
+    return low + __uint_as_float(b[1]);
 }
 
 // A log decay as the sums take it: -1e5 stands for everything below (its
@@ -286,24 +303,23 @@ template <typename T, int C, int D, bool QUICK> struct AttnTile {
             const uint32_t at = (uint32_t)(down ? R - 1 - row : row) * pitch + col * (uint32_t)sizeof(T);
             const char* low = reinterpret_cast<const char*>(base) - (down ? (uint64_t)((R - 1) * pitch) : 0);
             const int64_t turn = (int64_t)(R * sizeof(T)) * row_stride;
-            if (rows == C && d == D) {
+            if constexpr (DIRECT) {
+                if (rows == C && d == D) {
+#pragma unroll
+                    for (int n = 0; n < N; ++n, low += turn) direct(low + at, image, n, wave);
+                    return;
+                }
 #pragma unroll
                 for (int n = 0; n < N; ++n, low += turn) {
-                    if constexpr (DIRECT) direct(low + at, image, n, wave);
-                    else v[n] = vload_any(reinterpret_cast<const T*>(low + at));
+                    if (n * R + row < rows && col < d) direct(low + at, image, n, wave);
+                    else *reinterpret_cast<u32x4*>(image + (n * 256 + tid) * 8) = vzero();
                 }
             } else {
+                // (without a branch, so that the loads on their way are counted, and what came before them is not waited
+                // for with all of them: what is not the head's is read from its first row, and dropped by store())
 #pragma unroll
-                for (int n = 0; n < N; ++n, low += turn) {
-                    const bool in = n * R + row < rows && col < d;
-                    if constexpr (DIRECT) {
-                        if (in) direct(low + at, image, n, wave);
-                        else *reinterpret_cast<u32x4*>(image + (n * 256 + tid) * 8) = vzero();
-                    } else {
-                        v[n] = vzero();
-                        if (in) v[n] = vload_any(reinterpret_cast<const T*>(low + at));
-                    }
-                }
+                for (int n = 0; n < N; ++n, low += turn)
+                    v[n] = vload_any(n * R + row < rows && col < d ? reinterpret_cast<const T*>(low + at) : base);
             }
         } else {
 #pragma unroll
@@ -338,11 +354,13 @@ template <typename T, int C, int D, bool QUICK> struct AttnTile {
             for (int n = 0; n < N; ++n) v[n] = vzero();
     }
     // image[plane][position][column]
-    __device__ __forceinline__ void store(uint16_t* image, int tid) const {
+    __device__ __forceinline__ void store(uint16_t* image, int rows, int d, int tid) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             int row, col;
             unit(n, tid, row, col);
+            if constexpr (QUICK)
+                if (!(row < rows && col < d)) v[n] = vzero();
             uint32_t w[P][EPV / 2];
             if constexpr (std::is_same_v<T, bf16>) {
 #pragma unroll
@@ -399,8 +417,8 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
     // In fp32 the products of lesser planes have sums of their own, so that a large sum is rounded once for a product of
     // the first planes and once for the rest, not by each of six. 2 x 2048, 40 heads of 128 x 128: outputs and gradients
     // off by 1.7e-7 to 1.9e-7 instead of 3.4e-7 to 3.8e-7. Free in heads of 64; in those of 128 x 128 registers are
-    // short (TIGHT: x is read when it is wanted) and both directions take 14 % longer.
-    constexpr bool LESSER = std::is_same_v<T, float>, TIGHT = LESSER && DA * DC >= 128 * 128;
+    // short and both directions take 5 % longer.
+    constexpr bool LESSER = std::is_same_v<T, float>;
     constexpr int LI = LESSER ? C / 16 : 0, LP = LESSER ? PT : 0;
     constexpr int kPairs = PP * C * C, kA = STATES ? 0 : (P * C * DA > kPairs ? P * C * DA : kPairs);
     __shared__ __attribute__((aligned(16))) uint16_t lds[kA + P * C * DA + P * C * DC];
@@ -502,9 +520,9 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
     auto rows_at = [&](int r) { return r == r_first && head > 0 ? head : r_end - r < C ? r_end - r : C; };
     // A word of each 128 bytes of the next n rows, so that what goes straight into its image comes from the L2 cache when
     // its turn has come (two wavefronts to an operand). Not long before: the blocks of an XCD work on about as much as
-    // its L2 holds, and lines fetched a whole chunk ahead were gone when they were wanted. Backward of 4 x 2048, 40 heads
-    // of 128 x 128, bf16: 0.80 GB read and 310 us without, 1.32 GB and 275 us from the chunk's start, 0.95 GB and the
-    // same 275 us from its middle.
+    // its L2 holds, and lines fetched a whole chunk ahead were gone when they were wanted. 4 x 2048, 40 heads of 128 x
+    // 128, bf16: forward 187 us without, 161 from the chunk's start, 165 from its middle; backward 309 (0.88 GB read),
+    // 322 (1.47 GB) and 308 (0.99 GB).
     uint32_t ahead[2] = {0, 0};
     auto fetch = [&](int n, int t) {
         auto word = [&](const T* p, int64_t s, int d, int lines, uint32_t& to) {
@@ -528,26 +546,71 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
             if (over) job.over[at] = (over_lds[0][tid] + over_lds[1][tid]) + (over_lds[2][tid] + over_lds[3][tid]);
         }
     };
-    auto put_state = [&](const AttnState& to, int64_t place, float by, int lane) {
-        float* const at = to.p + place * to.s[0] + h * to.s[1];
-        const int s2 = (int)to.s[2], s3 = (int)to.s[3];
-#pragma unroll
-        for (int t = 0; t < TA; ++t)
-#pragma unroll
-            for (int m = 0; m < NT; ++m)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = tile_col(t, 4 * (lane >> 4) + e), col = tile_col(wave * NT + m, lane & 15);
-                    if (row < da && col < dc) at[(uint32_t)(row * s2 + col * s3)] = by * S[t][m][e];
-                }
+    // Where in the walk the state is wanted next, after `at`. (What it needs is read again each time: kept, it would take
+    // scalar registers that the loop has not got.)
+    auto job_again = [&]() -> const AttnJob& { return args.job[uniform32(opaque((int)jn))]; };
+    auto stop_after = [&](int at) {
+        const AttnJob& again = job_again();
+        int stop = 0x7fffffff;
+        if (again.mark != nullptr) {
+            const int piece = (int)again.piece, rest = (int)sp.len % piece, base = reverse && rest > 0 ? rest : piece;
+            stop = at < base ? base : base + ((at - base) / piece + 1) * piece;
+        }
+        const int tail = ((int)sp.len - 1) / C * C;
+        return again.tail != nullptr && tail > at && tail < stop ? tail : stop;
     };
-    // the position of the walk where the state is wanted next
-    int mark = 0x7fffffff;
-    if (GRADS && job.mark.p != nullptr) mark = reverse && sp.len % args.piece ? (int)(sp.len % args.piece) : (int)args.piece;
+    int stop = 0x7fffffff;
+    if constexpr (GRADS) stop = stop_after(r_first - 1);
+
+    // x, in vectors of XE values: for `dots` beside the outputs, a row's NT * 4 neighbours; for `over` as a left operand
+    // of NS products of 32 columns, 16 rows of x a wavefront (in chunks of 32 half of their columns). As many vectors
+    // either way, and no branch between them: it would wait for the loads.
+    constexpr int XE = sizeof(T) == 2 && NT == 2 ? 8 : 4, XR = NT * 4 / XE, XN = IT * XR, NS = C == 64 ? DC / 32 : DC / 64;
+    static_assert(XN * XE == NS * 8, "two layouts of as many values");
+    typedef uint32_t xvec __attribute__((ext_vector_type(XE * sizeof(T) / 4)));
+    typedef std::conditional_t<sizeof(xvec) == 16, typename AnyAddr<sizeof(T)>::v4, typename AnyAddr<sizeof(T)>::v2> xword;
+    xvec xr[GRADS ? XN : 1];
+    auto x_at = [&](int unit, int e) {
+        u32x4 w = vzero();
+#pragma unroll
+        for (int i = 0; i < (int)(XE * sizeof(T) / 4); ++i) w[i] = xr[unit][i];
+        return vget<T>(w, e);
+    };
+    const int xt = C == 64 ? wave : wave & 1, xs = C == 64 ? 0 : (wave >> 1) * NS;
+    auto load_x = [&](const T* const from, int count, int t) {
+        const int l16 = t & 15, g4 = (t >> 4) & 3, col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
+#pragma unroll
+        for (int i = 0; i < XN; ++i) {
+            const int tile = dots ? i / XR : xt;
+            const int c = dots ? col + XE * (i % XR) : 32 * (xs + i * XE / 8) + 8 * g4 + i * XE % 8;
+            const bool in = 16 * tile + l16 < count && c < dc;
+            u32x4 w = vzero();
+            if constexpr (QUICK) {
+                const char* const low = reinterpret_cast<const char*>(from) + ((reverse ? 15 : 0) + 16 * tile) * sx * (int64_t)sizeof(T);
+                const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(c * (int)sizeof(T));
+                xr[i] = xvec(0u);
+                if (in) xr[i] = *reinterpret_cast<const xword*>(low + at);
+            } else {
+                const T* const p = from + (16 * tile + l16) * sx + c * ex;
+                xr[i] = xvec(0u);
+                if (in && ex == 1 && c + XE <= dc) {
+                    xr[i] = *reinterpret_cast<const xword*>(p);
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < XE; ++e)  // (as AttnTile::load())
+                    if (in && c + e < dc) decltype(ta)::put(w, e, p[e * ex]);
+#pragma unroll
+                for (int k = 0; k < (int)(XE * sizeof(T) / 4); ++k) xr[i][k] = w[k];
+            }
+        }
+    };
 
     // Registers load a chunk while the block works on the one before; what goes straight into its image is waited for
     // while the CU's other blocks work. The first turn only loads (or only forms the decays).
     int r = r_first, n = 0, buf = 1;
+    if constexpr (GRADS && !DIRECT)
+        if (beside) load_x(px, rows_at(r_first), opaque(tid));
     ta.none();
     tb.none();
     tc.none();
@@ -561,67 +624,28 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
             if (wave == 3 && n_next > 0) g_next = g_load(r + n, n_next);
             asm volatile("s_waitcnt vmcnt(0)" ::"v"(ahead[0]), "v"(ahead[1]) : "memory");
         } else {
-            if (wave == 3 && n_next > 0) g_next = g_load(r + n, n_next);
-            if constexpr (!STATES) ta.store(ldsA, otid);
-            tb.store(ldsB, otid);
-            tc.store(ldsC, otid);
+            if constexpr (!STATES) ta.store(ldsA, n, da, otid);
+            tb.store(ldsB, n, da, otid);
+            tc.store(ldsC, n, dc, otid);
+            // (x is here by now; where it is used, a wait would be for the next chunk as well)
+            if constexpr (GRADS) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
         }
         __syncthreads();
+        const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
+        const bool full = n == C && dc == DC;
         if (n_next > 0) {
-            if constexpr (!DIRECT) load(n_next, otid);
-            else if (n == 0) fetch(n_next, otid);
+            if constexpr (!DIRECT) {
+                if (wave == 3) g_next = g_load(r + n, n_next);
+                load(n_next, otid);
+            } else if (n == 0) {
+                fetch(n_next, otid);
+            }
         }
         if (n > 0) {
             const uint32_t fragD = frag_base<DA / 8>(l16, g4, 0);
             const uint32_t fragC = frag_base<C / 8>(l16, g4, 0), halfC = frag_base<C / 8>(l16, g4 >> 1, g4 & 1);
             const uint32_t turnB = turn_base<DA / 8>(l16, g4), turnC = turn_base<DC / 8>(l16, g4);
             f32x4 O[IT][NT];
-            const int col = NT == 2 ? 32 * wave + 8 * g4 : 32 * (wave >> 1) + 4 * (wave & 1) + 8 * g4;
-            const bool full = n == C && dc == DC;
-            // x, in vectors of 16 bytes: for `dots` beside the outputs, a row's NT * 4 neighbours; for `over` as a left
-            // operand of NS products of 32 columns, 16 rows of x a wavefront (in chunks of 32 half of their columns)
-            constexpr int XV = sizeof(T) == 2 ? 1 : 2, NS = C == 64 ? DC / 32 : DC / 64;
-            constexpr int XD = sizeof(T) == 2 ? IT : IT * NT, XN = XD > NS * XV ? XD : NS * XV;
-            u32x4 x4[GRADS ? XN : 1];
-            const int xt = C == 64 ? wave : wave & 1, xs = C == 64 ? 0 : (wave >> 1) * NS;
-            auto load_x = [&]() {
-                constexpr int EPV = elems16<T>::value;
-                auto get = [&](u32x4& w, int tile, int c) {  // of the row of tile that is the lane's
-                    constexpr bool TWO = sizeof(T) == 2 && NT == 1;  // (for `dots`: half a vector)
-                    const bool part = TWO && dots;
-                    w = vzero();
-                    if (!(full || 16 * tile + l16 < n)) return;
-                    if constexpr (QUICK) {
-                        const char* const low = reinterpret_cast<const char*>(px) + ((reverse ? 15 : 0) + 16 * tile) * sx * (int64_t)sizeof(T);
-                        const uint32_t at = (uint32_t)(reverse ? 15 - l16 : l16) * (uint32_t)((reverse ? -sx : sx) * (int64_t)sizeof(T)) + (uint32_t)(c * (int)sizeof(T));
-                        if (c >= dc) return;
-                        if (part) {
-                            const u32x2 v = *reinterpret_cast<const typename AnyAddr<2>::v2*>(reinterpret_cast<const T*>(low + at));
-                            w[0] = v[0];
-                            w[1] = v[1];
-                        } else {
-                            w = vload_any(reinterpret_cast<const T*>(low + at));
-                        }
-                    } else {
-                        const T* const p = px + (16 * tile + l16) * sx + c * ex;
-                        const int count = part ? 4 : EPV;
-                        if (ex == 1 && !part && c + EPV <= dc) {
-                            w = vload_any(p);
-                            return;
-                        }
-#pragma unroll
-                        for (int e = 0; e < EPV; ++e)
-                            if (e < count && c + e < dc) decltype(ta)::put(w, e, p[e * ex]);
-                    }
-                };
-                if (dots) {
-#pragma unroll
-                    for (int i = 0; i < XD; ++i) get(x4[i], i / (XD / IT), col + 4 * (i % (XD / IT)));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NS * XV; ++i) get(x4[i], xt, 32 * (xs + i / XV) + 8 * g4 + 4 * (i % XV));
-                }
-            };
             if constexpr (!STATES) {
                 // ---- what the state gives, and the pairs, transposed (columns x rows), so that a lane gets four columns
                 // of a row: both from one reading of the rows
@@ -686,8 +710,8 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
                     }
                 }
                 if constexpr (LESSER) acc[0] += few[0];
-                if constexpr (GRADS && !TIGHT)
-                    if (beside) load_x();
+                if constexpr (GRADS && DIRECT)
+                    if (beside) load_x(px, n, otid);
                 uint32_t pw[PT][PP][2];
                 const int j = 16 * jt + 4 * g4;
                 const f32x4 jhi = *reinterpret_cast<const f32x4*>(&sums_hi[buf][j]), jlo = *reinterpret_cast<const f32x4*>(&sums_lo[buf][j]);
@@ -725,24 +749,25 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
                     for (int p = 0; p < PP; ++p)
                         *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(ldsP + p * C * C) + (halfC ^ frag_tile<C / 8>(2, 6))) = u32x2{0u, 0u};
                 __syncthreads();
-                if constexpr (GRADS && TIGHT)
-                    if (beside) load_x();
                 if constexpr (GRADS) if (dots) {
                     // ---- what the state gives, dotted
+                    float dot[IT];
 #pragma unroll
                     for (int it = 0; it < IT; ++it) {
-                        float dot = 0.0f;
+                        dot[it] = 0.0f;
 #pragma unroll
                         for (int m = 0; m < NT; ++m)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float x = sizeof(T) == 2 ? vget<T>(x4[it], 4 * m + e) : vget<T>(x4[it * (XD / IT) + (sizeof(T) == 2 ? 0 : m)], e);
-                                dot = __builtin_fmaf(O[it][m][e], x, dot);
-                            }
-                        dot += __shfl_xor(dot, 16);
-                        dot += __shfl_xor(dot, 32);
-                        if (g4 == 0) dot_lds[wave][16 * it + l16] = dot;
+                            for (int e = 0; e < 4; ++e) dot[it] = __builtin_fmaf(O[it][m][e], x_at(it * XR + (4 * m + e) / XE, (4 * m + e) % XE), dot[it]);
                     }
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        float unused;
+                        dot[it] = sum_rows(dot[it], g4, unused);
+                    }
+                    if (g4 == 0)
+#pragma unroll
+                        for (int it = 0; it < IT; ++it) dot_lds[wave][16 * it + l16] = dot[it];
                 }
                 if constexpr (GRADS) if (over) {
                     // ---- The chunk's pairs over a position: of its rows on one side and its columns on the other, the pair
@@ -756,58 +781,74 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
                     for (int s = 0; s < NS; ++s) {
                         if constexpr (std::is_same_v<T, bf16>) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) xw[s][0][i] = x4[s][i];
+                            for (int i = 0; i < 4; ++i) xw[s][0][i] = XE == 8 ? xr[XE == 8 ? s : 0][i % (XE / 2)] : xr[XE == 8 ? 0 : 2 * s + (i >> 1)][i & 1];
                         } else {
                             float f[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) f[i] = sizeof(T) == 2 ? vget<T>(x4[s], i) : vget<T>(x4[XV * s + i / 4 % XV], i & 3);
+                            for (int i = 0; i < 8; ++i) f[i] = x_at((8 * s + i) / XE, (8 * s + i) % XE);
                             to_planes<P, 4>(f, xw[s]);
                         }
                     }
                     // (every tile without a branch, so that they wait side by side; what is not the position's is dropped in
                     // the end, by a select, as it need not be finite)
-                    f32x4 w[IT];
+                    f32x4 w[IT], less[LESSER ? IT : 1];
 #pragma unroll
                     for (int jt = 0; jt < IT; ++jt) {
-                        f32x4 less = {0.0f, 0.0f, 0.0f, 0.0f};
-                        w[jt] = less;
+                        w[jt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        less[LESSER ? jt : 0] = w[jt];
+                    }
 #pragma unroll
-                        for (int s = 0; s < NS; ++s)
+                    for (int s = 0; s < NS; ++s)
 #pragma unroll
-                            for (int p = 0; p < P; ++p) {
-                                const bf16x8 fk = lds_at<bf16x8>(ldsC + p * C * DC, fragX ^ frag_tile<DC / 8>(jt, 4 * (xs + s)));
+                        for (int p = 0; p < P; ++p) {
+                            bf16x8 fk[IT];
 #pragma unroll
-                                for (int q = 0; q < P; ++q) {
-                                    f32x4& to = LESSER && p + q > 0 ? less : w[jt];
-                                    if (p + q <= ORD) to = mfma(fk, as_frag(xw[s][q]), to);
+                            for (int jt = 0; jt < IT; ++jt) fk[jt] = lds_at<bf16x8>(ldsC + p * C * DC, fragX ^ frag_tile<DC / 8>(jt, 4 * (xs + s)));
+#pragma unroll
+                            for (int q = 0; q < P; ++q)
+#pragma unroll
+                                for (int jt = 0; jt < IT; ++jt) {
+                                    f32x4& to = LESSER && p + q > 0 ? less[LESSER ? jt : 0] : w[jt];
+                                    if (p + q <= ORD) to = mfma(fk[jt], as_frag(xw[s][q]), to);
                                 }
-                            }
-                        if constexpr (LESSER) w[jt] += less;
-                        f32x4 pair = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int q = PP - 1; q >= 0; --q) {
-                            const u32x2 b = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(ldsP + q * C * C) + (halfC ^ frag_tile<C / 8>(xt, 2 * jt)));
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) pair[e] += __uint_as_float(e & 1 ? b[e >> 1] & 0xffff0000u : b[e >> 1] << 16);
                         }
-                        w[jt] *= pair;
-                    }
+                    u32x2 pair[IT][PP];
+#pragma unroll
+                    for (int jt = 0; jt < IT; ++jt)
+#pragma unroll
+                        for (int q = 0; q < PP; ++q)
+                            pair[jt][q] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const char*>(ldsP + q * C * C) + (halfC ^ frag_tile<C / 8>(xt, 2 * jt)));
+                    f32x4 sums[IT];
                     float tiles = 0.0f;  // of the tiles before
+                    const bool in = full || 16 * xt + l16 < n;
 #pragma unroll
                     for (int jt = 0; jt < IT; ++jt) {
-                        const float w01 = w[jt][0] + w[jt][1], w012 = w01 + w[jt][2], all = w012 + w[jt][3];
-                        const float one = __shfl_up(all, 16), near = g4 >= 1 ? one : 0.0f, two = __shfl_up(all + near, 32);
-                        const float lanes = near + (g4 >= 2 ? two : 0.0f), base = tiles + lanes;
-                        const float upto[5] = {base, base + w[jt][0], base + w01, base + w012, base + all};
-                        if (jt + 1 < IT) tiles += __shfl(lanes + all, 48 + l16);
-                        const int most = !(full || 16 * xt + l16 < n) || jt > xt ? -1 : jt < xt ? C : l16 - 4 * g4 - (reverse ? 1 : 0);
-                        f32x4 sums;
+                        if constexpr (LESSER) w[jt] += less[jt];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sums[e] = sum16(e <= most ? (reverse ? upto[e + 1] : upto[e]) : 0.0f);
-                        if (l16 == 0) *reinterpret_cast<f32x4*>(&over_lds[wave][16 * jt + 4 * g4]) = sums;
+                        for (int e = 0; e < 4; ++e) {
+                            float f = 0.0f;
+#pragma unroll
+                            for (int q = PP - 1; q >= 0; --q) f += __uint_as_float(e & 1 ? pair[jt][q][e >> 1] & 0xffff0000u : pair[jt][q][e >> 1] << 16);
+                            w[jt][e] *= f;
+                        }
+                        const float w01 = w[jt][0] + w[jt][1], w012 = w01 + w[jt][2], all = w012 + w[jt][3];
+                        float lanes;
+                        const float tile = sum_rows(all, g4, lanes), base = tiles + lanes;
+                        tiles += tile;
+                        const float upto[5] = {base, base + w[jt][0], base + w01, base + w012, base + all};
+                        const int most = !in || jt > xt ? -1 : jt < xt ? C : l16 - 4 * g4 - (reverse ? 1 : 0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sums[jt][e] = sum16(e <= most ? (reverse ? upto[e + 1] : upto[e]) : 0.0f);
                     }
+                    if (l16 == 0)
+#pragma unroll
+                        for (int jt = 0; jt < IT; ++jt) *reinterpret_cast<f32x4*>(&over_lds[wave][16 * jt + 4 * g4]) = sums[jt];
                 }
             }
+            // the next chunk's x, with the time until that chunk to arrive (waited for with its operands: a wait on its own
+            // would be for all that is on its way)
+            if constexpr (GRADS && !DIRECT)
+                if (beside && n_next > 0) load_x(px + n * sx, n_next, otid);
             if constexpr (DIRECT)
                 if (n_next > 0) fetch(n_next, otid);
             const float decay = whole[buf];
@@ -951,17 +992,25 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
         }
         if (n_next <= 0) break;
         if constexpr (GRADS)
-#pragma unroll 1
-            for (int want = 0; want < 2; ++want) {
-                const bool tail = want == 1;
-                if (tail ? job.tail.p == nullptr || r + n + n_next != (int)sp.len : r + n != mark) continue;
-                int64_t place = sp.seq;
-                if (!tail) {
-                    const int64_t p = (reverse ? sp.len - mark : (int64_t)mark) / args.piece;
-                    place = (args.cu ? sp.first / args.piece : sp.seq * (args.pieces - 1)) + p - 1;
-                    mark += (int)args.piece;
-                }
-                put_state(tail ? job.tail : job.mark, place, 1.0f, opaque(lane));
+            if (r + n == stop) {
+                // (a lane has four neighbouring rows of a column)
+                auto put = [&](float* states, int64_t place) {
+                    const int ol = opaque(lane), rows = (int)kept_rows(da), row0 = 8 * (ol >> 4);
+                    float* const at = states + (place * args.heads + h) * dc * rows + row0;
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) {
+                        const int col = tile_col(wave * NT + m, ol & 15);
+#pragma unroll
+                        for (int t = 0; t < TA; ++t)
+                            if (row0 + 32 * (t >> 1) + 4 * (t & 1) < da && col < dc)
+                                *reinterpret_cast<AnyAddr<4>::v4*>(at + col * rows + 32 * (t >> 1) + 4 * (t & 1)) = __builtin_bit_cast(u32x4, S[t][m]);
+                    }
+                };
+                const AttnJob& again = job_again();
+                const int64_t at = reverse ? sp.len - stop : (int64_t)stop, p = again.mark != nullptr ? at / again.piece : 0;
+                if (p > 0 && p * again.piece == at) put(again.mark, (args.cu ? sp.first / again.piece : sp.seq * (again.pieces - 1)) + p - 1);
+                if (again.tail != nullptr && stop == ((int)sp.len - 1) / C * C) put(again.tail, sp.seq);
+                stop = stop_after(stop);
             }
         if (wave == 3 && (STATES || n == 0)) decays(g_next, buf ^ 1);
         __syncthreads();
@@ -983,7 +1032,17 @@ __global__ void __launch_bounds__(256, QUICK && sizeof(T) == 2 && DC == 64 ? 3 :
         float by = 1.0f;
         // backwards, the state before the sequence has its first decay too
         if (!STATES && reverse && sp.len > 0) by = (float)exp(log_decay(to_f32(pg[sp.first * args.g_stride[1]])));
-        put_state(last, STATES ? sp.after(reverse) : sp.seq, by, lane);
+        float* const at = last.p + (STATES ? sp.after(reverse) : sp.seq) * last.s[0] + h * last.s[1];
+        const int s2 = (int)last.s[2], s3 = (int)last.s[3];
+#pragma unroll
+        for (int t = 0; t < TA; ++t)
+#pragma unroll
+            for (int m = 0; m < NT; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = tile_col(t, 4 * (lane >> 4) + e), col = tile_col(wave * NT + m, lane & 15);
+                    if (row < da && col < dc) at[(uint32_t)(row * s2 + col * s3)] = by * S[t][m][e];
+                }
     }
 
     if (STATES && tid == 3 * 64) job.decay[sp.after(reverse) * args.heads + h] = (float)exp2(total);
