@@ -562,8 +562,9 @@ int launch_attn_bwd(const cc1d_attn_bwd_params& b, hipStream_t stream) {
     st = with_dtype(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         static_assert(chunk_of<T>(64, 128) == chunk_of<T>(128, 64), "dq, dk and dv in the same chunks");
-        const bool wide = chunk_of<T>(attn_dim_of(dv), attn_dim_of(dk)) == 64;
-        return launch(wide ? attn_decay_grad_kernel<T, 16> : attn_decay_grad_kernel<T, 8>, dim3(dg.at.blocks), dim3(256), stream, dg);
+        constexpr int least = chunk_of<T>(128, 128), most = chunk_of<T>(64, 64);
+        const bool wide = chunk_of<T>(attn_dim_of(dv), attn_dim_of(dk)) == most;
+        return launch(wide ? attn_decay_grad_kernel<T, most / 4> : attn_decay_grad_kernel<T, least / 4>, dim3(dg.at.blocks), dim3(256), stream, dg);
     });
     if (st != CC1D_OK || !shared) return st;
     const GroupSumArgs gs{{dq_part, dk_part}, {b.dq, b.dk}, tokens * p.key_heads * p.dk, (int32_t)per, dk};
