@@ -48,8 +48,8 @@ int64_t piece_of(const cc1d_attn_params& p) { return p.dtype == CC1D_DTYPE_FP32 
 // that run side by side, from states that a first pass over keys and values
 // alone provides, which costs about half as much again. Measured, bf16 128 x 128,
 // both directions: batch 4 of 40 heads, 2048 positions 450 us whole and 552 in
-// three segments; fp32 80 x 72, 16 heads of 2048: 248 us in segments of 192 (this
-// rule's) or 256, 193 with 128, 1006 whole. Packed sequences are cut whatever
+// three segments (forward alone 151 and 149); fp32 80 x 72, 16 heads of 2048: 248
+// us in segments of 192 (this rule's), 193 with 128, 1006 whole. Packed sequences are cut whatever
 // their number, as their lengths are not known here and one of them may be nearly
 // all: a block's share is then 1 / 768 of the work or 192 positions, whichever
 // is more (8192 ragged positions, 32 heads, forward: 166 us, and 188 with segments
