@@ -61,6 +61,17 @@ def test_whole_and_long(dtype):
 
 
 @TYPES
+@pytest.mark.parametrize("size", [(61, 33), (72, 128), (30, 7)], ids=str)
+def test_whole_of_odd_sizes(size, dtype):
+    """States that are left on the way have rows of no whole vectors."""
+    p = rated(1, 1100 if dtype == FP32 else 2100, 43, 43, *size, dtype, True)
+    got = own(p)["dg"]
+    for h in (0, 15, 30, 39, 42):
+        close_dg(got[:, :, h:h + 1], {n: None if t is None else t[:, h:h + 1] if n in ("init", "dfinal") else t[:, :, h:h + 1]
+                                      for n, t in p.items()}, f"head {h}")
+
+
+@TYPES
 def test_batches(dtype):
     """Rows of a batch, whole: states on the way have places of their own."""
     check(rated(7, 1100, 7, 7, 8, 8, dtype, True))
